@@ -1,0 +1,315 @@
+// Decode attention over the 4-bit key/value cache (kv4.cuh): one query token per sequence, softmax(scale q k^T) v over its cached tokens or the last
+// `window` of them. One CTA of four warps per (sequence, key/value head and up to eight of its query heads, split of the tokens).
+//
+// Both products run as 16 x 8 x 16 tensor-core instructions whose 16-row operand comes from the codes in registers; the query heads are the eight columns:
+//     S^T[16 tokens, 8 heads] = K[16 tokens, dims] Q^T        O^T[16 dims, 8 heads] += V^T[16 dims, 16 tokens] P^T
+// A code c becomes the bf16 number 128 + c by one logic instruction for two of them (bits 0-3 of the mantissa). What that adds is taken off
+// exactly: from the keys by starting each product at -135.5 times the sum of the query's values, from the values by one more instruction per group of 32 dimensions that
+// sums the weights (a row of ones). Scales multiply the products of a group of keys, and the weights of a group of values, in 32 bits. The place of codes in a page is
+// such that a thread's registers are what it loads: no shuffle and no pass through shared memory. A thread's rows of S^T are the
+// tokens 4 (r / 2) + r % 2 and two later (r = lane / 4), so that the columns it has to hold of V^T are four consecutive tokens.
+//
+// tcgen05 would want the unpacked keys and values written to shared or tensor memory first; the unpacking is what bounds the kernel, not the products.
+//
+// The reference's counterpart is the paged attention behind vLLM's kv_cache_dtype (nemo_rl/models/generation/vllm/config.py).
+#include "kv4.cuh"
+
+#include <math.h>
+
+#include <atomic>
+
+namespace {
+using namespace rlb;
+
+constexpr int K4_WARPS = 4;
+constexpr int K4_STEP = 16;      // tokens a warp takes at a time
+constexpr float K4_SLACK = 8.f;  // how far (in powers of two) a score may pass the running maximum before the sums are rescaled: weights stay below 2^8
+
+struct K4Params {
+  const __nv_bfloat16* q;
+  long long q_stride;
+  const uint8_t* cache;
+  long long num_blocks;
+  const int* block_table;
+  long long table_stride;
+  int max_blocks;
+  const int* seq_lens;
+  int Hkv, G, chunks, block_size, window;
+  float scale;
+  int num_splits;
+  float* part_o;
+  float* part_ml;
+  __nv_bfloat16* out;
+  long long out_stride;
+  int* status;
+};
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Codes at nibble j of both halves of a word as two bf16 numbers 128 + code.
+__device__ __forceinline__ uint32_t unpack2(uint32_t w, int j) { return ((w >> (4 * j)) & 0x000f000fu) | 0x43004300u; }
+constexpr float K4_BIAS = 135.5f;      // 128 + 7.5
+
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
+  if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x; w[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+    }
+  }
+}
+__device__ __forceinline__ float bf16_of(uint32_t word, int i) { return __uint_as_float(i & 1 ? word & 0xffff0000u : word << 16); }
+
+// Shared memory after the token loop: [warps][8 heads][D] sums, then [warps][8][2] maximum and sum of the weights.
+template <int D>
+constexpr int k4_smem() { return K4_WARPS * 8 * (D + 2) * static_cast<int>(sizeof(float)); }
+
+template <int D>
+__global__ void __launch_bounds__(K4_WARPS * 32) kv4_decode_kernel(const K4Params p) {
+  extern __shared__ __align__(16) float k4_red[];
+  using Page = Kv4Page<D>;
+  constexpr int G = Page::G;      // groups of 32 dimensions
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
+  const int b = blockIdx.z, kvh = blockIdx.y / p.chunks, chunk = blockIdx.y % p.chunks, split = blockIdx.x;
+  const int heads = min(8, p.G - chunk * 8), head0 = kvh * p.G + chunk * 8;
+  pdl_sync();
+
+  int len = p.seq_lens[b];
+  const long long room = static_cast<long long>(p.max_blocks) * p.block_size;
+  if (len > room) {      // more tokens than the table has pages: recorded, the rest is left out
+    if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, RLB_ERR_BAD_ARG);
+    len = static_cast<int>(room);
+  }
+  len = max(len, 0);
+  const int first = p.window > 0 ? max(0, len - p.window) : 0;
+  const int step0 = first / K4_STEP, steps = len / K4_STEP + (len % K4_STEP != 0) - step0;
+  const int begin = step0 + static_cast<int>(static_cast<long long>(steps) * split / p.num_splits);
+  const int end = step0 + static_cast<int>(static_cast<long long>(steps) * (split + 1) / p.num_splits);
+
+  // the queries as the 8-column operand: pair j of group g is (dimension 32 g + 8 t + j, and four later) of head r
+  uint32_t qf[G][4];
+  float start[G][2];      // -135.5 * sum of the group's values, of heads 2 t and 2 t + 1
+  {
+    const __nv_bfloat16* q = p.q + static_cast<long long>(b) * p.q_stride + static_cast<long long>(head0 + r) * D + 8 * t;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (r < heads) v = *reinterpret_cast<const uint4*>(q + 32 * g);
+      qf[g][0] = __byte_perm(v.x, v.z, 0x5410);
+      qf[g][1] = __byte_perm(v.x, v.z, 0x7632);
+      qf[g][2] = __byte_perm(v.y, v.w, 0x5410);
+      qf[g][3] = __byte_perm(v.y, v.w, 0x7632);
+      const float2 a = unpack_bf16x2(v.x), c = unpack_bf16x2(v.y), d = unpack_bf16x2(v.z), e = unpack_bf16x2(v.w);
+      float s = ((a.x + a.y) + (c.x + c.y)) + ((d.x + d.y) + (e.x + e.y));
+      s += __shfl_xor_sync(0xffffffffu, s, 1);
+      s += __shfl_xor_sync(0xffffffffu, s, 2);
+      start[g][0] = -K4_BIAS * __shfl_sync(0xffffffffu, s, 8 * t);
+      start[g][1] = -K4_BIAS * __shfl_sync(0xffffffffu, s, 8 * t + 4);
+    }
+  }
+  const float c = p.scale * 1.4426950408889634f;
+
+  float o[2 * G][4], z[G][4], top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 2 * G; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+#pragma unroll
+  for (int g = 0; g < G; ++g) z[g][0] = z[g][1] = z[g][2] = z[g][3] = 0.f;
+
+  const int* table = p.block_table + static_cast<long long>(b) * p.table_stride;
+  const int tok = 4 * (r >> 1) + (r & 1);      // of a step; the thread's other row is two tokens later
+  for (int step = begin + warp; step < end; step += K4_WARPS) {
+    const int pos0 = step * K4_STEP, blk = pos0 / p.block_size, off = pos0 - blk * p.block_size;
+    long long page_no = table[blk];
+    if (page_no < 0 || page_no >= p.num_blocks) {      // outside the cache: recorded, its tokens are left out
+      if (lane == 0 && p.status) atomicCAS(p.status, 0, RLB_ERR_BAD_ARG);
+      continue;
+    }
+    const uint8_t* page = p.cache + (page_no * p.Hkv + kvh) * Page::bytes(p.block_size);
+    uint32_t ka[G], kb[G], va[G], vb[G], sa[G], sb[G];      // sa, sb: scales of keys, then of values
+    load_words(page + Page::key_word(off + tok, t, 0), ka);
+    load_words(page + Page::key_word(off + tok + 2, t, 0), kb);
+    const uint8_t* values = page + Page::values_at(p.block_size);
+    load_words(values + Page::value_unit(off + 4 * t, r, 0), va);
+    load_words(values + Page::value_unit(off + 4 * t + 2, r, 0), vb);
+    const uint8_t* scales = page + Page::scales_at(p.block_size);
+    load_words(scales + Page::scale(off + tok, 0, 0), sa);
+    load_words(scales + Page::scale(off + tok + 2, 0, 0), sb);
+
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      float acc[4] = {start[g][0], start[g][1], start[g][0], start[g][1]};
+      mma_bf16(acc, unpack2(ka[g], 0), unpack2(kb[g], 0), unpack2(ka[g], 1), unpack2(kb[g], 1), qf[g][0], qf[g][1]);
+      mma_bf16(acc, unpack2(ka[g], 2), unpack2(kb[g], 2), unpack2(ka[g], 3), unpack2(kb[g], 3), qf[g][2], qf[g][3]);
+      const float fa = bf16_of(sa[g >> 1], g), fb = bf16_of(sb[g >> 1], g);
+      s[0] = fmaf(acc[0], fa, s[0]);
+      s[1] = fmaf(acc[1], fa, s[1]);
+      s[2] = fmaf(acc[2], fb, s[2]);
+      s[3] = fmaf(acc[3], fb, s[3]);
+    }
+    const bool edge = pos0 < first || pos0 + K4_STEP > len;
+    const bool live_a = pos0 + tok >= first && pos0 + tok < len, live_b = pos0 + tok + 2 >= first && pos0 + tok + 2 < len;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] *= c;
+    if (edge) {      // (a place that was never written, or by another sequence, may hold anything)
+      if (!live_a) s[0] = s[1] = -INFINITY;
+      if (!live_b) s[2] = s[3] = -INFINITY;
+    }
+    // The running maximum moves only when a score passes it by K4_SLACK: weights are then at most 2^8, and any reference gives the same quotient.
+    if (__any_sync(0xffffffffu, fmaxf(s[0], s[2]) > top[0] + K4_SLACK || fmaxf(s[1], s[3]) > top[1] + K4_SLACK)) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float m = fmaxf(s[h], s[h + 2]);
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+        if (m > top[h]) {
+          const float f = exp2_fast(top[h] - m);      // (0 for the first)
+          top[h] = m;
+          sum[h] *= f;
+#pragma unroll
+          for (int i = 0; i < 2 * G; ++i) {
+            o[i][h] *= f;
+            o[i][h + 2] *= f;
+          }
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            z[g][h] *= f;
+            z[g][h + 2] *= f;
+          }
+        }
+      }
+    }
+    const float ref0 = top[0] == -INFINITY ? 0.f : top[0], ref1 = top[1] == -INFINITY ? 0.f : top[1];
+    const float p0 = exp2_fast(s[0] - ref0), p1 = exp2_fast(s[1] - ref1), p2 = exp2_fast(s[2] - ref0), p3 = exp2_fast(s[3] - ref1);
+    sum[0] += p0 + p2;
+    sum[1] += p1 + p3;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      float fa = bf16_of(sa[(G + g) >> 1], G + g), fb = bf16_of(sb[(G + g) >> 1], G + g);
+      if (edge) {
+        if (!live_a) fa = 0.f;
+        if (!live_b) fb = 0.f;
+      }
+      // weight * scale in 32 bits, rounded once to the operand's bf16: half a step, 2^-9, of each token's share, with either sign
+      const uint32_t w0 = transposed8x8(pack_bf16x2(p0 * fa, p1 * fa)), w1 = transposed8x8(pack_bf16x2(p2 * fb, p3 * fb));
+      mma_bf16(o[2 * g], unpack2(va[g], 0), unpack2(va[g], 1), unpack2(vb[g], 0), unpack2(vb[g], 1), w0, w1);
+      mma_bf16(o[2 * g + 1], unpack2(va[g], 2), unpack2(va[g], 3), unpack2(vb[g], 2), unpack2(vb[g], 3), w0, w1);
+      mma_bf16(z[g], 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, w0, w1);
+    }
+  }
+
+  // the warps' parts: heads 2 t and 2 t + 1, dimensions 32 g + 4 r .. + 3
+  float* red_ml = k4_red + K4_WARPS * 8 * D;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float l = sum[h];
+    l += __shfl_xor_sync(0xffffffffu, l, 4);
+    l += __shfl_xor_sync(0xffffffffu, l, 8);
+    l += __shfl_xor_sync(0xffffffffu, l, 16);
+    const int head = 2 * t + h;
+    if (r == 0) {
+      red_ml[(warp * 8 + head) * 2] = top[h];
+      red_ml[(warp * 8 + head) * 2 + 1] = l;
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+      *reinterpret_cast<float4*>(k4_red + (warp * 8 + head) * D + 32 * g + 4 * r) =
+          make_float4(o[2 * g][h] - K4_BIAS * z[g][h], o[2 * g][h + 2] - K4_BIAS * z[g][h], o[2 * g + 1][h] - K4_BIAS * z[g][h], o[2 * g + 1][h + 2] - K4_BIAS * z[g][h]);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < heads * D; i += blockDim.x) {
+    const int head = i / D, d = i - head * D;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < K4_WARPS; ++w) m = fmaxf(m, red_ml[(w * 8 + head) * 2]);
+    float l = 0.f, acc = 0.f;
+#pragma unroll
+    for (int w = 0; w < K4_WARPS; ++w) {
+      const float mw = red_ml[(w * 8 + head) * 2], f = mw == -INFINITY ? 0.f : exp2_fast(mw - m);
+      const float lw = red_ml[(w * 8 + head) * 2 + 1], ow = k4_red[(w * 8 + head) * D + d];
+      l += mw == -INFINITY ? lw : lw * f;      // (a part without a finite score: no tokens, or NaN)
+      acc += mw == -INFINITY ? ow : ow * f;
+    }
+    if (p.num_splits == 1) {
+      p.out[static_cast<long long>(b) * p.out_stride + static_cast<long long>(head0 + head) * D + d] = __float2bfloat16_rn(l == 0.f ? 0.f : acc / l);
+    } else {
+      const long long at = (static_cast<long long>(b) * p.Hkv * p.G + head0 + head) * p.num_splits + split;
+      p.part_o[at * D + d] = acc;
+      if (d == 0) {
+        p.part_ml[at * 2] = m;
+        p.part_ml[at * 2 + 1] = l;
+      }
+    }
+  }
+}
+
+// Joins the splits: one CTA per (sequence, query head), a thread per dimension.
+template <int D>
+__global__ void __launch_bounds__(D) kv4_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, __nv_bfloat16* __restrict__ out, long long out_stride, int Hq,
+                                                     int num_splits) {
+  pdl_sync();
+  const long long at = (static_cast<long long>(blockIdx.y) * Hq + blockIdx.x) * num_splits;
+  float m = -INFINITY;
+  for (int i = 0; i < num_splits; ++i) m = fmaxf(m, part_ml[(at + i) * 2]);
+  float l = 0.f, acc = 0.f;
+  for (int i = 0; i < num_splits; ++i) {
+    const float mi = part_ml[(at + i) * 2], f = mi == -INFINITY ? 1.f : exp2_fast(mi - m);
+    l += part_ml[(at + i) * 2 + 1] * f;
+    acc += part_o[(at + i) * D + threadIdx.x] * f;
+  }
+  out[blockIdx.y * out_stride + static_cast<long long>(blockIdx.x) * D + threadIdx.x] = __float2bfloat16_rn(l == 0.f ? 0.f : acc / l);
+}
+
+template <int D>
+int launch_decode(const K4Params& p, int B, cudaStream_t stream) {
+  static std::atomic<unsigned long long> ready{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (!(ready.load() >> (dev & 63) & 1)) {
+    e = cudaFuncSetAttribute(kv4_decode_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, k4_smem<D>());
+    if (e != cudaSuccess) return static_cast<int>(e);
+    ready.fetch_or(1ull << (dev & 63));
+  }
+  rlb_launch_pdl(kv4_decode_kernel<D>, dim3(p.num_splits, p.Hkv * p.chunks, B), dim3(K4_WARPS * 32), k4_smem<D>(), stream, p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || p.num_splits == 1) return static_cast<int>(e);
+  rlb_launch_pdl(kv4_join_kernel<D>, dim3(p.Hkv * p.G, B), dim3(D), 0, stream, p.part_o, p.part_ml, p.out, p.out_stride, p.Hkv * p.G, p.num_splits);
+  return static_cast<int>(cudaGetLastError());
+}
+}  // namespace
+
+// q [B, >= Hq D] bf16, 16-byte aligned rows; block_table [B, max_blocks] int32; seq_lens [B]; part_o [B Hq splits D] and part_ml [B Hq splits 2] fp32 with more than one split.
+RLB_API int rlb_kv4_paged_decode(const void* q, long long q_stride, const void* cache, long long num_blocks, const int* block_table, long long table_stride, int max_blocks,
+                                 const int* seq_lens, int B, int Hq, int Hkv, int D, int block_size, int window, float scale, int num_splits, float* part_o, float* part_ml, void* out,
+                                 long long out_stride, int* status, void* stream) {
+  if ((D != 64 && D != 128 && D != 256) || Hkv < 1 || Hq < 1 || Hq % Hkv || block_size < 16 || block_size % 16 || block_size > KV4_MAX_BLOCK || window < 0) return -2;
+  if (q_stride % 8 || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache)) & 15)) return -2;
+  if (B <= 0) return 0;
+  if (num_splits < 1 || (num_splits > 1 && (!part_o || !part_ml))) return -3;
+  const int group = Hq / Hkv, chunks = (group + 7) / 8;
+  if (B > 65535 || Hkv * chunks > 65535 || (num_splits > 1 && B > 65535)) return -4;
+  const K4Params p{static_cast<const __nv_bfloat16*>(q), q_stride, static_cast<const uint8_t*>(cache), num_blocks, block_table, table_stride, max_blocks, seq_lens, Hkv, group, chunks,
+                   block_size, window, scale, num_splits, part_o, part_ml, static_cast<__nv_bfloat16*>(out), out_stride, status};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return D == 64 ? launch_decode<64>(p, B, s) : D == 128 ? launch_decode<128>(p, B, s) : launch_decode<256>(p, B, s);
+}

@@ -1,0 +1,335 @@
+"""Kernels of the 4-bit key/value cache. The write and the read-back give the bytes and values of the definition exactly; decode attention is held to
+soft-max attention in 64 bits over the values that stand in the cache."""
+
+import math
+
+import pytest
+import torch
+
+from rl_b200.ops import kv4_ops as K
+from rl_b200.ops import lib as L
+
+pytestmark = pytest.mark.gpu
+
+HEADS = {64: [(14, 2), (16, 1), (8, 8)], 128: [(8, 2), (12, 2), (7, 1), (5, 5), (32, 2)], 256: [(8, 4), (10, 1)]}
+
+
+def _freq(D, base=500000.0):
+    return base ** (-torch.arange(0, D, 2).float() / D)
+
+
+def _rows(T, Hq, Hkv, D, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(T, (Hq + 2 * Hkv) * D, generator=g) * (1 + 3 * (torch.arange((Hq + 2 * Hkv) * D) % 29 == 3))).bfloat16()
+
+
+def _write_both(rows, pos, freq, slots, cache, Hq, Hkv, D):
+    """On the CPU and on the GPU: (rows, cache) of each."""
+    ref = cache.clone()
+    want = K.rope_kv4_cache_write(rows, pos, freq, slots, ref, Hq, Hkv, D)
+    dev, mine = rows.cuda(), cache.cuda()
+    got = K.rope_kv4_cache_write(dev, pos.cuda(), freq.cuda(), slots.cuda(), mine, Hq, Hkv, D)
+    assert got is dev
+    torch.cuda.synchronize()
+    return want, ref, got.cpu(), mine.cpu()
+
+
+@pytest.mark.parametrize("T", [1, 2, 3, 67, 500, 2400])
+@pytest.mark.parametrize("D,Hq,Hkv,block", [(64, 14, 2, 16), (64, 16, 1, 48), (128, 8, 2, 64), (128, 5, 5, 128), (256, 8, 1, 16)])
+def test_write_is_exact(native_lib, T, D, Hq, Hkv, block):
+    """Every rounding is the definition's: equal bytes."""
+    pages = T // block + 3
+    g = torch.Generator().manual_seed(T)
+    pos = torch.randint(0, 200_000, (T,), generator=g)
+    pos[0] = 2**31 - 1 if T == 2 else 0
+    slots = torch.randperm(pages * block, generator=g)[:T]
+    slots[T // 2 :: 9] = -1
+    cache = torch.randint(0, 255, (pages, Hkv, K.kv4_page_bytes(block, D)), generator=g, dtype=torch.uint8)      # what is not written stays
+    want, ref, got, mine = _write_both(_rows(T, Hq, Hkv, D, T), pos, _freq(D), slots, cache, Hq, Hkv, D)
+    assert torch.equal(got, want) and torch.equal(mine, ref) and L.check_status() == 0
+    back = K.kv4_cache_read(mine.cuda(), slots.cuda(), Hkv, D)
+    assert torch.equal(back.cpu(), K.kv4_cache_read(ref, slots, Hkv, D))
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_write_of_special_values(native_lib, D):
+    T, Hq, Hkv, block = 12, 1, 1, 16
+    x = torch.zeros(T, 3 * D)
+    x[1] = -0.0
+    x[2, D + 5], x[3, 2 * D + 40], x[4, 2 * D] = math.inf, math.nan, -math.inf
+    x[5] = 2.0 ** -101
+    x[6] = 2.0 ** -100
+    x[7] = torch.finfo(torch.bfloat16).max * torch.linspace(-1, 1, 3 * D)
+    x[8] = ((torch.arange(3 * D) % 32) - 16) * 0.125        # multiples of the scale: borders of codes
+    x[9] = (15 - (torch.arange(3 * D) % 32)) * 0.125
+    x[10] = 1e-39
+    x[11] = ((torch.arange(3 * D) * 37 % 256) - 128) * 2.0 ** -80
+    pos = torch.zeros(T, dtype=torch.int64)                  # no rotation: the values are what is held
+    want, ref, got, mine = _write_both(x.bfloat16(), pos, _freq(D), torch.arange(T), K.kv4_cache(1, Hkv, block, D, "cpu"), Hq, Hkv, D)
+    assert torch.equal(mine, ref)
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
+    kv, kr = K.kv4_cache_read(mine.cuda(), torch.arange(T).cuda(), Hkv, D).cpu(), K.kv4_cache_read(ref, torch.arange(T), Hkv, D)
+    assert torch.equal(kv.isnan(), kr.isnan()) and torch.equal(kv.nan_to_num(), kr.nan_to_num())
+
+
+def test_write_and_read_of_odd_views(native_lib):
+    """Rows that do not start on 16 bytes, wider buffers, 32-bit indices, an inner stride, rows of the output by number."""
+    T, Hq, Hkv, D, block = 37, 4, 2, 64, 16
+    rows, pos, freq, slots = _rows(T, Hq, Hkv, D), torch.arange(T), _freq(D), torch.randperm(64)[:T]
+    ref = K.kv4_cache(4, Hkv, block, D, "cpu")
+    want = K.rope_kv4_cache_write(rows, pos, freq, slots, ref, Hq, Hkv, D)
+    W = rows.shape[1]
+    wide = torch.zeros(T, W + 24, dtype=torch.bfloat16, device="cuda")
+    for view in (wide[:, 8 : 8 + W], wide[:, 3 : 3 + W], torch.zeros(W, T, dtype=torch.bfloat16, device="cuda").t()):
+        wide.fill_(5.0)
+        view.copy_(rows)
+        cache = K.kv4_cache(4, Hkv, block, D, "cuda")
+        assert K.rope_kv4_cache_write(view, pos.int().cuda(), freq.cuda(), slots.int().cuda(), cache, Hq, Hkv, D) is view
+        assert torch.equal(view.cpu(), want) and torch.equal(cache.cpu(), ref)
+    assert (wide[:, -4:] == 5).all()
+    kv = K.kv4_cache_read(ref, slots, Hkv, D)
+    to = torch.randperm(T)
+    for off, extra in ((0, 0), (8, 16), (1, 7)):
+        out = torch.full((T + 2, off + kv.shape[1] + extra), 3.0, dtype=torch.bfloat16, device="cuda")
+        got = K.kv4_cache_read(cache, slots.cuda(), Hkv, D, out=out[:, off:], rows=to.cuda())
+        assert got.data_ptr() == out[:, off:].data_ptr() and torch.equal(got[to.cuda(), : kv.shape[1]].cpu(), kv)
+        assert (out[T:] == 3).all() and (out[:, :off] == 3).all() and (out[:, off + kv.shape[1] :] == 3).all()
+    assert L.check_status() == 0
+
+
+def test_bad_slots_are_reported_and_skipped(native_lib):
+    T, Hq, Hkv, D, block = 3, 2, 1, 128, 16
+    rows, slots = _rows(T, Hq, Hkv, D), torch.tensor([32, 5, 10**12])
+    cache, ref = K.kv4_cache(2, Hkv, block, D, "cuda"), K.kv4_cache(2, Hkv, block, D, "cpu")
+    K.rope_kv4_cache_write(rows.cuda(), torch.arange(T).cuda(), _freq(D).cuda(), slots.cuda(), cache, Hq, Hkv, D)
+    assert L.check_status() == 6
+    K.rope_kv4_cache_write(rows, torch.arange(T), _freq(D), torch.tensor([-1, 5, -1]), ref, Hq, Hkv, D)
+    assert torch.equal(cache.cpu(), ref)
+    out = torch.full((2, 256), 9.0, dtype=torch.bfloat16, device="cuda")
+    K.kv4_cache_read(cache, torch.tensor([32, 5], device="cuda"), Hkv, D, out=out)
+    assert L.check_status() == 6 and (out[0] == 9).all() and torch.equal(out[1:].cpu(), K.kv4_cache_read(ref, torch.tensor([5]), Hkv, D))
+    K.kv4_cache_read(cache, torch.tensor([5], device="cuda"), Hkv, D, out=out, rows=torch.tensor([2], device="cuda"))
+    assert L.check_status() == 6
+    assert not K.kv4_cache_read(cache, torch.tensor([-1], device="cuda"), Hkv, D).any() and L.check_status() == 0
+
+
+# ------------------------------------------------------------------------------------------- decode
+def _pool(pages, Hkv, D, block, seed, big=1.0):
+    """A cache of normal values, and a garbage value in every byte that no token owns is made by the tests themselves."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(2, pages, Hkv, block, D, generator=g, device="cuda") * big
+    x[..., 3::29] *= 4
+    (kc, ks), (vc, vs) = (K.quantize_ref(t.bfloat16()) for t in x)
+    return K._pack_pages(kc, vc, ks, vs)
+
+
+def _check(got, q, cache, table, lens, Hq, Hkv, D, window=0, scale=None):
+    """Every output within what the roundings give: the result's to bf16 (2^-8 of it), each token's weight times its scale to bf16 (2^-8 of
+    the token's share), and the scores in 32 bits. A score's sum over a group starts at 135.5 times the sum of the query's values and has 33 terms of at most 143 |q|:
+    an error of 33 roundings at that size, times the key's scale; a score's error e changes a weight by e and the sum by as much."""
+    block, B = cache.shape[2] * 8 // (9 * D), q.shape[0]
+    scale = scale or 1 / math.sqrt(D)
+    for b in range(B):
+        n = int(lens[b])
+        lo = max(0, n - window) if window else 0
+        if n == 0:
+            assert not got[b].any()
+            continue
+        kc, vc, ks, vs = K._unpack_pages(cache[table[b, : -(-n // block)].long()].transpose(0, 1), D)
+        k, v = (((c.double() - 7.5) * s.double().unsqueeze(-1)).flatten(-2).flatten(1, 2)[:, lo:n] for c, s in ((kc, ks), (vc, vs)))
+        qb = q[b, : Hq * D].double().reshape(Hkv, Hq // Hkv, D)
+        p = torch.softmax(qb @ k.transpose(1, 2) * scale, -1)
+        want, share = p @ v, p @ v.abs()
+        e = scale * 33 * 2.0 ** -24 * 143 * torch.einsum("hgd,hd->hg", qb.abs(), ks.double().repeat_interleave(32, -1).flatten(1, 2)[:, lo:n].amax(1)).unsqueeze(-1)
+        tol = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2 * e + 2.0 ** -18) * share
+        off = (got[b].double().reshape(want.shape) - want).abs()
+        assert (off <= tol).all(), f"row {b}: {(off / tol).max().item():.2f} times the tolerance"
+
+
+def _decode_case(lens, Hq, Hkv, D, block, seed=0, spare=2, big=1.0):
+    need = [-(-n // block) for n in lens]
+    g = torch.Generator().manual_seed(seed)
+    pages = sum(need) + spare
+    cache = _pool(pages, Hkv, D, block, seed, big)
+    order, at = torch.randperm(pages, generator=g).int(), 0
+    table = torch.full((len(lens), max(1, max(need)) + 1), 10**9, dtype=torch.int32)      # entries behind a sequence's pages are never read
+    for i, k in enumerate(need):
+        table[i, :k] = order[at : at + k]
+        at += k
+    q = _rows(len(lens), Hq, Hkv, D, seed).cuda()
+    return q, cache, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda()
+
+
+LENGTHS = [[1], [0], [2, 15, 16, 17, 0, 31, 33], [63, 64, 65, 1, 127, 128, 129], [300, 0, 1025], [4100]]
+
+
+@pytest.mark.parametrize("lens", LENGTHS, ids=lambda l: "-".join(map(str, l)))
+@pytest.mark.parametrize("D,Hq,Hkv", [(D, *h) for D in HEADS for h in HEADS[D]])
+def test_decode(native_lib, lens, D, Hq, Hkv):
+    for block in (16, 64) if D != 128 else (48, 128):
+        q, cache, table, n = _decode_case(lens, Hq, Hkv, D, block, seed=len(lens))
+        for splits in (0, 1, 3, 9):
+            got = K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, num_splits=splits)
+            assert L.check_status() == 0
+            _check(got, q, cache, table, n, Hq, Hkv, D)
+            assert torch.equal(got, K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, num_splits=splits))      # the same bits again
+
+
+@pytest.mark.parametrize("window", [1, 5, 16, 100, 5000])
+@pytest.mark.parametrize("D,Hq,Hkv", [(64, 14, 2), (128, 8, 2), (256, 8, 4)])
+def test_decode_window(native_lib, window, D, Hq, Hkv):
+    q, cache, table, n = _decode_case([1, 17, 100, 0, 1000, 333, 16], Hq, Hkv, D, 32, seed=window)
+    for splits in (0, 1, 4):
+        _check(K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, window=window, num_splits=splits), q, cache, table, n, Hq, Hkv, D, window)
+    assert L.check_status() == 0
+
+
+@pytest.mark.parametrize("big,scale", [(1e-20, 0.1), (1e-3, 30.0), (40.0, None), (1e15, 1e-17)])
+def test_decode_of_small_large_and_peaked(native_lib, big, scale):
+    """Values far from one, and scores of hundreds: one token takes nearly all."""
+    q, cache, table, n = _decode_case([700, 33, 260], 8, 2, 128, 64, seed=5, big=big)
+    for splits in (1, 3):
+        _check(K.kv4_paged_decode(q, cache, table, n, 8, 2, 128, scale=scale, num_splits=splits), q, cache, table, n, 8, 2, 128, scale=scale)
+
+
+@pytest.mark.parametrize("splits", [1, 2, 10])
+def test_decode_ignores_what_stands_behind_the_end(native_lib, splits):
+    """NaN and infinite scales, and any codes, in places that the sequence does not see: before the window and behind its last token."""
+    Hq, Hkv, D, block, lens, window = 8, 2, 128, 64, [70, 129, 1, 64, 300], 50
+    q, cache, table, n = _decode_case(lens, Hq, Hkv, D, block, seed=3)
+    dirty = cache.clone()
+    for b, m in enumerate(lens):
+        for t in list(range(m, -(-m // block) * block)) + list(range(0, max(0, m - window))):
+            page, off = dirty[int(table[b, t // block])], t % block
+            s = page[:, block * D :].view(torch.bfloat16).view(Hkv, block, 8)
+            s[:, off] = torch.tensor([math.nan, math.inf, -math.inf, 3e38] * 2, device="cuda").bfloat16()
+            page[:, : block * D // 2].view(Hkv, block, -1)[:, off] = 0xA5
+    want = K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, window=window, num_splits=splits)
+    got = K.kv4_paged_decode(q, dirty, table, n, Hq, Hkv, D, window=window, num_splits=splits)
+    assert got.isfinite().all() and torch.equal(got, want)
+
+
+def test_decode_hands_on_what_is_not_finite(native_lib):
+    """A visible key with a NaN scale makes its heads NaN, a value's its group; other heads and sequences keep their numbers."""
+    Hq, Hkv, D, block = 4, 2, 128, 16
+    q, cache, table, n = _decode_case([40, 40], Hq, Hkv, D, block, seed=9)
+    for splits in (1, 2):
+        clean = K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, num_splits=splits)
+        for value, group in ((0, 2), (1, 1)):
+            c = cache.clone()
+            c[int(table[1, 1]), 1, block * D :].view(torch.bfloat16).view(block, 2, 4)[3, value, group] = math.nan
+            got = K.kv4_paged_decode(q, c, table, n, Hq, Hkv, D, num_splits=splits).view(2, Hq, D)
+            nan = torch.zeros(2, Hq, D, dtype=torch.bool, device="cuda")
+            nan[1, 2:, slice(None) if value == 0 else slice(32, 64)] = True
+            assert torch.equal(got.isnan(), nan) and torch.equal(got[~nan], clean.view(2, Hq, D)[~nan])
+
+
+def test_decode_of_odd_views(native_lib):
+    Hq, Hkv, D, block = 4, 2, 64, 16
+    q, cache, table, n = _decode_case([50, 3, 0, 77], Hq, Hkv, D, block)
+    want = K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D)
+    _check(want, q, cache, table, n, Hq, Hkv, D)
+    odd = torch.zeros(4, Hq * D + 5, dtype=torch.bfloat16, device="cuda")[:, 3 : 3 + Hq * D]
+    odd.copy_(q[:, : Hq * D])
+    wide = torch.full((4, 2 * Hq * D), 7.0, dtype=torch.bfloat16, device="cuda")
+    for out in (wide[:, 4 : 4 + Hq * D], wide[:, 1 : 1 + Hq * D], wide[:, ::2]):
+        wide.fill_(7.0)
+        got = K.kv4_paged_decode(odd, cache, table.long().t().contiguous().t(), n.long(), Hq, Hkv, D, out=out)
+        assert got is out and torch.equal(out, want) and int((wide == 7).sum()) >= 4 * Hq * D
+    assert K.kv4_paged_decode(q[:0], cache, table[:0], n[:0], Hq, Hkv, D).shape == (0, Hq * D)
+    scratch = tuple(torch.empty(s + 3, device="cuda") for s in K.kv4_scratch_sizes(4, Hq, 2, D))
+    _check(K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, num_splits=2, scratch=scratch), q, cache, table, n, Hq, Hkv, D)
+    for bad in ((scratch[0][:-4], scratch[1]), (scratch[0].double(), scratch[1]), (scratch[0], scratch[1].cpu())):
+        with pytest.raises(ValueError):
+            K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, num_splits=2, scratch=bad)
+    for bad in (q.float(), q.half(), q.cpu()):
+        with pytest.raises(ValueError):
+            K.kv4_paged_decode(bad, cache, table, n, Hq, Hkv, D)
+    with pytest.raises(ValueError):
+        K.rope_kv4_cache_write(q.float(), n, _freq(D).cuda(), n, cache, Hq, Hkv, D)
+    with pytest.raises(ValueError):
+        K.kv4_cache_read(cache, n, Hkv, D, out=torch.zeros(4, 2 * Hkv * D, device="cuda"))
+
+
+def test_bad_pages_and_lengths_are_reported(native_lib):
+    """Page numbers outside the cache are left out, lengths beyond the table end there: an error is on record and nothing else is read."""
+    Hq, Hkv, D, block = 8, 2, 128, 16
+    q, cache, table, n = _decode_case([64, 64], Hq, Hkv, D, block)
+    for splits in (1, 2):
+        want = K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, num_splits=splits)
+        for page in (-1, cache.shape[0], 2**31 - 1):
+            bad = table.clone()
+            bad[1, 2] = page
+            got = K.kv4_paged_decode(q, cache, bad, n, Hq, Hkv, D, num_splits=splits)
+            assert L.check_status() == 6 and torch.equal(got[0], want[0]) and got.isfinite().all()
+        got = K.kv4_paged_decode(q, cache, table[:, :4], torch.tensor([64, 2**31 - 1], dtype=torch.int32, device="cuda"), Hq, Hkv, D, num_splits=splits)
+        assert L.check_status() == 6 and torch.equal(got, want)
+        got = K.kv4_paged_decode(q, cache, table, torch.tensor([64, -5], dtype=torch.int32, device="cuda"), Hq, Hkv, D, num_splits=splits)
+        assert L.check_status() == 0 and torch.equal(got[0], want[0]) and not got[1].any()
+
+
+def test_places_beyond_32_bits(native_lib):
+    """A cache of more than 4 GiB: pages at its far end."""
+    Hq, Hkv, D, block = 8, 8, 128, 128
+    size = K.kv4_page_bytes(block, D) * Hkv
+    pages = 2**32 // size + 40
+    if torch.cuda.mem_get_info()[0] < 2 * pages * size:
+        pytest.skip("no room")
+    cache = K.kv4_cache(pages, Hkv, block, D, "cuda")
+    small = K.kv4_cache(4, Hkv, block, D, "cuda")
+    T = 300
+    rows, pos, freq = _rows(T, Hq, Hkv, D), torch.arange(T).cuda(), _freq(D).cuda()
+    at = torch.arange(T).cuda()
+    far = torch.tensor([pages - 1, pages - 7, pages - 3], device="cuda")
+    for c, page in ((cache, far), (small, torch.tensor([3, 0, 1], device="cuda"))):
+        K.rope_kv4_cache_write(rows.cuda(), pos, freq, page[at // block] * block + at % block, c, Hq, Hkv, D)
+    n = torch.tensor([T], dtype=torch.int32, device="cuda")
+    for i, j in zip(far.tolist(), (3, 0, 1)):
+        assert torch.equal(cache[i], small[j])
+    got = K.kv4_paged_decode(rows[:1].cuda(), cache, far[None].int(), n, Hq, Hkv, D)
+    assert torch.equal(got, K.kv4_paged_decode(rows[:1].cuda(), small, torch.tensor([[3, 0, 1]], device="cuda").int(), n, Hq, Hkv, D))
+    s = far[at // block] * block + at % block
+    assert torch.equal(K.kv4_cache_read(cache, s, Hkv, D), K.kv4_cache_read(small, torch.tensor([3, 0, 1], device="cuda")[at // block] * block + at % block, Hkv, D))
+    assert L.check_status() == 0
+
+
+def test_graphs_and_streams(native_lib):
+    """A decode step (write, then attention) captured twice, replayed in turn on changing inputs, next to eager calls on another stream."""
+    Hq, Hkv, D, block, B = 8, 2, 128, 16, 5
+    q, cache, table, n = _decode_case([30, 200, 1, 64, 17], Hq, Hkv, D, block, spare=8)
+    table = table.clamp(max=cache.shape[0] - 1)
+    freq = _freq(D).cuda()
+    state = dict(rows=q.clone(), pos=n.long() - 1, lens=n.clone())
+
+    def step(c, splits):
+        slots = table[torch.arange(B, device="cuda"), state["pos"] // block].long() * block + state["pos"] % block
+        rows = K.rope_kv4_cache_write(state["rows"].clone(), state["pos"], freq, slots, c, Hq, Hkv, D)
+        return K.kv4_paged_decode(rows, c, table, state["lens"], Hq, Hkv, D, num_splits=splits)
+
+    caches = [cache.clone(), cache.clone()]
+    graphs, outs = [], []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for s in (1, 4):
+            step(cache.clone(), s)
+    torch.cuda.current_stream().wait_stream(side)
+    for c, s in zip(caches, (1, 4)):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(c, s))
+        graphs.append(g)
+    for c in caches:
+        c.copy_(cache)
+    eager = cache.clone()
+    for i in range(3):
+        state["rows"].copy_(_rows(B, Hq, Hkv, D, 50 + i))
+        torch.cuda.synchronize()
+        for g in graphs:
+            g.replay()
+        with torch.cuda.stream(side):
+            want = step(eager, 1)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want) and torch.equal(caches[0], eager) and torch.equal(caches[1], eager)
+        _check(outs[1], K.rope_kv4_cache_write(state["rows"].clone(), state["pos"], freq, torch.full((B,), -1, device="cuda"), eager, Hq, Hkv, D), eager, table, n, Hq, Hkv, D)
+    assert L.check_status() == 0

@@ -1,0 +1,173 @@
+"""The 4-bit key/value cache on the CPU: what a page holds, against loops over the definition in 64 bits, and what the operators refuse."""
+
+import math
+
+import pytest
+import torch
+
+from rl_b200.ops import kv4_ops as K
+
+SHAPES = [(64, 2, 16), (128, 3, 48), (256, 1, 64)]      # D, Hkv, tokens of a page
+
+
+def _group(x):
+    """(scale, codes) of 32 Python floats."""
+    a = max(abs(v) for v in x)
+    if not all(map(math.isfinite, x)):
+        return math.nan, [8] * 32
+    if a < 2.0 ** -100:
+        return 0.0, [8] * 32
+    s = float(torch.tensor(a / 7.5, dtype=torch.float64).to(torch.bfloat16))
+    return s, [min(15, max(0, math.floor(v / s) + 8)) for v in x]
+
+
+def _place(page, D, block, off, value, d):
+    """(code, scale) of one number in a page's bytes, by the order that csrc/kv4.cuh states."""
+    G, n, (g, i) = D // 32, block * D // 2, divmod(d, 32)
+    if value:
+        unit = n + (off // 2) * D + ((i // 4) * G + g) * 4 + (off % 2) * 2
+    else:
+        unit = off * (D // 2) + ((i // 8) * G + g) * 4 + (i // 4 % 2) * 2
+    word = int(page[unit]) | int(page[unit + 1]) << 8
+    at = 2 * n + (off * 2 + value) * 2 * G + 2 * g
+    return word >> (4 * (i % 4)) & 15, float(page[at : at + 2].clone().view(torch.bfloat16))
+
+
+def _rows(T, Hq, Hkv, D, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(T, (Hq + 2 * Hkv) * D, generator=g) * (1 + 3 * (torch.arange((Hq + 2 * Hkv) * D) % 29 == 3))).bfloat16()
+
+
+def _freq(D):
+    return 10000.0 ** (-torch.arange(0, D, 2).float() / D)
+
+
+@pytest.mark.parametrize("D,Hkv,block", SHAPES)
+def test_page_order_and_codes(D, Hkv, block):
+    T, Hq = 5, Hkv
+    cache = K.kv4_cache(3, Hkv, block, D, "cpu")
+    assert cache.shape == (3, Hkv, block * D * 9 // 8)
+    slots = torch.tensor([2 * block + 7, 3, -1, block + block - 1, 0])
+    out = K.rope_kv4_cache_write(_rows(T, Hq, Hkv, D), torch.arange(T), _freq(D), slots, cache, Hq, Hkv, D)
+    back = K.kv4_cache_read(cache, slots, Hkv, D)
+    for t, slot in enumerate(slots.tolist()):
+        for value in (0, 1):
+            for h in range(Hkv):
+                at = (Hq + value * Hkv + h) * D
+                for g in range(D // 32):
+                    x = [float(v) for v in out[t, at + 32 * g : at + 32 * g + 32]]
+                    s, codes = _group(x)
+                    for i in range(32):
+                        if slot < 0:
+                            assert float(back[t, (value * Hkv + h) * D + 32 * g + i]) == 0.0
+                            continue
+                        assert _place(cache[slot // block, h], D, block, slot % block, value, 32 * g + i) == (codes[i], s)
+                        want = torch.tensor((codes[i] - 7.5) * s, dtype=torch.float64).to(torch.bfloat16)
+                        assert back[t, (value * Hkv + h) * D + 32 * g + i] == want
+                        assert abs(float(want) - x[i]) <= s * (0.5 + 2.0 ** -4)      # half a level, and 7.5 levels' worth of the scale's rounding 2^-8 and the result's
+    assert not cache[0, :, : block * D // 2].view(Hkv, block, -1)[:, [1, 2, 4, 5]].any()
+
+
+def test_rotation_is_that_of_the_formula():
+    T, Hq, Hkv, D = 7, 2, 1, 64
+    pos = torch.tensor([0, 1, 1000, 131071, 20_000_003, 2**31 - 1, 77])
+    x = _rows(T, Hq, Hkv, D)
+    out = K.rope_kv4_cache_write(x, pos, _freq(D), torch.full((T,), -1), K.kv4_cache(1, Hkv, 16, D, "cpu"), Hq, Hkv, D)
+    z = torch.polar(torch.ones((), dtype=torch.float64), pos.double()[:, None] * _freq(D).double())[:, None]
+    v = x.double().reshape(T, Hq + 2 * Hkv, D)[:, : Hq + Hkv]
+    want = torch.complex(v[..., : D // 2], v[..., D // 2 :]) * z
+    want = torch.cat([want.real, want.imag], -1).reshape(T, -1)
+    got = out[:, : (Hq + Hkv) * D].double()
+    # one rounding to bf16, and the cosine, sine, products and sum in 32 bits (4 roundings of at most 2 max|x|)
+    assert ((got - want).abs() <= want.abs() * 2.0 ** -8 + 4 * 2.0 ** -24 * 2 * v.abs().max()).all()
+    assert torch.equal(out[:, (Hq + Hkv) * D :], x[:, (Hq + Hkv) * D :])
+
+
+def test_special_values():
+    D = 64
+    x = torch.zeros(8, 64)
+    x[1] = -0.0
+    x[2, 5], x[3, 40], x[4, 0] = math.inf, math.nan, -math.inf
+    x[5] = 2.0 ** -101
+    x[6] = torch.finfo(torch.bfloat16).max * torch.linspace(-1, 1, 64)
+    x[7] = torch.cat([torch.arange(-16, 16), torch.arange(-15, 17)]) * 0.125      # multiples of the scale: the upper code
+    x = x.bfloat16()
+    codes, s = K.quantize_ref(x)
+    for i in range(8):
+        for g in range(2):
+            ws, wc = _group([float(v) for v in x[i, 32 * g : 32 * g + 32]])
+            assert (math.isnan(ws) and bool(s[i, g].isnan())) or float(s[i, g]) == ws
+            assert codes[i, g].tolist() == wc
+    kv = K._values(codes, s)
+    assert not kv[0].any() and not kv[1].any() and not kv[5].any() and kv[6].isfinite().all()
+    assert kv[2, :32].isnan().all() and not kv[2, 32:].any() and kv[3, 32:].isnan().all() and kv[4, :32].isnan().all()
+
+
+@pytest.mark.parametrize("D,Hkv,block", SHAPES)
+@pytest.mark.parametrize("window", [0, 1, 9, 40])
+def test_decode_and_write_together(D, Hkv, block, window):
+    """Tokens written one step at a time and attended to, as a decode loop does, against soft-max attention over the values that stand in the cache."""
+    Hq, n = 3 * Hkv, 2 * block + 3
+    cache = K.kv4_cache(5, Hkv, block, D, "cpu")
+    table = torch.tensor([[4, 0, 3, 1]], dtype=torch.int32)
+    kv = []
+    for t in range(n):
+        slot = int(table[0, t // block]) * block + t % block
+        row = K.rope_kv4_cache_write(_rows(1, Hq, Hkv, D, seed=t).float(), torch.tensor([t]), _freq(D), torch.tensor([slot]), cache, Hq, Hkv, D)
+        codes, s = K.quantize_ref(row[:, Hq * D :].reshape(2, Hkv, D))
+        kv.append(K._values(codes, s).double())
+        if t % 7 and t != n - 1:
+            continue
+        k, v = torch.stack(kv, 2)[:, :, max(0, t + 1 - window) if window else 0 :]
+        q = row[0, : Hq * D].double().reshape(Hkv, 3, D)
+        want = (torch.softmax(q @ k.transpose(1, 2) / math.sqrt(D), -1) @ v).reshape(-1)
+        got = K.kv4_paged_decode(row, cache, table, torch.tensor([t + 1], dtype=torch.int32), Hq, Hkv, D, window=window)[0].double()
+        # all in 32 bits: sums over D and over n, both below 2^9 terms
+        assert (got - want).abs().max() <= 2.0 ** -24 * 2 ** 9 * 8 * v.abs().max()
+    assert not K.kv4_paged_decode(row, cache, table, torch.tensor([0]), Hq, Hkv, D).any()
+
+
+def test_refusals():
+    cache = K.kv4_cache(2, 2, 16, 64, "cpu")
+    x, f, one = _rows(1, 4, 2, 64), _freq(64), torch.zeros(1, dtype=torch.int64)
+    bt, ln = torch.zeros((1, 2), dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    bad = [
+        lambda: K.kv4_page_bytes(16, 96),
+        lambda: K.kv4_page_bytes(24, 64),
+        lambda: K.kv4_page_bytes(0, 64),
+        lambda: K.kv4_page_bytes(2 * K.MAX_BLOCK, 64),
+        lambda: K.rope_kv4_cache_write(x, one, f, one, cache, 4, 2, 80),
+        lambda: K.rope_kv4_cache_write(x, one, f, one, cache, 3, 2, 64),
+        lambda: K.rope_kv4_cache_write(x, one, f.double(), one, cache, 4, 2, 64),
+        lambda: K.rope_kv4_cache_write(x, one, f[:-1], one, cache, 4, 2, 64),
+        lambda: K.rope_kv4_cache_write(x, one.float(), f, one, cache, 4, 2, 64),
+        lambda: K.rope_kv4_cache_write(x, one, f, torch.zeros(2, dtype=torch.int64), cache, 4, 2, 64),
+        lambda: K.rope_kv4_cache_write(x, one, f, one, cache.float(), 4, 2, 64),
+        lambda: K.rope_kv4_cache_write(x, one, f, one, cache[:, :, :-8], 4, 2, 64),
+        lambda: K.rope_kv4_cache_write(x, one, f, one, K.kv4_cache(2, 3, 16, 64, "cpu"), 4, 2, 64),
+        lambda: K.kv4_cache_read(cache, one, 2, 128),
+        lambda: K.kv4_cache_read(cache, one, 2, 64, rows=one),
+        lambda: K.kv4_cache_read(cache, one, 2, 64, out=torch.zeros(1, 255)),
+        lambda: K.kv4_cache_read(cache, one, 2, 64, out=torch.zeros(0, 256)),
+        lambda: K.kv4_cache_read(cache, one, 2, 64, out=torch.zeros(3, 256), rows=torch.zeros(2, dtype=torch.int64)),
+        lambda: K.kv4_paged_decode(x, cache, bt, ln, 3, 2, 64),
+        lambda: K.kv4_paged_decode(x, cache, bt, ln, 16, 2, 64),
+        lambda: K.kv4_paged_decode(x, cache, bt[0], ln, 4, 2, 64),
+        lambda: K.kv4_paged_decode(x, cache, bt, ln[:0], 4, 2, 64),
+        lambda: K.kv4_paged_decode(x, cache, bt.float(), ln, 4, 2, 64),
+        lambda: K.kv4_paged_decode(x, cache, bt, ln, 4, 2, 64, window=-1),
+        lambda: K.kv4_paged_decode(x, cache, bt, ln, 4, 2, 64, out=torch.zeros(1, 256)),
+        lambda: K.kv4_paged_decode(x, cache, bt, ln, 4, 2, 64, out=torch.zeros(2, 256).bfloat16()),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} went through")
+    assert not cache.any()
+
+
+def test_splits():
+    assert K.kv4_splits(1, 32, 8, 100) == 1 and K.kv4_splits(0, 32, 8, 100) == 1
+    for B, Hq, Hkv, n in ((1, 32, 8, 131072), (1, 8, 1, 10**6), (64, 32, 8, 4096), (512, 32, 8, 8192)):
+        s = K.kv4_splits(B, Hq, Hkv, n)
+        assert 1 <= s <= 128 and (s == 1 or n // s >= 256)
