@@ -23,6 +23,8 @@ using namespace rlb;
 
 constexpr int K4_WARPS = 4;
 constexpr int K4_STEP = 16;      // tokens a warp takes at a time
+constexpr int K4_STAGES = 4;     // steps whose words are in a warp's shared memory or on their way
+constexpr int K4_FOLD = 8;       // steps between two corrections of the sums
 constexpr float K4_SLACK = 8.f;  // how far (in powers of two) a score may pass the running maximum before the sums are rescaled: weights stay below 2^8
 
 struct K4Params {
@@ -63,28 +65,59 @@ __device__ __forceinline__ float exp2_fast(float x) {
 __device__ __forceinline__ uint32_t unpack2(uint32_t w, int j) { return ((w >> (4 * j)) & 0x000f000fu) | 0x43004300u; }
 constexpr float K4_BIAS = 135.5f;      // 128 + 7.5
 
+// N words of shared memory at once; and from global to shared memory, in the background.
 template <int N>
-__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
+__device__ __forceinline__ void load_words(uint32_t from, uint32_t (&w)[N]) {
   if constexpr (N == 2) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    w[0] = v.x; w[1] = v.y;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(from));
   } else {
 #pragma unroll
-    for (int i = 0; i < N / 4; ++i) {
-      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
-      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-    }
+    for (int i = 0; i < N; i += 4)
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]) : "r"(from + 4 * i));
+  }
+}
+template <int N>
+__device__ __forceinline__ void copy_words(uint32_t to, const uint8_t* from) {
+  if constexpr (N == 2) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 4 * i), "l"(from + 4 * i) : "memory");
   }
 }
 __device__ __forceinline__ float bf16_of(uint32_t word, int i) { return __uint_as_float(i & 1 ? word & 0xffff0000u : word << 16); }
 
-// Shared memory after the token loop: [warps][8 heads][D] sums, then [warps][8][2] maximum and sum of the weights.
+// A warp's stage: the words that each lane is going to use (its own copies, so that no other lane has to be waited for), and the scales of the 16 tokens.
 template <int D>
-constexpr int k4_smem() { return K4_WARPS * 8 * (D + 2) * static_cast<int>(sizeof(float)); }
+struct K4Stage {
+  static constexpr int PART = 32 * (D / 32) * 4;      // one word per lane and group
+  static constexpr int KA = 0, KB = PART, VA = 2 * PART, VB = 3 * PART, SCALES = 4 * PART, BYTES = 4 * PART + 2 * D;
+};
+// Shared memory: the warps' stages; after the token loop [warps][8 heads][D] sums, then [warps][8][2] maximum and sum of the weights.
+template <int D>
+constexpr int k4_smem() {
+  constexpr int fifo = K4_WARPS * K4_STAGES * K4Stage<D>::BYTES, red = K4_WARPS * 8 * (D + 2) * 4;
+  return fifo > red ? fifo : red;
+}
+
+// Takes the codes' offset off the sums.
+template <int G>
+__device__ __forceinline__ void fold(float (&o)[2 * G][4], float (&z)[G][4]) {
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      o[2 * g][j] = fmaf(-K4_BIAS, z[g][j & 1], o[2 * g][j]);
+      o[2 * g + 1][j] = fmaf(-K4_BIAS, z[g][j & 1], o[2 * g + 1][j]);
+    }
+    z[g][0] = z[g][1] = z[g][2] = z[g][3] = 0.f;
+  }
+}
 
 template <int D>
-__global__ void __launch_bounds__(K4_WARPS * 32) kv4_decode_kernel(const K4Params p) {
-  extern __shared__ __align__(16) float k4_red[];
+__global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 4 : 2) kv4_decode_kernel(const K4Params p) {
+  extern __shared__ __align__(128) uint8_t k4_smem_raw[];
+  using Stage = K4Stage<D>;
   using Page = Kv4Page<D>;
   constexpr int G = Page::G;      // groups of 32 dimensions
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
@@ -93,7 +126,7 @@ __global__ void __launch_bounds__(K4_WARPS * 32) kv4_decode_kernel(const K4Param
   pdl_sync();
 
   int len = p.seq_lens[b];
-  const long long room = static_cast<long long>(p.max_blocks) * p.block_size;
+  const long long room = p.num_blocks ? static_cast<long long>(p.max_blocks) * p.block_size : 0;
   if (len > room) {      // more tokens than the table has pages: recorded, the rest is left out
     if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, RLB_ERR_BAD_ARG);
     len = static_cast<int>(room);
@@ -104,6 +137,10 @@ __global__ void __launch_bounds__(K4_WARPS * 32) kv4_decode_kernel(const K4Param
   const int begin = step0 + static_cast<int>(static_cast<long long>(steps) * split / p.num_splits);
   const int end = step0 + static_cast<int>(static_cast<long long>(steps) * (split + 1) / p.num_splits);
 
+  // scores are compared before they are scaled: a negative scale turns the query's sign
+  const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
+  const float c = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-30f), slack = K4_SLACK / c;
+
   // the queries as the 8-column operand: pair j of group g is (dimension 32 g + 8 t + j, and four later) of head r
   uint32_t qf[G][4];
   float start[G][2];      // -135.5 * sum of the group's values, of heads 2 t and 2 t + 1
@@ -113,6 +150,7 @@ __global__ void __launch_bounds__(K4_WARPS * 32) kv4_decode_kernel(const K4Param
     for (int g = 0; g < G; ++g) {
       uint4 v = make_uint4(0, 0, 0, 0);
       if (r < heads) v = *reinterpret_cast<const uint4*>(q + 32 * g);
+      v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
       qf[g][0] = __byte_perm(v.x, v.z, 0x5410);
       qf[g][1] = __byte_perm(v.x, v.z, 0x7632);
       qf[g][2] = __byte_perm(v.y, v.w, 0x5410);
@@ -125,7 +163,6 @@ __global__ void __launch_bounds__(K4_WARPS * 32) kv4_decode_kernel(const K4Param
       start[g][1] = -K4_BIAS * __shfl_sync(0xffffffffu, s, 8 * t + 4);
     }
   }
-  const float c = p.scale * 1.4426950408889634f;
 
   float o[2 * G][4], z[G][4], top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
 #pragma unroll
@@ -133,26 +170,62 @@ __global__ void __launch_bounds__(K4_WARPS * 32) kv4_decode_kernel(const K4Param
 #pragma unroll
   for (int g = 0; g < G; ++g) z[g][0] = z[g][1] = z[g][2] = z[g][3] = 0.f;
 
+  // The warp's steps are begin + warp + 4 i. Each lane knows the page of one of 32 of them, and of one of the 32 after.
   const int* table = p.block_table + static_cast<long long>(b) * p.table_stride;
-  const int tok = 4 * (r >> 1) + (r & 1);      // of a step; the thread's other row is two tokens later
-  for (int step = begin + warp; step < end; step += K4_WARPS) {
-    const int pos0 = step * K4_STEP, blk = pos0 / p.block_size, off = pos0 - blk * p.block_size;
-    long long page_no = table[blk];
-    if (page_no < 0 || page_no >= p.num_blocks) {      // outside the cache: recorded, its tokens are left out
-      if (lane == 0 && p.status) atomicCAS(p.status, 0, RLB_ERR_BAD_ARG);
-      continue;
+  const int n = end - begin > warp ? (end - begin - warp + K4_WARPS - 1) / K4_WARPS : 0;
+  auto page_of = [&](int i, int& off) -> int {
+    if (i >= n) return 0;
+    const int pos0 = (begin + warp + i * K4_WARPS) * K4_STEP, blk = pos0 / p.block_size;
+    off = pos0 - blk * p.block_size;
+    int no = table[blk];
+    if (no < 0 || no >= p.num_blocks) {      // outside the cache: recorded, and page 0 read in its place
+      if (p.status) atomicCAS(p.status, 0, RLB_ERR_BAD_ARG);
+      no = 0;
     }
-    const uint8_t* page = p.cache + (page_no * p.Hkv + kvh) * Page::bytes(p.block_size);
-    uint32_t ka[G], kb[G], va[G], vb[G], sa[G], sb[G];      // sa, sb: scales of keys, then of values
-    load_words(page + Page::key_word(off + tok, t, 0), ka);
-    load_words(page + Page::key_word(off + tok + 2, t, 0), kb);
-    const uint8_t* values = page + Page::values_at(p.block_size);
-    load_words(values + Page::value_unit(off + 4 * t, r, 0), va);
-    load_words(values + Page::value_unit(off + 4 * t + 2, r, 0), vb);
-    const uint8_t* scales = page + Page::scales_at(p.block_size);
-    load_words(scales + Page::scale(off + tok, 0, 0), sa);
-    load_words(scales + Page::scale(off + tok + 2, 0, 0), sb);
+    return no;
+  };
+  int off_now = 0, off_next = 0;
+  int page_now = page_of(lane, off_now), page_next = page_of(32 + lane, off_next);
+  const uint32_t fifo = smem_u32(k4_smem_raw) + warp * (K4_STAGES * Stage::BYTES);
+  const int tok = 4 * (r >> 1) + (r & 1);      // of a step; the thread's other row is two tokens later
+  auto request = [&](int i) {
+    if (i < n) {
+      const int src = i & 31;
+      const int off = __shfl_sync(0xffffffffu, off_now, src);
+      const uint8_t* page = p.cache + (static_cast<long long>(__shfl_sync(0xffffffffu, page_now, src)) * p.Hkv + kvh) * Page::bytes(p.block_size);
+      const uint32_t to = fifo + (i % K4_STAGES) * Stage::BYTES;
+      const uint8_t* keys = page + Page::key_word(off + tok, t, 0);
+      const uint8_t* values = page + Page::values_at(p.block_size) + Page::value_unit(off + 4 * t, r, 0);
+      copy_words<G>(to + Stage::KA + lane * (G * 4), keys);
+      copy_words<G>(to + Stage::KB + lane * (G * 4), keys + D);               // two tokens of keys
+      copy_words<G>(to + Stage::VA + lane * (G * 4), values);
+      copy_words<G>(to + Stage::VB + lane * (G * 4), values + D);             // one pair of tokens of values
+      if (lane < D / 8) copy_words<4>(to + Stage::SCALES + lane * 16, page + Page::scales_at(p.block_size) + Page::scale(off, 0, 0) + lane * 16);
+      if (src == 31) {
+        page_now = page_next;
+        off_now = off_next;
+        page_next = page_of(i + 33 + lane, off_next);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < K4_STAGES - 1; ++i) request(i);
 
+  for (int i = 0; i < n; ++i) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(K4_STAGES - 2) : "memory");
+    __syncwarp();      // the scales were copied by other lanes; and every lane has read the stage that is requested next
+    const uint32_t from = fifo + (i % K4_STAGES) * Stage::BYTES;
+    uint32_t ka[G], kb[G], va[G], vb[G], sa[G], sb[G];      // sa, sb: scales of keys, then of values
+    load_words(from + Stage::KA + lane * (G * 4), ka);
+    load_words(from + Stage::KB + lane * (G * 4), kb);
+    load_words(from + Stage::SCALES + Page::scale(tok, 0, 0), sa);
+    load_words(from + Stage::SCALES + Page::scale(tok + 2, 0, 0), sb);
+    load_words(from + Stage::VA + lane * (G * 4), va);
+    load_words(from + Stage::VB + lane * (G * 4), vb);
+    request(i + K4_STAGES - 1);
+
+    const int pos0 = (begin + warp + i * K4_WARPS) * K4_STEP;
     float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int g = 0; g < G; ++g) {
@@ -167,14 +240,12 @@ __global__ void __launch_bounds__(K4_WARPS * 32) kv4_decode_kernel(const K4Param
     }
     const bool edge = pos0 < first || pos0 + K4_STEP > len;
     const bool live_a = pos0 + tok >= first && pos0 + tok < len, live_b = pos0 + tok + 2 >= first && pos0 + tok + 2 < len;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] *= c;
     if (edge) {      // (a place that was never written, or by another sequence, may hold anything)
       if (!live_a) s[0] = s[1] = -INFINITY;
       if (!live_b) s[2] = s[3] = -INFINITY;
     }
     // The running maximum moves only when a score passes it by K4_SLACK: weights are then at most 2^8, and any reference gives the same quotient.
-    if (__any_sync(0xffffffffu, fmaxf(s[0], s[2]) > top[0] + K4_SLACK || fmaxf(s[1], s[3]) > top[1] + K4_SLACK)) {
+    if (__any_sync(0xffffffffu, fmaxf(s[0], s[2]) > top[0] + slack || fmaxf(s[1], s[3]) > top[1] + slack)) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float m = fmaxf(s[h], s[h + 2]);
@@ -182,13 +253,13 @@ __global__ void __launch_bounds__(K4_WARPS * 32) kv4_decode_kernel(const K4Param
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
         if (m > top[h]) {
-          const float f = exp2_fast(top[h] - m);      // (0 for the first)
+          const float f = exp2_fast((top[h] - m) * c);      // (0 for the first)
           top[h] = m;
           sum[h] *= f;
 #pragma unroll
-          for (int i = 0; i < 2 * G; ++i) {
-            o[i][h] *= f;
-            o[i][h + 2] *= f;
+          for (int j = 0; j < 2 * G; ++j) {
+            o[j][h] *= f;
+            o[j][h + 2] *= f;
           }
 #pragma unroll
           for (int g = 0; g < G; ++g) {
@@ -198,26 +269,35 @@ __global__ void __launch_bounds__(K4_WARPS * 32) kv4_decode_kernel(const K4Param
         }
       }
     }
-    const float ref0 = top[0] == -INFINITY ? 0.f : top[0], ref1 = top[1] == -INFINITY ? 0.f : top[1];
-    const float p0 = exp2_fast(s[0] - ref0), p1 = exp2_fast(s[1] - ref1), p2 = exp2_fast(s[2] - ref0), p3 = exp2_fast(s[3] - ref1);
+    const float ref0 = top[0] == -INFINITY ? 0.f : -top[0] * c, ref1 = top[1] == -INFINITY ? 0.f : -top[1] * c;
+    const float p0 = exp2_fast(fmaf(s[0], c, ref0)), p1 = exp2_fast(fmaf(s[1], c, ref1)), p2 = exp2_fast(fmaf(s[2], c, ref0)), p3 = exp2_fast(fmaf(s[3], c, ref1));
     sum[0] += p0 + p2;
     sum[1] += p1 + p3;
+    if (edge) {
+#pragma unroll
+      for (int g = G / 2; g < G; ++g) {      // (the values' scales)
+        if (!live_a) sa[g] = 0u;
+        if (!live_b) sb[g] = 0u;
+      }
+    }
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      float fa = bf16_of(sa[(G + g) >> 1], G + g), fb = bf16_of(sb[(G + g) >> 1], G + g);
-      if (edge) {
-        if (!live_a) fa = 0.f;
-        if (!live_b) fb = 0.f;
-      }
-      // weight * scale in 32 bits, rounded once to the operand's bf16: half a step, 2^-9, of each token's share, with either sign
+      const float fa = bf16_of(sa[(G + g) >> 1], G + g), fb = bf16_of(sb[(G + g) >> 1], G + g);
+      // weight * scale in 32 bits, rounded once to the operand's bf16: half a step, 2^-8 of each token's share at most, with either sign
       const uint32_t w0 = transposed8x8(pack_bf16x2(p0 * fa, p1 * fa)), w1 = transposed8x8(pack_bf16x2(p2 * fb, p3 * fb));
       mma_bf16(o[2 * g], unpack2(va[g], 0), unpack2(va[g], 1), unpack2(vb[g], 0), unpack2(vb[g], 1), w0, w1);
       mma_bf16(o[2 * g + 1], unpack2(va[g], 2), unpack2(va[g], 3), unpack2(vb[g], 2), unpack2(vb[g], 3), w0, w1);
       mma_bf16(z[g], 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, w0, w1);
     }
+    // What the codes' offset has added is taken off again and again: left until the end it would outgrow the sums, which are to keep their last bits (32768 tokens: the
+    // result's error 2.8e-3 instead of 2.0e-3).
+    if (i % K4_FOLD == K4_FOLD - 1) fold(o, z);
   }
+  fold(o, z);
 
   // the warps' parts: heads 2 t and 2 t + 1, dimensions 32 g + 4 r .. + 3
+  __syncthreads();      // the FIFOs' memory is used again
+  float* k4_red = reinterpret_cast<float*>(k4_smem_raw);
   float* red_ml = k4_red + K4_WARPS * 8 * D;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -227,13 +307,13 @@ __global__ void __launch_bounds__(K4_WARPS * 32) kv4_decode_kernel(const K4Param
     l += __shfl_xor_sync(0xffffffffu, l, 16);
     const int head = 2 * t + h;
     if (r == 0) {
-      red_ml[(warp * 8 + head) * 2] = top[h];
+      red_ml[(warp * 8 + head) * 2] = top[h] * c;
       red_ml[(warp * 8 + head) * 2 + 1] = l;
     }
 #pragma unroll
     for (int g = 0; g < G; ++g)
       *reinterpret_cast<float4*>(k4_red + (warp * 8 + head) * D + 32 * g + 4 * r) =
-          make_float4(o[2 * g][h] - K4_BIAS * z[g][h], o[2 * g][h + 2] - K4_BIAS * z[g][h], o[2 * g + 1][h] - K4_BIAS * z[g][h], o[2 * g + 1][h + 2] - K4_BIAS * z[g][h]);
+          make_float4(o[2 * g][h], o[2 * g][h + 2], o[2 * g + 1][h], o[2 * g + 1][h + 2]);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < heads * D; i += blockDim.x) {
