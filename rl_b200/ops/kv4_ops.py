@@ -13,13 +13,13 @@ the PyTorch restatement. The cache is for inference: nothing here has a gradient
 from __future__ import annotations
 
 import math
-from contextlib import nullcontext
+from functools import lru_cache
 from typing import Optional
 
 import torch
 
 from . import lib as _L
-from .lib import call, ptr, stream_ptr, use_native
+from .lib import call, ptr, use_native
 
 _P, _I, _LL, _F = _L.P, _L.I, _L.L, _L.F
 _L.register("rlb_rope_kv4_cache_write", [_P, _P, _P, _P, _P, _LL, _I, _I, _I, _I, _LL, _LL, _P, _P])
@@ -47,33 +47,42 @@ def kv4_cache(num_blocks: int, Hkv: int, block_size: int, D: int, device) -> tor
     return torch.zeros((num_blocks, Hkv, kv4_page_bytes(block_size, D)), dtype=torch.uint8, device=device)
 
 
-def _block_size(cache: torch.Tensor, Hkv: int, D: int) -> int:
-    """Tokens of a page, from its bytes; refuses what is not a cache of this shape."""
+@lru_cache(maxsize=256)
+def _page_tokens(page_bytes: int, D: int) -> int:
+    """Tokens of a page of so many bytes; 0 where no page has as many."""
     if D not in HEAD_DIMS:
         raise ValueError(f"the 4-bit cache holds heads of {HEAD_DIMS} dimensions, not {D}")
-    if cache.dtype != torch.uint8 or cache.dim() != 3 or not cache.is_contiguous() or cache.data_ptr() % 16:
+    size = page_bytes * 8 // (9 * D)
+    return size if 16 <= size <= MAX_BLOCK and size % 16 == 0 and size * D * 9 // 8 == page_bytes else 0
+
+
+def _block_size(cache: torch.Tensor, Hkv: int, D: int) -> int:
+    """Tokens of a page, from its bytes; refuses what is not a cache of this shape."""
+    shape = cache.shape
+    if cache.dtype is not torch.uint8 or len(shape) != 3 or not cache.is_contiguous() or cache.data_ptr() % 16:
         raise ValueError("the 4-bit cache is a contiguous uint8 tensor [blocks, heads, page bytes] that starts on 16 bytes")
-    size = cache.shape[2] * 8 // (9 * D)
-    if cache.shape[1] != Hkv or size < 16 or kv4_page_bytes(size - size % 16, D) != cache.shape[2]:
-        raise ValueError(f"cache {tuple(cache.shape)} does not hold pages of {Hkv} heads of {D} dimensions")
+    size = _page_tokens(shape[2], D)
+    if shape[1] != Hkv or Hkv < 1 or not size:
+        raise ValueError(f"cache {tuple(shape)} does not hold pages of {Hkv} heads of {D} dimensions")
     return size
 
 
-def _same_device(*ts: Optional[torch.Tensor]) -> None:
-    devices = {t.device for t in ts if t is not None}
-    if len(devices) > 1:
-        raise ValueError(f"tensors on several devices: {sorted(map(str, devices))}")
+def _same_device(device: torch.device, *ts: torch.Tensor) -> None:
+    for t in ts:
+        if t.device != device:
+            raise ValueError(f"tensors on several devices: {device} and {t.device}")
 
 
-def _on(device: torch.device):
-    """Kernels go to the current stream of the tensors' device, whichever device is current."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _index(t: torch.Tensor, dtype: torch.dtype, shape: tuple, what: str) -> torch.Tensor:
+    if t.shape != shape or t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what} is an integer tensor {shape}, not {t.dtype} {tuple(t.shape)}")
+    return t if t.dtype is dtype and t.is_contiguous() else t.to(dtype).contiguous()
 
 
-def _index(t: torch.Tensor, dtype: torch.dtype, n: int, what: str) -> torch.Tensor:
-    if t.dim() != 1 or t.shape[0] != n or t.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{what} is a vector of {n} integers, not {t.dtype} {tuple(t.shape)}")
-    return t.to(dtype).contiguous()
+def _aligned(t: torch.Tensor) -> bool:
+    """Whether the kernels can move these rows 16 bytes at a time."""
+    stride = t.stride()
+    return stride[1] == 1 and stride[0] % 8 == 0 and t.data_ptr() % 16 == 0
 
 
 # --------------------------------------------------------------------------------------- PyTorch restatement
@@ -133,13 +142,13 @@ def rope_kv4_cache_write(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: t
     4-bit ``cache``, in one launch; returns the rotated fused rows. ``slots`` [T]: block * block_size + offset of each token (negative: rotate only);
     the slots of one call differ from each other. The angles are taken in 64 bits, whatever the position."""
     block = _block_size(cache, Hkv, D)
-    T = qkv.shape[0]
-    if qkv.dim() != 2 or qkv.shape[1] != (Hq + 2 * Hkv) * D:
+    if qkv.dim() != 2 or Hq < 0 or qkv.shape[1] != (Hq + 2 * Hkv) * D:
         raise ValueError(f"qkv is [T, {(Hq + 2 * Hkv) * D}], not {tuple(qkv.shape)}")
-    if inv_freq.dtype != torch.float32 or inv_freq.shape != (D // 2,):
+    if inv_freq.dtype is not torch.float32 or inv_freq.shape != (D // 2,):
         raise ValueError(f"inv_freq is a float32 vector of {D // 2}, not {inv_freq.dtype} {tuple(inv_freq.shape)}")
-    _same_device(qkv, positions, inv_freq, slots, cache)
-    positions, slots = _index(positions, torch.int32, T, "positions"), _index(slots, torch.int64, T, "slots")
+    T = qkv.shape[0]
+    _same_device(qkv.device, positions, inv_freq, slots, cache)
+    positions, slots = _index(positions, torch.int32, (T,), "positions"), _index(slots, torch.int64, (T,), "slots")
     if not use_native(qkv):
         out = qkv.clone()
         out[:, : (Hq + Hkv) * D] = _rotate_ref(qkv[:, : (Hq + Hkv) * D].reshape(T, Hq + Hkv, D), positions, inv_freq).reshape(T, -1)
@@ -155,16 +164,18 @@ def rope_kv4_cache_write(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: t
             ks[:, at], vs[:, at] = scales[mine][:, 0].transpose(0, 1), scales[mine][:, 1].transpose(0, 1)
             cache[b] = _pack_pages(kc, vc, ks, vs)
         return out
-    if qkv.dtype != BF16:
+    if qkv.dtype is not BF16:
         raise ValueError(f"the 4-bit cache takes bf16 rows, not {qkv.dtype}")
-    rows = qkv
-    if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.data_ptr() % 16:      # rows that do not start on 16 bytes: turned in a copy
-        rows = qkv.clone(memory_format=torch.contiguous_format)
-    with _on(qkv.device):
-        call("rlb_rope_kv4_cache_write", ptr(rows), ptr(positions), ptr(inv_freq.contiguous()), ptr(slots), ptr(cache), T, Hq, Hkv, D, block,
-             rows.stride(0), cache.shape[0], ptr(_L.status_word(qkv.device)), stream_ptr())
-        if rows is not qkv:
-            qkv.copy_(rows)
+    stream = torch.cuda.current_stream()
+    if stream.device_index != qkv.device.index:      # kernels go to the current stream of the tensors' device, whichever device is current
+        with torch.cuda.device(qkv.device):
+            return rope_kv4_cache_write(qkv, positions, inv_freq, slots, cache, Hq, Hkv, D)
+    rows = qkv if _aligned(qkv) else qkv.clone(memory_format=torch.contiguous_format)      # (rows that do not start on 16 bytes: turned in a copy)
+    inv_freq = inv_freq.contiguous()
+    call("rlb_rope_kv4_cache_write", ptr(rows), ptr(positions), ptr(inv_freq), ptr(slots), ptr(cache), T, Hq, Hkv, D, block, rows.stride(0), cache.shape[0],
+         ptr(_L.status_word(qkv.device)), stream.cuda_stream)
+    if rows is not qkv:
+        qkv.copy_(rows)
     return qkv
 
 
@@ -173,17 +184,20 @@ def kv4_cache_read(cache: torch.Tensor, slots: torch.Tensor, Hkv: int, D: int, *
     """Keys and values of the tokens at ``slots`` [n] as bf16 rows [k heads | v heads]. ``out`` [m, >= 2 Hkv D]: where they go (its other columns
     stay); ``rows`` [n]: token i goes to row ``rows[i]`` of ``out`` (None: row i), each row named once. A negative slot gives a row of zeros."""
     block = _block_size(cache, Hkv, D)
-    n, width = slots.shape[0], 2 * Hkv * D
-    _same_device(cache, slots, out, rows)
-    slots = _index(slots, torch.int64, n, "slots")
+    n, width, device = slots.numel(), 2 * Hkv * D, cache.device
+    _same_device(device, slots)
+    slots = _index(slots, torch.int64, (n,), "slots")
     if rows is not None:
         if out is None:
             raise ValueError("rows name rows of out: give both")
-        rows = _index(rows, torch.int64, n, "rows")
+        _same_device(device, rows)
+        rows = _index(rows, torch.int64, (n,), "rows")
     if out is None:
-        out = torch.empty((n, width), dtype=BF16, device=cache.device)
+        out = torch.empty((n, width), dtype=BF16, device=device)
     elif out.dim() != 2 or out.shape[1] < width or (rows is None and out.shape[0] < n):
         raise ValueError(f"out {tuple(out.shape)} has no room for {n} rows of {width}")
+    else:
+        _same_device(device, out)
     if not use_native(cache):
         kc, vc, ks, vs = _unpack_pages(cache[(slots // block).clamp(min=0)], D)      # [n, Hkv, block, ...]
         ar, off = torch.arange(n), slots.clamp(min=0) % block
@@ -191,18 +205,19 @@ def kv4_cache_read(cache: torch.Tensor, slots: torch.Tensor, Hkv: int, D: int, *
         kv = torch.where(slots[:, None] < 0, torch.zeros_like(kv), kv)
         out[torch.arange(n) if rows is None else rows, :width] = kv.to(out.dtype)
         return out
-    if out.dtype != BF16:
+    if out.dtype is not BF16:
         raise ValueError(f"the 4-bit cache is read into bf16 rows, not {out.dtype}")
+    stream = torch.cuda.current_stream()
+    if stream.device_index != device.index:
+        with torch.cuda.device(device):
+            return kv4_cache_read(cache, slots, Hkv, D, out=out, rows=rows)
     to = out
-    if out.stride(1) != 1 or out.stride(0) % 8 or out.data_ptr() % 16:      # rows that do not start on 16 bytes: read into a copy
-        to = out.clone(memory_format=torch.contiguous_format)
-        if to.stride(0) % 8:
-            to = torch.empty((out.shape[0], -(-out.shape[1] // 8) * 8), dtype=BF16, device=out.device)[:, : out.shape[1]].copy_(out)
-    with _on(cache.device):
-        call("rlb_kv4_cache_read", ptr(cache), ptr(slots), ptr(rows), ptr(to), n, to.stride(0), to.shape[0], Hkv, D, block, cache.shape[0],
-             ptr(_L.status_word(cache.device)), stream_ptr())
-        if to is not out:
-            out.copy_(to)
+    if not _aligned(out):      # rows that do not start on 16 bytes: read into a copy
+        to = torch.empty((out.shape[0], width), dtype=BF16, device=device).copy_(out[:, :width])
+    call("rlb_kv4_cache_read", ptr(cache), ptr(slots), ptr(rows), ptr(to), n, to.stride(0), to.shape[0], Hkv, D, block, cache.shape[0],
+         ptr(_L.status_word(device)), stream.cuda_stream)
+    if to is not out:
+        out[:, :width] = to
     return out
 
 
@@ -225,21 +240,28 @@ def kv4_paged_decode(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
     sequence without tokens gives zeros. ``num_splits``: parts that a sequence's tokens are cut into (0: by :func:`kv4_splits` from the table's width);
     ``scratch``: fp32 tensors of :func:`kv4_scratch_sizes` elements, for callers that keep their own. Returns [B, Hq D]."""
     block = _block_size(cache, Hkv, D)
+    device, width = q.device, Hq * D
+    if Hq < 1 or Hq % Hkv or q.dim() != 2 or q.shape[1] < width:
+        raise ValueError(f"q is [B, {width}] with {Hq} heads, a multiple of {Hkv}, not {tuple(q.shape)}")
+    if window < 0 or num_splits < 0:
+        raise ValueError(f"window {window} and num_splits {num_splits} are not negative")
     B = q.shape[0]
-    if Hq < 1 or Hq % Hkv or q.dim() != 2 or q.shape[1] < Hq * D:
-        raise ValueError(f"q is [B, {Hq * D}] with {Hq} heads, a multiple of {Hkv}, not {tuple(q.shape)}")
-    if block_table.dim() != 2 or block_table.shape[0] != B or seq_lens.shape != (B,):
-        raise ValueError(f"block_table is [{B}, pages] and seq_lens [{B}], not {tuple(block_table.shape)} and {tuple(seq_lens.shape)}")
-    if any(t.dtype not in (torch.int32, torch.int64) for t in (block_table, seq_lens)):
-        raise ValueError("block_table and seq_lens are integers")
-    if window < 0:
-        raise ValueError(f"window {window} is negative")
-    _same_device(q, cache, block_table, seq_lens, out, *(scratch or ()))
-    scale = scale if scale is not None else 1.0 / math.sqrt(D)
+    _same_device(device, cache, block_table, seq_lens)
+    if block_table.dim() != 2:
+        raise ValueError(f"block_table is [{B}, pages], not {tuple(block_table.shape)}")
+    pages = block_table.shape[1]
+    table = block_table
+    if table.dtype is not torch.int32 or table.shape[0] != B or table.stride(1) != 1:      # (rows of a wider table are read where they are)
+        table = _index(table, torch.int32, (B, pages), "block_table")
+    lens = _index(seq_lens, torch.int32, (B,), "seq_lens")
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
     if out is None:
-        out = torch.empty((B, Hq * D), dtype=q.dtype, device=q.device)
-    elif out.shape != (B, Hq * D) or out.dtype != q.dtype:
-        raise ValueError(f"out is {q.dtype} [{B}, {Hq * D}], not {out.dtype} {tuple(out.shape)}")
+        out = torch.empty((B, width), dtype=q.dtype, device=device)
+    elif out.shape != (B, width) or out.dtype != q.dtype:
+        raise ValueError(f"out is {q.dtype} [{B}, {width}], not {out.dtype} {tuple(out.shape)}")
+    else:
+        _same_device(device, out)
     if not use_native(q):
         for b in range(B):
             n = int(seq_lens[b])
@@ -252,28 +274,27 @@ def kv4_paged_decode(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
             p = torch.softmax(q[b, : Hq * D].reshape(Hkv, Hq // Hkv, D).float() * scale @ k.transpose(1, 2), dim=-1)
             out[b] = (p @ v).reshape(Hq * D).to(out.dtype)
         return out
-    if q.dtype != BF16:
+    if q.dtype is not BF16:
         raise ValueError(f"the 4-bit cache takes bf16 queries, not {q.dtype}")
-    if q.stride(1) != 1 or q.stride(0) % 8 or q.data_ptr() % 16:      # rows that do not start on 16 bytes
-        q = q[:, : Hq * D].clone(memory_format=torch.contiguous_format)
-    table = block_table.to(torch.int32)
-    if table.stride(1) != 1:
-        table = table.contiguous()
-    lens = seq_lens.to(torch.int32).contiguous()
-    num_splits = num_splits or kv4_splits(B, Hq, Hkv, table.shape[1] * block)
-    if num_splits < 1:
-        raise ValueError(f"num_splits {num_splits} is negative")
-    to = out if out.stride(1) == 1 and out.stride(0) % 4 == 0 and out.data_ptr() % 8 == 0 else torch.empty((B, Hq * D), dtype=BF16, device=q.device)
-    with _on(q.device):
-        po = pml = None
-        if num_splits > 1:
-            no, nml = kv4_scratch_sizes(B, Hq, num_splits, D)
-            po, pml = scratch if scratch is not None else (torch.empty(no, dtype=torch.float32, device=q.device),
-                                                           torch.empty(nml, dtype=torch.float32, device=q.device))
-            if any(t.dtype != torch.float32 or not t.is_contiguous() or t.numel() < size for t, size in ((po, no), (pml, nml))):
-                raise ValueError(f"scratch is two contiguous float32 tensors of {no} and {nml} elements")
-        call("rlb_kv4_paged_decode", ptr(q), q.stride(0), ptr(cache), cache.shape[0], ptr(table), table.stride(0), table.shape[1], ptr(lens), B, Hq, Hkv,
-             D, block, window, scale, num_splits, ptr(po), ptr(pml), ptr(to), to.stride(0), ptr(_L.status_word(q.device)), stream_ptr())
-        if to is not out:
-            out.copy_(to)
+    stream = torch.cuda.current_stream()
+    if stream.device_index != device.index:
+        with torch.cuda.device(device):
+            return kv4_paged_decode(q, cache, table, lens, Hq, Hkv, D, scale=scale, window=window, num_splits=num_splits, scratch=scratch, out=out)
+    if not _aligned(q):      # rows that do not start on 16 bytes
+        q = q[:, :width].clone(memory_format=torch.contiguous_format)
+    num_splits = num_splits or kv4_splits(B, Hq, Hkv, min(pages * block, window) if window else pages * block)
+    po = pml = None
+    if num_splits > 1:
+        no, nml = kv4_scratch_sizes(B, Hq, num_splits, D)
+        if scratch is None:
+            scratch = torch.empty(no, dtype=torch.float32, device=device), torch.empty(nml, dtype=torch.float32, device=device)
+        po, pml = scratch
+        _same_device(device, po, pml)
+        if any(t.dtype is not torch.float32 or not t.is_contiguous() or t.numel() < size for t, size in ((po, no), (pml, nml))):
+            raise ValueError(f"scratch is two contiguous float32 tensors of {no} and {nml} elements")
+    to = out if out.stride(1) == 1 else torch.empty((B, width), dtype=BF16, device=device)
+    call("rlb_kv4_paged_decode", ptr(q), q.stride(0), ptr(cache), cache.shape[0], ptr(table), table.stride(0), pages, ptr(lens), B, Hq, Hkv, D, block, window, scale,
+         num_splits, ptr(po), ptr(pml), ptr(to), to.stride(0), ptr(_L.status_word(device)), stream.cuda_stream)
+    if to is not out:
+        out.copy_(to)
     return out
