@@ -3,9 +3,11 @@
 //
 // Both products run as 16 x 8 x 16 tensor-core instructions whose 16-row operand comes from the codes in registers; the query heads are the eight columns:
 //     S^T[16 tokens, 8 heads] = K[16 tokens, dims] Q^T        O^T[16 dims, 8 heads] += V^T[16 dims, 16 tokens] P^T
-// A code c becomes the bf16 number 128 + c by one logic instruction for two of them (bits 0-3 of the mantissa). What that adds is taken off
-// exactly: from the keys by starting each product at -135.5 times the sum of the query's values, from the values by one more instruction per group of 32 dimensions that
-// sums the weights (a row of ones). Scales multiply the products of a group of keys, and the weights of a group of values, in 32 bits. The place of codes in a page is
+// A code is already a bf16 number where it stands: bits 0-3 alone are c * 2^-133, bits 4-7 alone (the top one is the exponent's lowest bit) c * 2^-129, both exact, as
+// bf16 numbers below 2^-125 are evenly spaced. So one AND makes two operands, and a shift by 8 the other two of a 16-bit unit. The powers of two go into the other
+// operand, which is bf16 with all of its exponents to spare: the query's values are multiplied by a power of two per head, the weights by one that follows the values' scales.
+// The offset of 7.5 levels is taken off in 32 bits: from the keys' products by the sum of the query's values, from the values' by a product with a row of equal codes that
+// sums the weights. Scales multiply the products of a group of keys, and the weights of a group of values, in 32 bits. The place of codes in a page is
 // such that a thread's registers are what it loads: no shuffle and no pass through shared memory. A thread's rows of S^T are the
 // tokens 4 (r / 2) + r % 2 and two later (r = lane / 4), so that the columns it has to hold of V^T are four consecutive tokens.
 //
@@ -24,7 +26,7 @@ using namespace rlb;
 constexpr int K4_WARPS = 4;
 constexpr int K4_STEP = 16;      // tokens a warp takes at a time
 constexpr int K4_STAGES = 4;     // steps whose words are in a warp's shared memory or on their way
-constexpr int K4_FOLD = 8;       // steps between two corrections of the sums
+constexpr int K4_FOLD = 16;      // steps between two corrections of the sums
 constexpr float K4_SLACK = 8.f;  // how far (in powers of two) a score may pass the running maximum before the sums are rescaled: weights stay below 2^8
 
 struct K4Params {
@@ -61,9 +63,13 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Codes at nibble j of both halves of a word as two bf16 numbers 128 + code.
-__device__ __forceinline__ uint32_t unpack2(uint32_t w, int j) { return ((w >> (4 * j)) & 0x000f000fu) | 0x43004300u; }
-constexpr float K4_BIAS = 135.5f;      // 128 + 7.5
+// Codes at nibble j of both halves of a word as two bf16 numbers: code * 2^-133 for even j, code * 2^-129 for odd j.
+__device__ __forceinline__ uint32_t unpack2(uint32_t w, int j) { return (j & 2 ? w >> 8 : w) & (j & 1 ? 0x00f000f0u : 0x000f000fu); }
+// 2^e for e from -252 to 254, as two factors where one would not do.
+__device__ __forceinline__ float times_pow2(float x, int e) {
+  const int h = e >> 1;
+  return x * __uint_as_float(static_cast<uint32_t>(h + 127) << 23) * __uint_as_float(static_cast<uint32_t>(e - h + 127) << 23);
+}
 
 // N words of shared memory at once; and from global to shared memory, in the background.
 template <int N>
@@ -100,15 +106,15 @@ constexpr int k4_smem() {
   return fifo > red ? fifo : red;
 }
 
-// Takes the codes' offset off the sums.
+// Takes the codes' offset off the sums: z is 15 * 2^-133 times the weights, 7.5 levels of what rows 0-7 of a tile count in, and 1/16 of that of rows 8-15.
 template <int G>
 __device__ __forceinline__ void fold(float (&o)[2 * G][4], float (&z)[G][4]) {
 #pragma unroll
   for (int g = 0; g < G; ++g) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      o[2 * g][j] = fmaf(-K4_BIAS, z[g][j & 1], o[2 * g][j]);
-      o[2 * g + 1][j] = fmaf(-K4_BIAS, z[g][j & 1], o[2 * g + 1][j]);
+      o[2 * g][j] = fmaf(j < 2 ? -0.5f : -8.f, z[g][j & 1], o[2 * g][j]);
+      o[2 * g + 1][j] = fmaf(j < 2 ? -0.5f : -8.f, z[g][j & 1], o[2 * g + 1][j]);
     }
     z[g][0] = z[g][1] = z[g][2] = z[g][3] = 0.f;
   }
@@ -137,34 +143,59 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 4 : 2) kv4_decode_ke
   const int begin = step0 + static_cast<int>(static_cast<long long>(steps) * split / p.num_splits);
   const int end = step0 + static_cast<int>(static_cast<long long>(steps) * (split + 1) / p.num_splits);
 
-  // scores are compared before they are scaled: a negative scale turns the query's sign
-  const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
-  const float c = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-30f), slack = K4_SLACK / c;
-
-  // the queries as the 8-column operand: pair j of group g is (dimension 32 g + 8 t + j, and four later) of head r
+  // The queries as the 8-column operand: pair j of group g is (dimension 32 g + 8 t + j, and four later) of head r, times 2^k with the head's largest value
+  // in [2^119, 2^120) (a sum of 32 stays finite), and 1/16 of that where the codes count 16 times. Scores are compared before they are scaled: a negative scale turns the
+  // query's sign. c[h]: from the products' unit to powers of two, of heads 2 t and 2 t + 1.
   uint32_t qf[G][4];
-  float start[G][2];      // -135.5 * sum of the group's values, of heads 2 t and 2 t + 1
+  float start[G][2], c[2], slack[2];      // start: -7.5 * sum of the group's values
   {
     const __nv_bfloat16* q = p.q + static_cast<long long>(b) * p.q_stride + static_cast<long long>(head0 + r) * D + 8 * t;
+    uint4 v[G];
+    uint32_t big = 0u;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (r < heads) v = *reinterpret_cast<const uint4*>(q + 32 * g);
-      v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
-      qf[g][0] = __byte_perm(v.x, v.z, 0x5410);
-      qf[g][1] = __byte_perm(v.x, v.z, 0x7632);
-      qf[g][2] = __byte_perm(v.y, v.w, 0x5410);
-      qf[g][3] = __byte_perm(v.y, v.w, 0x7632);
-      const float2 a = unpack_bf16x2(v.x), c = unpack_bf16x2(v.y), d = unpack_bf16x2(v.z), e = unpack_bf16x2(v.w);
-      float s = ((a.x + a.y) + (c.x + c.y)) + ((d.x + d.y) + (e.x + e.y));
+      v[g] = make_uint4(0, 0, 0, 0);
+      if (r < heads) v[g] = *reinterpret_cast<const uint4*>(q + 32 * g);
+      big = max(max(max(big, v[g].x & 0x7fffu), max(v[g].x >> 16 & 0x7fffu, v[g].y & 0x7fffu)), max(v[g].y >> 16 & 0x7fffu, v[g].z & 0x7fffu));
+      big = max(max(big, v[g].z >> 16 & 0x7fffu), max(v[g].w & 0x7fffu, v[g].w >> 16 & 0x7fffu));
+    }
+    big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+    big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+    const int k = 119 + 127 - static_cast<int>(big >> 7);
+    const float sign = p.scale < 0.f ? -1.f : 1.f;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const uint32_t w[4] = {v[g].x, v[g].y, v[g].z, v[g].w};
+      float f[8], s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 a = unpack_bf16x2(w[i]);
+        f[2 * i] = times_pow2(a.x * sign, k);
+        f[2 * i + 1] = times_pow2(a.y * sign, k);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s += f[j] + f[4 + j];
+        qf[g][j] = pack_bf16x2(f[j] * (j & 1 ? 0.0625f : 1.f), f[4 + j] * (j & 1 ? 0.0625f : 1.f));
+      }
       s += __shfl_xor_sync(0xffffffffu, s, 1);
       s += __shfl_xor_sync(0xffffffffu, s, 2);
-      start[g][0] = -K4_BIAS * __shfl_sync(0xffffffffu, s, 8 * t);
-      start[g][1] = -K4_BIAS * __shfl_sync(0xffffffffu, s, 8 * t + 4);
+      s = times_pow2(s * -7.5f, -133);
+      start[g][0] = __shfl_sync(0xffffffffu, s, 8 * t);
+      start[g][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
     }
+    const float unit = fminf(fmaxf(times_pow2(fabsf(p.scale) * 1.4426950408889634f, 133 - k), 1e-30f), 1e30f);
+    c[0] = __shfl_sync(0xffffffffu, unit, 8 * t);
+    c[1] = __shfl_sync(0xffffffffu, unit, 8 * t + 4);
+    slack[0] = K4_SLACK / c[0];
+    slack[1] = K4_SLACK / c[1];
   }
 
   float o[2 * G][4], z[G][4], top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+  // Weights are held 2^lift times as large, so that their products with the values' scales lie near 2^40 and keep clear of the ends of 32 bits (times 2^-133) and of
+  // bf16. limit: the largest scale, in bf16 bits in both halves, for which that holds.
+  float lift = 0.f;
+  uint32_t limit = 0u;
 #pragma unroll
   for (int i = 0; i < 2 * G; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
@@ -229,23 +260,48 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 4 : 2) kv4_decode_ke
     float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      float acc[4] = {start[g][0], start[g][1], start[g][0], start[g][1]};
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
       mma_bf16(acc, unpack2(ka[g], 0), unpack2(kb[g], 0), unpack2(ka[g], 1), unpack2(kb[g], 1), qf[g][0], qf[g][1]);
       mma_bf16(acc, unpack2(ka[g], 2), unpack2(kb[g], 2), unpack2(ka[g], 3), unpack2(kb[g], 3), qf[g][2], qf[g][3]);
       const float fa = bf16_of(sa[g >> 1], g), fb = bf16_of(sb[g >> 1], g);
-      s[0] = fmaf(acc[0], fa, s[0]);
-      s[1] = fmaf(acc[1], fa, s[1]);
-      s[2] = fmaf(acc[2], fb, s[2]);
-      s[3] = fmaf(acc[3], fb, s[3]);
+      s[0] = fmaf(acc[0] + start[g][0], fa, s[0]);
+      s[1] = fmaf(acc[1] + start[g][1], fa, s[1]);
+      s[2] = fmaf(acc[2] + start[g][0], fb, s[2]);
+      s[3] = fmaf(acc[3] + start[g][1], fb, s[3]);
     }
     const bool edge = pos0 < first || pos0 + K4_STEP > len;
     const bool live_a = pos0 + tok >= first && pos0 + tok < len, live_b = pos0 + tok + 2 >= first && pos0 + tok + 2 < len;
     if (edge) {      // (a place that was never written, or by another sequence, may hold anything)
       if (!live_a) s[0] = s[1] = -INFINITY;
       if (!live_b) s[2] = s[3] = -INFINITY;
+#pragma unroll
+      for (int g = G / 2; g < G; ++g) {      // (the values' scales)
+        if (!live_a) sa[g] = 0u;
+        if (!live_b) sb[g] = 0u;
+      }
     }
     // The running maximum moves only when a score passes it by K4_SLACK: weights are then at most 2^8, and any reference gives the same quotient.
-    if (__any_sync(0xffffffffu, fmaxf(s[0], s[2]) > top[0] + slack || fmaxf(s[1], s[3]) > top[1] + slack)) {
+    uint32_t widest = limit;
+#pragma unroll
+    for (int g = G / 2; g < G; ++g) widest = __vmaxu2(widest, __vmaxu2(sa[g], sb[g]));
+    if (__any_sync(0xffffffffu, fmaxf(s[0], s[2]) > top[0] + slack[0] || fmaxf(s[1], s[3]) > top[1] + slack[1] || widest != limit)) {
+      float f[2] = {1.f, 1.f};
+      uint32_t wide = 0u;      // the largest finite scale
+#pragma unroll
+      for (int g = G / 2; g < G; ++g) {
+        const uint32_t w[4] = {sa[g] & 0xffffu, sa[g] >> 16, sb[g] & 0xffffu, sb[g] >> 16};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) wide = max(wide, w[j] < 0x7f80u ? w[j] : 0u);
+      }
+      wide = __reduce_max_sync(0xffffffffu, wide);
+      if (wide > (limit & 0xffffu)) {
+        const int e = static_cast<int>(wide >> 7) - 127;
+        const float to = static_cast<float>(max(-100, min(96, 40 - e)));
+        f[0] = f[1] = exp2_fast(to - lift);
+        lift = to;
+        limit = static_cast<uint32_t>(min(254, max(1, e + 40 + 127))) << 7;
+        limit |= limit << 16;
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float m = fmaxf(s[h], s[h + 2]);
@@ -253,33 +309,26 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 4 : 2) kv4_decode_ke
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
         if (m > top[h]) {
-          const float f = exp2_fast((top[h] - m) * c);      // (0 for the first)
+          f[h] *= exp2_fast((top[h] - m) * c[h]);      // (0 for the first)
           top[h] = m;
-          sum[h] *= f;
+        }
+        sum[h] *= f[h];
 #pragma unroll
-          for (int j = 0; j < 2 * G; ++j) {
-            o[j][h] *= f;
-            o[j][h + 2] *= f;
-          }
+        for (int j = 0; j < 2 * G; ++j) {
+          o[j][h] *= f[h];
+          o[j][h + 2] *= f[h];
+        }
 #pragma unroll
-          for (int g = 0; g < G; ++g) {
-            z[g][h] *= f;
-            z[g][h + 2] *= f;
-          }
+        for (int g = 0; g < G; ++g) {
+          z[g][h] *= f[h];
+          z[g][h + 2] *= f[h];
         }
       }
     }
-    const float ref0 = top[0] == -INFINITY ? 0.f : -top[0] * c, ref1 = top[1] == -INFINITY ? 0.f : -top[1] * c;
-    const float p0 = exp2_fast(fmaf(s[0], c, ref0)), p1 = exp2_fast(fmaf(s[1], c, ref1)), p2 = exp2_fast(fmaf(s[2], c, ref0)), p3 = exp2_fast(fmaf(s[3], c, ref1));
+    const float ref0 = top[0] == -INFINITY ? 0.f : fmaf(-top[0], c[0], lift), ref1 = top[1] == -INFINITY ? 0.f : fmaf(-top[1], c[1], lift);
+    const float p0 = exp2_fast(fmaf(s[0], c[0], ref0)), p1 = exp2_fast(fmaf(s[1], c[1], ref1)), p2 = exp2_fast(fmaf(s[2], c[0], ref0)), p3 = exp2_fast(fmaf(s[3], c[1], ref1));
     sum[0] += p0 + p2;
     sum[1] += p1 + p3;
-    if (edge) {
-#pragma unroll
-      for (int g = G / 2; g < G; ++g) {      // (the values' scales)
-        if (!live_a) sa[g] = 0u;
-        if (!live_b) sb[g] = 0u;
-      }
-    }
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       const float fa = bf16_of(sa[(G + g) >> 1], G + g), fb = bf16_of(sb[(G + g) >> 1], G + g);
@@ -287,10 +336,9 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 4 : 2) kv4_decode_ke
       const uint32_t w0 = transposed8x8(pack_bf16x2(p0 * fa, p1 * fa)), w1 = transposed8x8(pack_bf16x2(p2 * fb, p3 * fb));
       mma_bf16(o[2 * g], unpack2(va[g], 0), unpack2(va[g], 1), unpack2(vb[g], 0), unpack2(vb[g], 1), w0, w1);
       mma_bf16(o[2 * g + 1], unpack2(va[g], 2), unpack2(va[g], 3), unpack2(vb[g], 2), unpack2(vb[g], 3), w0, w1);
-      mma_bf16(z[g], 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, w0, w1);
+      mma_bf16(z[g], 0x000f000fu, 0x000f000fu, 0x000f000fu, 0x000f000fu, w0, w1);
     }
-    // What the codes' offset has added is taken off again and again: left until the end it would outgrow the sums, which are to keep their last bits (32768 tokens: the
-    // result's error 2.8e-3 instead of 2.0e-3).
+    // The offset is taken off again and again: left until the end it would outgrow the sums, which are to keep their last bits.
     if (i % K4_FOLD == K4_FOLD - 1) fold(o, z);
   }
   fold(o, z);
@@ -307,13 +355,13 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 4 : 2) kv4_decode_ke
     l += __shfl_xor_sync(0xffffffffu, l, 16);
     const int head = 2 * t + h;
     if (r == 0) {
-      red_ml[(warp * 8 + head) * 2] = top[h] * c;
+      red_ml[(warp * 8 + head) * 2] = top[h] == -INFINITY ? -INFINITY : fmaf(top[h], c[h], -lift);      // what the weights are relative to
       red_ml[(warp * 8 + head) * 2 + 1] = l;
     }
 #pragma unroll
     for (int g = 0; g < G; ++g)
       *reinterpret_cast<float4*>(k4_red + (warp * 8 + head) * D + 32 * g + 4 * r) =
-          make_float4(o[2 * g][h], o[2 * g][h + 2], o[2 * g + 1][h], o[2 * g + 1][h + 2]);
+          make_float4(times_pow2(o[2 * g][h], 133), times_pow2(o[2 * g][h + 2], 129), times_pow2(o[2 * g + 1][h], 133), times_pow2(o[2 * g + 1][h + 2], 129));
   }
   __syncthreads();
   for (int i = threadIdx.x; i < heads * D; i += blockDim.x) {

@@ -125,7 +125,7 @@ def _pool(pages, Hkv, D, block, seed, big=1.0):
 
 def _check(got, q, cache, table, lens, Hq, Hkv, D, window=0, scale=None):
     """Every output within what the roundings give: the result's to bf16 (2^-8 of it), each token's weight times its scale to bf16 (2^-8 of
-    the token's share), and the scores in 32 bits. A score's sum over a group starts at 135.5 times the sum of the query's values and has 33 terms of at most 143 |q|:
+    the token's share), and the scores in 32 bits. A score's sum over a group has 32 terms of at most 15 |q| and the offset of 7.5 times the sum of the query's values:
     an error of 33 roundings at that size, times the key's scale; a score's error e changes a weight by e and the sum by as much."""
     block, B = cache.shape[2] * 8 // (9 * D), q.shape[0]
     scale = scale or 1 / math.sqrt(D)
@@ -140,7 +140,7 @@ def _check(got, q, cache, table, lens, Hq, Hkv, D, window=0, scale=None):
         qb = q[b, : Hq * D].double().reshape(Hkv, Hq // Hkv, D)
         p = torch.softmax(qb @ k.transpose(1, 2) * scale, -1)
         want, share = p @ v, p @ v.abs()
-        e = scale * 33 * 2.0 ** -24 * 143 * torch.einsum("hgd,hd->hg", qb.abs(), ks.double().repeat_interleave(32, -1).flatten(1, 2)[:, lo:n].amax(1)).unsqueeze(-1)
+        e = scale * 33 * 2.0 ** -24 * 15 * torch.einsum("hgd,hd->hg", qb.abs(), ks.double().repeat_interleave(32, -1).flatten(1, 2)[:, lo:n].amax(1)).unsqueeze(-1)
         tol = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2 * e + 2.0 ** -18) * share
         off = (got[b].double().reshape(want.shape) - want).abs()
         assert (off <= tol).all(), f"row {b}: {(off / tol).max().item():.2f} times the tolerance"
