@@ -1,5 +1,6 @@
 // Decode attention over the 4-bit key/value cache (kv4.cuh): one query token per sequence, softmax(scale q k^T) v over its cached tokens or the last
-// `window` of them. One CTA of four warps per (sequence, key/value head and up to eight of its query heads, split of the tokens).
+// `window` of them. A CTA of four warps takes a sequence and one key/value head with up to eight of its query heads; or as many CTAs as the device holds
+// share all tokens evenly, so that each gets a run of whole sequences and a part of one or two, and a second kernel joins the parts.
 //
 // Both products run as 16 x 8 x 16 tensor-core instructions whose 16-row operand comes from the codes in registers; the query heads are the eight columns:
 //     S^T[16 tokens, 8 heads] = K[16 tokens, dims] Q^T        O^T[16 dims, 8 heads] += V^T[16 dims, 16 tokens] P^T
@@ -24,7 +25,7 @@ namespace {
 using namespace rlb;
 
 constexpr int K4_WARPS = 4;
-constexpr int K4_STEP = 16;      // tokens a warp takes at a time
+constexpr int K4_STEP = 32;      // tokens a warp takes at a time: twice the 16 of an instruction
 constexpr int K4_STAGES = 4;     // steps whose words are in a warp's shared memory or on their way
 constexpr int K4_FOLD = 16;      // steps between two corrections of the sums
 constexpr float K4_SLACK = 8.f;  // how far (in powers of two) a score may pass the running maximum before the sums are rescaled: weights stay below 2^8
@@ -40,22 +41,23 @@ struct K4Params {
   const int* seq_lens;
   int Hkv, G, chunks, block_size, window;
   float scale;
-  int num_splits;
-  float* part_o;
-  float* part_ml;
+  int B, num_ctas;      // num_ctas: CTAs that share all tokens evenly, or 0: one CTA per (sequence, heads)
+  float* part_o;        // [num_ctas][2] parts of 8 heads x D sums
+  float2* part_ml;      // [num_ctas][2][8]
+  int4* joins;          // [min(num_ctas, sequences x heads)]
   __nv_bfloat16* out;
   long long out_stride;
   int* status;
 };
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transposed8x8(uint32_t v) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -65,10 +67,29 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 // Codes at nibble j of both halves of a word as two bf16 numbers: code * 2^-133 for even j, code * 2^-129 for odd j.
 __device__ __forceinline__ uint32_t unpack2(uint32_t w, int j) { return (j & 2 ? w >> 8 : w) & (j & 1 ? 0x00f000f0u : 0x000f000fu); }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }      // e from -126 to 127
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// Two sums or products at once.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
 // 2^e for e from -252 to 254, as two factors where one would not do.
 __device__ __forceinline__ float times_pow2(float x, int e) {
   const int h = e >> 1;
-  return x * __uint_as_float(static_cast<uint32_t>(h + 127) << 23) * __uint_as_float(static_cast<uint32_t>(e - h + 127) << 23);
+  return x * pow2(h) * pow2(e - h);
 }
 
 // N words of shared memory at once; and from global to shared memory, in the background.
@@ -93,16 +114,16 @@ __device__ __forceinline__ void copy_words(uint32_t to, const uint8_t* from) {
 }
 __device__ __forceinline__ float bf16_of(uint32_t word, int i) { return __uint_as_float(i & 1 ? word & 0xffff0000u : word << 16); }
 
-// A warp's stage: the words that each lane is going to use (its own copies, so that no other lane has to be waited for), and the scales of the 16 tokens.
+// A warp's stage: twice 16 tokens of the words that each lane is going to use (its own copies, so that no other lane has to be waited for), and their scales.
 template <int D>
 struct K4Stage {
   static constexpr int PART = 32 * (D / 32) * 4;      // one word per lane and group
-  static constexpr int KA = 0, KB = PART, VA = 2 * PART, VB = 3 * PART, SCALES = 4 * PART, BYTES = 4 * PART + 2 * D;
+  static constexpr int KA = 0, KB = PART, VA = 2 * PART, VB = 3 * PART, SCALES = 4 * PART, HALF = 4 * PART + 2 * D, BYTES = 2 * HALF;
 };
-// Shared memory: the warps' stages; after the token loop [warps][8 heads][D] sums, then [warps][8][2] maximum and sum of the weights.
+// Shared memory: the warps' stages; after the token loop [warps][8 heads] rows of D + 4 sums (4 more, for the banks).
 template <int D>
 constexpr int k4_smem() {
-  constexpr int fifo = K4_WARPS * K4_STAGES * K4Stage<D>::BYTES, red = K4_WARPS * 8 * (D + 2) * 4;
+  constexpr int fifo = K4_WARPS * K4_STAGES * K4Stage<D>::BYTES, red = K4_WARPS * 8 * (D + 4) * 4;
   return fifo > red ? fifo : red;
 }
 
@@ -120,69 +141,167 @@ __device__ __forceinline__ void fold(float (&o)[2 * G][4], float (&z)[G][4]) {
   }
 }
 
+// Tokens of a sequence that the table has room for, the first visible one, and the steps from there on.
+struct K4Span {
+  int len, first, step0, steps;
+};
+__device__ __forceinline__ K4Span k4_span(const K4Params& p, int b) {
+  K4Span s;
+  const long long room = p.num_blocks ? static_cast<long long>(p.max_blocks) * p.block_size : 0;
+  s.len = p.seq_lens[b];
+  if (s.len > room) {      // more tokens than the table has pages: recorded, the rest is left out
+    if (p.status) atomicCAS(p.status, 0, RLB_ERR_BAD_ARG);
+    s.len = static_cast<int>(room);
+  }
+  s.len = max(s.len, 0);
+  s.first = p.window > 0 ? max(0, s.len - p.window) : 0;
+  s.step0 = s.first / K4_STEP;
+  s.steps = max(1, s.len / K4_STEP + (s.len % K4_STEP != 0) - s.step0);      // (one for an empty sequence, whose output is written too)
+  return s;
+}
+
 template <int D>
-__global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 4 : 2) kv4_decode_kernel(const K4Params p) {
+__global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_kernel(const K4Params p) {
   extern __shared__ __align__(128) uint8_t k4_smem_raw[];
+  __shared__ float2 ml[K4_WARPS][8];      // of each warp and head: what its weights are relative to (a power of two), and their sum
+  __shared__ int found[3], sums[K4_WARPS];
   using Stage = K4Stage<D>;
   using Page = Kv4Page<D>;
   constexpr int G = Page::G;      // groups of 32 dimensions
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
-  const int b = blockIdx.z, kvh = blockIdx.y / p.chunks, chunk = blockIdx.y % p.chunks, split = blockIdx.x;
-  const int heads = min(8, p.G - chunk * 8), head0 = kvh * p.G + chunk * 8;
+  const int all_heads = p.Hkv * p.chunks;
   pdl_sync();
 
-  int len = p.seq_lens[b];
-  const long long room = p.num_blocks ? static_cast<long long>(p.max_blocks) * p.block_size : 0;
-  if (len > room) {      // more tokens than the table has pages: recorded, the rest is left out
-    if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, RLB_ERR_BAD_ARG);
-    len = static_cast<int>(room);
+  // Which steps are this CTA's: those of one (sequence, heads), or an even share [x, x_end) of all of them in the order (heads, sequence, step).
+  int b, hc, at, left = 1;             // sequence, heads, step within the sequence, steps from there on
+  if (p.num_ctas) {
+    const int per = (p.B + K4_WARPS * 32 - 1) / (K4_WARPS * 32), b0 = min(p.B, static_cast<int>(threadIdx.x) * per), b1 = min(p.B, b0 + per);
+    int mine = 0;
+    for (int i = b0; i < b1; ++i) mine += k4_span(p, i).steps;
+    int upto = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += v;
+    }
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int w = 0; w < K4_WARPS; ++w) {
+      if (w < warp) upto += sums[w];
+      all += sums[w];
+    }
+    const long long total = static_cast<long long>(all) * all_heads, ctas = min(total, static_cast<long long>(p.num_ctas)), x = total * blockIdx.x / ctas;
+    left = blockIdx.x < ctas ? static_cast<int>(total * (blockIdx.x + 1) / ctas - x) : 0;      // (no CTA between two others is without a step: the parts stand in a row)
+    hc = static_cast<int>(x / all);
+    int rest = static_cast<int>(x - static_cast<long long>(hc) * all) - (upto - mine);
+    if (left && rest >= 0 && rest < mine) {      // (one thread)
+      int i = b0;
+      for (int n; (n = k4_span(p, i).steps) <= rest; ++i) rest -= n;
+      found[0] = i;
+      found[1] = rest;
+      found[2] = all;
+    }
+    __syncthreads();
+    if (!left) {
+      if (threadIdx.x == 0 && p.B * all_heads > p.num_ctas) p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
+      return;
+    }
+    b = found[0];
+    at = found[1];
+  } else {
+    b = blockIdx.y;
+    hc = blockIdx.x;
+    at = 0;
   }
-  len = max(len, 0);
-  const int first = p.window > 0 ? max(0, len - p.window) : 0;
-  const int step0 = first / K4_STEP, steps = len / K4_STEP + (len % K4_STEP != 0) - step0;
-  const int begin = step0 + static_cast<int>(static_cast<long long>(steps) * split / p.num_splits);
-  const int end = step0 + static_cast<int>(static_cast<long long>(steps) * (split + 1) / p.num_splits);
+  bool opened = false;      // whether a sequence begins here that goes on in the next CTA
+
+  for (;;) {
+  const int kvh = hc / p.chunks, chunk = hc - kvh * p.chunks, heads = min(8, p.G - chunk * 8), head0 = kvh * p.G + chunk * 8;
+  const K4Span span = k4_span(p, b);
+  const int len = span.len, first = span.first, begin = span.step0 + at;
+  const int count = p.num_ctas ? min(span.steps - at, left) : span.steps;
+  uint4 qv[G];
+  {
+    const __nv_bfloat16* q = p.q + static_cast<long long>(b) * p.q_stride + static_cast<long long>(head0 + r) * D + 8 * t;
+#pragma unroll
+    for (int g = 0; g < G; ++g) qv[g] = r < heads ? *reinterpret_cast<const uint4*>(q + 32 * g) : make_uint4(0, 0, 0, 0);
+  }
+  // The warp's steps are begin + warp + 4 i. Each lane knows the page of one half of a step (j = 2 i + half) among 16 of them, and of one among the 16 after.
+  const int* table = p.block_table + static_cast<long long>(b) * p.table_stride;
+  const int n = len && count > warp ? (count - warp + K4_WARPS - 1) / K4_WARPS : 0;
+  auto page_of = [&](int j, int& off) -> int {
+    const int pos0 = (begin + warp + (j >> 1) * K4_WARPS) * K4_STEP + (j & 1) * 16;
+    off = 0;
+    if (j >= 2 * n || pos0 >= len) return 0;
+    const int blk = pos0 / p.block_size;
+    off = pos0 - blk * p.block_size;
+    int no = table[blk];
+    if (no < 0 || no >= p.num_blocks) {      // outside the cache: recorded, and page 0 read in its place
+      if (p.status) atomicCAS(p.status, 0, RLB_ERR_BAD_ARG);
+      no = 0;
+    }
+    return no;
+  };
+  int off_now = 0, off_next = 0;
+  int page_now = page_of(lane, off_now), page_next = page_of(32 + lane, off_next);
+  const uint32_t fifo = smem_u32(k4_smem_raw) + warp * (K4_STAGES * Stage::BYTES);
+  const int tok = 4 * (r >> 1) + (r & 1);      // of 16; the thread's other row is two tokens later
+  const int key_at = Page::key_word(tok, t, 0), value_at = Page::values_at(p.block_size) + Page::value_unit(4 * t, r, 0), scale_at = Page::scales_at(p.block_size) + lane * 16;
+  const uint8_t* cache = p.cache + kvh * Page::bytes(p.block_size);
+  const long long page_stride = p.Hkv * Page::bytes(p.block_size);
+  auto request = [&](int i) {
+    if (i < n) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int src = (2 * i + h) & 31, off = __shfl_sync(0xffffffffu, off_now, src);
+        const uint8_t* page = cache + __shfl_sync(0xffffffffu, page_now, src) * page_stride;
+        const uint8_t *keys = page + (off * (D / 2) + key_at), *values = page + (off * (D / 2) + value_at);
+        const uint32_t to = fifo + (i % K4_STAGES) * Stage::BYTES + h * Stage::HALF;
+        copy_words<G>(to + Stage::KA + lane * (G * 4), keys);
+        copy_words<G>(to + Stage::KB + lane * (G * 4), keys + D);               // two tokens of keys
+        copy_words<G>(to + Stage::VA + lane * (G * 4), values);
+        copy_words<G>(to + Stage::VB + lane * (G * 4), values + D);             // one pair of tokens of values
+        if (lane < D / 8) copy_words<4>(to + Stage::SCALES + lane * 16, page + (off * (D / 8) + scale_at));
+      }
+      if ((i & 15) == 15) {
+        page_now = page_next;
+        off_now = off_next;
+        page_next = page_of(2 * i + 34 + lane, off_next);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < K4_STAGES - 1; ++i) request(i);
 
   // The queries as the 8-column operand: pair j of group g is (dimension 32 g + 8 t + j, and four later) of head r, times 2^k with the head's largest value
   // in [2^119, 2^120) (a sum of 32 stays finite), and 1/16 of that where the codes count 16 times. Scores are compared before they are scaled: a negative scale turns the
   // query's sign. c[h]: from the products' unit to powers of two, of heads 2 t and 2 t + 1.
   uint32_t qf[G][4];
-  float start[G][2], c[2], slack[2];      // start: -7.5 * sum of the group's values
+  float2 start[G];      // -7.5 * sum of the group's values, of heads 2 t and 2 t + 1: a product with a row of codes 15, halved
+  float c[2], slack[2];
   {
-    const __nv_bfloat16* q = p.q + static_cast<long long>(b) * p.q_stride + static_cast<long long>(head0 + r) * D + 8 * t;
-    uint4 v[G];
     uint32_t big = 0u;
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      v[g] = make_uint4(0, 0, 0, 0);
-      if (r < heads) v[g] = *reinterpret_cast<const uint4*>(q + 32 * g);
-      big = max(max(max(big, v[g].x & 0x7fffu), max(v[g].x >> 16 & 0x7fffu, v[g].y & 0x7fffu)), max(v[g].y >> 16 & 0x7fffu, v[g].z & 0x7fffu));
-      big = max(max(big, v[g].z >> 16 & 0x7fffu), max(v[g].w & 0x7fffu, v[g].w >> 16 & 0x7fffu));
-    }
+    for (int g = 0; g < G; ++g)
+      big = __vmaxu2(__vmaxu2(big, __vmaxu2(qv[g].x & 0x7fff7fffu, qv[g].y & 0x7fff7fffu)), __vmaxu2(qv[g].z & 0x7fff7fffu, qv[g].w & 0x7fff7fffu));
+    big = max(big & 0xffffu, big >> 16);
     big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
     big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
-    const int k = 119 + 127 - static_cast<int>(big >> 7);
-    const float sign = p.scale < 0.f ? -1.f : 1.f;
+    const int k = 119 + 127 - static_cast<int>(big >> 7);      // -9 to 246: in two factors, the second also with the sign, and with 1/16
+    const float half = pow2(k >> 1), rest = pow2(k - (k >> 1)) * (p.scale < 0.f ? -1.f : 1.f);
+    const uint32_t by = pack_bf16x2(half, half), by_even = pack_bf16x2(rest, rest), by_odd = pack_bf16x2(rest * 0.0625f, rest * 0.0625f);
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      const uint32_t w[4] = {v[g].x, v[g].y, v[g].z, v[g].w};
-      float f[8], s = 0.f;
+      const uint32_t w[4] = {__byte_perm(qv[g].x, qv[g].z, 0x5410), __byte_perm(qv[g].x, qv[g].z, 0x7632), __byte_perm(qv[g].y, qv[g].w, 0x5410), __byte_perm(qv[g].y, qv[g].w, 0x7632)};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 a = unpack_bf16x2(w[i]);
-        f[2 * i] = times_pow2(a.x * sign, k);
-        f[2 * i + 1] = times_pow2(a.y * sign, k);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s += f[j] + f[4 + j];
-        qf[g][j] = pack_bf16x2(f[j] * (j & 1 ? 0.0625f : 1.f), f[4 + j] * (j & 1 ? 0.0625f : 1.f));
-      }
-      s += __shfl_xor_sync(0xffffffffu, s, 1);
-      s += __shfl_xor_sync(0xffffffffu, s, 2);
-      s = times_pow2(s * -7.5f, -133);
-      start[g][0] = __shfl_sync(0xffffffffu, s, 8 * t);
-      start[g][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
+      for (int j = 0; j < 4; ++j) qf[g][j] = mul_bf16x2(mul_bf16x2(w[j], by), j & 1 ? by_odd : by_even);
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+      mma_bf16(acc, 0x000f000fu, 0x000f000fu, 0x00f000f0u, 0x00f000f0u, qf[g][0], qf[g][1]);
+      mma_bf16(acc, 0x000f000fu, 0x000f000fu, 0x00f000f0u, 0x00f000f0u, qf[g][2], qf[g][3]);
+      start[g] = make_float2(-0.5f * acc[0], -0.5f * acc[1]);
     }
     const float unit = fminf(fmaxf(times_pow2(fabsf(p.scale) * 1.4426950408889634f, 133 - k), 1e-30f), 1e30f);
     c[0] = __shfl_sync(0xffffffffu, unit, 8 * t);
@@ -201,95 +320,65 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 4 : 2) kv4_decode_ke
 #pragma unroll
   for (int g = 0; g < G; ++g) z[g][0] = z[g][1] = z[g][2] = z[g][3] = 0.f;
 
-  // The warp's steps are begin + warp + 4 i. Each lane knows the page of one of 32 of them, and of one of the 32 after.
-  const int* table = p.block_table + static_cast<long long>(b) * p.table_stride;
-  const int n = end - begin > warp ? (end - begin - warp + K4_WARPS - 1) / K4_WARPS : 0;
-  auto page_of = [&](int i, int& off) -> int {
-    if (i >= n) return 0;
-    const int pos0 = (begin + warp + i * K4_WARPS) * K4_STEP, blk = pos0 / p.block_size;
-    off = pos0 - blk * p.block_size;
-    int no = table[blk];
-    if (no < 0 || no >= p.num_blocks) {      // outside the cache: recorded, and page 0 read in its place
-      if (p.status) atomicCAS(p.status, 0, RLB_ERR_BAD_ARG);
-      no = 0;
-    }
-    return no;
-  };
-  int off_now = 0, off_next = 0;
-  int page_now = page_of(lane, off_now), page_next = page_of(32 + lane, off_next);
-  const uint32_t fifo = smem_u32(k4_smem_raw) + warp * (K4_STAGES * Stage::BYTES);
-  const int tok = 4 * (r >> 1) + (r & 1);      // of a step; the thread's other row is two tokens later
-  auto request = [&](int i) {
-    if (i < n) {
-      const int src = i & 31;
-      const int off = __shfl_sync(0xffffffffu, off_now, src);
-      const uint8_t* page = p.cache + (static_cast<long long>(__shfl_sync(0xffffffffu, page_now, src)) * p.Hkv + kvh) * Page::bytes(p.block_size);
-      const uint32_t to = fifo + (i % K4_STAGES) * Stage::BYTES;
-      const uint8_t* keys = page + Page::key_word(off + tok, t, 0);
-      const uint8_t* values = page + Page::values_at(p.block_size) + Page::value_unit(off + 4 * t, r, 0);
-      copy_words<G>(to + Stage::KA + lane * (G * 4), keys);
-      copy_words<G>(to + Stage::KB + lane * (G * 4), keys + D);               // two tokens of keys
-      copy_words<G>(to + Stage::VA + lane * (G * 4), values);
-      copy_words<G>(to + Stage::VB + lane * (G * 4), values + D);             // one pair of tokens of values
-      if (lane < D / 8) copy_words<4>(to + Stage::SCALES + lane * 16, page + Page::scales_at(p.block_size) + Page::scale(off, 0, 0) + lane * 16);
-      if (src == 31) {
-        page_now = page_next;
-        off_now = off_next;
-        page_next = page_of(i + 33 + lane, off_next);
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-#pragma unroll
-  for (int i = 0; i < K4_STAGES - 1; ++i) request(i);
-
   for (int i = 0; i < n; ++i) {
     asm volatile("cp.async.wait_group %0;" ::"n"(K4_STAGES - 2) : "memory");
     __syncwarp();      // the scales were copied by other lanes; and every lane has read the stage that is requested next
-    const uint32_t from = fifo + (i % K4_STAGES) * Stage::BYTES;
-    uint32_t ka[G], kb[G], va[G], vb[G], sa[G], sb[G];      // sa, sb: scales of keys, then of values
-    load_words(from + Stage::KA + lane * (G * 4), ka);
-    load_words(from + Stage::KB + lane * (G * 4), kb);
-    load_words(from + Stage::SCALES + Page::scale(tok, 0, 0), sa);
-    load_words(from + Stage::SCALES + Page::scale(tok + 2, 0, 0), sb);
-    load_words(from + Stage::VA + lane * (G * 4), va);
-    load_words(from + Stage::VB + lane * (G * 4), vb);
     request(i + K4_STAGES - 1);
-
-    const int pos0 = (begin + warp + i * K4_WARPS) * K4_STEP;
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    const uint32_t from = fifo + (i % K4_STAGES) * Stage::BYTES;
+    float s[2][4];
+    uint32_t va[2][G / 2], vb[2][G / 2];      // the values' scales
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      float acc[4] = {0.f, 0.f, 0.f, 0.f};
-      mma_bf16(acc, unpack2(ka[g], 0), unpack2(kb[g], 0), unpack2(ka[g], 1), unpack2(kb[g], 1), qf[g][0], qf[g][1]);
-      mma_bf16(acc, unpack2(ka[g], 2), unpack2(kb[g], 2), unpack2(ka[g], 3), unpack2(kb[g], 3), qf[g][2], qf[g][3]);
-      const float fa = bf16_of(sa[g >> 1], g), fb = bf16_of(sb[g >> 1], g);
-      s[0] = fmaf(acc[0] + start[g][0], fa, s[0]);
-      s[1] = fmaf(acc[1] + start[g][1], fa, s[1]);
-      s[2] = fmaf(acc[2] + start[g][0], fb, s[2]);
-      s[3] = fmaf(acc[3] + start[g][1], fb, s[3]);
+    for (int h = 0; h < 2; ++h) {
+      uint32_t ka[G], kb[G], sa[G], sb[G];
+      load_words(from + h * Stage::HALF + Stage::KA + lane * (G * 4), ka);
+      load_words(from + h * Stage::HALF + Stage::KB + lane * (G * 4), kb);
+      load_words(from + h * Stage::HALF + Stage::SCALES + Page::scale(tok, 0, 0), sa);
+      load_words(from + h * Stage::HALF + Stage::SCALES + Page::scale(tok + 2, 0, 0), sb);
+      float2 lo = make_float2(0.f, 0.f), hi = lo;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        mma_bf16(acc, unpack2(ka[g], 0), unpack2(kb[g], 0), unpack2(ka[g], 1), unpack2(kb[g], 1), qf[g][0], qf[g][1]);
+        mma_bf16(acc, unpack2(ka[g], 2), unpack2(kb[g], 2), unpack2(ka[g], 3), unpack2(kb[g], 3), qf[g][2], qf[g][3]);
+        const float fa = bf16_of(sa[g >> 1], g), fb = bf16_of(sb[g >> 1], g);
+        lo = fma2(add2(make_float2(acc[0], acc[1]), start[g]), make_float2(fa, fa), lo);
+        hi = fma2(add2(make_float2(acc[2], acc[3]), start[g]), make_float2(fb, fb), hi);
+      }
+      s[h][0] = lo.x; s[h][1] = lo.y; s[h][2] = hi.x; s[h][3] = hi.y;
+#pragma unroll
+      for (int g = 0; g < G / 2; ++g) {
+        va[h][g] = sa[G / 2 + g];
+        vb[h][g] = sb[G / 2 + g];
+      }
     }
-    const bool edge = pos0 < first || pos0 + K4_STEP > len;
-    const bool live_a = pos0 + tok >= first && pos0 + tok < len, live_b = pos0 + tok + 2 >= first && pos0 + tok + 2 < len;
-    if (edge) {      // (a place that was never written, or by another sequence, may hold anything)
-      if (!live_a) s[0] = s[1] = -INFINITY;
-      if (!live_b) s[2] = s[3] = -INFINITY;
+    const int pos0 = (begin + warp + i * K4_WARPS) * K4_STEP;
+    if (pos0 < first || pos0 + K4_STEP > len) {      // (a place that was never written, or by another sequence, may hold anything)
 #pragma unroll
-      for (int g = G / 2; g < G; ++g) {      // (the values' scales)
-        if (!live_a) sa[g] = 0u;
-        if (!live_b) sb[g] = 0u;
+      for (int h = 0; h < 2; ++h) {
+        const int at = pos0 + 16 * h + tok;
+        if (at < first || at >= len) {
+          s[h][0] = s[h][1] = -INFINITY;
+#pragma unroll
+          for (int g = 0; g < G / 2; ++g) va[h][g] = 0u;
+        }
+        if (at + 2 < first || at + 2 >= len) {
+          s[h][2] = s[h][3] = -INFINITY;
+#pragma unroll
+          for (int g = 0; g < G / 2; ++g) vb[h][g] = 0u;
+        }
       }
     }
     // The running maximum moves only when a score passes it by K4_SLACK: weights are then at most 2^8, and any reference gives the same quotient.
+    const float m0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2])), m1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]));
     uint32_t widest = limit;
 #pragma unroll
-    for (int g = G / 2; g < G; ++g) widest = __vmaxu2(widest, __vmaxu2(sa[g], sb[g]));
-    if (__any_sync(0xffffffffu, fmaxf(s[0], s[2]) > top[0] + slack[0] || fmaxf(s[1], s[3]) > top[1] + slack[1] || widest != limit)) {
+    for (int g = 0; g < G / 2; ++g) widest = __vmaxu2(__vmaxu2(widest, __vmaxu2(va[0][g], vb[0][g])), __vmaxu2(va[1][g], vb[1][g]));
+    if (__any_sync(0xffffffffu, m0 > top[0] + slack[0] || m1 > top[1] + slack[1] || widest != limit)) {
       float f[2] = {1.f, 1.f};
       uint32_t wide = 0u;      // the largest finite scale
 #pragma unroll
-      for (int g = G / 2; g < G; ++g) {
-        const uint32_t w[4] = {sa[g] & 0xffffu, sa[g] >> 16, sb[g] & 0xffffu, sb[g] >> 16};
+      for (int g = 0; g < G; ++g) {
+        const uint32_t w[4] = {va[g & 1][g >> 1] & 0xffffu, va[g & 1][g >> 1] >> 16, vb[g & 1][g >> 1] & 0xffffu, vb[g & 1][g >> 1] >> 16};
 #pragma unroll
         for (int j = 0; j < 4; ++j) wide = max(wide, w[j] < 0x7f80u ? w[j] : 0u);
       }
@@ -304,7 +393,7 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 4 : 2) kv4_decode_ke
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float m = fmaxf(s[h], s[h + 2]);
+        float m = h ? m1 : m0;
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
@@ -326,89 +415,167 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 4 : 2) kv4_decode_ke
       }
     }
     const float ref0 = top[0] == -INFINITY ? 0.f : fmaf(-top[0], c[0], lift), ref1 = top[1] == -INFINITY ? 0.f : fmaf(-top[1], c[1], lift);
-    const float p0 = exp2_fast(fmaf(s[0], c[0], ref0)), p1 = exp2_fast(fmaf(s[1], c[1], ref1)), p2 = exp2_fast(fmaf(s[2], c[0], ref0)), p3 = exp2_fast(fmaf(s[3], c[1], ref1));
-    sum[0] += p0 + p2;
-    sum[1] += p1 + p3;
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const float fa = bf16_of(sa[(G + g) >> 1], G + g), fb = bf16_of(sb[(G + g) >> 1], G + g);
-      // weight * scale in 32 bits, rounded once to the operand's bf16: half a step, 2^-8 of each token's share at most, with either sign
-      const uint32_t w0 = transposed8x8(pack_bf16x2(p0 * fa, p1 * fa)), w1 = transposed8x8(pack_bf16x2(p2 * fb, p3 * fb));
-      mma_bf16(o[2 * g], unpack2(va[g], 0), unpack2(va[g], 1), unpack2(vb[g], 0), unpack2(vb[g], 1), w0, w1);
-      mma_bf16(o[2 * g + 1], unpack2(va[g], 2), unpack2(va[g], 3), unpack2(vb[g], 2), unpack2(vb[g], 3), w0, w1);
-      mma_bf16(z[g], 0x000f000fu, 0x000f000fu, 0x000f000fu, 0x000f000fu, w0, w1);
+    for (int h = 0; h < 2; ++h) {
+      uint32_t wa[G], wb[G];
+      load_words(from + h * Stage::HALF + Stage::VA + lane * (G * 4), wa);
+      load_words(from + h * Stage::HALF + Stage::VB + lane * (G * 4), wb);
+      const float2 pa = make_float2(exp2_fast(fmaf(s[h][0], c[0], ref0)), exp2_fast(fmaf(s[h][1], c[1], ref1)));
+      const float2 pb = make_float2(exp2_fast(fmaf(s[h][2], c[0], ref0)), exp2_fast(fmaf(s[h][3], c[1], ref1)));
+      sum[0] += pa.x + pb.x;
+      sum[1] += pa.y + pb.y;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float fa = bf16_of(va[h][g >> 1], g), fb = bf16_of(vb[h][g >> 1], g);
+        // weight * scale in 32 bits, rounded once to the operand's bf16: half a step, 2^-8 of each token's share at most, with either sign
+        const uint32_t w0 = transposed8x8(pack_bf16x2(pa.x * fa, pa.y * fa)), w1 = transposed8x8(pack_bf16x2(pb.x * fb, pb.y * fb));
+        mma_bf16(o[2 * g], unpack2(wa[g], 0), unpack2(wa[g], 1), unpack2(wb[g], 0), unpack2(wb[g], 1), w0, w1);
+        mma_bf16(o[2 * g + 1], unpack2(wa[g], 2), unpack2(wa[g], 3), unpack2(wb[g], 2), unpack2(wb[g], 3), w0, w1);
+        mma_bf16(z[g], 0x000f000fu, 0x000f000fu, 0x000f000fu, 0x000f000fu, w0, w1);
+      }
     }
     // The offset is taken off again and again: left until the end it would outgrow the sums, which are to keep their last bits.
     if (i % K4_FOLD == K4_FOLD - 1) fold(o, z);
   }
   fold(o, z);
 
-  // the warps' parts: heads 2 t and 2 t + 1, dimensions 32 g + 4 r .. + 3
-  __syncthreads();      // the FIFOs' memory is used again
-  float* k4_red = reinterpret_cast<float*>(k4_smem_raw);
-  float* red_ml = k4_red + K4_WARPS * 8 * D;
+  // The warps' parts are brought to one reference and added: heads 2 t and 2 t + 1, dimensions 32 g + 4 r .. + 3 of each lane.
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    float l = sum[h];
-    l += __shfl_xor_sync(0xffffffffu, l, 4);
-    l += __shfl_xor_sync(0xffffffffu, l, 8);
-    l += __shfl_xor_sync(0xffffffffu, l, 16);
+    sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 4);
+    sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 8);
+    sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 16);
+    top[h] = top[h] == -INFINITY ? -INFINITY : fmaf(top[h], c[h], -lift);
+    if (r == 0) ml[warp][2 * t + h] = make_float2(top[h], sum[h]);
+  }
+  __syncthreads();      // (the stages' memory is used again, too)
+  float* red = reinterpret_cast<float*>(k4_smem_raw);
+  constexpr int ROW = D + 4;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
     const int head = 2 * t + h;
-    if (r == 0) {
-      red_ml[(warp * 8 + head) * 2] = top[h] == -INFINITY ? -INFINITY : fmaf(top[h], c[h], -lift);      // what the weights are relative to
-      red_ml[(warp * 8 + head) * 2 + 1] = l;
-    }
+    float m = ml[0][head].x;
+#pragma unroll
+    for (int w = 1; w < K4_WARPS; ++w) m = fmaxf(m, ml[w][head].x);
+    // (a part without a finite score has no tokens, or NaN, which is to stay)
+    const float f = top[h] == -INFINITY ? 1.f : exp2_fast(top[h] - m), f0 = f * 0x1p67f, f1 = f * 0x1p63f;
 #pragma unroll
     for (int g = 0; g < G; ++g)
-      *reinterpret_cast<float4*>(k4_red + (warp * 8 + head) * D + 32 * g + 4 * r) =
-          make_float4(times_pow2(o[2 * g][h], 133), times_pow2(o[2 * g][h + 2], 129), times_pow2(o[2 * g + 1][h], 133), times_pow2(o[2 * g + 1][h + 2], 129));
+      *reinterpret_cast<float4*>(red + (warp * 8 + head) * ROW + 32 * g + 4 * r) =
+          make_float4(o[2 * g][h] * 0x1p66f * f0, o[2 * g][h + 2] * 0x1p66f * f1, o[2 * g + 1][h] * 0x1p66f * f0, o[2 * g + 1][h + 2] * 0x1p66f * f1);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < heads * D; i += blockDim.x) {
-    const int head = i / D, d = i - head * D;
-    float m = -INFINITY;
+  for (int i = threadIdx.x; i < heads * (D / 4); i += K4_WARPS * 32) {
+    const int head = i / (D / 4), d = i % (D / 4) * 4;
+    float m = ml[0][head].x, l = 0.f;
 #pragma unroll
-    for (int w = 0; w < K4_WARPS; ++w) m = fmaxf(m, red_ml[(w * 8 + head) * 2]);
-    float l = 0.f, acc = 0.f;
+    for (int w = 1; w < K4_WARPS; ++w) m = fmaxf(m, ml[w][head].x);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < K4_WARPS; ++w) {
-      const float mw = red_ml[(w * 8 + head) * 2], f = mw == -INFINITY ? 0.f : exp2_fast(mw - m);
-      const float lw = red_ml[(w * 8 + head) * 2 + 1], ow = k4_red[(w * 8 + head) * D + d];
-      l += mw == -INFINITY ? lw : lw * f;      // (a part without a finite score: no tokens, or NaN)
-      acc += mw == -INFINITY ? ow : ow * f;
+      const float2 part = ml[w][head];
+      l += part.y * (part.x == -INFINITY ? 1.f : exp2_fast(part.x - m));
+      const float4 v = *reinterpret_cast<const float4*>(red + (w * 8 + head) * ROW + d);
+      acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
     }
-    if (p.num_splits == 1) {
-      p.out[static_cast<long long>(b) * p.out_stride + static_cast<long long>(head0 + head) * D + d] = __float2bfloat16_rn(l == 0.f ? 0.f : acc / l);
-    } else {
-      const long long at = (static_cast<long long>(b) * p.Hkv * p.G + head0 + head) * p.num_splits + split;
-      p.part_o[at * D + d] = acc;
-      if (d == 0) {
-        p.part_ml[at * 2] = m;
-        p.part_ml[at * 2 + 1] = l;
-      }
+    if (count == span.steps) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      *reinterpret_cast<uint2*>(p.out + static_cast<long long>(b) * p.out_stride + static_cast<long long>(head0 + head) * D + d) =
+          make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+    } else {      // a part: of a sequence that began in an earlier CTA, or of one that begins here
+      const long long part = static_cast<long long>(blockIdx.x) * 2 + (at == 0);
+      *reinterpret_cast<float4*>(p.part_o + (part * 8 + head) * D + d) = acc;
+      if (d == 0) p.part_ml[part * 8 + head] = make_float2(m, l);
     }
   }
+  if (!p.num_ctas) return;
+  // A sequence that begins here is joined from this CTA's part and those of the CTAs up to the one that has its last step.
+  if (at == 0) {
+    int4 job = make_int4(-1, 0, 0, 0);
+    if (count < span.steps) {
+      opened = true;
+      const long long total = static_cast<long long>(found[2]) * all_heads, ctas = min(total, static_cast<long long>(p.num_ctas));
+      const long long past = total * (blockIdx.x + 1) / ctas - count + span.steps;
+      job = make_int4(static_cast<int>(blockIdx.x), static_cast<int>((past * ctas - 1) / total), b, hc);
+    }
+    if (threadIdx.x == 0) {
+      if (p.B * all_heads <= p.num_ctas) p.joins[hc * p.B + b] = job;
+      else if (opened) p.joins[blockIdx.x] = job;
+    }
+  }
+  left -= count;
+  if (!left) break;
+  at = 0;
+  if (++b == p.B) {
+    b = 0;
+    ++hc;
+  }
+  __syncthreads();      // the sums' memory becomes the stages' again
+  }
+  if (threadIdx.x == 0 && !opened && p.B * all_heads > p.num_ctas) p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
 }
 
-// Joins the splits: one CTA per (sequence, query head), a thread per dimension.
+// Joins the parts of the sequences that several CTAs shared: a CTA per possible one, a warp per head and fourth part.
 template <int D>
-__global__ void __launch_bounds__(D) kv4_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, __nv_bfloat16* __restrict__ out, long long out_stride, int Hq,
-                                                     int num_splits) {
+__global__ void __launch_bounds__(1024) kv4_join_kernel(const K4Params p) {
+  __shared__ float4 red[3][8][D / 4];
+  __shared__ float reds[4][8];
   pdl_sync();
-  const long long at = (static_cast<long long>(blockIdx.y) * Hq + blockIdx.x) * num_splits;
+  const int4 job = p.joins[blockIdx.x];      // first and last CTA, sequence, heads
+  if (job.x < 0) return;
+  const int head = threadIdx.x >> 5 & 7, quarter = threadIdx.x >> 8, lane = threadIdx.x & 31, n = job.y - job.x + 1;
+  auto part = [&](int i) { return (static_cast<long long>(job.x + i) * 2 + (i == 0)) * 8 + head; };
   float m = -INFINITY;
-  for (int i = 0; i < num_splits; ++i) m = fmaxf(m, part_ml[(at + i) * 2]);
-  float l = 0.f, acc = 0.f;
-  for (int i = 0; i < num_splits; ++i) {
-    const float mi = part_ml[(at + i) * 2], f = mi == -INFINITY ? 1.f : exp2_fast(mi - m);
-    l += part_ml[(at + i) * 2 + 1] * f;
-    acc += part_o[(at + i) * D + threadIdx.x] * f;
+  for (int i = lane; i < n; i += 32) m = fmaxf(m, p.part_ml[part(i)].x);
+  m = warp_max(m);
+  constexpr int V = D / 128 > 0 ? D / 128 : 1;
+  float4 acc[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+#pragma unroll 4
+  for (int i = quarter; i < n; i += 4) {
+    const long long at = part(i);
+    const float2 w = p.part_ml[at];
+    const float f = w.x == -INFINITY ? 1.f : exp2_fast(w.x - m);      // (a part without a finite score has no tokens, or NaN)
+    l += w.y * f;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (lane + 32 * v < D / 4) {
+        const float4 o = reinterpret_cast<const float4*>(p.part_o + at * D)[lane + 32 * v];
+        acc[v].x = fmaf(o.x, f, acc[v].x);
+        acc[v].y = fmaf(o.y, f, acc[v].y);
+        acc[v].z = fmaf(o.z, f, acc[v].z);
+        acc[v].w = fmaf(o.w, f, acc[v].w);
+      }
   }
-  out[blockIdx.y * out_stride + static_cast<long long>(blockIdx.x) * D + threadIdx.x] = __float2bfloat16_rn(l == 0.f ? 0.f : acc / l);
+  if (lane == 0) reds[quarter][head] = l;
+  if (quarter) {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (lane + 32 * v < D / 4) red[quarter - 1][head][lane + 32 * v] = acc[v];
+  }
+  __syncthreads();
+  const int kvh = job.w / p.chunks, chunk = job.w - kvh * p.chunks;
+  if (quarter || head >= min(8, p.G - chunk * 8)) return;
+  l = (reds[0][head] + reds[1][head]) + (reds[2][head] + reds[3][head]);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  __nv_bfloat16* out = p.out + job.z * p.out_stride + static_cast<long long>(kvh * p.G + chunk * 8 + head) * D;
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    if (lane + 32 * v < D / 4) {
+      float4 o = acc[v];
+#pragma unroll
+      for (int q = 0; q < 3; ++q) {
+        const float4 w = red[q][head][lane + 32 * v];
+        o.x += w.x; o.y += w.y; o.z += w.z; o.w += w.w;
+      }
+      reinterpret_cast<uint2*>(out)[lane + 32 * v] = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+    }
 }
 
 template <int D>
-int launch_decode(const K4Params& p, int B, cudaStream_t stream) {
+int launch_decode(const K4Params& p, cudaStream_t stream) {
   static std::atomic<unsigned long long> ready{0};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -418,26 +585,32 @@ int launch_decode(const K4Params& p, int B, cudaStream_t stream) {
     if (e != cudaSuccess) return static_cast<int>(e);
     ready.fetch_or(1ull << (dev & 63));
   }
-  rlb_launch_pdl(kv4_decode_kernel<D>, dim3(p.num_splits, p.Hkv * p.chunks, B), dim3(K4_WARPS * 32), k4_smem<D>(), stream, p);
+  const int all_heads = p.Hkv * p.chunks;
+  const dim3 grid = p.num_ctas ? dim3(p.num_ctas) : dim3(all_heads, p.B);
+  rlb_launch_pdl(kv4_decode_kernel<D>, grid, dim3(K4_WARPS * 32), k4_smem<D>(), stream, p);
   e = cudaGetLastError();
-  if (e != cudaSuccess || p.num_splits == 1) return static_cast<int>(e);
-  rlb_launch_pdl(kv4_join_kernel<D>, dim3(p.Hkv * p.G, B), dim3(D), 0, stream, p.part_o, p.part_ml, p.out, p.out_stride, p.Hkv * p.G, p.num_splits);
+  if (e != cudaSuccess || !p.num_ctas) return static_cast<int>(e);
+  const long long segments = static_cast<long long>(p.B) * all_heads;
+  rlb_launch_pdl(kv4_join_kernel<D>, dim3(static_cast<unsigned>(segments < p.num_ctas ? segments : p.num_ctas)), dim3(1024), 0, stream, p);
   return static_cast<int>(cudaGetLastError());
 }
 }  // namespace
 
-// q [B, >= Hq D] bf16, 16-byte aligned rows; block_table [B, max_blocks] int32; seq_lens [B]; part_o [B Hq splits D] and part_ml [B Hq splits 2] fp32 with more than one split.
+// q [B, >= Hq D] bf16, 16-byte aligned rows; block_table [B, max_blocks] int32; seq_lens [B]; out: 8-byte aligned rows. num_ctas: 0, or CTAs that share all
+// tokens evenly, with scratch part_o [num_ctas 16 D] and part_ml [num_ctas 36] fp32 (16-byte aligned).
 RLB_API int rlb_kv4_paged_decode(const void* q, long long q_stride, const void* cache, long long num_blocks, const int* block_table, long long table_stride, int max_blocks,
-                                 const int* seq_lens, int B, int Hq, int Hkv, int D, int block_size, int window, float scale, int num_splits, float* part_o, float* part_ml, void* out,
+                                 const int* seq_lens, int B, int Hq, int Hkv, int D, int block_size, int window, float scale, int num_ctas, float* part_o, float* part_ml, void* out,
                                  long long out_stride, int* status, void* stream) {
   if ((D != 64 && D != 128 && D != 256) || Hkv < 1 || Hq < 1 || Hq % Hkv || block_size < 16 || block_size % 16 || block_size > KV4_MAX_BLOCK || window < 0) return -2;
   if (q_stride % 8 || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache)) & 15)) return -2;
+  if (out_stride % 4 || (reinterpret_cast<uintptr_t>(out) & 7)) return -2;
   if (B <= 0) return 0;
-  if (num_splits < 1 || (num_splits > 1 && (!part_o || !part_ml))) return -3;
   const int group = Hq / Hkv, chunks = (group + 7) / 8;
-  if (B > 65535 || Hkv * chunks > 65535 || (num_splits > 1 && B > 65535)) return -4;
+  if (num_ctas < 0 || (num_ctas && (!part_o || !part_ml || ((reinterpret_cast<uintptr_t>(part_o) | reinterpret_cast<uintptr_t>(part_ml)) & 15)))) return -3;
+  if ((!num_ctas && B > 65535) || B * (static_cast<long long>(max_blocks) * block_size / K4_STEP + 1) > 0x7fffffffll || static_cast<long long>(B) * Hkv * chunks > 0x7fffffffll) return -4;
   const K4Params p{static_cast<const __nv_bfloat16*>(q), q_stride, static_cast<const uint8_t*>(cache), num_blocks, block_table, table_stride, max_blocks, seq_lens, Hkv, group, chunks,
-                   block_size, window, scale, num_splits, part_o, part_ml, static_cast<__nv_bfloat16*>(out), out_stride, status};
+                   block_size, window, scale, B, num_ctas, part_o, reinterpret_cast<float2*>(part_ml), reinterpret_cast<int4*>(part_ml + static_cast<long long>(num_ctas) * 32),
+                   static_cast<__nv_bfloat16*>(out), out_stride, status};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return D == 64 ? launch_decode<64>(p, B, s) : D == 128 ? launch_decode<128>(p, B, s) : launch_decode<256>(p, B, s);
+  return D == 64 ? launch_decode<64>(p, s) : D == 128 ? launch_decode<128>(p, s) : launch_decode<256>(p, s);
 }

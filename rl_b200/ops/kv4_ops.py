@@ -221,30 +221,33 @@ def kv4_cache_read(cache: torch.Tensor, slots: torch.Tensor, Hkv: int, D: int, *
     return out
 
 
-def kv4_splits(B: int, Hq: int, Hkv: int, max_len: int, sm_count: int = 148) -> int:
-    """KV splits of decode attention over the 4-bit cache: as many CTAs as the device holds at a time, no split of less than 256 tokens."""
-    ctas = max(1, B) * Hkv * -(-(Hq // Hkv) // 8)
-    return int(max(1, min(4 * sm_count // ctas, max_len // 256, 128)))
+def kv4_ctas(B: int, Hq: int, Hkv: int, D: int, max_len: int, sm_count: int = 148) -> int:
+    """CTAs that share the tokens of decode attention over the 4-bit cache evenly: as many as the device holds at a time, none with less than 256 tokens.
+    0: one per sequence and heads, without a second kernel that joins parts, where sequences have no more than that."""
+    if max_len <= 256:
+        return 0
+    work = max(1, B) * Hkv * -(-(Hq // Hkv) // 8) * (-(-max_len // 256))
+    return min((3 if D <= 128 else 2) * sm_count, work)
 
 
-def kv4_scratch_sizes(B: int, Hq: int, num_splits: int, D: int) -> tuple[int, int]:
-    """Floats of the two scratch tensors of :func:`kv4_paged_decode` with this many splits."""
-    return B * Hq * num_splits * D, B * Hq * num_splits * 2
+def kv4_scratch_sizes(num_ctas: int, D: int) -> tuple[int, int]:
+    """Floats of the two scratch tensors of :func:`kv4_paged_decode` with this many CTAs."""
+    return num_ctas * 16 * D, num_ctas * 36
 
 
 def kv4_paged_decode(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, Hq: int, Hkv: int, D: int, *,
-                     scale: Optional[float] = None, window: int = 0, num_splits: int = 0,
+                     scale: Optional[float] = None, window: int = 0, num_ctas: Optional[int] = None,
                      scratch: Optional[tuple[torch.Tensor, torch.Tensor]] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of one query token per sequence, ``q`` [B, >= Hq D] (rows may be strided: the fused rows do), against the 4-bit ``cache``:
     ``seq_lens`` [B] int32 tokens in the pages that ``block_table`` [B, pages] int32 names, of which ``window`` > 0 leaves the last ``window``. A
-    sequence without tokens gives zeros. ``num_splits``: parts that a sequence's tokens are cut into (0: by :func:`kv4_splits` from the table's width);
-    ``scratch``: fp32 tensors of :func:`kv4_scratch_sizes` elements, for callers that keep their own. Returns [B, Hq D]."""
+    sequence without tokens gives zeros. ``num_ctas``: CTAs that share the work evenly, 0: one per sequence and heads (None: by :func:`kv4_ctas` from the
+    table's width); ``scratch``: fp32 tensors of :func:`kv4_scratch_sizes` elements, for callers that keep their own. Returns [B, Hq D]."""
     block = _block_size(cache, Hkv, D)
     device, width = q.device, Hq * D
     if Hq < 1 or Hq % Hkv or q.dim() != 2 or q.shape[1] < width:
         raise ValueError(f"q is [B, {width}] with {Hq} heads, a multiple of {Hkv}, not {tuple(q.shape)}")
-    if window < 0 or num_splits < 0:
-        raise ValueError(f"window {window} and num_splits {num_splits} are not negative")
+    if window < 0 or (num_ctas or 0) < 0:
+        raise ValueError(f"window {window} or num_ctas {num_ctas} is negative")
     B = q.shape[0]
     _same_device(device, cache, block_table, seq_lens)
     if block_table.dim() != 2:
@@ -279,22 +282,23 @@ def kv4_paged_decode(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
     stream = torch.cuda.current_stream()
     if stream.device_index != device.index:
         with torch.cuda.device(device):
-            return kv4_paged_decode(q, cache, table, lens, Hq, Hkv, D, scale=scale, window=window, num_splits=num_splits, scratch=scratch, out=out)
+            return kv4_paged_decode(q, cache, table, lens, Hq, Hkv, D, scale=scale, window=window, num_ctas=num_ctas, scratch=scratch, out=out)
     if not _aligned(q):      # rows that do not start on 16 bytes
         q = q[:, :width].clone(memory_format=torch.contiguous_format)
-    num_splits = num_splits or kv4_splits(B, Hq, Hkv, min(pages * block, window) if window else pages * block)
+    if num_ctas is None:
+        num_ctas = kv4_ctas(B, Hq, Hkv, D, min(pages * block, window) if window else pages * block)
     po = pml = None
-    if num_splits > 1:
-        no, nml = kv4_scratch_sizes(B, Hq, num_splits, D)
+    if num_ctas:
+        no, nml = kv4_scratch_sizes(num_ctas, D)
         if scratch is None:
             scratch = torch.empty(no, dtype=torch.float32, device=device), torch.empty(nml, dtype=torch.float32, device=device)
         po, pml = scratch
         _same_device(device, po, pml)
-        if any(t.dtype is not torch.float32 or not t.is_contiguous() or t.numel() < size for t, size in ((po, no), (pml, nml))):
-            raise ValueError(f"scratch is two contiguous float32 tensors of {no} and {nml} elements")
-    to = out if out.stride(1) == 1 else torch.empty((B, width), dtype=BF16, device=device)
+        if any(t.dtype is not torch.float32 or not t.is_contiguous() or t.numel() < size or t.data_ptr() % 16 for t, size in ((po, no), (pml, nml))):
+            raise ValueError(f"scratch is two contiguous float32 tensors of {no} and {nml} elements that start on 16 bytes")
+    to = out if out.stride(1) == 1 and out.stride(0) % 4 == 0 and out.data_ptr() % 8 == 0 else torch.empty((B, width), dtype=BF16, device=device)
     call("rlb_kv4_paged_decode", ptr(q), q.stride(0), ptr(cache), cache.shape[0], ptr(table), table.stride(0), pages, ptr(lens), B, Hq, Hkv, D, block, window, scale,
-         num_splits, ptr(po), ptr(pml), ptr(to), to.stride(0), ptr(_L.status_word(device)), stream.cuda_stream)
+         num_ctas, ptr(po), ptr(pml), ptr(to), to.stride(0), ptr(_L.status_word(device)), stream.cuda_stream)
     if to is not out:
         out.copy_(to)
     return out

@@ -156,6 +156,7 @@ def test_refusals():
         lambda: K.kv4_paged_decode(x, cache, bt, ln[:0], 4, 2, 64),
         lambda: K.kv4_paged_decode(x, cache, bt.float(), ln, 4, 2, 64),
         lambda: K.kv4_paged_decode(x, cache, bt, ln, 4, 2, 64, window=-1),
+        lambda: K.kv4_paged_decode(x, cache, bt, ln, 4, 2, 64, num_ctas=-1),
         lambda: K.kv4_paged_decode(x, cache, bt, ln, 4, 2, 64, out=torch.zeros(1, 256)),
         lambda: K.kv4_paged_decode(x, cache, bt, ln, 4, 2, 64, out=torch.zeros(2, 256).bfloat16()),
     ]
@@ -166,8 +167,7 @@ def test_refusals():
     assert not cache.any()
 
 
-def test_splits():
-    assert K.kv4_splits(1, 32, 8, 100) == 1 and K.kv4_splits(0, 32, 8, 100) == 1
-    for B, Hq, Hkv, n in ((1, 32, 8, 131072), (1, 8, 1, 10**6), (64, 32, 8, 4096), (512, 32, 8, 8192)):
-        s = K.kv4_splits(B, Hq, Hkv, n)
-        assert 1 <= s <= 128 and (s == 1 or n // s >= 256)
+def test_ctas():
+    assert K.kv4_ctas(64, 32, 8, 128, 256) == 0 and K.kv4_ctas(0, 32, 8, 128, 0) == 0
+    assert K.kv4_ctas(1, 8, 1, 128, 257) == 2 and K.kv4_ctas(1, 16, 1, 128, 257) == 4
+    assert K.kv4_ctas(512, 32, 8, 128, 8192) == 3 * 148 and K.kv4_ctas(512, 32, 8, 256, 8192) == 2 * 148
