@@ -65,13 +65,18 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }      // e from -126 to 127
 // Codes at nibble j of both halves of a word as two bf16 numbers: code * 2^-133 for even j, code * 2^-129 for odd j.
 __device__ __forceinline__ uint32_t unpack2(uint32_t w, int j) { return (j & 2 ? w >> 8 : w) & (j & 1 ? 0x00f000f0u : 0x000f000fu); }
-__device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }      // e from -126 to 127
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
+}
+// 16 tokens' products of a group of 32 dimensions: wa, wb are the thread's words of its two tokens, q its pairs of the query.
+__device__ __forceinline__ void score_group(float (&acc)[4], uint32_t wa, uint32_t wb, const uint32_t (&q)[4]) {
+  mma_bf16(acc, unpack2(wa, 0), unpack2(wb, 0), unpack2(wa, 1), unpack2(wb, 1), q[0], q[1]);
+  mma_bf16(acc, unpack2(wa, 2), unpack2(wb, 2), unpack2(wa, 3), unpack2(wb, 3), q[2], q[3]);
 }
 // Two sums or products at once.
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
@@ -160,14 +165,15 @@ __device__ __forceinline__ K4Span k4_span(const K4Params& p, int b) {
   return s;
 }
 
-template <int D>
+template <int D, bool PAIR>
 __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_kernel(const K4Params p) {
   extern __shared__ __align__(128) uint8_t k4_smem_raw[];
-  __shared__ float2 ml[K4_WARPS][8];      // of each warp and head: what its weights are relative to (a power of two), and their sum
+  __shared__ float2 ml[K4_WARPS][8];      // of each warp and column: what its weights are relative to (a power of two), and their sum
   __shared__ int found[3], sums[K4_WARPS];
   using Stage = K4Stage<D>;
   using Page = Kv4Page<D>;
-  constexpr int G = Page::G;      // groups of 32 dimensions
+  constexpr int G = Page::G, W = G < 4 ? G : 4;      // groups of 32 dimensions; words of a load
+  constexpr int NS = PAIR ? 1 : 2;                   // times 16 tokens of a step that a column stands for
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
   const int all_heads = p.Hkv * p.chunks;
   pdl_sync();
@@ -219,14 +225,15 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
 
   for (;;) {
   const int kvh = hc / p.chunks, chunk = hc - kvh * p.chunks, heads = min(8, p.G - chunk * 8), head0 = kvh * p.G + chunk * 8;
+  const int col_head = PAIR ? r & 3 : r;      // the query head of column r
   const K4Span span = k4_span(p, b);
   const int len = span.len, first = span.first, begin = span.step0 + at;
   const int count = p.num_ctas ? min(span.steps - at, left) : span.steps;
   uint4 qv[G];
   {
-    const __nv_bfloat16* q = p.q + static_cast<long long>(b) * p.q_stride + static_cast<long long>(head0 + r) * D + 8 * t;
+    const __nv_bfloat16* q = p.q + static_cast<long long>(b) * p.q_stride + static_cast<long long>(head0 + col_head) * D + 8 * t;
 #pragma unroll
-    for (int g = 0; g < G; ++g) qv[g] = r < heads ? *reinterpret_cast<const uint4*>(q + 32 * g) : make_uint4(0, 0, 0, 0);
+    for (int g = 0; g < G; ++g) qv[g] = col_head < heads ? *reinterpret_cast<const uint4*>(q + 32 * g) : make_uint4(0, 0, 0, 0);
   }
   // The warp's steps are begin + warp + 4 i. Each lane knows the page of one half of a step (j = 2 i + half) among 16 of them, and of one among the 16 after.
   const int* table = p.block_table + static_cast<long long>(b) * p.table_stride;
@@ -276,11 +283,11 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
 #pragma unroll
   for (int i = 0; i < K4_STAGES - 1; ++i) request(i);
 
-  // The queries as the 8-column operand: pair j of group g is (dimension 32 g + 8 t + j, and four later) of head r, times 2^k with the head's largest value
+  // The queries as the 8-column operand: pair j of group g is (dimension 32 g + 8 t + j, and four later) of a head, times 2^k with the head's largest value
   // in [2^119, 2^120) (a sum of 32 stays finite), and 1/16 of that where the codes count 16 times. Scores are compared before they are scaled: a negative scale turns the
-  // query's sign. c[h]: from the products' unit to powers of two, of heads 2 t and 2 t + 1.
+  // query's sign. c[h]: from the products' unit to powers of two, of columns 2 t and 2 t + 1.
   uint32_t qf[G][4];
-  float2 start[G];      // -7.5 * sum of the group's values, of heads 2 t and 2 t + 1: a product with a row of codes 15, halved
+  float2 start[G];      // -7.5 * sum of the group's values, of columns 2 t and 2 t + 1: a product with a row of codes 15, halved
   float c[2], slack[2];
   {
     uint32_t big = 0u;
@@ -299,8 +306,7 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
 #pragma unroll
       for (int j = 0; j < 4; ++j) qf[g][j] = mul_bf16x2(mul_bf16x2(w[j], by), j & 1 ? by_odd : by_even);
       float acc[4] = {0.f, 0.f, 0.f, 0.f};
-      mma_bf16(acc, 0x000f000fu, 0x000f000fu, 0x00f000f0u, 0x00f000f0u, qf[g][0], qf[g][1]);
-      mma_bf16(acc, 0x000f000fu, 0x000f000fu, 0x00f000f0u, 0x00f000f0u, qf[g][2], qf[g][3]);
+      score_group(acc, 0xffffffffu, 0xffffffffu, qf[g]);
       start[g] = make_float2(-0.5f * acc[0], -0.5f * acc[1]);
     }
     const float unit = fminf(fmaxf(times_pow2(fabsf(p.scale) * 1.4426950408889634f, 133 - k), 1e-30f), 1e30f);
@@ -325,24 +331,39 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
     __syncwarp();      // the scales were copied by other lanes; and every lane has read the stage that is requested next
     request(i + K4_STAGES - 1);
     const uint32_t from = fifo + (i % K4_STAGES) * Stage::BYTES;
-    float s[2][4];
-    uint32_t va[2][G / 2], vb[2][G / 2];      // the values' scales
+    float s[NS][4];
+    uint32_t va[NS][G / 2], vb[NS][G / 2];      // the values' scales
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t ka[G], kb[G], sa[G], sb[G];
-      load_words(from + h * Stage::HALF + Stage::KA + lane * (G * 4), ka);
-      load_words(from + h * Stage::HALF + Stage::KB + lane * (G * 4), kb);
-      load_words(from + h * Stage::HALF + Stage::SCALES + Page::scale(tok, 0, 0), sa);
-      load_words(from + h * Stage::HALF + Stage::SCALES + Page::scale(tok + 2, 0, 0), sb);
+    for (int h = 0; h < NS; ++h) {
+      const uint32_t mine = from + (PAIR ? t >> 1 : h) * Stage::HALF;      // (columns 0-3: the first 16 tokens, 4-7: the others)
+      uint32_t sa[G], sb[G];
+      load_words(mine + Stage::SCALES + Page::scale(tok, 0, 0), sa);
+      load_words(mine + Stage::SCALES + Page::scale(tok + 2, 0, 0), sb);
       float2 lo = make_float2(0.f, 0.f), hi = lo;
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        mma_bf16(acc, unpack2(ka[g], 0), unpack2(kb[g], 0), unpack2(ka[g], 1), unpack2(kb[g], 1), qf[g][0], qf[g][1]);
-        mma_bf16(acc, unpack2(ka[g], 2), unpack2(kb[g], 2), unpack2(ka[g], 3), unpack2(kb[g], 3), qf[g][2], qf[g][3]);
-        const float fa = bf16_of(sa[g >> 1], g), fb = bf16_of(sb[g >> 1], g);
-        lo = fma2(add2(make_float2(acc[0], acc[1]), start[g]), make_float2(fa, fa), lo);
-        hi = fma2(add2(make_float2(acc[2], acc[3]), start[g]), make_float2(fb, fb), hi);
+      for (int g0 = 0; g0 < G; g0 += W) {
+        uint32_t ka[W], kb[W], kc[W], kd[W];
+        load_words(from + h * Stage::HALF + Stage::KA + lane * (G * 4) + g0 * 4, ka);
+        load_words(from + h * Stage::HALF + Stage::KB + lane * (G * 4) + g0 * 4, kb);
+        if constexpr (PAIR) {
+          load_words(from + Stage::HALF + Stage::KA + lane * (G * 4) + g0 * 4, kc);
+          load_words(from + Stage::HALF + Stage::KB + lane * (G * 4) + g0 * 4, kd);
+        }
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+          const int g = g0 + j;
+          float acc[4] = {0.f, 0.f, 0.f, 0.f};
+          score_group(acc, ka[j], kb[j], qf[g]);
+          if constexpr (PAIR) {
+            float other[4] = {0.f, 0.f, 0.f, 0.f};
+            score_group(other, kc[j], kd[j], qf[g]);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[q] = t < 2 ? acc[q] : other[q];
+          }
+          const float fa = bf16_of(sa[g >> 1], g), fb = bf16_of(sb[g >> 1], g);
+          lo = fma2(add2(make_float2(acc[0], acc[1]), start[g]), make_float2(fa, fa), lo);
+          hi = fma2(add2(make_float2(acc[2], acc[3]), start[g]), make_float2(fb, fb), hi);
+        }
       }
       s[h][0] = lo.x; s[h][1] = lo.y; s[h][2] = hi.x; s[h][3] = hi.y;
 #pragma unroll
@@ -354,8 +375,8 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
     const int pos0 = (begin + warp + i * K4_WARPS) * K4_STEP;
     if (pos0 < first || pos0 + K4_STEP > len) {      // (a place that was never written, or by another sequence, may hold anything)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int at = pos0 + 16 * h + tok;
+      for (int h = 0; h < NS; ++h) {
+        const int at = pos0 + 16 * (PAIR ? t >> 1 : h) + tok;
         if (at < first || at >= len) {
           s[h][0] = s[h][1] = -INFINITY;
 #pragma unroll
@@ -369,19 +390,27 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
       }
     }
     // The running maximum moves only when a score passes it by K4_SLACK: weights are then at most 2^8, and any reference gives the same quotient.
-    const float m0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2])), m1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]));
+    float m0 = fmaxf(s[0][0], s[0][2]), m1 = fmaxf(s[0][1], s[0][3]);
+    if constexpr (!PAIR) {
+      m0 = fmaxf(m0, fmaxf(s[NS - 1][0], s[NS - 1][2]));
+      m1 = fmaxf(m1, fmaxf(s[NS - 1][1], s[NS - 1][3]));
+    }
     uint32_t widest = limit;
 #pragma unroll
-    for (int g = 0; g < G / 2; ++g) widest = __vmaxu2(__vmaxu2(widest, __vmaxu2(va[0][g], vb[0][g])), __vmaxu2(va[1][g], vb[1][g]));
+    for (int h = 0; h < NS; ++h)
+#pragma unroll
+      for (int g = 0; g < G / 2; ++g) widest = __vmaxu2(widest, __vmaxu2(va[h][g], vb[h][g]));
     if (__any_sync(0xffffffffu, m0 > top[0] + slack[0] || m1 > top[1] + slack[1] || widest != limit)) {
       float f[2] = {1.f, 1.f};
       uint32_t wide = 0u;      // the largest finite scale
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const uint32_t w[4] = {va[g & 1][g >> 1] & 0xffffu, va[g & 1][g >> 1] >> 16, vb[g & 1][g >> 1] & 0xffffu, vb[g & 1][g >> 1] >> 16};
+      for (int h = 0; h < NS; ++h)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) wide = max(wide, w[j] < 0x7f80u ? w[j] : 0u);
-      }
+        for (int g = 0; g < G / 2; ++g) {
+          const uint32_t w[4] = {va[h][g] & 0xffffu, va[h][g] >> 16, vb[h][g] & 0xffffu, vb[h][g] >> 16};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) wide = max(wide, w[j] < 0x7f80u ? w[j] : 0u);
+        }
       wide = __reduce_max_sync(0xffffffffu, wide);
       if (wide > (limit & 0xffffu)) {
         const int e = static_cast<int>(wide >> 7) - 127;
@@ -416,22 +445,37 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
     }
     const float ref0 = top[0] == -INFINITY ? 0.f : fmaf(-top[0], c[0], lift), ref1 = top[1] == -INFINITY ? 0.f : fmaf(-top[1], c[1], lift);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t wa[G], wb[G];
-      load_words(from + h * Stage::HALF + Stage::VA + lane * (G * 4), wa);
-      load_words(from + h * Stage::HALF + Stage::VB + lane * (G * 4), wb);
+    for (int h = 0; h < NS; ++h) {
       const float2 pa = make_float2(exp2_fast(fmaf(s[h][0], c[0], ref0)), exp2_fast(fmaf(s[h][1], c[1], ref1)));
       const float2 pb = make_float2(exp2_fast(fmaf(s[h][2], c[0], ref0)), exp2_fast(fmaf(s[h][3], c[1], ref1)));
       sum[0] += pa.x + pb.x;
       sum[1] += pa.y + pb.y;
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const float fa = bf16_of(va[h][g >> 1], g), fb = bf16_of(vb[h][g >> 1], g);
-        // weight * scale in 32 bits, rounded once to the operand's bf16: half a step, 2^-8 of each token's share at most, with either sign
-        const uint32_t w0 = transposed8x8(pack_bf16x2(pa.x * fa, pa.y * fa)), w1 = transposed8x8(pack_bf16x2(pb.x * fb, pb.y * fb));
-        mma_bf16(o[2 * g], unpack2(wa[g], 0), unpack2(wa[g], 1), unpack2(wb[g], 0), unpack2(wb[g], 1), w0, w1);
-        mma_bf16(o[2 * g + 1], unpack2(wa[g], 2), unpack2(wa[g], 3), unpack2(wb[g], 2), unpack2(wb[g], 3), w0, w1);
-        mma_bf16(z[g], 0x000f000fu, 0x000f000fu, 0x000f000fu, 0x000f000fu, w0, w1);
+      for (int g0 = 0; g0 < G; g0 += W) {
+        uint32_t wa[W], wb[W], wc[W], wd[W];
+        load_words(from + h * Stage::HALF + Stage::VA + lane * (G * 4) + g0 * 4, wa);
+        load_words(from + h * Stage::HALF + Stage::VB + lane * (G * 4) + g0 * 4, wb);
+        if constexpr (PAIR) {
+          load_words(from + Stage::HALF + Stage::VA + lane * (G * 4) + g0 * 4, wc);
+          load_words(from + Stage::HALF + Stage::VB + lane * (G * 4) + g0 * 4, wd);
+        }
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+          const int g = g0 + j;
+          const float fa = bf16_of(va[h][g >> 1], g), fb = bf16_of(vb[h][g >> 1], g);
+          // weight * scale in 32 bits, rounded once to the operand's bf16: half a step, 2^-8 of each token's share at most, with either sign
+          uint32_t w0 = transposed8x8(pack_bf16x2(pa.x * fa, pa.y * fa)), w1 = transposed8x8(pack_bf16x2(pb.x * fb, pb.y * fb));
+          mma_bf16(z[g], 0x000f000fu, 0x000f000fu, 0x000f000fu, 0x000f000fu, w0, w1);
+          if constexpr (PAIR) {      // columns 4-7 hold the weights of the other 16 tokens
+            const uint32_t x0 = r < 4 ? 0u : w0, x1 = r < 4 ? 0u : w1;
+            mma_bf16(o[2 * g], unpack2(wc[j], 0), unpack2(wc[j], 1), unpack2(wd[j], 0), unpack2(wd[j], 1), x0, x1);
+            mma_bf16(o[2 * g + 1], unpack2(wc[j], 2), unpack2(wc[j], 3), unpack2(wd[j], 2), unpack2(wd[j], 3), x0, x1);
+            w0 = r < 4 ? w0 : 0u;
+            w1 = r < 4 ? w1 : 0u;
+          }
+          mma_bf16(o[2 * g], unpack2(wa[j], 0), unpack2(wa[j], 1), unpack2(wb[j], 0), unpack2(wb[j], 1), w0, w1);
+          mma_bf16(o[2 * g + 1], unpack2(wa[j], 2), unpack2(wa[j], 3), unpack2(wb[j], 2), unpack2(wb[j], 3), w0, w1);
+        }
       }
     }
     // The offset is taken off again and again: left until the end it would outgrow the sums, which are to keep their last bits.
@@ -439,7 +483,10 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
   }
   fold(o, z);
 
-  // The warps' parts are brought to one reference and added: heads 2 t and 2 t + 1, dimensions 32 g + 4 r .. + 3 of each lane.
+  // The warps' parts (and, where four heads have two columns each, the columns') are brought to one reference and added: columns 2 t and 2 t + 1, dimensions
+  // 32 g + 4 r .. + 3 of each lane.
+  constexpr int PARTS = PAIR ? 2 * K4_WARPS : K4_WARPS;
+  auto part_of = [&](int head, int i) -> float2 { return PAIR ? ml[i >> 1][head + 4 * (i & 1)] : ml[i][head]; };
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 4);
@@ -453,29 +500,29 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
   constexpr int ROW = D + 4;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int head = 2 * t + h;
-    float m = ml[0][head].x;
+    const int column = 2 * t + h, head = PAIR ? column & 3 : column;
+    float m = part_of(head, 0).x;
 #pragma unroll
-    for (int w = 1; w < K4_WARPS; ++w) m = fmaxf(m, ml[w][head].x);
+    for (int i = 1; i < PARTS; ++i) m = fmaxf(m, part_of(head, i).x);
     // (a part without a finite score has no tokens, or NaN, which is to stay)
     const float f = top[h] == -INFINITY ? 1.f : exp2_fast(top[h] - m), f0 = f * 0x1p67f, f1 = f * 0x1p63f;
 #pragma unroll
     for (int g = 0; g < G; ++g)
-      *reinterpret_cast<float4*>(red + (warp * 8 + head) * ROW + 32 * g + 4 * r) =
+      *reinterpret_cast<float4*>(red + (warp * 8 + column) * ROW + 32 * g + 4 * r) =
           make_float4(o[2 * g][h] * 0x1p66f * f0, o[2 * g][h + 2] * 0x1p66f * f1, o[2 * g + 1][h] * 0x1p66f * f0, o[2 * g + 1][h + 2] * 0x1p66f * f1);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < heads * (D / 4); i += K4_WARPS * 32) {
     const int head = i / (D / 4), d = i % (D / 4) * 4;
-    float m = ml[0][head].x, l = 0.f;
+    float m = part_of(head, 0).x, l = 0.f;
 #pragma unroll
-    for (int w = 1; w < K4_WARPS; ++w) m = fmaxf(m, ml[w][head].x);
+    for (int w = 1; w < PARTS; ++w) m = fmaxf(m, part_of(head, w).x);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < K4_WARPS; ++w) {
-      const float2 part = ml[w][head];
+    for (int w = 0; w < PARTS; ++w) {
+      const float2 part = part_of(head, w);
       l += part.y * (part.x == -INFINITY ? 1.f : exp2_fast(part.x - m));
-      const float4 v = *reinterpret_cast<const float4*>(red + (w * 8 + head) * ROW + d);
+      const float4 v = *reinterpret_cast<const float4*>(red + (PAIR ? (w >> 1) * 8 + head + 4 * (w & 1) : w * 8 + head) * ROW + d);
       acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
     }
     if (count == span.steps) {
@@ -574,20 +621,20 @@ __global__ void __launch_bounds__(1024) kv4_join_kernel(const K4Params p) {
     }
 }
 
-template <int D>
+template <int D, bool PAIR>
 int launch_decode(const K4Params& p, cudaStream_t stream) {
   static std::atomic<unsigned long long> ready{0};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return static_cast<int>(e);
   if (!(ready.load() >> (dev & 63) & 1)) {
-    e = cudaFuncSetAttribute(kv4_decode_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, k4_smem<D>());
+    e = cudaFuncSetAttribute(kv4_decode_kernel<D, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, k4_smem<D>());
     if (e != cudaSuccess) return static_cast<int>(e);
     ready.fetch_or(1ull << (dev & 63));
   }
   const int all_heads = p.Hkv * p.chunks;
   const dim3 grid = p.num_ctas ? dim3(p.num_ctas) : dim3(all_heads, p.B);
-  rlb_launch_pdl(kv4_decode_kernel<D>, grid, dim3(K4_WARPS * 32), k4_smem<D>(), stream, p);
+  rlb_launch_pdl(kv4_decode_kernel<D, PAIR>, grid, dim3(K4_WARPS * 32), k4_smem<D>(), stream, p);
   e = cudaGetLastError();
   if (e != cudaSuccess || !p.num_ctas) return static_cast<int>(e);
   const long long segments = static_cast<long long>(p.B) * all_heads;
@@ -612,5 +659,6 @@ RLB_API int rlb_kv4_paged_decode(const void* q, long long q_stride, const void* 
                    block_size, window, scale, B, num_ctas, part_o, reinterpret_cast<float2*>(part_ml), reinterpret_cast<int4*>(part_ml + static_cast<long long>(num_ctas) * 32),
                    static_cast<__nv_bfloat16*>(out), out_stride, status};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return D == 64 ? launch_decode<64>(p, s) : D == 128 ? launch_decode<128>(p, s) : launch_decode<256>(p, s);
+  if (group <= 4) return D == 64 ? launch_decode<64, true>(p, s) : D == 128 ? launch_decode<128, true>(p, s) : launch_decode<256, true>(p, s);
+  return D == 64 ? launch_decode<64, false>(p, s) : D == 128 ? launch_decode<128, false>(p, s) : launch_decode<256, false>(p, s);
 }

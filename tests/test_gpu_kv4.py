@@ -125,8 +125,8 @@ def _pool(pages, Hkv, D, block, seed, big=1.0):
 
 def _check(got, q, cache, table, lens, Hq, Hkv, D, window=0, scale=None):
     """Every output within what the roundings give: the result's to bf16 (2^-8 of it), each token's weight times its scale to bf16 (2^-8 of
-    the token's share), and the scores in 32 bits. A score's sum over a group has 32 terms of at most 15 |q| and the offset of 7.5 times the sum of the query's values:
-    an error of 33 roundings at that size, times the key's scale; a score's error e changes a weight by e and the sum by as much."""
+    the token's share), and the scores' to 32 bits. A score's sum over a group has 32 terms of at most 15 |q| and the offset of 7.5 times the sum of the query's values: 33
+    roundings at that size, times the key's scale; a score's error e changes a weight by e and the sum by as much."""
     block, B = cache.shape[2] * 8 // (9 * D), q.shape[0]
     scale = scale or 1 / math.sqrt(D)
     for b in range(B):
