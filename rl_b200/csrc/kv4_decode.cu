@@ -26,7 +26,7 @@ using namespace rlb;
 
 constexpr int K4_WARPS = 4;
 constexpr int K4_STEP = 32;      // tokens a warp takes at a time: twice the 16 of an instruction
-constexpr int K4_STAGES = 4;     // steps whose words are in a warp's shared memory or on their way
+constexpr int K4_STAGES = 3;     // steps whose words are in a warp's shared memory or on their way
 constexpr int K4_FOLD = 16;      // steps between two corrections of the sums
 constexpr float K4_SLACK = 8.f;  // how far (in powers of two) a score may pass the running maximum before the sums are rescaled: weights stay below 2^8
 
@@ -67,16 +67,25 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }      // e from -126 to 127
 // Codes at nibble j of both halves of a word as two bf16 numbers: code * 2^-133 for even j, code * 2^-129 for odd j.
-__device__ __forceinline__ uint32_t unpack2(uint32_t w, int j) { return (j & 2 ? w >> 8 : w) & (j & 1 ? 0x00f000f0u : 0x000f000fu); }
+__device__ __forceinline__ uint32_t unpack2(uint32_t w, int j) { return w & (j & 1 ? 0x00f000f0u : 0x000f000fu); }
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 // 16 tokens' products of a group of 32 dimensions: wa, wb are the thread's words of its two tokens, q its pairs of the query.
-__device__ __forceinline__ void score_group(float (&acc)[4], uint32_t wa, uint32_t wb, const uint32_t (&q)[4]) {
-  mma_bf16(acc, unpack2(wa, 0), unpack2(wb, 0), unpack2(wa, 1), unpack2(wb, 1), q[0], q[1]);
-  mma_bf16(acc, unpack2(wa, 2), unpack2(wb, 2), unpack2(wa, 3), unpack2(wb, 3), q[2], q[3]);
+__device__ __forceinline__ void score_group(float (&acc)[4], uint32_t wa, uint32_t wb, uint4 q) {
+  mma_bf16(acc, unpack2(wa, 0), unpack2(wb, 0), unpack2(wa, 1), unpack2(wb, 1), q.x, q.y);
+  wa >>= 8;
+  wb >>= 8;
+  mma_bf16(acc, unpack2(wa, 0), unpack2(wb, 0), unpack2(wa, 1), unpack2(wb, 1), q.z, q.w);
+}
+// 32 dimensions of 16 tokens' values added to the sums of a group: weights w0, w1.
+__device__ __forceinline__ void add_group(float (&o0)[4], float (&o1)[4], uint32_t wa, uint32_t wb, uint32_t w0, uint32_t w1) {
+  mma_bf16(o0, unpack2(wa, 0), unpack2(wa, 1), unpack2(wb, 0), unpack2(wb, 1), w0, w1);
+  wa >>= 8;
+  wb >>= 8;
+  mma_bf16(o1, unpack2(wa, 0), unpack2(wa, 1), unpack2(wb, 0), unpack2(wb, 1), w0, w1);
 }
 // Two sums or products at once.
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
@@ -117,6 +126,8 @@ __device__ __forceinline__ void copy_words(uint32_t to, const uint8_t* from) {
     for (int i = 0; i < N; i += 4) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 4 * i), "l"(from + 4 * i) : "memory");
   }
 }
+// p + a * b, in one multiplication.
+__device__ __forceinline__ const uint8_t* wide(const uint8_t* p, uint32_t a, uint32_t b) { return p + static_cast<unsigned long long>(a) * b; }
 __device__ __forceinline__ float bf16_of(uint32_t word, int i) { return __uint_as_float(i & 1 ? word & 0xffff0000u : word << 16); }
 
 // A warp's stage: twice 16 tokens of the words that each lane is going to use (its own copies, so that no other lane has to be waited for), and their scales.
@@ -132,18 +143,20 @@ constexpr int k4_smem() {
   return fifo > red ? fifo : red;
 }
 
-// Takes the codes' offset off the sums: z is 15 * 2^-133 times the weights, 7.5 levels of what rows 0-7 of a tile count in, and 1/16 of that of rows 8-15.
+// Takes the codes' offset off the sums: z (of two groups, in rows 0-7 and 8-15) is 15 * 2^-133 times the weights, 7.5 levels of what rows 0-7 of a tile count in, and 1/16 of that of rows 8-15.
 template <int G>
-__device__ __forceinline__ void fold(float (&o)[2 * G][4], float (&z)[G][4]) {
+__device__ __forceinline__ void fold(float (&o)[2 * G][4], float (&z)[G / 2][4]) {
 #pragma unroll
   for (int g = 0; g < G; ++g) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      o[2 * g][j] = fmaf(j < 2 ? -0.5f : -8.f, z[g][j & 1], o[2 * g][j]);
-      o[2 * g + 1][j] = fmaf(j < 2 ? -0.5f : -8.f, z[g][j & 1], o[2 * g + 1][j]);
+      const float w = z[g >> 1][(g & 1) * 2 + (j & 1)];
+      o[2 * g][j] = fmaf(j < 2 ? -0.5f : -8.f, w, o[2 * g][j]);
+      o[2 * g + 1][j] = fmaf(j < 2 ? -0.5f : -8.f, w, o[2 * g + 1][j]);
     }
-    z[g][0] = z[g][1] = z[g][2] = z[g][3] = 0.f;
   }
+#pragma unroll
+  for (int g = 0; g < G / 2; ++g) z[g][0] = z[g][1] = z[g][2] = z[g][3] = 0.f;
 }
 
 // Tokens of a sequence that the table has room for, the first visible one, and the steps from there on.
@@ -170,6 +183,8 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
   extern __shared__ __align__(128) uint8_t k4_smem_raw[];
   __shared__ float2 ml[K4_WARPS][8];      // of each warp and column: what its weights are relative to (a power of two), and their sum
   __shared__ int found[3], sums[K4_WARPS];
+  __shared__ uint4 query[PAIR ? 2 : 1][D / 32][32];      // each lane's operands of a group (PAIR: with zeros in columns 4-7, and in columns 0-3); what its products start from
+  __shared__ float2 offset[D / 32][32];
   using Stage = K4Stage<D>;
   using Page = Kv4Page<D>;
   constexpr int G = Page::G, W = G < 4 ? G : 4;      // groups of 32 dimensions; words of a load
@@ -255,22 +270,24 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
   int page_now = page_of(lane, off_now), page_next = page_of(32 + lane, off_next);
   const uint32_t fifo = smem_u32(k4_smem_raw) + warp * (K4_STAGES * Stage::BYTES);
   const int tok = 4 * (r >> 1) + (r & 1);      // of 16; the thread's other row is two tokens later
-  const int key_at = Page::key_word(tok, t, 0), value_at = Page::values_at(p.block_size) + Page::value_unit(4 * t, r, 0), scale_at = Page::scales_at(p.block_size) + lane * 16;
   const uint8_t* cache = p.cache + kvh * Page::bytes(p.block_size);
-  const long long page_stride = p.Hkv * Page::bytes(p.block_size);
+  const uint8_t *key_base = cache + Page::key_word(tok, t, 0), *value_base = cache + Page::values_at(p.block_size) + Page::value_unit(4 * t, r, 0);
+  const uint8_t* scale_base = cache + Page::scales_at(p.block_size) + lane * 16;
+  const uint32_t page_stride = static_cast<uint32_t>(p.Hkv * Page::bytes(p.block_size));
   auto request = [&](int i) {
     if (i < n) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int src = (2 * i + h) & 31, off = __shfl_sync(0xffffffffu, off_now, src);
-        const uint8_t* page = cache + __shfl_sync(0xffffffffu, page_now, src) * page_stride;
-        const uint8_t *keys = page + (off * (D / 2) + key_at), *values = page + (off * (D / 2) + value_at);
+        const int src = (2 * i + h) & 31;
+        const uint32_t off = __shfl_sync(0xffffffffu, off_now, src), no = __shfl_sync(0xffffffffu, page_now, src);
+        const uint8_t* keys = wide(wide(key_base, no, page_stride), off, D / 2);
+        const uint8_t* values = wide(wide(value_base, no, page_stride), off, D / 2);
         const uint32_t to = fifo + (i % K4_STAGES) * Stage::BYTES + h * Stage::HALF;
         copy_words<G>(to + Stage::KA + lane * (G * 4), keys);
         copy_words<G>(to + Stage::KB + lane * (G * 4), keys + D);               // two tokens of keys
         copy_words<G>(to + Stage::VA + lane * (G * 4), values);
         copy_words<G>(to + Stage::VB + lane * (G * 4), values + D);             // one pair of tokens of values
-        if (lane < D / 8) copy_words<4>(to + Stage::SCALES + lane * 16, page + (off * (D / 8) + scale_at));
+        if (lane < D / 8) copy_words<4>(to + Stage::SCALES + lane * 16, wide(wide(scale_base, no, page_stride), off, D / 8));
       }
       if ((i & 15) == 15) {
         page_now = page_next;
@@ -286,8 +303,7 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
   // The queries as the 8-column operand: pair j of group g is (dimension 32 g + 8 t + j, and four later) of a head, times 2^k with the head's largest value
   // in [2^119, 2^120) (a sum of 32 stays finite), and 1/16 of that where the codes count 16 times. Scores are compared before they are scaled: a negative scale turns the
   // query's sign. c[h]: from the products' unit to powers of two, of columns 2 t and 2 t + 1.
-  uint32_t qf[G][4];
-  float2 start[G];      // -7.5 * sum of the group's values, of columns 2 t and 2 t + 1: a product with a row of codes 15, halved
+  // They stay in shared memory, for the registers' sake, with -7.5 times the sum of the group's values of columns 2 t and 2 t + 1 (a product with a row of codes 15, halved).
   float c[2], slack[2];
   {
     uint32_t big = 0u;
@@ -302,12 +318,17 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
     const uint32_t by = pack_bf16x2(half, half), by_even = pack_bf16x2(rest, rest), by_odd = pack_bf16x2(rest * 0.0625f, rest * 0.0625f);
 #pragma unroll
     for (int g = 0; g < G; ++g) {
+      if ((g & (K4_WARPS - 1)) != warp) continue;      // (the warps take turns)
       const uint32_t w[4] = {__byte_perm(qv[g].x, qv[g].z, 0x5410), __byte_perm(qv[g].x, qv[g].z, 0x7632), __byte_perm(qv[g].y, qv[g].w, 0x5410), __byte_perm(qv[g].y, qv[g].w, 0x7632)};
+      uint32_t qf[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) qf[g][j] = mul_bf16x2(mul_bf16x2(w[j], by), j & 1 ? by_odd : by_even);
+      for (int j = 0; j < 4; ++j) qf[j] = mul_bf16x2(mul_bf16x2(w[j], by), j & 1 ? by_odd : by_even);
       float acc[4] = {0.f, 0.f, 0.f, 0.f};
-      score_group(acc, 0xffffffffu, 0xffffffffu, qf[g]);
-      start[g] = make_float2(-0.5f * acc[0], -0.5f * acc[1]);
+      const uint4 all = make_uint4(qf[0], qf[1], qf[2], qf[3]), none = make_uint4(0u, 0u, 0u, 0u);
+      score_group(acc, 0xffffffffu, 0xffffffffu, all);
+      query[0][g][lane] = PAIR && r >= 4 ? none : all;
+      if constexpr (PAIR) query[NS][g][lane] = r >= 4 ? all : none;
+      offset[g][lane] = make_float2(-0.5f * acc[0], -0.5f * acc[1]);
     }
     const float unit = fminf(fmaxf(times_pow2(fabsf(p.scale) * 1.4426950408889634f, 133 - k), 1e-30f), 1e30f);
     c[0] = __shfl_sync(0xffffffffu, unit, 8 * t);
@@ -315,16 +336,17 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
     slack[0] = K4_SLACK / c[0];
     slack[1] = K4_SLACK / c[1];
   }
+  __syncthreads();
 
-  float o[2 * G][4], z[G][4], top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+  float o[2 * G][4], z[G / 2][4], top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
   // Weights are held 2^lift times as large, so that their products with the values' scales lie near 2^40 and keep clear of the ends of 32 bits (times 2^-133) and of
   // bf16. limit: the largest scale, in bf16 bits in both halves, for which that holds.
-  float lift = 0.f;
+  float lift = 0.f, ref[2] = {0.f, 0.f};      // ref: what is added to a score's power of two
   uint32_t limit = 0u;
 #pragma unroll
   for (int i = 0; i < 2 * G; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
-  for (int g = 0; g < G; ++g) z[g][0] = z[g][1] = z[g][2] = z[g][3] = 0.f;
+  for (int g = 0; g < G / 2; ++g) z[g][0] = z[g][1] = z[g][2] = z[g][3] = 0.f;
 
   for (int i = 0; i < n; ++i) {
     asm volatile("cp.async.wait_group %0;" ::"n"(K4_STAGES - 2) : "memory");
@@ -353,16 +375,12 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
         for (int j = 0; j < W; ++j) {
           const int g = g0 + j;
           float acc[4] = {0.f, 0.f, 0.f, 0.f};
-          score_group(acc, ka[j], kb[j], qf[g]);
-          if constexpr (PAIR) {
-            float other[4] = {0.f, 0.f, 0.f, 0.f};
-            score_group(other, kc[j], kd[j], qf[g]);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) acc[q] = t < 2 ? acc[q] : other[q];
-          }
+          score_group(acc, ka[j], kb[j], query[0][g][lane]);
+          if constexpr (PAIR) score_group(acc, kc[j], kd[j], query[NS][g][lane]);
+          const float2 start = offset[g][lane];
           const float fa = bf16_of(sa[g >> 1], g), fb = bf16_of(sb[g >> 1], g);
-          lo = fma2(add2(make_float2(acc[0], acc[1]), start[g]), make_float2(fa, fa), lo);
-          hi = fma2(add2(make_float2(acc[2], acc[3]), start[g]), make_float2(fb, fb), hi);
+          lo = fma2(add2(make_float2(acc[0], acc[1]), start), make_float2(fa, fa), lo);
+          hi = fma2(add2(make_float2(acc[2], acc[3]), start), make_float2(fb, fb), hi);
         }
       }
       s[h][0] = lo.x; s[h][1] = lo.y; s[h][2] = hi.x; s[h][3] = hi.y;
@@ -402,18 +420,33 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
       for (int g = 0; g < G / 2; ++g) widest = __vmaxu2(widest, __vmaxu2(va[h][g], vb[h][g]));
     if (__any_sync(0xffffffffu, m0 > top[0] + slack[0] || m1 > top[1] + slack[1] || widest != limit)) {
       float f[2] = {1.f, 1.f};
-      uint32_t wide = 0u;      // the largest finite scale
+      uint32_t most = 0u, lost = 0u;      // the largest scale; groups with one that is not finite, which are NaN from here on (and count as zeros, for z's sake)
 #pragma unroll
       for (int h = 0; h < NS; ++h)
 #pragma unroll
-        for (int g = 0; g < G / 2; ++g) {
-          const uint32_t w[4] = {va[h][g] & 0xffffu, va[h][g] >> 16, vb[h][g] & 0xffffu, vb[h][g] >> 16};
+        for (int g = 0; g < G / 2; ++g)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) wide = max(wide, w[j] < 0x7f80u ? w[j] : 0u);
-        }
-      wide = __reduce_max_sync(0xffffffffu, wide);
-      if (wide > (limit & 0xffffu)) {
-        const int e = static_cast<int>(wide >> 7) - 127;
+          for (int j = 0; j < 2; ++j) {
+            uint32_t& w = j ? vb[h][g] : va[h][g];
+            if ((w & 0xffffu) >= 0x7f80u) {
+              lost |= 1u << (2 * g);
+              w &= 0xffff0000u;
+            }
+            if (w >> 16 >= 0x7f80u) {
+              lost |= 2u << (2 * g);
+              w &= 0xffffu;
+            }
+            most = max(most, max(w & 0xffffu, w >> 16));
+          }
+      most = __reduce_max_sync(0xffffffffu, most);
+      lost = __reduce_or_sync(0xffffffffu, lost);
+      if (lost) {
+#pragma unroll
+        for (int j = 0; j < 2 * G; ++j)
+          if (lost >> (j >> 1) & 1u) o[j][0] = o[j][1] = o[j][2] = o[j][3] = __uint_as_float(0x7fc00000u);
+      }
+      if (most > (limit & 0xffffu)) {
+        const int e = static_cast<int>(most >> 7) - 127;
         const float to = static_cast<float>(max(-100, min(96, 40 - e)));
         f[0] = f[1] = exp2_fast(to - lift);
         lift = to;
@@ -430,6 +463,7 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
           f[h] *= exp2_fast((top[h] - m) * c[h]);      // (0 for the first)
           top[h] = m;
         }
+        ref[h] = top[h] == -INFINITY ? 0.f : fmaf(-top[h], c[h], lift);
         sum[h] *= f[h];
 #pragma unroll
         for (int j = 0; j < 2 * G; ++j) {
@@ -437,17 +471,16 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
           o[j][h + 2] *= f[h];
         }
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
+        for (int g = 0; g < G / 2; ++g) {
           z[g][h] *= f[h];
           z[g][h + 2] *= f[h];
         }
       }
     }
-    const float ref0 = top[0] == -INFINITY ? 0.f : fmaf(-top[0], c[0], lift), ref1 = top[1] == -INFINITY ? 0.f : fmaf(-top[1], c[1], lift);
 #pragma unroll
     for (int h = 0; h < NS; ++h) {
-      const float2 pa = make_float2(exp2_fast(fmaf(s[h][0], c[0], ref0)), exp2_fast(fmaf(s[h][1], c[1], ref1)));
-      const float2 pb = make_float2(exp2_fast(fmaf(s[h][2], c[0], ref0)), exp2_fast(fmaf(s[h][3], c[1], ref1)));
+      const float2 pa = make_float2(exp2_fast(fmaf(s[h][0], c[0], ref[0])), exp2_fast(fmaf(s[h][1], c[1], ref[1])));
+      const float2 pb = make_float2(exp2_fast(fmaf(s[h][2], c[0], ref[0])), exp2_fast(fmaf(s[h][3], c[1], ref[1])));
       sum[0] += pa.x + pb.x;
       sum[1] += pa.y + pb.y;
 #pragma unroll
@@ -465,23 +498,20 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
           const float fa = bf16_of(va[h][g >> 1], g), fb = bf16_of(vb[h][g >> 1], g);
           // weight * scale in 32 bits, rounded once to the operand's bf16: half a step, 2^-8 of each token's share at most, with either sign
           uint32_t w0 = transposed8x8(pack_bf16x2(pa.x * fa, pa.y * fa)), w1 = transposed8x8(pack_bf16x2(pb.x * fb, pb.y * fb));
-          mma_bf16(z[g], 0x000f000fu, 0x000f000fu, 0x000f000fu, 0x000f000fu, w0, w1);
+          mma_bf16(z[g >> 1], g & 1 ? 0u : 0x000f000fu, g & 1 ? 0x000f000fu : 0u, g & 1 ? 0u : 0x000f000fu, g & 1 ? 0x000f000fu : 0u, w0, w1);
           if constexpr (PAIR) {      // columns 4-7 hold the weights of the other 16 tokens
-            const uint32_t x0 = r < 4 ? 0u : w0, x1 = r < 4 ? 0u : w1;
-            mma_bf16(o[2 * g], unpack2(wc[j], 0), unpack2(wc[j], 1), unpack2(wd[j], 0), unpack2(wd[j], 1), x0, x1);
-            mma_bf16(o[2 * g + 1], unpack2(wc[j], 2), unpack2(wc[j], 3), unpack2(wd[j], 2), unpack2(wd[j], 3), x0, x1);
+            add_group(o[2 * g], o[2 * g + 1], wc[j], wd[j], r < 4 ? 0u : w0, r < 4 ? 0u : w1);
             w0 = r < 4 ? w0 : 0u;
             w1 = r < 4 ? w1 : 0u;
           }
-          mma_bf16(o[2 * g], unpack2(wa[j], 0), unpack2(wa[j], 1), unpack2(wb[j], 0), unpack2(wb[j], 1), w0, w1);
-          mma_bf16(o[2 * g + 1], unpack2(wa[j], 2), unpack2(wa[j], 3), unpack2(wb[j], 2), unpack2(wb[j], 3), w0, w1);
+          add_group(o[2 * g], o[2 * g + 1], wa[j], wb[j], w0, w1);
         }
       }
     }
     // The offset is taken off again and again: left until the end it would outgrow the sums, which are to keep their last bits.
-    if (i % K4_FOLD == K4_FOLD - 1) fold(o, z);
+    if (i % K4_FOLD == K4_FOLD - 1) fold<G>(o, z);
   }
-  fold(o, z);
+  fold<G>(o, z);
 
   // The warps' parts (and, where four heads have two columns each, the columns') are brought to one reference and added: columns 2 t and 2 t + 1, dimensions
   // 32 g + 4 r .. + 3 of each lane.
@@ -654,7 +684,9 @@ RLB_API int rlb_kv4_paged_decode(const void* q, long long q_stride, const void* 
   if (B <= 0) return 0;
   const int group = Hq / Hkv, chunks = (group + 7) / 8;
   if (num_ctas < 0 || (num_ctas && (!part_o || !part_ml || ((reinterpret_cast<uintptr_t>(part_o) | reinterpret_cast<uintptr_t>(part_ml)) & 15)))) return -3;
-  if ((!num_ctas && B > 65535) || B * (static_cast<long long>(max_blocks) * block_size / K4_STEP + 1) > 0x7fffffffll || static_cast<long long>(B) * Hkv * chunks > 0x7fffffffll) return -4;
+  if ((!num_ctas && B > 65535) || B * (static_cast<long long>(max_blocks) * block_size / K4_STEP + 1) > 0x7fffffffll || static_cast<long long>(B) * Hkv * chunks > 0x7fffffffll ||
+      static_cast<long long>(Hkv) * block_size * D * 9 / 8 > 0xffffffffll)
+    return -4;
   const K4Params p{static_cast<const __nv_bfloat16*>(q), q_stride, static_cast<const uint8_t*>(cache), num_blocks, block_table, table_stride, max_blocks, seq_lens, Hkv, group, chunks,
                    block_size, window, scale, B, num_ctas, part_o, reinterpret_cast<float2*>(part_ml), reinterpret_cast<int4*>(part_ml + static_cast<long long>(num_ctas) * 32),
                    static_cast<__nv_bfloat16*>(out), out_stride, status};
