@@ -26,7 +26,7 @@ using namespace rlb;
 
 constexpr int K4_WARPS = 4;
 constexpr int K4_STEP = 32;      // tokens a warp takes at a time: twice the 16 of an instruction
-constexpr int K4_STAGES = 3;     // steps whose words are in a warp's shared memory or on their way
+constexpr int K4_CLUSTER = 8;    // CTAs of a cluster at most
 constexpr int K4_FOLD = 16;      // steps between two corrections of the sums
 constexpr float K4_SLACK = 8.f;  // how far (in powers of two) a score may pass the running maximum before the sums are rescaled: weights stay below 2^8
 
@@ -41,7 +41,7 @@ struct K4Params {
   const int* seq_lens;
   int Hkv, G, chunks, block_size, window;
   float scale;
-  int B, num_ctas;      // num_ctas: CTAs that share all tokens evenly, or 0: one CTA per (sequence, heads)
+  int B, num_ctas, cluster;      // num_ctas: CTAs that share all tokens evenly, or 0: a cluster of `cluster` CTAs per (sequence, heads)
   float* part_o;        // [num_ctas][2] parts of 8 heads x D sums
   float2* part_ml;      // [num_ctas][2][8]
   int4* joins;          // [min(num_ctas, sequences x heads)]
@@ -126,6 +126,11 @@ __device__ __forceinline__ void copy_words(uint32_t to, const uint8_t* from) {
     for (int i = 0; i < N; i += 4) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 4 * i), "l"(from + 4 * i) : "memory");
   }
 }
+__device__ __forceinline__ float2 ld_cluster2(uint32_t from) {      // of another CTA of the cluster
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(from) : "memory");
+  return v;
+}
 // p + a * b, in one multiplication.
 __device__ __forceinline__ const uint8_t* wide(const uint8_t* p, uint32_t a, uint32_t b) { return p + static_cast<unsigned long long>(a) * b; }
 __device__ __forceinline__ float bf16_of(uint32_t word, int i) { return __uint_as_float(i & 1 ? word & 0xffff0000u : word << 16); }
@@ -135,11 +140,12 @@ template <int D>
 struct K4Stage {
   static constexpr int PART = 32 * (D / 32) * 4;      // one word per lane and group
   static constexpr int KA = 0, KB = PART, VA = 2 * PART, VB = 3 * PART, SCALES = 4 * PART, HALF = 4 * PART + 2 * D, BYTES = 2 * HALF;
+  static constexpr int COUNT = D == 64 ? 4 : D == 128 ? 3 : 2;      // steps whose words are in a warp's shared memory or on their way
 };
-// Shared memory: the warps' stages; after the token loop [warps][8 heads] rows of D + 4 sums (4 more, for the banks).
+// Shared memory: the warps' stages; after the token loop [warps][8 heads] rows of D + 4 sums (4 more, for the banks) and [8 heads][D] of the CTA.
 template <int D>
 constexpr int k4_smem() {
-  constexpr int fifo = K4_WARPS * K4_STAGES * K4Stage<D>::BYTES, red = K4_WARPS * 8 * (D + 4) * 4;
+  constexpr int fifo = K4_WARPS * K4Stage<D>::COUNT * K4Stage<D>::BYTES, red = K4_WARPS * 8 * (D + 4) * 4 + 8 * D * 4;
   return fifo > red ? fifo : red;
 }
 
@@ -179,15 +185,16 @@ __device__ __forceinline__ K4Span k4_span(const K4Params& p, int b) {
 }
 
 template <int D, bool PAIR>
-__global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_kernel(const K4Params p) {
+__global__ void __launch_bounds__(K4_WARPS * 32, D == 64 ? 4 : D == 128 ? 3 : 2) kv4_decode_kernel(const K4Params p) {
   extern __shared__ __align__(128) uint8_t k4_smem_raw[];
   __shared__ float2 ml[K4_WARPS][8];      // of each warp and column: what its weights are relative to (a power of two), and their sum
-  __shared__ int found[3], sums[K4_WARPS];
+  __shared__ float2 joined_ml[8];
+  __shared__ int found[2], sums[K4_WARPS];
   __shared__ uint4 query[PAIR ? 2 : 1][D / 32][32];      // each lane's operands of a group (PAIR: with zeros in columns 4-7, and in columns 0-3); what its products start from
   __shared__ float2 offset[D / 32][32];
   using Stage = K4Stage<D>;
   using Page = Kv4Page<D>;
-  constexpr int G = Page::G, W = G < 4 ? G : 4;      // groups of 32 dimensions; words of a load
+  constexpr int STAGES = Stage::COUNT, G = Page::G, W = G < 4 ? G : 4;      // groups of 32 dimensions; words of a load
   constexpr int NS = PAIR ? 1 : 2;                   // times 16 tokens of a step that a column stands for
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
   const int all_heads = p.Hkv * p.chunks;
@@ -195,6 +202,7 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
 
   // Which steps are this CTA's: those of one (sequence, heads), or an even share [x, x_end) of all of them in the order (heads, sequence, step).
   int b, hc, at, left = 1;             // sequence, heads, step within the sequence, steps from there on
+  uint32_t share = 0;
   if (p.num_ctas) {
     const int per = (p.B + K4_WARPS * 32 - 1) / (K4_WARPS * 32), b0 = min(p.B, static_cast<int>(threadIdx.x) * per), b1 = min(p.B, b0 + per);
     int mine = 0;
@@ -213,16 +221,15 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
       if (w < warp) upto += sums[w];
       all += sums[w];
     }
-    const long long total = static_cast<long long>(all) * all_heads, ctas = min(total, static_cast<long long>(p.num_ctas)), x = total * blockIdx.x / ctas;
-    left = blockIdx.x < ctas ? static_cast<int>(total * (blockIdx.x + 1) / ctas - x) : 0;      // (no CTA between two others is without a step: the parts stand in a row)
+    const uint32_t total = static_cast<uint32_t>(all) * all_heads, x = blockIdx.x * (share = (total + p.num_ctas - 1) / p.num_ctas);
+    left = x < total ? static_cast<int>(min(share, total - x)) : 0;
     hc = static_cast<int>(x / all);
-    int rest = static_cast<int>(x - static_cast<long long>(hc) * all) - (upto - mine);
+    int rest = static_cast<int>(x - hc * all) - (upto - mine);
     if (left && rest >= 0 && rest < mine) {      // (one thread)
       int i = b0;
       for (int n; (n = k4_span(p, i).steps) <= rest; ++i) rest -= n;
       found[0] = i;
       found[1] = rest;
-      found[2] = all;
     }
     __syncthreads();
     if (!left) {
@@ -233,7 +240,7 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
     at = found[1];
   } else {
     b = blockIdx.y;
-    hc = blockIdx.x;
+    hc = blockIdx.x / p.cluster;
     at = 0;
   }
   bool opened = false;      // whether a sequence begins here that goes on in the next CTA
@@ -242,8 +249,15 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
   const int kvh = hc / p.chunks, chunk = hc - kvh * p.chunks, heads = min(8, p.G - chunk * 8), head0 = kvh * p.G + chunk * 8;
   const int col_head = PAIR ? r & 3 : r;      // the query head of column r
   const K4Span span = k4_span(p, b);
+  int count = span.steps;
+  if (p.num_ctas) {
+    count = min(span.steps - at, left);
+  } else if (p.cluster > 1) {      // (the clusters stand in a row)
+    const int rank = blockIdx.x - hc * p.cluster;
+    at = static_cast<int>(static_cast<long long>(span.steps) * rank / p.cluster);
+    count = static_cast<int>(static_cast<long long>(span.steps) * (rank + 1) / p.cluster) - at;
+  }
   const int len = span.len, first = span.first, begin = span.step0 + at;
-  const int count = p.num_ctas ? min(span.steps - at, left) : span.steps;
   uint4 qv[G];
   {
     const __nv_bfloat16* q = p.q + static_cast<long long>(b) * p.q_stride + static_cast<long long>(head0 + col_head) * D + 8 * t;
@@ -252,53 +266,50 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
   }
   // The warp's steps are begin + warp + 4 i. Each lane knows the page of one half of a step (j = 2 i + half) among 16 of them, and of one among the 16 after.
   const int* table = p.block_table + static_cast<long long>(b) * p.table_stride;
-  const int n = len && count > warp ? (count - warp + K4_WARPS - 1) / K4_WARPS : 0;
-  auto page_of = [&](int j, int& off) -> int {
-    const int pos0 = (begin + warp + (j >> 1) * K4_WARPS) * K4_STEP + (j & 1) * 16;
-    off = 0;
-    if (j >= 2 * n || pos0 >= len) return 0;
-    const int blk = pos0 / p.block_size;
-    off = pos0 - blk * p.block_size;
-    int no = table[blk];
-    if (no < 0 || no >= p.num_blocks) {      // outside the cache: recorded, and page 0 read in its place
-      if (p.status) atomicCAS(p.status, 0, RLB_ERR_BAD_ARG);
-      no = 0;
-    }
-    return no;
+  const int pos0 = (begin + warp) * K4_STEP, n = len && count > warp ? (count - warp + K4_WARPS - 1) / K4_WARPS : 0;
+  // (Entries behind the sequence's pages may hold anything; page 0 is read in their place, and in that of a wrong one, which is recorded.)
+  auto place = [&](int j, int& off) -> int {
+    const int pos = pos0 + (j >> 1) * (K4_WARPS * K4_STEP) + (j & 1) * 16, blk = static_cast<int>(static_cast<uint32_t>(pos) / static_cast<uint32_t>(p.block_size));
+    off = pos - blk * p.block_size;
+    return blk < p.max_blocks ? table[blk] : 0;
+  };
+  auto checked = [&](int j, int no) -> int {
+    const bool mine = j < 2 * n && pos0 + (j >> 1) * (K4_WARPS * K4_STEP) + (j & 1) * 16 < len, good = static_cast<uint32_t>(no) < static_cast<uint32_t>(p.num_blocks);
+    if (mine && !good && p.status) atomicCAS(p.status, 0, RLB_ERR_BAD_ARG);
+    return (mine && good ? no : 0) * p.Hkv + kvh;
   };
   int off_now = 0, off_next = 0;
-  int page_now = page_of(lane, off_now), page_next = page_of(32 + lane, off_next);
-  const uint32_t fifo = smem_u32(k4_smem_raw) + warp * (K4_STAGES * Stage::BYTES);
+  int page_next = place(32 + lane, off_next), page_now = checked(lane, place(lane, off_now));
+  const uint32_t fifo = smem_u32(k4_smem_raw) + warp * (STAGES * Stage::BYTES);
   const int tok = 4 * (r >> 1) + (r & 1);      // of 16; the thread's other row is two tokens later
-  const uint8_t* cache = p.cache + kvh * Page::bytes(p.block_size);
-  const uint8_t *key_base = cache + Page::key_word(tok, t, 0), *value_base = cache + Page::values_at(p.block_size) + Page::value_unit(4 * t, r, 0);
-  const uint8_t* scale_base = cache + Page::scales_at(p.block_size) + lane * 16;
-  const uint32_t page_stride = static_cast<uint32_t>(p.Hkv * Page::bytes(p.block_size));
+  const uint8_t *key_base = p.cache + Page::key_word(tok, t, 0), *value_base = p.cache + Page::values_at(p.block_size) + Page::value_unit(4 * t, r, 0);
+  const uint8_t* scale_base = p.cache + Page::scales_at(p.block_size) + lane * 16;
+  const uint32_t page_bytes = static_cast<uint32_t>(Page::bytes(p.block_size));
   auto request = [&](int i) {
     if (i < n) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int src = (2 * i + h) & 31;
         const uint32_t off = __shfl_sync(0xffffffffu, off_now, src), no = __shfl_sync(0xffffffffu, page_now, src);
-        const uint8_t* keys = wide(wide(key_base, no, page_stride), off, D / 2);
-        const uint8_t* values = wide(wide(value_base, no, page_stride), off, D / 2);
-        const uint32_t to = fifo + (i % K4_STAGES) * Stage::BYTES + h * Stage::HALF;
+        const uint8_t* keys = wide(wide(key_base, no, page_bytes), off, D / 2);
+        const uint8_t* values = wide(wide(value_base, no, page_bytes), off, D / 2);
+        const uint32_t to = fifo + (i % STAGES) * Stage::BYTES + h * Stage::HALF;
         copy_words<G>(to + Stage::KA + lane * (G * 4), keys);
         copy_words<G>(to + Stage::KB + lane * (G * 4), keys + D);               // two tokens of keys
         copy_words<G>(to + Stage::VA + lane * (G * 4), values);
         copy_words<G>(to + Stage::VB + lane * (G * 4), values + D);             // one pair of tokens of values
-        if (lane < D / 8) copy_words<4>(to + Stage::SCALES + lane * 16, wide(wide(scale_base, no, page_stride), off, D / 8));
+        if (lane < D / 8) copy_words<4>(to + Stage::SCALES + lane * 16, wide(wide(scale_base, no, page_bytes), off, D / 8));
       }
-      if ((i & 15) == 15) {
-        page_now = page_next;
+      if ((i & 15) == 15) {      // (an entry is looked at 16 steps after it was asked for)
+        page_now = checked(2 * i + 2 + lane, page_next);
         off_now = off_next;
-        page_next = page_of(2 * i + 34 + lane, off_next);
+        page_next = place(2 * i + 34 + lane, off_next);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
-  for (int i = 0; i < K4_STAGES - 1; ++i) request(i);
+  for (int i = 0; i < STAGES - 1; ++i) request(i);
 
   // The queries as the 8-column operand: pair j of group g is (dimension 32 g + 8 t + j, and four later) of a head, times 2^k with the head's largest value
   // in [2^119, 2^120) (a sum of 32 stays finite), and 1/16 of that where the codes count 16 times. Scores are compared before they are scaled: a negative scale turns the
@@ -349,10 +360,10 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
   for (int g = 0; g < G / 2; ++g) z[g][0] = z[g][1] = z[g][2] = z[g][3] = 0.f;
 
   for (int i = 0; i < n; ++i) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(K4_STAGES - 2) : "memory");
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
     __syncwarp();      // the scales were copied by other lanes; and every lane has read the stage that is requested next
-    request(i + K4_STAGES - 1);
-    const uint32_t from = fifo + (i % K4_STAGES) * Stage::BYTES;
+    request(i + STAGES - 1);
+    const uint32_t from = fifo + (i % STAGES) * Stage::BYTES;
     float s[NS][4];
     uint32_t va[NS][G / 2], vb[NS][G / 2];      // the values' scales
 #pragma unroll
@@ -390,17 +401,17 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
         vb[h][g] = sb[G / 2 + g];
       }
     }
-    const int pos0 = (begin + warp + i * K4_WARPS) * K4_STEP;
-    if (pos0 < first || pos0 + K4_STEP > len) {      // (a place that was never written, or by another sequence, may hold anything)
+    const int pos = pos0 + i * (K4_WARPS * K4_STEP);
+    if (pos < first || pos + K4_STEP > len) {      // (a place that was never written, or by another sequence, may hold anything)
 #pragma unroll
       for (int h = 0; h < NS; ++h) {
-        const int at = pos0 + 16 * (PAIR ? t >> 1 : h) + tok;
-        if (at < first || at >= len) {
+        const int token = pos + 16 * (PAIR ? t >> 1 : h) + tok;
+        if (token < first || token >= len) {
           s[h][0] = s[h][1] = -INFINITY;
 #pragma unroll
           for (int g = 0; g < G / 2; ++g) va[h][g] = 0u;
         }
-        if (at + 2 < first || at + 2 >= len) {
+        if (token + 2 < first || token + 2 >= len) {
           s[h][2] = s[h][3] = -INFINITY;
 #pragma unroll
           for (int g = 0; g < G / 2; ++g) vb[h][g] = 0u;
@@ -542,6 +553,7 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
           make_float4(o[2 * g][h] * 0x1p66f * f0, o[2 * g][h + 2] * 0x1p66f * f1, o[2 * g + 1][h] * 0x1p66f * f0, o[2 * g + 1][h + 2] * 0x1p66f * f1);
   }
   __syncthreads();
+  float* joined = red + K4_WARPS * 8 * ROW;
   for (int i = threadIdx.x; i < heads * (D / 4); i += K4_WARPS * 32) {
     const int head = i / (D / 4), d = i % (D / 4) * 4;
     float m = part_of(head, 0).x, l = 0.f;
@@ -555,7 +567,10 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
       const float4 v = *reinterpret_cast<const float4*>(red + (PAIR ? (w >> 1) * 8 + head + 4 * (w & 1) : w * 8 + head) * ROW + d);
       acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
     }
-    if (count == span.steps) {
+    if (p.cluster > 1) {
+      *reinterpret_cast<float4*>(joined + head * D + d) = acc;
+      if (d == 0) joined_ml[head] = make_float2(m, l);
+    } else if (count == span.steps) {
       const float inv = l == 0.f ? 0.f : 1.f / l;
       *reinterpret_cast<uint2*>(p.out + static_cast<long long>(b) * p.out_stride + static_cast<long long>(head0 + head) * D + d) =
           make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
@@ -565,15 +580,45 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
       if (d == 0) p.part_ml[part * 8 + head] = make_float2(m, l);
     }
   }
+  if (p.cluster > 1) {      // each CTA of the cluster writes its share of the output, from what all of them have
+    cluster_sync();
+    const uint32_t sums_at = smem_u32(joined), ml_at = smem_u32(joined_ml);
+    for (int i = (blockIdx.x - hc * p.cluster) * (K4_WARPS * 32) + threadIdx.x; i < heads * (D / 4); i += p.cluster * (K4_WARPS * 32)) {
+      const int head = i / (D / 4), d = i % (D / 4) * 4;
+      float2 parts[K4_CLUSTER];
+      float m = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int c = 0; c < K4_CLUSTER; ++c)
+        if (c < p.cluster) {
+          parts[c] = ld_cluster2(mapa_shared(ml_at + head * 8, c));
+          m = fmaxf(m, parts[c].x);
+        }
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < K4_CLUSTER; ++c)
+        if (c < p.cluster) {
+          const float f = parts[c].x == -INFINITY ? 1.f : exp2_fast(parts[c].x - m);
+          const uint32_t from = mapa_shared(sums_at + (head * D + d) * 4, c);
+          const float2 u = ld_cluster2(from), v = ld_cluster2(from + 8);
+          l = fmaf(parts[c].y, f, l);
+          acc.x = fmaf(u.x, f, acc.x);
+          acc.y = fmaf(u.y, f, acc.y);
+          acc.z = fmaf(v.x, f, acc.z);
+          acc.w = fmaf(v.y, f, acc.w);
+        }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      *reinterpret_cast<uint2*>(p.out + static_cast<long long>(b) * p.out_stride + static_cast<long long>(head0 + head) * D + d) =
+          make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+    }
+    cluster_sync();      // (the others may still read this CTA's sums)
+  }
   if (!p.num_ctas) return;
   // A sequence that begins here is joined from this CTA's part and those of the CTAs up to the one that has its last step.
   if (at == 0) {
     int4 job = make_int4(-1, 0, 0, 0);
     if (count < span.steps) {
       opened = true;
-      const long long total = static_cast<long long>(found[2]) * all_heads, ctas = min(total, static_cast<long long>(p.num_ctas));
-      const long long past = total * (blockIdx.x + 1) / ctas - count + span.steps;
-      job = make_int4(static_cast<int>(blockIdx.x), static_cast<int>((past * ctas - 1) / total), b, hc);
+      job = make_int4(static_cast<int>(blockIdx.x), static_cast<int>(((blockIdx.x + 1) * share - count + span.steps - 1) / share), b, hc);
     }
     if (threadIdx.x == 0) {
       if (p.B * all_heads <= p.num_ctas) p.joins[hc * p.B + b] = job;
@@ -592,63 +637,71 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D <= 128 ? 3 : 2) kv4_decode_ke
   if (threadIdx.x == 0 && !opened && p.B * all_heads > p.num_ctas) p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
 }
 
-// Joins the parts of the sequences that several CTAs shared: a CTA per possible one, a warp per head and fourth part.
-template <int D>
-__global__ void __launch_bounds__(1024) kv4_join_kernel(const K4Params p) {
-  __shared__ float4 red[3][8][D / 4];
-  __shared__ float reds[4][8];
+// Joins the parts of the sequences that several CTAs shared. Few sequences: a CTA per sequence and head, whose eight warps take every eighth part. More than CTAs: at most
+// one sequence begins in a CTA and ends in another, most of two parts; a CTA each, a warp per head.
+template <int D, bool FEW>
+__global__ void __launch_bounds__(256) kv4_join_kernel(const K4Params p) {
+  __shared__ float4 red[FEW ? 8 : 1][D / 4];
+  __shared__ float reds[8];
+  constexpr int V = D / 128 > 0 ? D / 128 : 1, BY = FEW ? 8 : 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, head = FEW ? blockIdx.y : warp;
   pdl_sync();
   const int4 job = p.joins[blockIdx.x];      // first and last CTA, sequence, heads
-  if (job.x < 0) return;
-  const int head = threadIdx.x >> 5 & 7, quarter = threadIdx.x >> 8, lane = threadIdx.x & 31, n = job.y - job.x + 1;
+  const int kvh = job.w / p.chunks, chunk = job.w - kvh * p.chunks;
+  if (job.x < 0 || head >= min(8, p.G - chunk * 8)) return;      // (FEW: the whole CTA)
+  const int n = job.y - job.x + 1;
   auto part = [&](int i) { return (static_cast<long long>(job.x + i) * 2 + (i == 0)) * 8 + head; };
   float m = -INFINITY;
   for (int i = lane; i < n; i += 32) m = fmaxf(m, p.part_ml[part(i)].x);
   m = warp_max(m);
-  constexpr int V = D / 128 > 0 ? D / 128 : 1;
   float4 acc[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
   float l = 0.f;
 #pragma unroll 4
-  for (int i = quarter; i < n; i += 4) {
-    const long long at = part(i);
-    const float2 w = p.part_ml[at];
+  for (int i = FEW ? warp : 0; i < n; i += BY) {
+    const long long from = part(i);
+    const float2 w = p.part_ml[from];
     const float f = w.x == -INFINITY ? 1.f : exp2_fast(w.x - m);      // (a part without a finite score has no tokens, or NaN)
     l += w.y * f;
 #pragma unroll
     for (int v = 0; v < V; ++v)
       if (lane + 32 * v < D / 4) {
-        const float4 o = reinterpret_cast<const float4*>(p.part_o + at * D)[lane + 32 * v];
+        const float4 o = reinterpret_cast<const float4*>(p.part_o + from * D)[lane + 32 * v];
         acc[v].x = fmaf(o.x, f, acc[v].x);
         acc[v].y = fmaf(o.y, f, acc[v].y);
         acc[v].z = fmaf(o.z, f, acc[v].z);
         acc[v].w = fmaf(o.w, f, acc[v].w);
       }
   }
-  if (lane == 0) reds[quarter][head] = l;
-  if (quarter) {
+  if constexpr (FEW) {
+    if (lane == 0) reds[warp] = l;
 #pragma unroll
     for (int v = 0; v < V; ++v)
-      if (lane + 32 * v < D / 4) red[quarter - 1][head][lane + 32 * v] = acc[v];
+      if (lane + 32 * v < D / 4) red[warp][lane + 32 * v] = acc[v];
+    __syncthreads();
+    if (warp >= V) return;
+    l = 0.f;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) l += reds[q];
   }
-  __syncthreads();
-  const int kvh = job.w / p.chunks, chunk = job.w - kvh * p.chunks;
-  if (quarter || head >= min(8, p.G - chunk * 8)) return;
-  l = (reds[0][head] + reds[1][head]) + (reds[2][head] + reds[3][head]);
   const float inv = l == 0.f ? 0.f : 1.f / l;
   __nv_bfloat16* out = p.out + job.z * p.out_stride + static_cast<long long>(kvh * p.G + chunk * 8 + head) * D;
 #pragma unroll
-  for (int v = 0; v < V; ++v)
-    if (lane + 32 * v < D / 4) {
-      float4 o = acc[v];
+  for (int v = 0; v < V; ++v) {
+    const int d = lane + 32 * (FEW ? warp : v);
+    if (d >= D / 4 || (FEW && v)) continue;
+    float4 o = acc[v];
+    if constexpr (FEW) {
+      o = red[0][d];
 #pragma unroll
-      for (int q = 0; q < 3; ++q) {
-        const float4 w = red[q][head][lane + 32 * v];
+      for (int q = 1; q < 8; ++q) {
+        const float4 w = red[q][d];
         o.x += w.x; o.y += w.y; o.z += w.z; o.w += w.w;
       }
-      reinterpret_cast<uint2*>(out)[lane + 32 * v] = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
     }
+    reinterpret_cast<uint2*>(out)[d] = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+  }
 }
 
 template <int D, bool PAIR>
@@ -663,32 +716,52 @@ int launch_decode(const K4Params& p, cudaStream_t stream) {
     ready.fetch_or(1ull << (dev & 63));
   }
   const int all_heads = p.Hkv * p.chunks;
-  const dim3 grid = p.num_ctas ? dim3(p.num_ctas) : dim3(all_heads, p.B);
-  rlb_launch_pdl(kv4_decode_kernel<D, PAIR>, grid, dim3(K4_WARPS * 32), k4_smem<D>(), stream, p);
-  e = cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = p.num_ctas ? dim3(p.num_ctas) : dim3(all_heads * p.cluster, p.B);
+  cfg.blockDim = dim3(K4_WARPS * 32);
+  cfg.dynamicSmemBytes = k4_smem<D>();
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  unsigned n = 0;
+  if (p.cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = p.cluster;
+    attr[n].val.clusterDim.y = 1;
+    attr[n++].val.clusterDim.z = 1;
+  }
+  if (rlb_pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  e = cudaLaunchKernelEx(&cfg, kv4_decode_kernel<D, PAIR>, p);
   if (e != cudaSuccess || !p.num_ctas) return static_cast<int>(e);
   const long long segments = static_cast<long long>(p.B) * all_heads;
-  rlb_launch_pdl(kv4_join_kernel<D>, dim3(static_cast<unsigned>(segments < p.num_ctas ? segments : p.num_ctas)), dim3(1024), 0, stream, p);
+  if (segments <= p.num_ctas) rlb_launch_pdl(kv4_join_kernel<D, true>, dim3(static_cast<unsigned>(segments), p.G < 8 ? p.G : 8), dim3(256), 0, stream, p);
+  else rlb_launch_pdl(kv4_join_kernel<D, false>, dim3(p.num_ctas), dim3(256), 0, stream, p);
   return static_cast<int>(cudaGetLastError());
 }
 }  // namespace
 
-// q [B, >= Hq D] bf16, 16-byte aligned rows; block_table [B, max_blocks] int32; seq_lens [B]; out: 8-byte aligned rows. num_ctas: 0, or CTAs that share all
-// tokens evenly, with scratch part_o [num_ctas 16 D] and part_ml [num_ctas 36] fp32 (16-byte aligned).
+// q [B, >= Hq D] bf16, 16-byte aligned rows; block_table [B, max_blocks] int32; seq_lens [B]; out: 8-byte aligned rows. num_ctas: 0, for a cluster of `cluster` (1 to
+// 8) CTAs per sequence and key/value head (and eight query heads), or CTAs that share all tokens evenly (cluster 1), with scratch part_o [num_ctas 16 D] and part_ml [num_ctas 36] fp32 (16-byte aligned).
 RLB_API int rlb_kv4_paged_decode(const void* q, long long q_stride, const void* cache, long long num_blocks, const int* block_table, long long table_stride, int max_blocks,
-                                 const int* seq_lens, int B, int Hq, int Hkv, int D, int block_size, int window, float scale, int num_ctas, float* part_o, float* part_ml, void* out,
+                                 const int* seq_lens, int B, int Hq, int Hkv, int D, int block_size, int window, float scale, int cluster, int num_ctas, float* part_o, float* part_ml, void* out,
                                  long long out_stride, int* status, void* stream) {
   if ((D != 64 && D != 128 && D != 256) || Hkv < 1 || Hq < 1 || Hq % Hkv || block_size < 16 || block_size % 16 || block_size > KV4_MAX_BLOCK || window < 0) return -2;
   if (q_stride % 8 || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache)) & 15)) return -2;
   if (out_stride % 4 || (reinterpret_cast<uintptr_t>(out) & 7)) return -2;
   if (B <= 0) return 0;
   const int group = Hq / Hkv, chunks = (group + 7) / 8;
+  if (cluster < 1 || cluster > K4_CLUSTER || (num_ctas && cluster != 1)) return -3;
   if (num_ctas < 0 || (num_ctas && (!part_o || !part_ml || ((reinterpret_cast<uintptr_t>(part_o) | reinterpret_cast<uintptr_t>(part_ml)) & 15)))) return -3;
-  if ((!num_ctas && B > 65535) || B * (static_cast<long long>(max_blocks) * block_size / K4_STEP + 1) > 0x7fffffffll || static_cast<long long>(B) * Hkv * chunks > 0x7fffffffll ||
-      static_cast<long long>(Hkv) * block_size * D * 9 / 8 > 0xffffffffll)
+  if (static_cast<long long>(max_blocks) * block_size > 0x7fff0000ll || (!num_ctas && B > 65535) ||
+      (num_ctas && static_cast<long long>(B) * Hkv * chunks * (static_cast<long long>(max_blocks) * block_size / K4_STEP + 2) + num_ctas > 0x7fffffffll) || static_cast<long long>(B) * Hkv * chunks > 0x7fffffffll || static_cast<long long>(Hkv) * chunks * cluster > 0x7fffffffll ||
+      num_blocks * Hkv > 0x7fffffffll)
     return -4;
   const K4Params p{static_cast<const __nv_bfloat16*>(q), q_stride, static_cast<const uint8_t*>(cache), num_blocks, block_table, table_stride, max_blocks, seq_lens, Hkv, group, chunks,
-                   block_size, window, scale, B, num_ctas, part_o, reinterpret_cast<float2*>(part_ml), reinterpret_cast<int4*>(part_ml + static_cast<long long>(num_ctas) * 32),
+                   block_size, window, scale, B, num_ctas, cluster, part_o, reinterpret_cast<float2*>(part_ml), reinterpret_cast<int4*>(part_ml + static_cast<long long>(num_ctas) * 32),
                    static_cast<__nv_bfloat16*>(out), out_stride, status};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (group <= 4) return D == 64 ? launch_decode<64, true>(p, s) : D == 128 ? launch_decode<128, true>(p, s) : launch_decode<256, true>(p, s);

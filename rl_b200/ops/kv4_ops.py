@@ -24,13 +24,15 @@ from .lib import call, ptr, use_native
 _P, _I, _LL, _F = _L.P, _L.I, _L.L, _L.F
 _L.register("rlb_rope_kv4_cache_write", [_P, _P, _P, _P, _P, _LL, _I, _I, _I, _I, _LL, _LL, _P, _P])
 _L.register("rlb_kv4_cache_read", [_P, _P, _P, _P, _LL, _LL, _LL, _I, _I, _I, _LL, _P, _P])
-_L.register("rlb_kv4_paged_decode", [_P, _LL, _P, _LL, _P, _LL, _I, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P, _LL, _P, _P])
+_L.register("rlb_kv4_paged_decode", [_P, _LL, _P, _LL, _P, _LL, _I, _P, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P, _P, _P, _LL, _P, _P])
 
 BF16 = torch.bfloat16
 HEAD_DIMS = (64, 128, 256)
 GROUP = 32
 TINY = 2.0 ** -100
 MAX_BLOCK = 65536
+MAX_CLUSTER = 8
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else lambda index: torch.cuda.current_stream(index).cuda_stream
 
 
 def kv4_page_bytes(block_size: int, D: int) -> int:
@@ -166,14 +168,14 @@ def rope_kv4_cache_write(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: t
         return out
     if qkv.dtype is not BF16:
         raise ValueError(f"the 4-bit cache takes bf16 rows, not {qkv.dtype}")
-    stream = torch.cuda.current_stream()
-    if stream.device_index != qkv.device.index:      # kernels go to the current stream of the tensors' device, whichever device is current
+    index = qkv.device.index
+    if torch.cuda.current_device() != index:      # kernels go to the current stream of the tensors' device, whichever device is current
         with torch.cuda.device(qkv.device):
             return rope_kv4_cache_write(qkv, positions, inv_freq, slots, cache, Hq, Hkv, D)
     rows = qkv if _aligned(qkv) else qkv.clone(memory_format=torch.contiguous_format)      # (rows that do not start on 16 bytes: turned in a copy)
     inv_freq = inv_freq.contiguous()
-    call("rlb_rope_kv4_cache_write", ptr(rows), ptr(positions), ptr(inv_freq), ptr(slots), ptr(cache), T, Hq, Hkv, D, block, rows.stride(0), cache.shape[0],
-         ptr(_L.status_word(qkv.device)), stream.cuda_stream)
+    call("rlb_rope_kv4_cache_write", rows.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), slots.data_ptr(), cache.data_ptr(), T, Hq, Hkv, D, block,
+         rows.stride(0), cache.shape[0], _L.status_word(qkv.device).data_ptr(), _raw_stream(index))
     if rows is not qkv:
         qkv.copy_(rows)
     return qkv
@@ -207,47 +209,59 @@ def kv4_cache_read(cache: torch.Tensor, slots: torch.Tensor, Hkv: int, D: int, *
         return out
     if out.dtype is not BF16:
         raise ValueError(f"the 4-bit cache is read into bf16 rows, not {out.dtype}")
-    stream = torch.cuda.current_stream()
-    if stream.device_index != device.index:
+    index = device.index
+    if torch.cuda.current_device() != index:
         with torch.cuda.device(device):
             return kv4_cache_read(cache, slots, Hkv, D, out=out, rows=rows)
     to = out
     if not _aligned(out):      # rows that do not start on 16 bytes: read into a copy
         to = torch.empty((out.shape[0], width), dtype=BF16, device=device).copy_(out[:, :width])
-    call("rlb_kv4_cache_read", ptr(cache), ptr(slots), ptr(rows), ptr(to), n, to.stride(0), to.shape[0], Hkv, D, block, cache.shape[0],
-         ptr(_L.status_word(device)), stream.cuda_stream)
+    call("rlb_kv4_cache_read", cache.data_ptr(), slots.data_ptr(), ptr(rows), to.data_ptr(), n, to.stride(0), to.shape[0], Hkv, D, block, cache.shape[0],
+         _L.status_word(device).data_ptr(), _raw_stream(index))
     if to is not out:
         out[:, :width] = to
     return out
 
 
-def kv4_ctas(B: int, Hq: int, Hkv: int, D: int, max_len: int, sm_count: int = 148) -> int:
-    """CTAs that share the tokens of decode attention over the 4-bit cache evenly: as many as the device holds at a time, none with less than 256 tokens.
-    0: one per sequence and heads, without a second kernel that joins parts, where sequences have no more than that."""
-    if max_len <= 256:
-        return 0
-    work = max(1, B) * Hkv * -(-(Hq // Hkv) // 8) * (-(-max_len // 256))
-    return min((3 if D <= 128 else 2) * sm_count, work)
+@lru_cache(maxsize=4096)
+def kv4_plan(B: int, Hq: int, Hkv: int, D: int, max_len: int, sm_count: int = 148) -> tuple[int, int]:
+    """How decode attention over the 4-bit cache is cut up: (cluster, 0): a cluster of CTAs per sequence and key/value head (with up to eight query
+    heads), or (1, n): n CTAs, as many as the device holds, share all tokens evenly, and a second kernel joins what they cut through.
+
+    Sharing costs some 4 us and pays off for sequences of 3200 tokens and more (8 KV heads of 128, four query heads each, us in a graph, one CTA each / shared: 64
+    sequences of 16000 tokens 259 / 222, of 4000 73 / 70, of 1280 30 / 34; 16 of 4000 29 / 27, of 1000 11 / 16), where there are no more than two CTAs for each that
+    the device holds (128 of 4000: 118 / 125). Few sequences are cut into a cluster of at least eight steps of 32 tokens per CTA, one CTA on most SMs
+    (us with one, four, eight CTAs: one sequence of 1000 tokens 9.7, 7.0, 6.6, of 4000 27, 12, 9.4 and shared 14; four of 4000 28, 14, 14 and shared 16; 16 of 1000
+    11, 18, 24)."""
+    segments, steps = max(1, B) * Hkv * -(-(Hq // Hkv) // 8), -(-max_len // 32)
+    slots = (3 if D > 64 else 4) * sm_count if D <= 128 else 2 * sm_count
+    if steps >= 100 and segments < 2 * slots and (steps >= 400 or steps * segments >= 10000) and segments * (steps + 2) < 2**30:
+        return 1, slots
+    cluster = 1
+    while cluster < MAX_CLUSTER and 2 * cluster * segments <= 200 and 16 * cluster <= steps:
+        cluster *= 2
+    return cluster, 0
 
 
-def kv4_scratch_sizes(num_ctas: int, D: int) -> tuple[int, int]:
-    """Floats of the two scratch tensors of :func:`kv4_paged_decode` with this many CTAs."""
-    return num_ctas * 16 * D, num_ctas * 36
+def kv4_scratch_size(num_ctas: int, D: int) -> int:
+    """Floats of the scratch tensor of :func:`kv4_paged_decode` with this many CTAs."""
+    return num_ctas * (16 * D + 36)
 
 
 def kv4_paged_decode(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, Hq: int, Hkv: int, D: int, *,
-                     scale: Optional[float] = None, window: int = 0, num_ctas: Optional[int] = None,
-                     scratch: Optional[tuple[torch.Tensor, torch.Tensor]] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                     scale: Optional[float] = None, window: int = 0, plan: Optional[tuple[int, int]] = None,
+                     scratch: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of one query token per sequence, ``q`` [B, >= Hq D] (rows may be strided: the fused rows do), against the 4-bit ``cache``:
     ``seq_lens`` [B] int32 tokens in the pages that ``block_table`` [B, pages] int32 names, of which ``window`` > 0 leaves the last ``window``. A
-    sequence without tokens gives zeros. ``num_ctas``: CTAs that share the work evenly, 0: one per sequence and heads (None: by :func:`kv4_ctas` from the
-    table's width); ``scratch``: fp32 tensors of :func:`kv4_scratch_sizes` elements, for callers that keep their own. Returns [B, Hq D]."""
+    sequence without tokens gives zeros. ``plan``: (cluster, num_ctas): a cluster of up to eight CTAs per sequence and key/value head, or with (1, n) n CTAs
+    that share all tokens evenly (None: :func:`kv4_plan` for the table's width); ``scratch``: float32 tensor of :func:`kv4_scratch_size` elements, for callers that
+    keep their own. Returns [B, Hq D]."""
     block = _block_size(cache, Hkv, D)
     device, width = q.device, Hq * D
     if Hq < 1 or Hq % Hkv or q.dim() != 2 or q.shape[1] < width:
         raise ValueError(f"q is [B, {width}] with {Hq} heads, a multiple of {Hkv}, not {tuple(q.shape)}")
-    if window < 0 or (num_ctas or 0) < 0:
-        raise ValueError(f"window {window} or num_ctas {num_ctas} is negative")
+    if window < 0:
+        raise ValueError(f"window {window} is negative")
     B = q.shape[0]
     _same_device(device, cache, block_table, seq_lens)
     if block_table.dim() != 2:
@@ -279,26 +293,31 @@ def kv4_paged_decode(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
         return out
     if q.dtype is not BF16:
         raise ValueError(f"the 4-bit cache takes bf16 queries, not {q.dtype}")
-    stream = torch.cuda.current_stream()
-    if stream.device_index != device.index:
+    if plan is None:
+        plan = kv4_plan(B, Hq, Hkv, D, min(pages * block, window) if window else pages * block)
+    cluster, num_ctas = plan
+    if not 1 <= cluster <= MAX_CLUSTER or num_ctas < 0 or (num_ctas and cluster != 1):
+        raise ValueError(f"plan {plan} is neither (1 to {MAX_CLUSTER}, 0) nor (1, CTAs)")
+    if num_ctas:
+        size = kv4_scratch_size(num_ctas, D)
+        if scratch is None:
+            scratch = torch.empty(size, dtype=torch.float32, device=device)
+        elif scratch.dtype is not torch.float32 or not scratch.is_contiguous() or scratch.numel() < size or scratch.data_ptr() % 16 or scratch.device != device:
+            raise ValueError(f"scratch is a contiguous float32 tensor of {size} elements on {device} that starts on 16 bytes")
+        sums = scratch.data_ptr()
+        parts = sums + num_ctas * 64 * D
+    else:
+        sums = parts = None
+    index = device.index
+    if torch.cuda.current_device() != index:
         with torch.cuda.device(device):
-            return kv4_paged_decode(q, cache, table, lens, Hq, Hkv, D, scale=scale, window=window, num_ctas=num_ctas, scratch=scratch, out=out)
+            return kv4_paged_decode(q, cache, table, lens, Hq, Hkv, D, scale=scale, window=window, plan=plan, scratch=scratch, out=out)
     if not _aligned(q):      # rows that do not start on 16 bytes
         q = q[:, :width].clone(memory_format=torch.contiguous_format)
-    if num_ctas is None:
-        num_ctas = kv4_ctas(B, Hq, Hkv, D, min(pages * block, window) if window else pages * block)
-    po = pml = None
-    if num_ctas:
-        no, nml = kv4_scratch_sizes(num_ctas, D)
-        if scratch is None:
-            scratch = torch.empty(no, dtype=torch.float32, device=device), torch.empty(nml, dtype=torch.float32, device=device)
-        po, pml = scratch
-        _same_device(device, po, pml)
-        if any(t.dtype is not torch.float32 or not t.is_contiguous() or t.numel() < size or t.data_ptr() % 16 for t, size in ((po, no), (pml, nml))):
-            raise ValueError(f"scratch is two contiguous float32 tensors of {no} and {nml} elements that start on 16 bytes")
-    to = out if out.stride(1) == 1 and out.stride(0) % 4 == 0 and out.data_ptr() % 8 == 0 else torch.empty((B, width), dtype=BF16, device=device)
-    call("rlb_kv4_paged_decode", ptr(q), q.stride(0), ptr(cache), cache.shape[0], ptr(table), table.stride(0), pages, ptr(lens), B, Hq, Hkv, D, block, window, scale,
-         num_ctas, ptr(po), ptr(pml), ptr(to), to.stride(0), ptr(_L.status_word(device)), stream.cuda_stream)
+    stride = out.stride()
+    to = out if stride[1] == 1 and stride[0] % 4 == 0 and out.data_ptr() % 8 == 0 else torch.empty((B, width), dtype=BF16, device=device)
+    call("rlb_kv4_paged_decode", q.data_ptr(), q.stride(0), cache.data_ptr(), cache.shape[0], table.data_ptr(), table.stride(0), pages, lens.data_ptr(), B, Hq, Hkv,
+         D, block, window, scale, cluster, num_ctas, sums, parts, to.data_ptr(), to.stride(0), _L.status_word(device).data_ptr(), _raw_stream(index))
     if to is not out:
         out.copy_(to)
     return out

@@ -127,7 +127,7 @@ def _check(got, q, cache, table, lens, Hq, Hkv, D, window=0, scale=None):
     """Every output within what the roundings give: the result's to bf16 (2^-8 of it), each token's weight times its scale to bf16 (2^-8 of
     the token's share), and the scores' to 32 bits. A score's sum over a group has 32 terms of at most 15 |q| and the offset of 7.5 times the sum of the query's values: 33
     roundings at that size, times the key's scale; a score's error e changes a weight by e and the sum by as much."""
-    block, B = cache.shape[2] * 8 // (9 * D), q.shape[0]
+    block, B = cache.shape[2] * 8 // (9 * D), got.shape[0]
     scale = scale or 1 / math.sqrt(D)
     for b in range(B):
         n = int(lens[b])
@@ -168,19 +168,19 @@ LENGTHS = [[1], [0], [2, 15, 16, 17, 0, 31, 33], [63, 64, 65, 1, 127, 128, 129],
 def test_decode(native_lib, lens, D, Hq, Hkv):
     for block in (16, 64) if D != 128 else (48, 128):
         q, cache, table, n = _decode_case(lens, Hq, Hkv, D, block, seed=len(lens))
-        for ctas in (None, 0, 1, 5, 37):
-            got = K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, num_ctas=ctas)
+        for plan in (None, (1, 0), (3, 0), (8, 0), (1, 1), (1, 5), (1, 37)):
+            got = K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, plan=plan)
             assert L.check_status() == 0
             _check(got, q, cache, table, n, Hq, Hkv, D)
-            assert torch.equal(got, K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, num_ctas=ctas))      # the same bits again
+            assert torch.equal(got, K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, plan=plan))      # the same bits again
 
 
 @pytest.mark.parametrize("window", [1, 5, 16, 100, 5000])
 @pytest.mark.parametrize("D,Hq,Hkv", [(64, 14, 2), (128, 8, 2), (256, 8, 4)])
 def test_decode_window(native_lib, window, D, Hq, Hkv):
     q, cache, table, n = _decode_case([1, 17, 100, 0, 1000, 333, 16], Hq, Hkv, D, 32, seed=window)
-    for ctas in (None, 0, 3, 40):
-        _check(K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, window=window, num_ctas=ctas), q, cache, table, n, Hq, Hkv, D, window)
+    for plan in (None, (1, 0), (2, 0), (7, 0), (1, 3), (1, 40)):
+        _check(K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, window=window, plan=plan), q, cache, table, n, Hq, Hkv, D, window)
     assert L.check_status() == 0
 
 
@@ -188,12 +188,12 @@ def test_decode_window(native_lib, window, D, Hq, Hkv):
 def test_decode_of_small_large_and_peaked(native_lib, big, scale):
     """Values far from one, and scores of hundreds: one token takes nearly all."""
     q, cache, table, n = _decode_case([700, 33, 260], 8, 2, 128, 64, seed=5, big=big)
-    for ctas in (0, 7):
-        _check(K.kv4_paged_decode(q, cache, table, n, 8, 2, 128, scale=scale, num_ctas=ctas), q, cache, table, n, 8, 2, 128, scale=scale)
+    for plan in ((1, 0), (4, 0), (1, 7)):
+        _check(K.kv4_paged_decode(q, cache, table, n, 8, 2, 128, scale=scale, plan=plan), q, cache, table, n, 8, 2, 128, scale=scale)
 
 
-@pytest.mark.parametrize("ctas", [0, 2, 33])
-def test_decode_ignores_what_stands_behind_the_end(native_lib, ctas):
+@pytest.mark.parametrize("plan", [(1, 0), (5, 0), (1, 2), (1, 33)])
+def test_decode_ignores_what_stands_behind_the_end(native_lib, plan):
     """NaN and infinite scales, and any codes, in places that the sequence does not see: before the window and behind its last token."""
     Hq, Hkv, D, block, lens, window = 8, 2, 128, 64, [70, 129, 1, 64, 300], 50
     q, cache, table, n = _decode_case(lens, Hq, Hkv, D, block, seed=3)
@@ -204,8 +204,8 @@ def test_decode_ignores_what_stands_behind_the_end(native_lib, ctas):
             s = page[:, block * D :].view(torch.bfloat16).view(Hkv, block, 8)
             s[:, off] = torch.tensor([math.nan, math.inf, -math.inf, 3e38] * 2, device="cuda").bfloat16()
             page[:, : block * D // 2].view(Hkv, block, -1)[:, off] = 0xA5
-    want = K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, window=window, num_ctas=ctas)
-    got = K.kv4_paged_decode(q, dirty, table, n, Hq, Hkv, D, window=window, num_ctas=ctas)
+    want = K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, window=window, plan=plan)
+    got = K.kv4_paged_decode(q, dirty, table, n, Hq, Hkv, D, window=window, plan=plan)
     assert got.isfinite().all() and torch.equal(got, want)
 
 
@@ -213,12 +213,12 @@ def test_decode_hands_on_what_is_not_finite(native_lib):
     """A visible key with a NaN scale makes its heads NaN, a value's its group; other heads and sequences keep their numbers."""
     Hq, Hkv, D, block = 4, 2, 128, 16
     q, cache, table, n = _decode_case([40, 40], Hq, Hkv, D, block, seed=9)
-    for ctas in (0, 3):
-        clean = K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, num_ctas=ctas)
+    for plan in ((1, 0), (2, 0), (1, 3)):
+        clean = K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, plan=plan)
         for value, group in ((0, 2), (1, 1)):
             c = cache.clone()
             c[int(table[1, 1]), 1, block * D :].view(torch.bfloat16).view(block, 2, 4)[3, value, group] = math.nan
-            got = K.kv4_paged_decode(q, c, table, n, Hq, Hkv, D, num_ctas=ctas).view(2, Hq, D)
+            got = K.kv4_paged_decode(q, c, table, n, Hq, Hkv, D, plan=plan).view(2, Hq, D)
             nan = torch.zeros(2, Hq, D, dtype=torch.bool, device="cuda")
             nan[1, 2:, slice(None) if value == 0 else slice(32, 64)] = True
             assert torch.equal(got.isnan(), nan) and torch.equal(got[~nan], clean.view(2, Hq, D)[~nan])
@@ -237,11 +237,14 @@ def test_decode_of_odd_views(native_lib):
         got = K.kv4_paged_decode(odd, cache, table.long().t().contiguous().t(), n.long(), Hq, Hkv, D, out=out)
         assert got is out and torch.equal(out, want) and int((wide == 7).sum()) >= 4 * Hq * D
     assert K.kv4_paged_decode(q[:0], cache, table[:0], n[:0], Hq, Hkv, D).shape == (0, Hq * D)
-    scratch = tuple(torch.empty(s + 3, device="cuda") for s in K.kv4_scratch_sizes(3, D))
-    _check(K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, num_ctas=3, scratch=scratch), q, cache, table, n, Hq, Hkv, D)
-    for bad in ((scratch[0][:-4], scratch[1]), (scratch[0].double(), scratch[1]), (scratch[0], scratch[1].cpu()), (scratch[0][1:], scratch[1])):
+    scratch = torch.empty(K.kv4_scratch_size(3, D) + 4, device="cuda")
+    _check(K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, plan=(1, 3), scratch=scratch), q, cache, table, n, Hq, Hkv, D)
+    for bad in (scratch[:-5], scratch.double(), scratch.cpu(), scratch[1:], scratch[::2]):
         with pytest.raises(ValueError):
-            K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, num_ctas=3, scratch=bad)
+            K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, plan=(1, 3), scratch=bad)
+    for bad in ((0, 0), (9, 0), (2, 5), (1, -1)):
+        with pytest.raises(ValueError):
+            K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, plan=bad)
     for bad in (q.float(), q.half(), q.cpu()):
         with pytest.raises(ValueError):
             K.kv4_paged_decode(bad, cache, table, n, Hq, Hkv, D)
@@ -255,17 +258,18 @@ def test_bad_pages_and_lengths_are_reported(native_lib):
     """Page numbers outside the cache are left out, lengths beyond the table end there: an error is on record and nothing else is read."""
     Hq, Hkv, D, block = 8, 2, 128, 16
     q, cache, table, n = _decode_case([64, 64], Hq, Hkv, D, block)
-    for ctas in (0, 3):
-        want = K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, num_ctas=ctas)
+    for plan in ((1, 0), (2, 0), (1, 3)):
+        want = K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, plan=plan)
         for page in (-1, cache.shape[0], 2**31 - 1):
             bad = table.clone()
             bad[1, 2] = page
-            got = K.kv4_paged_decode(q, cache, bad, n, Hq, Hkv, D, num_ctas=ctas)
+            got = K.kv4_paged_decode(q, cache, bad, n, Hq, Hkv, D, plan=plan)
             assert L.check_status() == 6 and torch.equal(got[0], want[0]) and got.isfinite().all()
-        got = K.kv4_paged_decode(q, cache, table[:, :4], torch.tensor([64, 2**31 - 1], dtype=torch.int32, device="cuda"), Hq, Hkv, D, num_ctas=ctas)
+        got = K.kv4_paged_decode(q, cache, table[:, :4], torch.tensor([64, 2**31 - 1], dtype=torch.int32, device="cuda"), Hq, Hkv, D, plan=plan)
         assert L.check_status() == 6 and torch.equal(got, want)
-        got = K.kv4_paged_decode(q, cache, table, torch.tensor([64, -5], dtype=torch.int32, device="cuda"), Hq, Hkv, D, num_ctas=ctas)
-        assert L.check_status() == 0 and torch.equal(got[0], want[0]) and not got[1].any()
+        got = K.kv4_paged_decode(q, cache, table, torch.tensor([64, -5], dtype=torch.int32, device="cuda"), Hq, Hkv, D, plan=plan)
+        assert L.check_status() == 0 and not got[1].any()
+        _check(got[:1], q, cache, table, n, Hq, Hkv, D)
 
 
 def test_places_beyond_32_bits(native_lib):
@@ -301,20 +305,20 @@ def test_graphs_and_streams(native_lib):
     freq = _freq(D).cuda()
     state = dict(rows=q.clone(), pos=n.long() - 1, lens=n.clone())
 
-    def step(c, ctas):
+    def step(c, plan):
         slots = table[torch.arange(B, device="cuda"), state["pos"] // block].long() * block + state["pos"] % block
         rows = K.rope_kv4_cache_write(state["rows"].clone(), state["pos"], freq, slots, c, Hq, Hkv, D)
-        return K.kv4_paged_decode(rows, c, table, state["lens"], Hq, Hkv, D, num_ctas=ctas)
+        return K.kv4_paged_decode(rows, c, table, state["lens"], Hq, Hkv, D, plan=plan)
 
-    caches = [cache.clone(), cache.clone()]
+    caches = [cache.clone() for _ in range(3)]
     graphs, outs = [], []
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
-        for s in (0, 40):
+        for s in ((1, 0), (1, 40), (4, 0)):
             step(cache.clone(), s)
     torch.cuda.current_stream().wait_stream(side)
-    for c, s in zip(caches, (0, 40)):
+    for c, s in zip(caches, ((1, 0), (1, 40), (4, 0))):
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             outs.append(step(c, s))
@@ -328,8 +332,9 @@ def test_graphs_and_streams(native_lib):
         for g in graphs:
             g.replay()
         with torch.cuda.stream(side):
-            want = step(eager, 0)
+            want = step(eager, (1, 0))
         torch.cuda.synchronize()
-        assert torch.equal(outs[0], want) and torch.equal(caches[0], eager) and torch.equal(caches[1], eager)
-        _check(outs[1], K.rope_kv4_cache_write(state["rows"].clone(), state["pos"], freq, torch.full((B,), -1, device="cuda"), eager, Hq, Hkv, D), eager, table, n, Hq, Hkv, D)
+        assert torch.equal(outs[0], want) and all(torch.equal(c, eager) for c in caches)
+        for got in outs[1:]:
+            _check(got, K.rope_kv4_cache_write(state["rows"].clone(), state["pos"], freq, torch.full((B,), -1, device="cuda"), eager, Hq, Hkv, D), eager, table, n, Hq, Hkv, D)
     assert L.check_status() == 0

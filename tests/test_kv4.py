@@ -156,7 +156,6 @@ def test_refusals():
         lambda: K.kv4_paged_decode(x, cache, bt, ln[:0], 4, 2, 64),
         lambda: K.kv4_paged_decode(x, cache, bt.float(), ln, 4, 2, 64),
         lambda: K.kv4_paged_decode(x, cache, bt, ln, 4, 2, 64, window=-1),
-        lambda: K.kv4_paged_decode(x, cache, bt, ln, 4, 2, 64, num_ctas=-1),
         lambda: K.kv4_paged_decode(x, cache, bt, ln, 4, 2, 64, out=torch.zeros(1, 256)),
         lambda: K.kv4_paged_decode(x, cache, bt, ln, 4, 2, 64, out=torch.zeros(2, 256).bfloat16()),
     ]
@@ -167,7 +166,12 @@ def test_refusals():
     assert not cache.any()
 
 
-def test_ctas():
-    assert K.kv4_ctas(64, 32, 8, 128, 256) == 0 and K.kv4_ctas(0, 32, 8, 128, 0) == 0
-    assert K.kv4_ctas(1, 8, 1, 128, 257) == 2 and K.kv4_ctas(1, 16, 1, 128, 257) == 4
-    assert K.kv4_ctas(512, 32, 8, 128, 8192) == 3 * 148 and K.kv4_ctas(512, 32, 8, 256, 8192) == 2 * 148
+def test_plan():
+    """A cluster or CTAs that share, never both; no cluster without eight steps for each of its CTAs."""
+    for D in (64, 128, 256):
+        for B in (0, 1, 3, 16, 64, 500, 5000):
+            for Hq, Hkv in ((32, 8), (16, 1), (8, 8)):
+                for n in (0, 1, 256, 300, 1000, 4000, 20000, 10**6):
+                    cluster, ctas = K.kv4_plan(B, Hq, Hkv, D, n)
+                    assert 1 <= cluster <= K.MAX_CLUSTER and (ctas == 0 or cluster == 1) and (cluster == 1 or n > 32 * 8 * (cluster - 1))
+                    assert ctas in (0, 148 * {64: 4, 128: 3, 256: 2}[D])
