@@ -108,13 +108,16 @@ __device__ __forceinline__ float times_pow2(float x, int e) {
 
 // N words of shared memory at once; 16 bytes from global to shared memory, in the background.
 template <int N>
-__device__ __forceinline__ void load_words(uint32_t from, uint32_t (&w)[N]) {
+__device__ __forceinline__ void load_words(const uint8_t* from, uint32_t (&w)[N]) {
   if constexpr (N == 2) {
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(from));
+    const uint2 v = *reinterpret_cast<const uint2*>(from);
+    w[0] = v.x; w[1] = v.y;
   } else {
 #pragma unroll
-    for (int i = 0; i < N; i += 4)
-      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]) : "r"(from + 4 * i));
+    for (int i = 0; i < N; i += 4) {
+      const uint4 v = reinterpret_cast<const uint4*>(from)[i / 4];
+      w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w;
+    }
   }
 }
 __device__ __forceinline__ void copy16(uint32_t to, const uint8_t* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
@@ -382,12 +385,12 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D == 64 ? 4 : D == 128 ? 3 : 2)
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
     __syncwarp();      // every lane copied for the others; and has read the stage that is requested next
     request(i + STAGES - 1);
-    const uint32_t from = fifo + (i % STAGES) * Stage::BYTES;
+    const uint8_t* from = k4_smem_raw + (warp * STAGES + i % STAGES) * Stage::BYTES;
     float s[NS][4];
     uint32_t va[NS][G / 2], vb[NS][G / 2];      // the values' scales
 #pragma unroll
     for (int h = 0; h < NS; ++h) {
-      const uint32_t mine = from + (PAIR ? t >> 1 : h) * Stage::HALF;      // (columns 0-3: the first 16 tokens, 4-7: the others)
+      const uint8_t* mine = from + (PAIR ? t >> 1 : h) * Stage::HALF;      // (columns 0-3: the first 16 tokens, 4-7: the others)
       uint32_t sa[G], sb[G];
       load_words(mine + Stage::SCALES + Page::scale(tok, 0, 0), sa);
       load_words(mine + Stage::SCALES + Page::scale(tok + 2, 0, 0), sb);
