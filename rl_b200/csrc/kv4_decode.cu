@@ -131,10 +131,11 @@ __device__ __forceinline__ const uint8_t* wide(const uint8_t* p, uint32_t a, uin
 __device__ __forceinline__ float bf16_of(uint32_t word, int i) { return __uint_as_float(i & 1 ? word & 0xffff0000u : word << 16); }
 
 // A warp's stage: twice 16 tokens of keys, values and scales. They are copied as they lie, 512 bytes by a warp's instruction (each lane the words that it uses would be four
-// times as many requests for the values: the load alone took 254 instead of 177 us for 1.2 GB), into places of which 16 lie in 16 banks for the copy and for the lanes that read:
-//   keys    words of a lane's token a at lane * 4 G, of token b (two later) 16 D / 4 bytes behind; heads of 256 in two halves of 16 bytes
-//   values  pair a of a lane (r, t) in 128 t + 16 (r ^ 2 t), likewise pair b and halves
-// and one bit of the address turned for b or the second half.
+// times as many requests for the values: 32 sequences of 32768 tokens 225 instead of 216 us), 32 bytes to one place. The places are such that neither the copies nor the lanes that read
+// meet in a bank:
+//   keys    words of a lane's token a at lane * 4 G, those of token b (two later) 4 D bytes behind
+//   values  pair a of a lane (r, t) at 4 G (8 t + (r ^ 2 t)), pair b 4 D bytes behind
+// but with a bit of the address turned where more than 128 bytes are read at once: for b with heads of 64, for the second 16 bytes of a lane with heads of 256.
 template <int D>
 struct K4Stage {
   static constexpr int KEYS = 0, VALUES = 8 * D, SCALES = 16 * D, HALF = 18 * D, BYTES = 2 * HALF;
@@ -144,25 +145,25 @@ struct K4Stage {
     const int token = D == 64 ? lane >> 1 : D == 128 ? 8 * k + (lane >> 2) : 4 * k + (lane >> 3), r = (token >> 2) * 2 + (token & 1), b = token >> 1 & 1;
     if constexpr (D == 64) return b * 256 + ((r * 32 + (lane & 1) * 16) ^ (b * 64));
     if constexpr (D == 128) return b * 512 + (4 * r + (lane & 3)) * 16;
-    return b * 1024 + (lane & 1) * 512 + (((4 * r + (lane >> 1 & 3)) * 16) ^ ((lane & 1) * 64));
+    return b * 1024 + (4 * r + (lane >> 1 & 3)) * 32 + ((lane ^ r) & 1) * 16;
   }
   __device__ static __forceinline__ int value_to(int lane, int k) {
     const int pair = D == 64 ? lane >> 2 : D == 128 ? 4 * k + (lane >> 3) : 2 * k + (lane >> 4), t = pair >> 1, b = pair & 1;
     if constexpr (D == 64) return b * 256 + (t >> 1) * 128 + ((((t & 1) * 4 + ((lane & 3) ^ (t & 2))) ^ (b * 4)) * 16);
     if constexpr (D == 128) return b * 512 + t * 128 + ((lane & 7) ^ (2 * t)) * 16;
-    return b * 1024 + (lane & 1) * 512 + t * 128 + ((lane >> 1 & 7) ^ (2 * t) ^ ((lane & 1) * 4)) * 16;
+    return b * 1024 + t * 256 + ((lane >> 1 & 7) ^ (2 * t)) * 32 + ((lane ^ (t >> 1)) & 1) * 16;
   }
   // where a lane's words of its token or pair b stand, groups from 4 q on
   __device__ static __forceinline__ int key_at(int lane, int b, int q) {
     if constexpr (D == 64) return b * 256 + ((lane * 8) ^ (b * 64));
     if constexpr (D == 128) return b * 512 + lane * 16;
-    return b * 1024 + q * 512 + ((lane * 16) ^ (q * 64));
+    return b * 1024 + lane * 32 + (q ^ (lane >> 2 & 1)) * 16;
   }
   __device__ static __forceinline__ int value_at(int lane, int b, int q) {
     const int r = lane >> 2, t = lane & 3;
     if constexpr (D == 64) return b * 256 + (t >> 1) * 128 + ((((t & 1) * 4 + ((r >> 1) ^ (t & 2))) ^ (b * 4)) * 16) + (r & 1) * 8;
     if constexpr (D == 128) return b * 512 + t * 128 + (r ^ (2 * t)) * 16;
-    return b * 1024 + q * 512 + t * 128 + (r ^ (2 * t) ^ (q * 4)) * 16;
+    return b * 1024 + t * 256 + (r ^ (2 * t)) * 32 + (q ^ (t >> 1)) * 16;
   }
 };
 // Shared memory: the warps' stages; after the token loop [warps][8 heads] rows of D + 4 sums (4 more, for the banks) and [8 heads][D] of the CTA.
