@@ -7,8 +7,12 @@
 // The reference reaches its quantised caches through vLLM's kv_cache_dtype (nemo_rl/models/generation/vllm/config.py).
 #include "kv4.cuh"
 
+#include <algorithm>
+
 namespace {
 using namespace rlb;
+
+constexpr int KV4_READ_ROWS = 64;      // places a block of the read-back takes at most
 
 // Sine and cosine of the product of a position and a frequency in 64 bits: at position p the rounding of the angle to 32 bits alone would be off by p
 // / 2^25. Reduced to |r| <= pi/4 by a multiple of pi/2 that is subtracted in two parts (exact products by fma), then the Taylor series: the first term left out is
@@ -82,143 +86,200 @@ __device__ __forceinline__ uint32_t codes8(const uint4& v, uint32_t scale) {
   return out;
 }
 
+// Page and place in it of a slot; page -1: none (negative, or outside the cache, which is recorded).
+__device__ __forceinline__ int2 place_of(long long slot, int block_size, long long num_slots, int* status) {
+  if (slot < 0) return make_int2(-1, 0);
+  if (slot >= num_slots) {
+    if (status) atomicCAS(status, 0, RLB_ERR_BAD_ARG);
+    return make_int2(-1, 0);
+  }
+  const long long page = slot >> 32 ? slot / block_size : static_cast<long long>(static_cast<uint32_t>(slot) / static_cast<uint32_t>(block_size));
+  return make_int2(static_cast<int>(page), static_cast<int>(slot - page * block_size));
+}
+
 // Rotates the q and k heads of the fused rows in place and puts the rotated k and v into the cache. A block takes `rows` tokens and heads [h0, h0 +
-// heads_per_block) of them; their angles are computed once.
+// heads_per_block) of them, a row at a time: D / 16 threads a head, the next row's values on their way. The angles and the slots' places are worked out once per token.
 template <int D>
-__global__ void __launch_bounds__(256) kv4_write_kernel(__nv_bfloat16* __restrict__ qkv, const int* __restrict__ pos, const float* __restrict__ inv_freq,
+__global__ void __launch_bounds__(512) kv4_write_kernel(__nv_bfloat16* __restrict__ qkv, const int* __restrict__ pos, const float* __restrict__ inv_freq,
                                                         const long long* __restrict__ slots, uint8_t* __restrict__ cache, long long T, int Hq, int Hkv, int block_size,
                                                         long long row_stride, long long num_slots, int* status, int rows, int heads_per_block) {
-  extern __shared__ __align__(16) float2 kv4_cs[];
+  extern __shared__ __align__(16) float2 kv4_cs[];      // [rows][D / 2], then [rows] places
   using Page = Kv4Page<D>;
-  constexpr int LPH = D / 16, HALF = D / 2;
+  constexpr int LPH = D / 16, HALF = D / 2, UP = D / 64;      // UP: the upper half's groups follow the lower half's
+  int2* places = reinterpret_cast<int2*>(kv4_cs + rows * HALF);
   const long long t0 = static_cast<long long>(blockIdx.x) * rows;
   const int n = static_cast<int>(T - t0 < rows ? T - t0 : rows);
-  const int h0 = blockIdx.y * heads_per_block, total_heads = Hq + 2 * Hkv;
-  const int nh = min(heads_per_block, total_heads - h0);
+  const int h0 = blockIdx.y * heads_per_block, nh = min(heads_per_block, Hq + 2 * Hkv - h0);
+  const int per_row = nh * LPH;
   pdl_sync();
-  if (h0 < Hq + Hkv) {
-    for (int i = threadIdx.x; i < n * HALF; i += blockDim.x) kv4_cs[i] = turn(pos[t0 + i / HALF], inv_freq[i % HALF]);
-  }
-  __syncthreads();
-  const int per_row = nh * LPH, total = n * per_row, lane = threadIdx.x & 31;
-  for (int base = threadIdx.x - lane; base < total; base += blockDim.x) {      // (whole warps, for the shuffles)
-    const int i = base + lane;
-    const bool live = i < total;
-    const int r = live ? i / per_row : 0, w = live ? i - r * per_row : 0, h = h0 + w / LPH, c = w % LPH;
-    uint4* p = reinterpret_cast<uint4*>(qkv + (t0 + r) * row_stride + static_cast<long long>(h) * D + c * 8);
-    const long long slot = live && h >= Hq ? slots[t0 + r] : -1;
-    const bool store = slot >= 0 && slot < num_slots;
-    if (slot >= num_slots && status && c == 0) atomicCAS(status, 0, RLB_ERR_BAD_ARG);      // outside the cache: recorded, rotated in place, not written
-    uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-    if (live && (h < Hq + Hkv || store)) {
+  const int padded = (per_row + 31) / 32 * 32;      // (whole warps, for the shuffles)
+  const long long next = row_stride / 8;
+  uint4* p = nullptr;
+  uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+  auto first_row = [&](int w) {
+    p = reinterpret_cast<uint4*>(qkv + t0 * row_stride + static_cast<long long>(h0) * D + (w / LPH) * D + w % LPH * 8);
+    if (w < per_row) {
       lo = p[0];
       hi = p[HALF / 8];
     }
-    if (live && h < Hq + Hkv) {
-      const float4* t = reinterpret_cast<const float4*>(kv4_cs + r * HALF + c * 8);
-      turn2(lo.x, hi.x, t[0]);
-      turn2(lo.y, hi.y, t[1]);
-      turn2(lo.z, hi.z, t[2]);
-      turn2(lo.w, hi.w, t[3]);
-      p[0] = lo;
-      p[HALF / 8] = hi;
-    }
-    if (!__any_sync(0xffffffffu, store)) continue;
-    const uint32_t s_lo = group_scale(lo), s_hi = group_scale(hi);
-    if (!store) continue;
-    const bool value = h >= Hq + Hkv;
-    const int head = value ? h - Hq - Hkv : h - Hq;
-    const long long blk = slot / block_size;
-    const int off = static_cast<int>(slot - blk * block_size), t = c & 3, g = c >> 2;
-    uint8_t* page = cache + (blk * Hkv + head) * Page::bytes(block_size);
-    const uint32_t c_lo = codes8(lo, s_lo), c_hi = codes8(hi, s_hi);
-    constexpr int UP = D / 64;      // the upper half's groups follow the lower half's
-    if (value) {
-      uint8_t* v = page + Page::values_at(block_size);
-      *reinterpret_cast<uint16_t*>(v + Page::value_unit(off, 2 * t, g)) = static_cast<uint16_t>(c_lo);
-      *reinterpret_cast<uint16_t*>(v + Page::value_unit(off, 2 * t + 1, g)) = static_cast<uint16_t>(c_lo >> 16);
-      *reinterpret_cast<uint16_t*>(v + Page::value_unit(off, 2 * t, g + UP)) = static_cast<uint16_t>(c_hi);
-      *reinterpret_cast<uint16_t*>(v + Page::value_unit(off, 2 * t + 1, g + UP)) = static_cast<uint16_t>(c_hi >> 16);
-    } else {
-      *reinterpret_cast<uint32_t*>(page + Page::key_word(off, t, g)) = c_lo;
-      *reinterpret_cast<uint32_t*>(page + Page::key_word(off, t, g + UP)) = c_hi;
-    }
-    if (t == 0) {
-      uint8_t* s = page + Page::scales_at(block_size);
-      *reinterpret_cast<uint16_t*>(s + Page::scale(off, value, g)) = static_cast<uint16_t>(s_lo);
-      *reinterpret_cast<uint16_t*>(s + Page::scale(off, value, g + UP)) = static_cast<uint16_t>(s_hi);
+  };
+  first_row(threadIdx.x);
+  for (int i = threadIdx.x; i < n; i += blockDim.x) places[i] = place_of(slots[t0 + i], block_size, num_slots, status);
+  if (h0 < Hq + Hkv)
+    for (int i = threadIdx.x; i < n * HALF; i += blockDim.x) kv4_cs[i] = turn(pos[t0 + i / HALF], inv_freq[i % HALF]);
+  __syncthreads();
+  for (int w = threadIdx.x; w < padded; w += blockDim.x) {
+    if (w != threadIdx.x) first_row(w);
+    const int h = h0 + w / LPH, c = w % LPH;
+    const bool live = w < per_row, value = h >= Hq + Hkv, held = live && h >= Hq;
+    for (int r = 0; r < n; ++r, p += next) {
+      uint4 lo_next = lo, hi_next = hi;
+      if (live && r + 1 < n) {
+        lo_next = p[next];
+        hi_next = p[next + HALF / 8];
+      }
+      if (live && !value) {
+        const float4* t = reinterpret_cast<const float4*>(kv4_cs + r * HALF + c * 8);
+        turn2(lo.x, hi.x, t[0]);
+        turn2(lo.y, hi.y, t[1]);
+        turn2(lo.z, hi.z, t[2]);
+        turn2(lo.w, hi.w, t[3]);
+        p[0] = lo;
+        p[HALF / 8] = hi;
+      }
+      const int2 place = places[r];
+      if (__any_sync(0xffffffffu, held) && place.x >= 0) {      // (the place is the whole warp's)
+        const uint32_t s_lo = group_scale(lo), s_hi = group_scale(hi);
+        if (held) {
+          const int t = c & 3, g = c >> 2, off = place.y;
+          uint8_t* page = cache + (static_cast<long long>(place.x) * Hkv + (value ? h - Hq - Hkv : h - Hq)) * Page::bytes(block_size);
+          const uint32_t c_lo = codes8(lo, s_lo), c_hi = codes8(hi, s_hi);
+          if (value) {
+            uint8_t* v = page + Page::values_at(block_size);
+            *reinterpret_cast<uint16_t*>(v + Page::value_unit(off, 2 * t, g)) = static_cast<uint16_t>(c_lo);
+            *reinterpret_cast<uint16_t*>(v + Page::value_unit(off, 2 * t + 1, g)) = static_cast<uint16_t>(c_lo >> 16);
+            *reinterpret_cast<uint16_t*>(v + Page::value_unit(off, 2 * t, g + UP)) = static_cast<uint16_t>(c_hi);
+            *reinterpret_cast<uint16_t*>(v + Page::value_unit(off, 2 * t + 1, g + UP)) = static_cast<uint16_t>(c_hi >> 16);
+          } else {
+            *reinterpret_cast<uint32_t*>(page + Page::key_word(off, t, g)) = c_lo;
+            *reinterpret_cast<uint32_t*>(page + Page::key_word(off, t, g + UP)) = c_hi;
+          }
+          if (t == 0) {
+            uint8_t* s = page + Page::scales_at(block_size);
+            *reinterpret_cast<uint16_t*>(s + Page::scale(off, value, g)) = static_cast<uint16_t>(s_lo);
+            *reinterpret_cast<uint16_t*>(s + Page::scale(off, value, g + UP)) = static_cast<uint16_t>(s_hi);
+          }
+        }
+      }
+      lo = lo_next;
+      hi = hi_next;
     }
   }
 }
 
-__device__ __forceinline__ uint4 values8(uint32_t codes, uint32_t scale) {
-  const float s = __uint_as_float(scale << 16);
-  uint32_t out[4];
+template <int N>
+__device__ __forceinline__ void words_of(const uint8_t* from, uint32_t (&w)[N]) {
+  if constexpr (N == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(from);
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(from);
+    w[0] = v.x; w[1] = v.y;
+  } else {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    out[i] = pack_bf16x2((static_cast<float>(codes >> (8 * i) & 15u) - 7.5f) * s, (static_cast<float>(codes >> (8 * i + 4) & 15u) - 7.5f) * s);
-  return make_uint4(out[0], out[1], out[2], out[3]);
+    for (int i = 0; i < N; i += 4) {
+      const uint4 v = reinterpret_cast<const uint4*>(from)[i / 4];
+      w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w;
+    }
+  }
+}
+// The numbers of codes at bits 3-6 of both halves times a scale: 16 + c as bf16, less 23.5, exactly; one rounding in the product.
+__device__ __forceinline__ uint32_t values2(uint32_t codes, uint32_t scale) {
+  uint32_t v;
+  asm("{\n\t.reg .b32 x;\n\tsub.rn.bf16x2 x, %1, %2;\n\tmul.rn.bf16x2 %0, x, %3;\n\t}" : "=r"(v) : "r"((codes & 0x00780078u) | 0x41804180u), "r"(0x41bc41bcu), "r"(scale));
+  return v;
+}
+// Eight values of a word (the first in the low bits) by their scale in both halves.
+__device__ __forceinline__ uint4 values8(uint32_t codes, uint32_t scale) {
+  const uint32_t a = values2(codes << 3, scale), b = values2(codes >> 1, scale), c = values2(codes >> 5, scale), d = values2(codes >> 9, scale);      // (0, 4), (1, 5), (2, 6), (3, 7)
+  return make_uint4(__byte_perm(a, b, 0x5410), __byte_perm(c, d, 0x5410), __byte_perm(a, b, 0x7632), __byte_perm(c, d, 0x7632));
 }
 
-// Keys and values of places of the cache as bf16 rows [k | v]. out_rows: which row of `out` a place goes to (null: its own number). A negative slot gives zeros.
+// Keys and values of places of the cache as bf16 rows [k | v]. out_rows: which row of `out` a place goes to (null: its own number). A negative slot gives zeros. A block
+// takes `rows` places; four threads a head of each, with eight dimensions of every group.
 template <int D>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const uint8_t* __restrict__ cache, const long long* __restrict__ slots, const long long* __restrict__ out_rows,
                                                        __nv_bfloat16* __restrict__ out, long long n, long long out_stride, long long num_out, int Hkv, int block_size,
-                                                       long long num_slots, int* status) {
+                                                       long long num_slots, int* status, int rows) {
   using Page = Kv4Page<D>;
-  constexpr int LPH = D / 16, UP = D / 64;
+  constexpr int G = Page::G;
+  __shared__ int2 places[KV4_READ_ROWS];
+  __shared__ long long targets[KV4_READ_ROWS];
+  const long long first = static_cast<long long>(blockIdx.x) * rows;
+  const int here = static_cast<int>(n - first < rows ? n - first : rows);
   pdl_sync();
-  const int per_row = 2 * Hkv * LPH;
-  const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const long long row = i / per_row;
-  if (row >= n) return;
-  const int w = static_cast<int>(i - row * per_row), h = w / LPH, c = w % LPH, t = c & 3, g = c >> 2;
-  const long long to = out_rows ? out_rows[row] : row;
-  const long long slot = slots[row];
-  if (to < 0 || to >= num_out || slot >= num_slots) {      // outside the cache or the output: recorded, nothing written
-    if (status && w == 0) atomicCAS(status, 0, RLB_ERR_BAD_ARG);
-    return;
-  }
-  uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-  if (slot >= 0) {
-    const bool value = h >= Hkv;
-    const long long blk = slot / block_size;
-    const int off = static_cast<int>(slot - blk * block_size);
-    const uint8_t* page = cache + (blk * Hkv + (value ? h - Hkv : h)) * Page::bytes(block_size);
-    uint32_t c_lo, c_hi;
-    if (value) {
-      const uint8_t* v = page + Page::values_at(block_size);
-      c_lo = *reinterpret_cast<const uint16_t*>(v + Page::value_unit(off, 2 * t, g)) | *reinterpret_cast<const uint16_t*>(v + Page::value_unit(off, 2 * t + 1, g)) << 16;
-      c_hi = *reinterpret_cast<const uint16_t*>(v + Page::value_unit(off, 2 * t, g + UP)) | *reinterpret_cast<const uint16_t*>(v + Page::value_unit(off, 2 * t + 1, g + UP)) << 16;
-    } else {
-      c_lo = *reinterpret_cast<const uint32_t*>(page + Page::key_word(off, t, g));
-      c_hi = *reinterpret_cast<const uint32_t*>(page + Page::key_word(off, t, g + UP));
+  if (threadIdx.x < here) {
+    const long long slot = slots[first + threadIdx.x];
+    long long to = out_rows ? out_rows[first + threadIdx.x] : first + threadIdx.x;
+    const int2 place = place_of(slot, block_size, num_slots, status);
+    if (to < 0 || to >= num_out) {      // outside the output: recorded, nothing written
+      if (status) atomicCAS(status, 0, RLB_ERR_BAD_ARG);
+      to = -1;
     }
-    const uint8_t* s = page + Page::scales_at(block_size);
-    lo = values8(c_lo, *reinterpret_cast<const uint16_t*>(s + Page::scale(off, value, g)));
-    hi = values8(c_hi, *reinterpret_cast<const uint16_t*>(s + Page::scale(off, value, g + UP)));
+    places[threadIdx.x] = place;
+    targets[threadIdx.x] = place.x < 0 && slot >= 0 ? -1 : to;
   }
-  uint4* p = reinterpret_cast<uint4*>(out + to * out_stride + static_cast<long long>(h) * D + c * 8);
-  p[0] = lo;
-  p[D / 16] = hi;
+  __syncthreads();
+  const uint32_t per_row = 2 * Hkv * 4;
+  for (uint32_t i = threadIdx.x; i < here * per_row; i += blockDim.x) {
+    const uint32_t row = i / per_row, w = i - row * per_row;
+    const int h = static_cast<int>(w >> 2), t = static_cast<int>(w & 3);
+    const int2 place = places[row];
+    const long long to = targets[row];
+    if (to < 0) continue;
+    uint4* p = reinterpret_cast<uint4*>(out + to * out_stride + static_cast<long long>(h) * D + t * 8);
+    if (place.x < 0) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) p[g * 4] = make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    const bool value = h >= Hkv;
+    const int off = place.y;
+    const uint8_t* page = cache + (static_cast<long long>(place.x) * Hkv + (value ? h - Hkv : h)) * Page::bytes(block_size);
+    uint32_t words[G], scales[G / 2];
+    if (value) {      // units of two tokens lie side by side: both are read, one is taken
+      uint32_t a[G], b[G];
+      words_of(page + Page::values_at(block_size) + Page::value_unit(off & ~1, 2 * t, 0), a);
+      words_of(page + Page::values_at(block_size) + Page::value_unit(off & ~1, 2 * t + 1, 0), b);
+#pragma unroll
+      for (int g = 0; g < G; ++g) words[g] = __byte_perm(a[g], b[g], off & 1 ? 0x7632 : 0x5410);
+    } else {
+      words_of(page + Page::key_word(off, t, 0), words);
+    }
+    words_of(page + Page::scales_at(block_size) + Page::scale(off, value, 0), scales);
+#pragma unroll
+    for (int g = 0; g < G; ++g) p[g * 4] = values8(words[g], __byte_perm(scales[g >> 1], 0u, g & 1 ? 0x3232 : 0x1010));
+  }
 }
 
 template <int D>
 int launch_write(void* qkv, const int* pos, const float* inv_freq, const long long* slots, void* cache, long long T, int Hq, int Hkv, int block_size, long long row_stride,
                  long long num_blocks, int* status, cudaStream_t stream) {
-  const int heads = Hq + 2 * Hkv, threads = 128, rows = 1, per_block = threads * 16 / D;
+  const int heads = Hq + 2 * Hkv, per_head = D / 16;
+  const bool many = T * heads * per_head > 148 * 2048;      // more than the device holds threads: whole rows, four tokens a block
+  const int rows = many ? 4 : 1, per_block = many ? heads : 128 / per_head;
+  const int threads = many ? std::min(512, (heads * per_head + 31) / 32 * 32) : 128;
   const dim3 grid(static_cast<unsigned>((T + rows - 1) / rows), static_cast<unsigned>((heads + per_block - 1) / per_block));
-  rlb_launch_pdl(kv4_write_kernel<D>, grid, dim3(threads), rows * D / 2 * sizeof(float2), stream, static_cast<__nv_bfloat16*>(qkv), pos, inv_freq, slots, static_cast<uint8_t*>(cache), T, Hq,
-                 Hkv, block_size, row_stride, num_blocks * block_size, status, rows, per_block);
+  rlb_launch_pdl(kv4_write_kernel<D>, grid, dim3(threads), rows * (D / 2 * sizeof(float2) + sizeof(int2)), stream, static_cast<__nv_bfloat16*>(qkv), pos, inv_freq, slots,
+                 static_cast<uint8_t*>(cache), T, Hq, Hkv, block_size, row_stride, num_blocks * block_size, status, rows, per_block);
   return static_cast<int>(cudaGetLastError());
 }
 
 template <int D>
 int launch_read(const void* cache, const long long* slots, const long long* out_rows, void* out, long long n, long long out_stride, long long num_out, int Hkv, int block_size,
                 long long num_blocks, int* status, cudaStream_t stream) {
-  const long long items = n * 2 * Hkv * (D / 16);
-  rlb_launch_pdl(kv4_read_kernel<D>, dim3(static_cast<unsigned>((items + 255) / 256)), dim3(256), 0, stream, static_cast<const uint8_t*>(cache), slots, out_rows,
-                 static_cast<__nv_bfloat16*>(out), n, out_stride, num_out, Hkv, block_size, num_blocks * block_size, status);
+  const int per_row = 8 * Hkv, rows = std::max(1, std::min({KV4_READ_ROWS, 512 / per_row, static_cast<int>(std::min<long long>(n / 296 + 1, KV4_READ_ROWS))}));
+  rlb_launch_pdl(kv4_read_kernel<D>, dim3(static_cast<unsigned>((n + rows - 1) / rows)), dim3(256), 0, stream, static_cast<const uint8_t*>(cache), slots, out_rows,
+                 static_cast<__nv_bfloat16*>(out), n, out_stride, num_out, Hkv, block_size, num_blocks * block_size, status, rows);
   return static_cast<int>(cudaGetLastError());
 }
 bool bad_shape(int D, int Hkv, int block_size) { return (D != 64 && D != 128 && D != 256) || Hkv < 1 || block_size < 16 || block_size % 16 || block_size > KV4_MAX_BLOCK; }
@@ -229,7 +290,7 @@ RLB_API int rlb_rope_kv4_cache_write(void* qkv, const int* pos, const float* inv
                                      long long row_stride, long long num_blocks, int* status, void* stream) {
   if (bad_shape(D, Hkv, block_size) || Hq < 0 || row_stride % 8 || ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(cache)) & 15)) return -2;
   if (T <= 0) return 0;
-  if (T > 0x7fffffffll) return -3;
+  if (T > 0x7fffffffll || num_blocks > 0x7fffffffll || (Hq + 2ll * Hkv) * (D / 16) / 128 + 1 > 65535) return -3;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   auto launch = D == 64 ? launch_write<64> : D == 128 ? launch_write<128> : launch_write<256>;
   return launch(qkv, pos, inv_freq, slots, cache, T, Hq, Hkv, block_size, row_stride, num_blocks, status, s);
@@ -240,7 +301,7 @@ RLB_API int rlb_kv4_cache_read(const void* cache, const long long* slots, const 
                                int block_size, long long num_blocks, int* status, void* stream) {
   if (bad_shape(D, Hkv, block_size) || out_stride % 8 || ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(cache)) & 15)) return -2;
   if (n <= 0) return 0;
-  if (n * 2 * Hkv * (D / 16) / 256 >= 0x7fffffffll) return -3;
+  if (n > 0x7fffffffll || num_blocks > 0x7fffffffll || Hkv > (1 << 20)) return -3;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   auto launch = D == 64 ? launch_read<64> : D == 128 ? launch_read<128> : launch_read<256>;
   return launch(cache, slots, out_rows, out, n, out_stride, num_out, Hkv, block_size, num_blocks, status, s);
