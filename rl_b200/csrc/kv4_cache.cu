@@ -65,23 +65,21 @@ __device__ __forceinline__ uint32_t group_scale(const uint4& v) {
   return __bfloat16_as_ushort(__float2bfloat16_rn(a * (1.f / 7.5f)));
 }
 
-// floor(x / s) + 8 in 0..15, exactly: the quotient by the reciprocal is off by one at most, and the multiples of s that x lies between are exact in
-// 32 bits (4 bits times 8).
-__device__ __forceinline__ uint32_t code4(float x, float s, float inv) {
-  float t = floorf(x * inv);
-  t = __fmul_rn(t, s) > x ? t - 1.f : __fmul_rn(t + 1.f, s) <= x ? t + 1.f : t;
-  return static_cast<uint32_t>(fminf(fmaxf(t + 8.f, 0.f), 15.f));
-}
-// Eight values' codes, the first in the low bits.
+// Eight values' codes, the first in the low bits: floor(x / s) + 8, which lies in 0..15 by itself (|x / s| < 7.6), exactly. x and s have eight bits each, so that x / s is an
+// integer or at least 2^-10 from every one but 0: the quotient by the reciprocal, off by less than 2^-19, plus 2^-12 has the right integer part, and below 0 it is kept below.
+// Adding 1.5 * 2^23 rounds to an integer in the low bits; these bits are put together by multiplications, and what stands above them in each word comes off at the end.
 __device__ __forceinline__ uint32_t codes8(const uint4& v, uint32_t scale) {
   if (scale == 0u || scale == 0x7fc0u) return 0x88888888u;
-  const float s = __uint_as_float(scale << 16), inv = 1.f / s;
+  const float inv = 1.f / __uint_as_float(scale << 16);
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-  uint32_t out = 0;
+  uint32_t out = 0u - 0x4b400000u * 0x11111111u;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 f = unpack_bf16x2(w[i]);
-    out |= code4(f.x, s, inv) << (8 * i) | code4(f.y, s, inv) << (8 * i + 4);
+    float a = fmaf(f.x, inv, 7.5f + 0x1p-12f), b = fmaf(f.y, inv, 7.5f + 0x1p-12f);
+    if (f.x < 0.f) a = fminf(a, 7.5f - 0x1p-12f);
+    if (f.y < 0.f) b = fminf(b, 7.5f - 0x1p-12f);
+    out += __float_as_uint(a + 12582912.f) * (1u << (8 * i)) + __float_as_uint(b + 12582912.f) * (16u << (8 * i));
   }
   return out;
 }
@@ -100,7 +98,7 @@ __device__ __forceinline__ int2 place_of(long long slot, int block_size, long lo
 // Rotates the q and k heads of the fused rows in place and puts the rotated k and v into the cache. A block takes `rows` tokens and heads [h0, h0 +
 // heads_per_block) of them, a row at a time: D / 16 threads a head, the next row's values on their way. The angles and the slots' places are worked out once per token.
 template <int D>
-__global__ void __launch_bounds__(512) kv4_write_kernel(__nv_bfloat16* __restrict__ qkv, const int* __restrict__ pos, const float* __restrict__ inv_freq,
+__global__ void __launch_bounds__(256, 5) kv4_write_kernel(__nv_bfloat16* __restrict__ qkv, const int* __restrict__ pos, const float* __restrict__ inv_freq,
                                                         const long long* __restrict__ slots, uint8_t* __restrict__ cache, long long T, int Hq, int Hkv, int block_size,
                                                         long long row_stride, long long num_slots, int* status, int rows, int heads_per_block) {
   extern __shared__ __align__(16) float2 kv4_cs[];      // [rows][D / 2], then [rows] places
@@ -126,7 +124,10 @@ __global__ void __launch_bounds__(512) kv4_write_kernel(__nv_bfloat16* __restric
   first_row(threadIdx.x);
   for (int i = threadIdx.x; i < n; i += blockDim.x) places[i] = place_of(slots[t0 + i], block_size, num_slots, status);
   if (h0 < Hq + Hkv)
-    for (int i = threadIdx.x; i < n * HALF; i += blockDim.x) kv4_cs[i] = turn(pos[t0 + i / HALF], inv_freq[i % HALF]);
+    for (int i = threadIdx.x; i < n * HALF; i += blockDim.x) {      // (in the order in which a head's threads read 16 bytes each)
+      const int j = i % HALF;
+      kv4_cs[i - j + (j % 8 / 2 * LPH + j / 8) * 2 + j % 2] = turn(pos[t0 + i / HALF], inv_freq[j]);
+    }
   __syncthreads();
   for (int w = threadIdx.x; w < padded; w += blockDim.x) {
     if (w != threadIdx.x) first_row(w);
@@ -139,11 +140,11 @@ __global__ void __launch_bounds__(512) kv4_write_kernel(__nv_bfloat16* __restric
         hi_next = p[next + HALF / 8];
       }
       if (live && !value) {
-        const float4* t = reinterpret_cast<const float4*>(kv4_cs + r * HALF + c * 8);
+        const float4* t = reinterpret_cast<const float4*>(kv4_cs + r * HALF) + c;
         turn2(lo.x, hi.x, t[0]);
-        turn2(lo.y, hi.y, t[1]);
-        turn2(lo.z, hi.z, t[2]);
-        turn2(lo.w, hi.w, t[3]);
+        turn2(lo.y, hi.y, t[LPH]);
+        turn2(lo.z, hi.z, t[2 * LPH]);
+        turn2(lo.w, hi.w, t[3 * LPH]);
         p[0] = lo;
         p[HALF / 8] = hi;
       }
@@ -265,9 +266,9 @@ template <int D>
 int launch_write(void* qkv, const int* pos, const float* inv_freq, const long long* slots, void* cache, long long T, int Hq, int Hkv, int block_size, long long row_stride,
                  long long num_blocks, int* status, cudaStream_t stream) {
   const int heads = Hq + 2 * Hkv, per_head = D / 16;
-  const bool many = T * heads * per_head > 148 * 2048;      // more than the device holds threads: whole rows, four tokens a block
-  const int rows = many ? 4 : 1, per_block = many ? heads : 128 / per_head;
-  const int threads = many ? std::min(512, (heads * per_head + 31) / 32 * 32) : 128;
+  const bool many = T * heads * per_head > 148 * 2048;      // more than the device holds threads: whole rows, some tokens a block (15003 tokens of 32 + 2 * 8 heads of 128, us with 2, 4, 8: 62, 64, 69; 32 + 2 * 4 of 64: 31, 29, 30)
+  const int rows = many ? (D == 64 ? 4 : 2) : 1, per_block = many ? heads : 128 / per_head;
+  const int per_row = heads * per_head, times = (per_row + 255) / 256, threads = many ? ((per_row + times - 1) / times + 31) / 32 * 32 : 128;
   const dim3 grid(static_cast<unsigned>((T + rows - 1) / rows), static_cast<unsigned>((heads + per_block - 1) / per_block));
   rlb_launch_pdl(kv4_write_kernel<D>, grid, dim3(threads), rows * (D / 2 * sizeof(float2) + sizeof(int2)), stream, static_cast<__nv_bfloat16*>(qkv), pos, inv_freq, slots,
                  static_cast<uint8_t*>(cache), T, Hq, Hkv, block_size, row_stride, num_blocks * block_size, status, rows, per_block);
