@@ -184,7 +184,7 @@ GENERATION = dict(backend=F(str, choices=("native", "vllm", "sglang", "megatron"
                   top_p=F(float, int), top_k=F(int), stop_token_ids=F(list), stop_strings=F(list), model_name=F(str),
                   block_size=F(int), gpu_memory_utilization=F(float, int), kv_cache_tokens=F(int), max_model_len=F(int), max_running=F(int),
                   max_prefill_tokens=F(int), use_cuda_graphs=F(bool), free_kv_cache_on_sleep=F(bool), seed=F(int),
-                  precision=F(str, choices=("bfloat16", "bf16", "fp8", "mxfp8")), decode_window=F(int),
+                  precision=F(str, choices=("bfloat16", "bf16", "fp8", "mxfp8")), decode_window=F(int), kv_cache_dtype=F(str),
                   native_cfg=F(dict, sub=NATIVE_GEN), vllm_cfg=F(dict, sub=NATIVE_GEN), sglang_cfg=OPAQUE, mcore_generation_config=OPAQUE,
                   colocated=F(dict, sub=COLOCATED), vllm_kwargs=F(dict), pad_token_id=F(int), _pad_token_id=F(int),
                   port_range_low=F(int), port_range_high=F(int), val_temperature=F(float, int), val_top_p=F(float, int), val_top_k=F(int),

@@ -24,6 +24,8 @@ RLB_EXTERN int rlb_qk_rmsnorm_fwd(const void* x, const void* wq, const void* wk,
 RLB_EXTERN int rlb_rope(void* x, const int* pos, const float* inv_freq, long long rows, int heads, int D, long long row_stride, int backward, void* stream);
 RLB_EXTERN int rlb_rope_kv_cache_write(void* qkv, const int* pos, const float* inv_freq, const long long* slots, void* k_cache, void* v_cache, long long T,
                                        int Hq, int Hkv, int D, int block_size, long long row_stride, long long num_blocks, int* status, void* stream);
+RLB_EXTERN int rlb_rope_kv4_cache_write(void* qkv, const int* pos, const float* inv_freq, const long long* slots, void* cache, long long T, int Hq, int Hkv, int D,
+                                        int block_size, long long row_stride, long long num_blocks, int* status, void* stream);
 RLB_EXTERN int rlb_flash_attn_fwd(const void* qkv, long long qkv_stride, const int* cu_seqlens, int num_seqs, int T, int Hq, int Hkv, int D, float scale,
                                   void* out, long long out_stride, float* lse, int max_tiles, int* status, void* stream);
 RLB_EXTERN int rlb_flash_attn_fwd_d64(const void* qkv, long long qkv_stride, const int* cu_seqlens, int num_seqs, int T, int Hq, int Hkv, int D, float scale,
@@ -36,7 +38,7 @@ struct RlbDenseLayer {
   const void *q_norm, *k_norm;                               // or null
   const float* qkv_bias;                                     // or null
   const float* inv_freq;
-  void *k_cache, *v_cache;                                   // with `slots`
+  void *k_cache, *v_cache;                                   // with `slots`; kv4: the first is the 4-bit cache of both
 };
 struct RlbDenseForward {
   const RlbDenseLayer* layers;
@@ -46,7 +48,7 @@ struct RlbDenseForward {
   const int *positions, *cu_seqlens;
   const long long* slots;         // where keys and values go in the caches, or null
   int* status;
-  int L, T, B, d, Hq, Hkv, D, F, block_size;
+  int L, T, B, d, Hq, Hkv, D, F, block_size, kv4;
   long long num_blocks;
   float eps, scale;
 };
@@ -72,7 +74,9 @@ extern "C" __attribute__((visibility("default"))) int rlb_dense_forward(const Rl
     RLB_TRY(rlb_rmsnorm_fwd(h, nullptr, w.norm1, p.x, nullptr, nullptr, p.T, p.d, p.d, p.d, p.eps, stream));
     RLB_TRY(linear(p, p.x, w.qkv, p.qkv, width, p.d, w.qkv_bias, nullptr, stream));
     if (w.q_norm) RLB_TRY(rlb_qk_rmsnorm_fwd(p.qkv, w.q_norm, w.k_norm, p.qkv, nullptr, p.T, p.Hq, p.Hkv, p.D, width, width, p.eps, stream));
-    if (p.slots)
+    if (p.slots && p.kv4)
+      RLB_TRY(rlb_rope_kv4_cache_write(p.qkv, p.positions, w.inv_freq, p.slots, w.k_cache, p.T, p.Hq, p.Hkv, p.D, p.block_size, width, p.num_blocks, p.status, stream));
+    else if (p.slots)
       RLB_TRY(rlb_rope_kv_cache_write(p.qkv, p.positions, w.inv_freq, p.slots, w.k_cache, w.v_cache, p.T, p.Hq, p.Hkv, p.D, p.block_size, width, p.num_blocks,
                                       p.status, stream));
     else

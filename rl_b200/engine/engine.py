@@ -25,6 +25,7 @@ from rl_b200.models.config import RECURRENT_MIXERS
 from rl_b200.models.transformer import CausalLM, PackedBatch
 from rl_b200.ops import engine_ops as E
 from rl_b200.ops import functional as F
+from rl_b200.ops import kv4_ops as K4
 from rl_b200.ops import layer_ops as Y
 from rl_b200.ops import lib as _L
 from rl_b200.ops import mixer_ops as X
@@ -412,9 +413,10 @@ class GenerationEngine:
                  kv_cache_tokens: Optional[int] = None, gpu_memory_utilization: float = 0.5, max_running: int = 512,
                  max_prefill_tokens: int = 16384, max_model_len: int = 8192, use_cuda_graphs: bool = True,
                  logits_fp32: bool = True, tokenizer=None, quantization: Optional[str] = None, decode_window: int = 16,
-                 enable_prefix_caching: bool = True):
+                 enable_prefix_caching: bool = True, kv_cache_dtype: Optional[str] = None):
         """``quantization``: None (bf16), ``"mxfp8"`` or ``"fp8"``: serve quantised copies of the linear weights
-        (see ``engine/quantized.py``); call :meth:`requantize` after the weights changed."""
+        (see ``engine/quantized.py``); call :meth:`requantize` after the weights changed. ``kv_cache_dtype``: None or ``"auto"`` (the model's type) or
+        ``"int4"``: keys and values in 4 bits (``ops/kv4_ops.py``), 3.6 times as many tokens in the same memory."""
         self.model = model
         self.quantization = quantization if quantization not in (None, "", "bfloat16", "bf16", "none") else None
         self.cfg = model.cfg
@@ -464,6 +466,16 @@ class GenerationEngine:
         attn0 = model.layers[self._attn_layers[0]].self_attn if self._attn_layers else None
         self.hq = attn0.hq if attn0 is not None else self.cfg.num_attention_heads
         self.hkv = attn0.hkv if attn0 is not None else self.cfg.num_key_value_heads
+        # keys and values in 4 bits: one pool per attention layer, in the place of the keys' (see ``ops/kv4_ops.py``)
+        if kv_cache_dtype not in (None, "auto", "int4"):
+            raise ValueError(f"kv_cache_dtype {kv_cache_dtype!r}: 'auto' or 'int4'")
+        self.kv4 = kv_cache_dtype == "int4"
+        if self.kv4:
+            if self.mixer or self.cfg.is_mla:
+                raise NotImplementedError("the 4-bit key/value cache serves attention layers with keys and values of their own, not layer-list models or latent attention")
+            if self.native and model.dtype != torch.bfloat16:
+                raise ValueError(f"the 4-bit key/value cache serves bf16 models, not {model.dtype}")
+            K4.kv4_page_bytes(block_size, self.cfg.head_dim)      # (refuses shapes that no page has)
         # tensor-parallel decode is captured too when the fused GEMM + all-reduce kernel (device-resident epoch) carries the
         # collectives; NCCL broadcasts / all-gathers of the sampled tokens and logits are capturable as well
         # mixture-of-experts decode is captured as well: its few-token layer (csrc/moe_decode.cu) has fixed shapes and no
@@ -480,6 +492,8 @@ class GenerationEngine:
             elif self.device.type == "cuda":
                 free, _ = torch.cuda.mem_get_info(self.device)
                 per_block = 2 * max(1, len(self._attn_layers)) * self.hkv * block_size * c.head_dim * 2
+                if self.kv4:
+                    per_block = max(1, len(self._attn_layers)) * self.hkv * K4.kv4_page_bytes(block_size, c.head_dim)
                 if self.mixer:
                     per_block = max(1, sum(self._cache_width(i) for i, _ in self.runs)) * block_size * model.embed_tokens.element_size()
                 num_blocks = max(16, int(free * gpu_memory_utilization) // per_block)
@@ -550,8 +564,13 @@ class GenerationEngine:
         shape = (self.num_blocks, self.hkv, self.block_size, c.head_dim)
         dt = self.model.dtype
         attn = set(self._attn_layers)
-        self.k_cache = [torch.zeros(shape, dtype=dt, device=self.device) if i in attn else None for i in range(len(self.model.layers))]
-        self.v_cache = [torch.zeros(shape, dtype=dt, device=self.device) if i in attn else None for i in range(len(self.model.layers))]
+        layers = range(len(self.model.layers))
+        if self.kv4:
+            self.k_cache = [K4.kv4_cache(self.num_blocks, self.hkv, self.block_size, c.head_dim, self.device) if i in attn else None for i in layers]
+            self.v_cache = [None] * len(self.model.layers)
+        else:
+            self.k_cache = [torch.zeros(shape, dtype=dt, device=self.device) if i in attn else None for i in layers]
+            self.v_cache = [torch.zeros(shape, dtype=dt, device=self.device) if i in attn else None for i in layers]
         if self.hybrid:   # row 0 is scratch (padding rows of a decode batch write there)
             R = self.max_running + 1
             self.mamba_conv = [torch.zeros((R, c.mamba_conv_dim, c.mamba_d_conv - 1), dtype=dt, device=self.device) if l.kind == "mamba" else None
@@ -611,6 +630,8 @@ class GenerationEngine:
         c = self.cfg
         if self.mixer:
             return sum(self._cache_width(i) for i, _ in self.runs) * self.num_blocks * self.block_size * self.model.embed_tokens.element_size()
+        if self.kv4:
+            return len(self._attn_layers) * self.num_blocks * self.hkv * K4.kv4_page_bytes(self.block_size, c.head_dim)
         return 2 * len(self._attn_layers) * self.num_blocks * self.hkv * self.block_size * c.head_dim * self.model.dtype.itemsize if hasattr(self.model.dtype, "itemsize") else 0
 
     # ------------------------------------------------------------------ routed-expert recording (rollout routing replay)
@@ -710,6 +731,35 @@ class GenerationEngine:
             return self._zero_freq
         return m.inv_freq_local if (layer.window and m.inv_freq_local is not None) else m.inv_freq
 
+    def _write_kv(self, li: int, qkv, positions, freq, slots):
+        """Rotates q and k of the fused rows and puts k and v into layer ``li``'s cache; returns the rotated rows."""
+        if self.kv4:
+            return K4.rope_kv4_cache_write(qkv, positions, freq, slots, self.k_cache[li], self.hq, self.hkv, self.cfg.head_dim)
+        return E.rope_kv_cache_write(qkv, positions, freq, slots, self.k_cache[li], self.v_cache[li], self.hq, self.hkv, self.cfg.head_dim)
+
+    def _attend(self, li: int, qkv, block_table, seq_lens, num_splits, scratch, **kw):
+        """Decode attention of the rows over layer ``li``'s cache. ``num_splits`` and ``scratch``: from :meth:`_decode_splits`."""
+        if self.kv4:
+            windowed = bool(kw.get("window"))      # (a window is far shorter than what the step's plan was made for)
+            return K4.kv4_paged_decode(qkv, self.k_cache[li], block_table, seq_lens, self.hq, self.hkv, self.cfg.head_dim, plan=None if windowed else num_splits,
+                                       scratch=None if windowed else scratch, **kw)
+        return E.paged_decode(qkv, self.k_cache[li], self.v_cache[li], block_table, seq_lens, self.hq, self.hkv, self.cfg.head_dim,
+                              num_splits=num_splits, scratch=scratch, **kw)
+
+    def _decode_splits(self, B: int):
+        """How a decode step of ``B`` rows cuts up its attention."""
+        most = max(self.max_model_len // 2, 1)
+        if self.kv4:
+            return K4.kv4_plan(B, self.hq, self.hkv, self.cfg.head_dim, most, self._sm_count)
+        return E.choose_splits(B, self.hkv, most, self.block_size, self._sm_count, self.hq)
+
+    def _decode_scratch(self, B: int, num_splits):
+        new = lambda n: torch.empty(n, dtype=torch.float32, device=self.device)   # noqa: E731
+        if self.kv4:
+            return new(K4.kv4_scratch_size(num_splits[1], self.cfg.head_dim)) if num_splits[1] else None
+        no, nml = E.decode_scratch_sizes(B, self.hq, num_splits, self.cfg.head_dim)
+        return (new(no), new(nml)) if num_splits > 1 else None
+
     def _output_logits(self, h, out=None):
         """[n, V] logits: the local vocabulary slice is projected here and the slices are gathered over the tp group."""
         z = F.gemm(h, self.model.output_weight, out=out if self.tpw == 1 else None, out_dtype=self.logits_dtype)
@@ -740,7 +790,7 @@ class GenerationEngine:
         slots = torch.full((1,), -1, dtype=torch.int64, device=dev)
         if decode:
             bt = torch.zeros((1, self.max_blocks_per_seq), dtype=torch.int32, device=dev)
-            self._decode_forward(ids, pos, slots, bt, torch.zeros(1, dtype=torch.int32, device=dev), 1, None)
+            self._decode_forward(ids, pos, slots, bt, torch.zeros(1, dtype=torch.int32, device=dev), None if self.kv4 else 1, None)
         else:
             cu = torch.tensor([0, 1], dtype=torch.int32, device=dev)
             self._prefill_forward(PackedBatch(ids, pos, cu, 1), slots, torch.zeros(1, dtype=torch.int64, device=dev))
@@ -765,7 +815,7 @@ class GenerationEngine:
         if not self.native or self.hybrid or getattr(m, "sharder", None) is not None:
             return None
         return dense_forward(m.layers, h, positions, [self._freq(layer) for layer in m.layers], cu_seqlens, max_seqlen, slots=slots,
-                             k_caches=self.k_cache, v_caches=self.v_cache)
+                             k_caches=self.k_cache, v_caches=() if self.kv4 else self.v_cache)
 
     @torch.no_grad()
     def _prefill_forward(self, batch: PackedBatch, slots: torch.Tensor, last_idx: torch.Tensor, state_rows=None) -> torch.Tensor:
@@ -780,7 +830,7 @@ class GenerationEngine:
                 continue
             x = F.rmsnorm(h, layer.input_layernorm, c.rms_norm_eps)
             qkv = layer.self_attn.project_qkv(x, batch.positions, m.inv_freq, apply_rope=False)
-            qkv = E.rope_kv_cache_write(qkv, batch.positions, self._freq(layer), slots, self.k_cache[li], self.v_cache[li], self.hq, self.hkv, c.head_dim)
+            qkv = self._write_kv(li, qkv, batch.positions, self._freq(layer), slots)
             a = F.attention_varlen(qkv, batch.cu_seqlens, batch.max_seqlen, self.hq, self.hkv, c.head_dim, scale=c.attn_scale, window=layer.window)
             h = self._layer_tail(layer, h, a)
         hl = E.gather_rows(h if whole is None else whole, last_idx.to(torch.int32))
@@ -827,9 +877,8 @@ class GenerationEngine:
                 qkv = E.skinny_linear(hw, at.qkv_proj, bias=at.qkv_bias, ssq_in=ssq, eps=eps)
             if c.qk_norm:
                 qkv = F.qk_rmsnorm(qkv, at.q_norm, at.k_norm, at.hq, at.hkv, c.head_dim, eps)
-            qkv = E.rope_kv_cache_write(qkv, positions, m.inv_freq, slots, self.k_cache[li], self.v_cache[li], self.hq, self.hkv, c.head_dim)
-            a = E.paged_decode(qkv, self.k_cache[li], self.v_cache[li], block_table, seq_lens, self.hq, self.hkv, c.head_dim,
-                               num_splits=num_splits, scratch=scratch)
+            qkv = self._write_kv(li, qkv, positions, m.inv_freq, slots)
+            a = self._attend(li, qkv, block_table, seq_lens, num_splits, scratch)
             h = E.skinny_linear(a, at.o_proj, residual=h, ssq_out=ssq2, norm_w=layer.post_attention_layernorm, out2=hw2)
             act = E.skinny_linear(hw2, layer.mlp.gate_up_proj, ssq_in=ssq2, eps=eps, swiglu=True)
             next_w = m.layers[li + 1].input_layernorm if li + 1 < L else m.norm
@@ -872,9 +921,8 @@ class GenerationEngine:
             qkv = E.skinny_linear(x, at.qkv_proj, bias=at.qkv_bias)
             if c.qk_norm:
                 qkv = F.qk_rmsnorm(qkv, at.q_norm, at.k_norm, at.hq, at.hkv, c.head_dim, eps)
-            qkv = E.rope_kv_cache_write(qkv, positions, m.inv_freq, slots, self.k_cache[li], self.v_cache[li], self.hq, self.hkv, c.head_dim)
-            a = E.paged_decode(qkv, self.k_cache[li], self.v_cache[li], block_table, seq_lens, self.hq, self.hkv, c.head_dim,
-                               num_splits=num_splits, scratch=scratch)
+            qkv = self._write_kv(li, qkv, positions, m.inv_freq, slots)
+            a = self._attend(li, qkv, block_table, seq_lens, num_splits, scratch)
             part = E.skinny_linear(a, at.o_proj, out_dtype=torch.float32)
             h, x2 = comm.allreduce_rows(part, h, layer.post_attention_layernorm, eps)
             act = E.skinny_linear(x2, layer.mlp.gate_up_proj, swiglu=True)
@@ -1104,9 +1152,8 @@ class GenerationEngine:
                 continue
             x = F.rmsnorm(h, layer.input_layernorm, c.rms_norm_eps)
             qkv = layer.self_attn.project_qkv(x, positions, m.inv_freq, apply_rope=False)
-            qkv = E.rope_kv_cache_write(qkv, positions, self._freq(layer), slots, self.k_cache[li], self.v_cache[li], self.hq, self.hkv, c.head_dim)
-            a = E.paged_decode(qkv, self.k_cache[li], self.v_cache[li], block_table, seq_lens, self.hq,
-                               self.hkv, c.head_dim, scale=c.attn_scale, window=layer.window, num_splits=num_splits, scratch=scratch)
+            qkv = self._write_kv(li, qkv, positions, self._freq(layer), slots)
+            a = self._attend(li, qkv, block_table, seq_lens, num_splits, scratch, scale=c.attn_scale, window=layer.window)
             h = self._layer_tail(layer, h, a)
         h = F.rmsnorm(h, m.norm, c.rms_norm_eps)
         return self._output_logits(h, logits_out)
@@ -1176,11 +1223,11 @@ class GenerationEngine:
         st = self._static_buffers()
         B = self._bucket(n)
         c = self.cfg
-        num_splits = E.choose_splits(B, self.hkv, max(self.max_model_len // 2, 1), self.block_size, self._sm_count, self.hq) if self.native else 1
+        num_splits = self._decode_splits(B) if self.native else 1
         if not self.native:
             self._decode_rows = st["state_rows"][:n]
             logits = self._decode_forward(st["ids"][:n].long(), st["positions"][:n], st["slots"][:n], st["block_table"][:n],
-                                          st["seq_lens"][:n], 1, None)
+                                          st["seq_lens"][:n], None if self.kv4 else 1, None)
             tok, lp = E.sample(logits, temperature=sp.temperature, top_k=sp.top_k or 0, top_p=sp.top_p, greedy=sp.greedy,
                                seed=self.BASE_SEED, row_keys=st["keys"][:n])
             tok, lp = self._agree(tok, lp)
@@ -1214,8 +1261,7 @@ class GenerationEngine:
         if use_graphs:
             g = self._graphs.get(key)
             if g is None:
-                no, nml = E.decode_scratch_sizes(B, self.hq, num_splits, c.head_dim)
-                scratch = (torch.empty(no, dtype=torch.float32, device=self.device), torch.empty(nml, dtype=torch.float32, device=self.device)) if num_splits > 1 else None
+                scratch = self._decode_scratch(B, num_splits)
                 # warm-up outside capture (sets kernel attributes, sizes the allocator), then capture. The warm-up must leave no trace:
                 # it writes no cache slot, works on the scratch state row, and the step inputs and outputs are put back
                 saved, saved_out = st["blob"].clone(), st["out_blob"].clone()
@@ -1244,8 +1290,7 @@ class GenerationEngine:
                 self._ev_pending = True
             _L.Counters.graph_replayed(g[2] * steps)
         else:
-            no, nml = E.decode_scratch_sizes(B, self.hq, num_splits, c.head_dim)
-            scratch = (torch.empty(no, dtype=torch.float32, device=self.device), torch.empty(nml, dtype=torch.float32, device=self.device)) if num_splits > 1 else None
+            scratch = self._decode_scratch(B, num_splits)
             for _ in range(steps):
                 self._decode_body(st, B, sp, num_splits, scratch)
         return st["tok"][:n], st["lp"][:n]
@@ -1370,13 +1415,16 @@ class GenerationEngine:
                 continue
             x = F.rmsnorm(h, layer.input_layernorm, c.rms_norm_eps)
             qkv = layer.self_attn.project_qkv(x, positions, m.inv_freq, apply_rope=False)
-            qkv = E.rope_kv_cache_write(qkv, positions, self._freq(layer), slots, self.k_cache[li], self.v_cache[li], hq, hkv, D)
+            qkv = self._write_kv(li, qkv, positions, self._freq(layer), slots)
             if pre_slots:
                 # rows of the cached prefix carry keys / values from the cache pages (already rotated) and a zero query
                 full = torch.zeros((total, W), dtype=qkv.dtype, device=dev)
                 full[new_rows] = qkv
-                full[pre_rows, hq * D : (hq + hkv) * D] = self.k_cache[li][pre_blk, :, pre_off, :].reshape(-1, hkv * D)
-                full[pre_rows, (hq + hkv) * D :] = self.v_cache[li][pre_blk, :, pre_off, :].reshape(-1, hkv * D)
+                if self.kv4:
+                    K4.kv4_cache_read(self.k_cache[li], ps, hkv, D, out=full[:, hq * D :], rows=pre_rows)
+                else:
+                    full[pre_rows, hq * D : (hq + hkv) * D] = self.k_cache[li][pre_blk, :, pre_off, :].reshape(-1, hkv * D)
+                    full[pre_rows, (hq + hkv) * D :] = self.v_cache[li][pre_blk, :, pre_off, :].reshape(-1, hkv * D)
                 a = F.attention_varlen(full, cu, max(full_lens), hq, hkv, D, scale=c.attn_scale, window=layer.window)[new_rows]
             else:
                 a = F.attention_varlen(qkv, cu, max(full_lens), hq, hkv, D, scale=c.attn_scale, window=layer.window)
@@ -1665,7 +1713,11 @@ class GenerationEngine:
                                 raw = cache.view(torch.bfloat16)
                                 E.block_copy(raw, raw, src, dst)
                     for li in self._attn_layers:
-                        E.block_copy(self.k_cache[li], self.v_cache[li], src, dst)
+                        if self.kv4:
+                            raw = self.k_cache[li].view(torch.bfloat16)
+                            E.block_copy(raw, raw, src, dst)
+                        else:
+                            E.block_copy(self.k_cache[li], self.v_cache[li], src, dst)
                 new = list(prefill) + list(shared)
                 rows = torch.stack([last_logits[sid] if sid in last_logits else last_logits[reqs[sid].share_with] for sid in new])
                 self._step_counter += 1

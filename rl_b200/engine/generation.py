@@ -34,6 +34,7 @@ GENERATION_DEFAULTS = dict(
     use_cuda_graphs=True,
     free_kv_cache_on_sleep=False,
     seed=0,
+    kv_cache_dtype="auto",  # what keys and values are held in: auto (the model's type) | int4 (vllm_cfg.kv_cache_dtype in the reference)
     precision="bfloat16",   # rollout precision of the linear layers: bfloat16 | mxfp8 | fp8 (vllm_cfg.precision in the reference)
 )
 
@@ -85,9 +86,14 @@ class NativeGeneration:
             model, block_size=c["block_size"], kv_cache_tokens=c["kv_cache_tokens"],
             gpu_memory_utilization=c["gpu_memory_utilization"], max_running=c["max_running"],
             max_prefill_tokens=c["max_prefill_tokens"], max_model_len=c["max_model_len"] or 8192,
-            use_cuda_graphs=c["use_cuda_graphs"], tokenizer=tokenizer,
+            use_cuda_graphs=c["use_cuda_graphs"], tokenizer=tokenizer, kv_cache_dtype="int4" if self._kv_cache_dtype() == "int4" else None,
             quantization=(c.get("native_cfg") or {}).get("precision") or (c.get("vllm_cfg") or {}).get("precision") or c.get("precision"))
         self._calls = 0
+
+    def _kv_cache_dtype(self) -> str:
+        """``int4`` where the configuration asks for it; other names of the reference (fp8 and its forms) have no cache here and serve the model's type."""
+        c = self.cfg
+        return str((c.get("native_cfg") or {}).get("kv_cache_dtype") or (c.get("vllm_cfg") or {}).get("kv_cache_dtype") or c.get("kv_cache_dtype"))
 
     # lifecycle hooks of the generation contract
     def prepare_for_generation(self, *args, **kw) -> bool:

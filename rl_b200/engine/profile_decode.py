@@ -34,6 +34,7 @@ def main(argv=None):
                     "(shares only: durations taken under a profiler are not benchmark figures)")
     ap.add_argument("--trace-out", default="", help="write the traced (kernel, start us, duration us) list to this JSON file")
     ap.add_argument("--quantization", default="", help="mxfp8 | fp8: serve quantised copies of the linear weights (low-precision rollout)")
+    ap.add_argument("--kv-cache-dtype", default="auto", help="int4: keys and values in 4 bits")
     a = ap.parse_args(argv)
     mc = preset(a.model)
     if a.layers:
@@ -41,7 +42,8 @@ def main(argv=None):
     dev = torch.device("cuda", 0)
     model = CausalLM(mc, dtype=torch.bfloat16, device=dev, seed=0)
     eng = GenerationEngine(model, block_size=64, kv_cache_tokens=a.batch * (a.context + a.steps + 64), max_running=max(64, a.batch),
-                           max_model_len=a.context + a.steps + 64, use_cuda_graphs=not a.eager, quantization=a.quantization or None)
+                           max_model_len=a.context + a.steps + 64, use_cuda_graphs=not a.eager, quantization=a.quantization or None,
+                           kv_cache_dtype=a.kv_cache_dtype)
     quant = eng.requantize()
     g = torch.Generator().manual_seed(0)
     n_unique = a.batch if a.distinct_prompts else max(1, a.batch // 8)

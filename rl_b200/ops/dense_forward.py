@@ -13,6 +13,7 @@ from torch.nn.modules import module as _module
 from . import attention as _attention
 from . import functional as F
 from . import lib as _L
+from .kv4_ops import block_size_of as _kv4_block
 from .lib import Counters, call, ptr, stream_ptr, use_native
 
 _P, _I, _LL, _F = C.c_void_p, C.c_int, C.c_longlong, C.c_float
@@ -25,7 +26,7 @@ class _Layer(C.Structure):
 
 class _Forward(C.Structure):
     _fields_ = [(n, _P) for n in ("layers", "h", "out", "mid", "x", "qkv", "att", "gate_up", "act", "positions", "cu_seqlens", "slots", "status")]
-    _fields_ += [(n, _I) for n in ("L", "T", "B", "d", "Hq", "Hkv", "D", "F", "block_size")]
+    _fields_ += [(n, _I) for n in ("L", "T", "B", "d", "Hq", "Hkv", "D", "F", "block_size", "kv4")]
     _fields_ += [("num_blocks", _LL), ("eps", _F), ("scale", _F)]
 
 
@@ -62,7 +63,7 @@ def _weights(layer) -> Optional[tuple]:
 def dense_forward(layers: Sequence, h: torch.Tensor, positions: torch.Tensor, inv_freqs: Sequence[torch.Tensor], cu_seqlens: torch.Tensor, max_seqlen: int, *,
                   slots: Optional[torch.Tensor] = None, k_caches: Sequence = (), v_caches: Sequence = ()) -> Optional[torch.Tensor]:
     """The residual stream after ``layers``, or None where this path does not cover them: then nothing has been done. ``inv_freqs``: one per layer.
-    ``slots``: the rotated keys and the values also go to these places of the layers' caches."""
+    ``slots``: the rotated keys and the values also go to these places of the layers' caches (``v_caches`` empty: ``k_caches`` are the 4-bit caches of both)."""
     c = layers[0].cfg if len(layers) else None
     if c is None or torch.is_grad_enabled() or not use_native(h) or h.dtype != torch.bfloat16 or not h.is_contiguous() or h.shape[0] == 0 or h.data_ptr() % 16:
         return None
@@ -71,7 +72,8 @@ def dense_forward(layers: Sequence, h: torch.Tensor, positions: torch.Tensor, in
         return None
     if c.hidden_size % 8 or any(layer.window and max_seqlen > layer.window for layer in layers):
         return None
-    if slots is not None and not all(k.dtype == torch.bfloat16 and k.is_contiguous() for k in (*k_caches, *v_caches)):
+    kv4 = slots is not None and not len(v_caches)
+    if slots is not None and not all(k.dtype == (torch.uint8 if kv4 else torch.bfloat16) and k.is_contiguous() for k in (*k_caches, *v_caches)):
         return None
     weights = [_weights(layer) for layer in layers]
     if any(w is None for w in weights):
@@ -91,7 +93,7 @@ def dense_forward(layers: Sequence, h: torch.Tensor, positions: torch.Tensor, in
             setattr(slot, name, ptr(t))
         slot.inv_freq = freq.data_ptr()
         if slots is not None:
-            slot.k_cache, slot.v_cache = k_caches[i].data_ptr(), v_caches[i].data_ptr()
+            slot.k_cache, slot.v_cache = k_caches[i].data_ptr(), None if kv4 else v_caches[i].data_ptr()
     positions, cu = positions.to(torch.int32), cu_seqlens.to(torch.int32)
     new = lambda *shape: torch.empty(shape, dtype=torch.bfloat16, device=h.device)      # noqa: E731
     out, mid, x, qkv, att, act = new(T, d), new(T, d), new(T, d), new(T, (Hq + 2 * Hkv) * D), new(T, Hq * D), new(T, ff)
@@ -100,7 +102,7 @@ def dense_forward(layers: Sequence, h: torch.Tensor, positions: torch.Tensor, in
         layers=C.cast(array, _P), h=ptr(h), out=ptr(out), mid=ptr(mid), x=ptr(x), qkv=ptr(qkv), att=ptr(att), gate_up=ptr(gu), act=ptr(act),
         positions=ptr(positions), cu_seqlens=ptr(cu), slots=ptr(slots),
         status=ptr(_L.status_word(h.device)), L=len(layers), T=T, B=cu.numel() - 1, d=d, Hq=Hq, Hkv=Hkv, D=D, F=ff,
-        block_size=k_caches[0].shape[2] if slots is not None else 0,
+        block_size=(_kv4_block(k_caches[0], Hkv, D) if kv4 else k_caches[0].shape[2]) if slots is not None else 0, kv4=int(kv4),
         num_blocks=k_caches[0].shape[0] if slots is not None else 0, eps=c.rms_norm_eps,
         scale=c.attn_scale if c.attn_scale is not None else 1.0 / math.sqrt(D))), stream_ptr())
     Counters.launches += len(layers) * (9 + bool(c.qk_norm)) - 1

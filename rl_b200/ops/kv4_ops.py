@@ -58,7 +58,7 @@ def _page_tokens(page_bytes: int, D: int) -> int:
     return size if 16 <= size <= MAX_BLOCK and size % 16 == 0 and size * D * 9 // 8 == page_bytes else 0
 
 
-def _block_size(cache: torch.Tensor, Hkv: int, D: int) -> int:
+def block_size_of(cache: torch.Tensor, Hkv: int, D: int) -> int:
     """Tokens of a page, from its bytes; refuses what is not a cache of this shape."""
     shape = cache.shape
     if cache.dtype is not torch.uint8 or len(shape) != 3 or not cache.is_contiguous() or cache.data_ptr() % 16:
@@ -143,7 +143,7 @@ def rope_kv4_cache_write(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: t
     """Rotary embedding of the q and k heads of fused rows [T, (Hq + 2 Hkv) D] (in place on CUDA) and the write of the rotated k and of v into the
     4-bit ``cache``, in one launch; returns the rotated fused rows. ``slots`` [T]: block * block_size + offset of each token (negative: rotate only);
     the slots of one call differ from each other. The angles are taken in 64 bits, whatever the position."""
-    block = _block_size(cache, Hkv, D)
+    block = block_size_of(cache, Hkv, D)
     if qkv.dim() != 2 or Hq < 0 or qkv.shape[1] != (Hq + 2 * Hkv) * D:
         raise ValueError(f"qkv is [T, {(Hq + 2 * Hkv) * D}], not {tuple(qkv.shape)}")
     if inv_freq.dtype is not torch.float32 or inv_freq.shape != (D // 2,):
@@ -185,7 +185,7 @@ def kv4_cache_read(cache: torch.Tensor, slots: torch.Tensor, Hkv: int, D: int, *
                    rows: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Keys and values of the tokens at ``slots`` [n] as bf16 rows [k heads | v heads]. ``out`` [m, >= 2 Hkv D]: where they go (its other columns
     stay); ``rows`` [n]: token i goes to row ``rows[i]`` of ``out`` (None: row i), each row named once. A negative slot gives a row of zeros."""
-    block = _block_size(cache, Hkv, D)
+    block = block_size_of(cache, Hkv, D)
     n, width, device = slots.numel(), 2 * Hkv * D, cache.device
     _same_device(device, slots)
     slots = _index(slots, torch.int64, (n,), "slots")
@@ -256,7 +256,7 @@ def kv4_paged_decode(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
     sequence without tokens gives zeros. ``plan``: (cluster, num_ctas): a cluster of up to eight CTAs per sequence and key/value head, or with (1, n) n CTAs
     that share all tokens evenly (None: :func:`kv4_plan` for the table's width); ``scratch``: float32 tensor of :func:`kv4_scratch_size` elements, for callers that
     keep their own. Returns [B, Hq D]."""
-    block = _block_size(cache, Hkv, D)
+    block = block_size_of(cache, Hkv, D)
     device, width = q.device, Hq * D
     if Hq < 1 or Hq % Hkv or q.dim() != 2 or q.shape[1] < width:
         raise ValueError(f"q is [B, {width}] with {Hq} heads, a multiple of {Hkv}, not {tuple(q.shape)}")

@@ -548,7 +548,7 @@ class PolicyWorker:
         g.update(gen_cfg or {})
         native_cfg = dict(g.get("native_cfg") or g.get("vllm_cfg") or {})
         merged = {k: v for k, v in g.items() if k not in ("native_cfg", "vllm_cfg", "colocated", "sglang_cfg")}
-        for k in ("gpu_memory_utilization", "max_model_len", "block_size", "kv_cache_tokens", "max_running", "use_cuda_graphs"):
+        for k in ("gpu_memory_utilization", "max_model_len", "block_size", "kv_cache_tokens", "max_running", "use_cuda_graphs", "kv_cache_dtype"):
             if k in native_cfg:
                 merged[k] = native_cfg[k]
         if native_cfg.get("enforce_eager"):

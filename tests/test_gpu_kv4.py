@@ -5,6 +5,7 @@ import math
 
 import pytest
 import torch
+from kv4_oracle import replayed
 
 from rl_b200.ops import kv4_ops as K
 from rl_b200.ops import lib as L
@@ -338,3 +339,94 @@ def test_graphs_and_streams(native_lib):
         for got in outs[1:]:
             _check(got, K.rope_kv4_cache_write(state["rows"].clone(), state["pos"], freq, torch.full((B,), -1, device="cuda"), eager, Hq, Hkv, D), eager, table, n, Hq, Hkv, D)
     assert L.check_status() == 0
+
+
+# ------------------------------------------------------------------------------------------- the engine
+def _model(**kw):
+    from rl_b200.models.config import ModelConfig
+    from rl_b200.models.transformer import CausalLM
+
+    mc = ModelConfig(**{**dict(model_type="llama", vocab_size=4096, hidden_size=512, intermediate_size=1408, num_hidden_layers=2, num_attention_heads=8,
+                               num_key_value_heads=2, head_dim=128, rope_theta=500000.0), **kw})
+    return CausalLM(mc, dtype=torch.bfloat16, device="cuda", seed=3)
+
+
+def _engine(model, **kw):
+    from rl_b200.engine.engine import GenerationEngine
+
+    return GenerationEngine(model, **{**dict(block_size=16, num_blocks=600, max_running=16, max_model_len=1024, kv_cache_dtype="int4"), **kw})
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(head_dim=64, num_key_value_heads=4), dict(num_attention_heads=7, num_key_value_heads=1, qk_norm=True), dict(head_dim=256, num_attention_heads=4)],
+                         ids=["128", "64", "7-heads", "256"])
+def test_engine_on_the_4_bit_cache(native_lib, kw):
+    """Decoding by graphs and without, prompts in portions and after cached prefixes, against the layers in plain PyTorch over what the cache holds. The bound is that
+    of the bf16 engine against the trainer's pass."""
+    from rl_b200.engine.engine import SamplingParams
+
+    model = _model(**kw)
+    g = torch.Generator().manual_seed(0)
+    prompts = [torch.randint(1, 4096, (n,), generator=g).tolist() for n in (40, 3, 100, 17, 64)]
+    prompts += [prompts[0], prompts[2]]
+    sp = SamplingParams(max_new_tokens=24, stop_token_ids=[], seed=3, temperature=1.0)
+    results = []
+    for opts in (dict(use_cuda_graphs=True), dict(use_cuda_graphs=False), dict(max_prefill_tokens=48)):
+        eng = _engine(model, **opts)
+        seen = {}
+        rounds = eng._prefill_round
+        eng._prefill_round = lambda items, *a, **k: ([seen.setdefault(tuple(q), []).append(p + n) for _, q, p, n in items], rounds(items, *a, **k))[1]
+        recs = eng.generate(prompts, sp)
+        assert L.check_status() == 0
+        results.append([r.out_tokens for r in recs])
+        gaps = []
+        for r in recs:
+            want = replayed(model, r, sorted(set(seen.get(tuple(r.prompt), [len(r.prompt)]))), 1.0).cpu()
+            gaps.append((want - torch.tensor(r.out_logprobs)).abs())
+        gaps = torch.cat(gaps)
+        assert gaps.mean() < 0.03 and gaps.max() < 0.5, (opts, gaps.mean(), gaps.max())
+    assert results[0] == results[1]
+    # a later prompt that begins with cached pages
+    eng = _engine(model)
+    eng.generate([prompts[2]], SamplingParams(max_new_tokens=2, stop_token_ids=[], seed=3))
+    eng.generate([prompts[2] + prompts[3]], SamplingParams(max_new_tokens=4, stop_token_ids=[], seed=3))
+    assert eng.stats["cached_prefix_tokens"] >= 96 and L.check_status() == 0
+
+
+def test_engine_sliding_windows(native_lib):
+    from rl_b200.engine.engine import SamplingParams
+    from rl_b200.models.config import preset
+    from rl_b200.models.transformer import CausalLM
+
+    mc = preset("gemma3-1b", vocab_size=2048, hidden_size=256, intermediate_size=512, num_hidden_layers=3, num_attention_heads=4, num_key_value_heads=2, head_dim=256,
+                sliding_window=32, embed_scale=1.0, layer_types=["sliding_attention", "full_attention", "sliding_attention"])
+    model = CausalLM(mc, dtype=torch.bfloat16, device="cuda", seed=1)
+    g = torch.Generator().manual_seed(0)
+    prompts = [torch.randint(1, 2048, (n,), generator=g).tolist() for n in (70, 5, 33)]
+    eng = _engine(model)
+    recs = eng.generate(prompts, SamplingParams(max_new_tokens=40, stop_token_ids=[], seed=3, temperature=1.0))
+    assert L.check_status() == 0
+    gaps = torch.cat([(replayed(model, r, [len(r.prompt)], 1.0).cpu() - torch.tensor(r.out_logprobs)).abs() for r in recs])
+    assert gaps.mean() < 0.03 and gaps.max() < 0.5, (gaps.mean(), gaps.max())
+
+
+def test_generation_by_configuration(native_lib):
+    """``generation.kv_cache_dtype: int4`` through the policy worker: half and more of the cache's memory is saved, the rollout stays near the policy."""
+    from rl_b200.distributed.batched_data_dict import BatchedDataDict
+    from rl_b200.models.config import ModelConfig
+    from rl_b200.policy.worker import PolicyWorker
+
+    mc = ModelConfig(model_type="llama", vocab_size=4096, hidden_size=512, intermediate_size=1408, num_hidden_layers=2, num_attention_heads=8, num_key_value_heads=2,
+                     head_dim=128, rope_theta=500000.0)
+    g = dict(max_new_tokens=24, stop_token_ids=[], kv_cache_tokens=8192, block_size=64, max_running=32, vllm_cfg=dict(kv_cache_dtype="int4"))
+    p = PolicyWorker(dict(precision="bfloat16", train_global_batch_size=8, train_micro_batch_size=4, max_total_sequence_length=256,
+                          optimizer=dict(name="torch.optim.AdamW", kwargs=dict(lr=1e-4)), generation=g), model_cfg=mc, device="cuda:0", init_reference_model=False, seed=3)
+    gen = p.build_generation()
+    assert gen.engine.kv4
+    gen.prepare_for_generation()
+    ids = torch.randint(1, 4095, (8, 40), generator=torch.Generator().manual_seed(0))
+    out = gen.generate(BatchedDataDict(input_ids=ids, input_lengths=torch.full((8,), 40)))
+    lp = p.get_logprobs(BatchedDataDict(input_ids=out["output_ids"], input_lengths=out["unpadded_sequence_lengths"]))["logprobs"]
+    err = (lp - out["logprobs"]).abs()[out["logprobs"] != 0]
+    assert L.check_status() == 0 and (out["generation_lengths"] == 24).all()
+    assert 0 < err.mean().item() < 0.3 and err.max().item() < 2.0      # the bounds of the other quantised rollouts
+    assert gen.engine.kv_cache_bytes() * 32 == 2 * 2 * gen.engine.num_blocks * 2 * 64 * 128 * 2 * 9

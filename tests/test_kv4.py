@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+from kv4_oracle import replayed
 
 from rl_b200.ops import kv4_ops as K
 
@@ -175,3 +176,89 @@ def test_plan():
                     cluster, ctas = K.kv4_plan(B, Hq, Hkv, D, n)
                     assert 1 <= cluster <= K.MAX_CLUSTER and (ctas == 0 or cluster == 1) and (cluster == 1 or n > 32 * 8 * (cluster - 1))
                     assert ctas in (0, 148 * {64: 4, 128: 3, 256: 2}[D])
+
+
+# ------------------------------------------------------------------------------------------- the engine
+def _model(**kw):
+    from rl_b200.models.config import ModelConfig
+    from rl_b200.models.transformer import CausalLM
+
+    torch.manual_seed(0)
+    mc = ModelConfig(**{**dict(vocab_size=97, hidden_size=64, intermediate_size=96, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2,
+                               head_dim=64, torch_dtype="float32"), **kw})
+    return CausalLM(mc, dtype=torch.float32, device="cpu", seed=1)
+
+
+def _engine(model, **kw):
+    from rl_b200.engine.engine import GenerationEngine
+
+    return GenerationEngine(model, **{**dict(block_size=16, num_blocks=64, max_running=8, max_model_len=128, use_cuda_graphs=False, kv_cache_dtype="int4"), **kw})
+
+
+@pytest.mark.parametrize("kind", ["llama", "qk_norm", "window"])
+def test_engine_on_the_4_bit_cache(kind):
+    """Whole prompts, shared prompts, prompts in portions and cached prefixes give the log-probabilities of the model whose cached keys and values are what 4 bits hold."""
+    from rl_b200.engine.engine import SamplingParams
+    from rl_b200.models.config import preset
+    from rl_b200.models.transformer import CausalLM
+
+    model = _model(qk_norm=True) if kind == "qk_norm" else _model()
+    if kind == "window":
+        mc = preset("gemma3-1b", torch_dtype="float32", vocab_size=97, hidden_size=32, intermediate_size=64, num_hidden_layers=3, num_attention_heads=4,
+                    num_key_value_heads=2, head_dim=64, sliding_window=6, attn_scale=0.1, embed_scale=32 ** 0.5,
+                    layer_types=["sliding_attention", "full_attention", "sliding_attention"])
+        model = CausalLM(mc, dtype=torch.float32, device="cpu", seed=1)
+    long = [(7 * i) % 90 + 1 for i in range(37)]
+    prompts = [long, long, [9, 8, 7], [11] * 16, [5] * 17]
+    sp = SamplingParams(max_new_tokens=9, stop_token_ids=[], seed=3, temperature=0.8)
+    for kw, portions in ((dict(), lambda n: [n]), (dict(max_prefill_tokens=16), None)):
+        eng = _engine(model, **kw)
+        seen = {}
+        if portions is None:      # (a round's budget is shared by its prompts: what each portion is, is looked at)
+            rounds = eng._prefill_round
+            eng._prefill_round = lambda items, *a, **k: ([seen.setdefault(tuple(q), []).append(p + n) for _, q, p, n in items], rounds(items, *a, **k))[1]
+        for r in eng.generate(prompts, sp):
+            n = len(r.prompt)
+            cut = portions(n) if portions else seen.get(tuple(r.prompt), [n])
+            want = replayed(model, r, cut, 0.8)
+            # float32 on both sides, sums in other orders; a value may fall on the other side of its code's border: one level of one value of 64
+            assert (want - torch.tensor(r.out_logprobs)).abs().max() < 5e-3, (kw, n)
+        assert portions is not None or any(len(v) > 1 for v in seen.values())
+
+
+def test_engine_shares_and_evicts_like_the_other_cache():
+    """Siblings of a prompt whose last page is copied, and sequences that lose their pages and are prefilled again, are greedy alike."""
+    from rl_b200.engine.engine import SamplingParams
+
+    model = _model()
+    prompt = [(5 * i) % 90 + 1 for i in range(21)]
+    sp = SamplingParams(max_new_tokens=20, stop_token_ids=[], seed=3, temperature=0.0)
+    one = _engine(model).generate([prompt], sp)[0].out_tokens
+    assert all(r.out_tokens == one for r in _engine(model).generate([prompt] * 6, sp))
+    tight = _engine(model, num_blocks=9)
+    assert all(len(r.out_tokens) == 20 for r in tight.generate([prompt, [3] * 20, [4] * 30], sp))
+
+
+def test_engine_memory_and_refusals():
+    from rl_b200.engine.engine import GenerationEngine
+    from rl_b200.engine.generation import NativeGeneration
+    from rl_b200.models.config import preset
+    from rl_b200.models.transformer import CausalLM
+
+    model = _model()
+    small, big = _engine(model), _engine(model, kv_cache_dtype="auto")
+    small.wake()
+    big.wake()
+    assert small.kv_cache_bytes() == sum(t.numel() for t in small.k_cache) and small.v_cache == [None, None]
+    assert small.kv_cache_bytes() * 32 == big.kv_cache_bytes() * 9 // 2      # 4.5 bits a value; the model here has 32
+    for bad in (dict(kv_cache_dtype="int3"), dict(block_size=24), dict(block_size=4)):
+        with pytest.raises(ValueError):
+            _engine(model, **bad)
+    with pytest.raises(ValueError):
+        _engine(_model(head_dim=32))
+    layered = CausalLM(preset("tiny-gadarax", torch_dtype="float32"), dtype=torch.float32, device="cpu", seed=1)
+    with pytest.raises(NotImplementedError):
+        GenerationEngine(layered, block_size=16, num_blocks=8, max_running=2, max_model_len=64, use_cuda_graphs=False, kv_cache_dtype="int4")
+    cfg = dict(block_size=16, kv_cache_tokens=256, max_running=4, max_model_len=64, use_cuda_graphs=False)
+    assert NativeGeneration(model, dict(cfg, kv_cache_dtype="int4")).engine.kv4 and NativeGeneration(model, dict(cfg, vllm_cfg=dict(kv_cache_dtype="int4"))).engine.kv4
+    assert not NativeGeneration(model, dict(cfg, vllm_cfg=dict(kv_cache_dtype="fp8"))).engine.kv4 and not NativeGeneration(model, cfg).engine.kv4
