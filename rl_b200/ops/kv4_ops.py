@@ -87,6 +87,16 @@ def _aligned(t: torch.Tensor) -> bool:
     return stride[1] == 1 and stride[0] % 8 == 0 and t.data_ptr() % 16 == 0
 
 
+def _apart(t: torch.Tensor, width: int) -> bool:
+    """Whether the rows that are written do not overlap (copying to rows that do is refused by PyTorch)."""
+    return t.shape[0] < 2 or t.stride(0) >= width
+
+
+def _no_gradient(t: torch.Tensor) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError("the 4-bit cache has no gradient: call under torch.no_grad()")
+
+
 # --------------------------------------------------------------------------------------- PyTorch restatement
 def quantize_ref(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """[..., D] -> codes uint8 [..., D / 32, 32] and bf16 scales [..., D / 32]."""
@@ -149,6 +159,7 @@ def rope_kv4_cache_write(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: t
     if inv_freq.dtype is not torch.float32 or inv_freq.shape != (D // 2,):
         raise ValueError(f"inv_freq is a float32 vector of {D // 2}, not {inv_freq.dtype} {tuple(inv_freq.shape)}")
     T = qkv.shape[0]
+    _no_gradient(qkv)
     _same_device(qkv.device, positions, inv_freq, slots, cache)
     positions, slots = _index(positions, torch.int32, (T,), "positions"), _index(slots, torch.int64, (T,), "slots")
     if not use_native(qkv):
@@ -172,7 +183,7 @@ def rope_kv4_cache_write(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: t
     if torch.cuda.current_device() != index:      # kernels go to the current stream of the tensors' device, whichever device is current
         with torch.cuda.device(qkv.device):
             return rope_kv4_cache_write(qkv, positions, inv_freq, slots, cache, Hq, Hkv, D)
-    rows = qkv if _aligned(qkv) else qkv.clone(memory_format=torch.contiguous_format)      # (rows that do not start on 16 bytes: turned in a copy)
+    rows = qkv if _aligned(qkv) and _apart(qkv, qkv.shape[1]) else qkv.clone(memory_format=torch.contiguous_format)      # (rows that do not start on 16 bytes: turned in a copy)
     inv_freq = inv_freq.contiguous()
     call("rlb_rope_kv4_cache_write", rows.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), slots.data_ptr(), cache.data_ptr(), T, Hq, Hkv, D, block,
          rows.stride(0), cache.shape[0], _L.status_word(qkv.device).data_ptr(), _raw_stream(index))
@@ -202,10 +213,10 @@ def kv4_cache_read(cache: torch.Tensor, slots: torch.Tensor, Hkv: int, D: int, *
         _same_device(device, out)
     if not use_native(cache):
         kc, vc, ks, vs = _unpack_pages(cache[(slots // block).clamp(min=0)], D)      # [n, Hkv, block, ...]
-        ar, off = torch.arange(n), slots.clamp(min=0) % block
+        ar, off = torch.arange(n, device=device), slots.clamp(min=0) % block
         kv = torch.stack([_values(kc, ks)[ar, :, off], _values(vc, vs)[ar, :, off]], 1).reshape(n, width)
         kv = torch.where(slots[:, None] < 0, torch.zeros_like(kv), kv)
-        out[torch.arange(n) if rows is None else rows, :width] = kv.to(out.dtype)
+        out[ar if rows is None else rows, :width] = kv.to(out.dtype)
         return out
     if out.dtype is not BF16:
         raise ValueError(f"the 4-bit cache is read into bf16 rows, not {out.dtype}")
@@ -214,7 +225,7 @@ def kv4_cache_read(cache: torch.Tensor, slots: torch.Tensor, Hkv: int, D: int, *
         with torch.cuda.device(device):
             return kv4_cache_read(cache, slots, Hkv, D, out=out, rows=rows)
     to = out
-    if not _aligned(out):      # rows that do not start on 16 bytes: read into a copy
+    if not (_aligned(out) and _apart(out, width)):      # rows that do not start on 16 bytes: read into a copy
         to = torch.empty((out.shape[0], width), dtype=BF16, device=device).copy_(out[:, :width])
     call("rlb_kv4_cache_read", cache.data_ptr(), slots.data_ptr(), ptr(rows), to.data_ptr(), n, to.stride(0), to.shape[0], Hkv, D, block, cache.shape[0],
          _L.status_word(device).data_ptr(), _raw_stream(index))
@@ -255,22 +266,23 @@ def kv4_paged_decode(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
     ``seq_lens`` [B] int32 tokens in the pages that ``block_table`` [B, pages] int32 names, of which ``window`` > 0 leaves the last ``window``. A
     sequence without tokens gives zeros. ``plan``: (cluster, num_ctas): a cluster of up to eight CTAs per sequence and key/value head, or with (1, n) n CTAs
     that share all tokens evenly (None: :func:`kv4_plan` for the table's width); ``scratch``: float32 tensor of :func:`kv4_scratch_size` elements, for callers that
-    keep their own. Returns [B, Hq D]."""
+    keep their own (one call at a time). Returns [B, Hq D]."""
     block = block_size_of(cache, Hkv, D)
     device, width = q.device, Hq * D
     if Hq < 1 or Hq % Hkv or q.dim() != 2 or q.shape[1] < width:
         raise ValueError(f"q is [B, {width}] with {Hq} heads, a multiple of {Hkv}, not {tuple(q.shape)}")
-    if window < 0:
-        raise ValueError(f"window {window} is negative")
+    if window < 0 or (scale is not None and not math.isfinite(scale)):
+        raise ValueError(f"window {window} is negative, or scale {scale} not a number")
     B = q.shape[0]
     _same_device(device, cache, block_table, seq_lens)
     if block_table.dim() != 2:
         raise ValueError(f"block_table is [{B}, pages], not {tuple(block_table.shape)}")
     pages = block_table.shape[1]
-    table = block_table
-    if table.dtype is not torch.int32 or table.shape[0] != B or table.stride(1) != 1:      # (rows of a wider table are read where they are)
-        table = _index(table, torch.int32, (B, pages), "block_table")
-    lens = _index(seq_lens, torch.int32, (B,), "seq_lens")
+    if block_table.shape[0] != B or seq_lens.shape != (B,) or block_table.dtype is not torch.int32 or seq_lens.dtype is not torch.int32:
+        raise ValueError(f"block_table is int32 [{B}, pages] and seq_lens int32 [{B}], not {block_table.dtype} {tuple(block_table.shape)} and {seq_lens.dtype} {tuple(seq_lens.shape)}")
+    _no_gradient(q)
+    table = block_table if block_table.stride(1) == 1 else block_table.contiguous()      # (rows of a wider table are read where they are)
+    lens = seq_lens.contiguous()
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     if out is None:
@@ -315,7 +327,7 @@ def kv4_paged_decode(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
     if not _aligned(q):      # rows that do not start on 16 bytes
         q = q[:, :width].clone(memory_format=torch.contiguous_format)
     stride = out.stride()
-    to = out if stride[1] == 1 and stride[0] % 4 == 0 and out.data_ptr() % 8 == 0 else torch.empty((B, width), dtype=BF16, device=device)
+    to = out if stride[1] == 1 and stride[0] % 4 == 0 and out.data_ptr() % 8 == 0 and _apart(out, width) else torch.empty((B, width), dtype=BF16, device=device)
     call("rlb_kv4_paged_decode", q.data_ptr(), q.stride(0), cache.data_ptr(), cache.shape[0], table.data_ptr(), table.stride(0), pages, lens.data_ptr(), B, Hq, Hkv,
          D, block, window, scale, cluster, num_ctas, sums, parts, to.data_ptr(), to.stride(0), _L.status_word(device).data_ptr(), _raw_stream(index))
     if to is not out:

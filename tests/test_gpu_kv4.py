@@ -141,7 +141,7 @@ def _check(got, q, cache, table, lens, Hq, Hkv, D, window=0, scale=None):
         qb = q[b, : Hq * D].double().reshape(Hkv, Hq // Hkv, D)
         p = torch.softmax(qb @ k.transpose(1, 2) * scale, -1)
         want, share = p @ v, p @ v.abs()
-        e = scale * 33 * 2.0 ** -24 * 15 * torch.einsum("hgd,hd->hg", qb.abs(), ks.double().repeat_interleave(32, -1).flatten(1, 2)[:, lo:n].amax(1)).unsqueeze(-1)
+        e = abs(scale) * 33 * 2.0 ** -24 * 15 * torch.einsum("hgd,hd->hg", qb.abs(), ks.double().repeat_interleave(32, -1).flatten(1, 2)[:, lo:n].amax(1)).unsqueeze(-1)
         tol = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2 * e + 2.0 ** -18) * share
         off = (got[b].double().reshape(want.shape) - want).abs()
         assert (off <= tol).all(), f"row {b}: {(off / tol).max().item():.2f} times the tolerance"
@@ -193,6 +193,32 @@ def test_decode_of_small_large_and_peaked(native_lib, big, scale):
         _check(K.kv4_paged_decode(q, cache, table, n, 8, 2, 128, scale=scale, plan=plan), q, cache, table, n, 8, 2, 128, scale=scale)
 
 
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1e-38])
+def test_decode_scales(native_lib, scale):
+    """A negative scale, and scales that leave every token the same weight."""
+    for Hq in (4, 10):
+        q, cache, table, n = _decode_case([700, 33, 1], Hq, 2, 64, 16, seed=6)
+        for plan in ((1, 0), (4, 0), (1, 7)):
+            got = K.kv4_paged_decode(q, cache, table, n, Hq, 2, 64, scale=scale, plan=plan)
+            _check(got, q, cache, table, n, Hq, 2, 64, scale=scale or 1e-300)
+    with pytest.raises(ValueError):
+        K.kv4_paged_decode(q, cache, table, n, 10, 2, 64, scale=math.nan)
+
+
+@pytest.mark.parametrize("Hq", [4, 16])
+def test_a_query_that_is_not_finite_spoils_its_head_alone(native_lib, Hq):
+    q, cache, table, n = _decode_case([50, 300], Hq, 2, 128, 16, seed=2)
+    for plan in ((1, 0), (3, 0), (1, 5)):
+        clean = K.kv4_paged_decode(q, cache, table, n, Hq, 2, 128, plan=plan).view(2, Hq, 128)
+        for bad in (math.nan, math.inf):
+            x = q.clone()
+            x[1, 128 + 77] = bad
+            got = K.kv4_paged_decode(x, cache, table, n, Hq, 2, 128, plan=plan).view(2, Hq, 128)
+            assert got[1, 1].isnan().all()
+            got[1, 1] = clean[1, 1]
+            assert torch.equal(got, clean)
+
+
 @pytest.mark.parametrize("plan", [(1, 0), (5, 0), (1, 2), (1, 33)])
 def test_decode_ignores_what_stands_behind_the_end(native_lib, plan):
     """NaN and infinite scales, and any codes, in places that the sequence does not see: before the window and behind its last token."""
@@ -235,7 +261,7 @@ def test_decode_of_odd_views(native_lib):
     wide = torch.full((4, 2 * Hq * D), 7.0, dtype=torch.bfloat16, device="cuda")
     for out in (wide[:, 4 : 4 + Hq * D], wide[:, 1 : 1 + Hq * D], wide[:, ::2]):
         wide.fill_(7.0)
-        got = K.kv4_paged_decode(odd, cache, table.long().t().contiguous().t(), n.long(), Hq, Hkv, D, out=out)
+        got = K.kv4_paged_decode(odd, cache, table.t().contiguous().t(), torch.stack([n, n], 1)[:, 0], Hq, Hkv, D, out=out)
         assert got is out and torch.equal(out, want) and int((wide == 7).sum()) >= 4 * Hq * D
     assert K.kv4_paged_decode(q[:0], cache, table[:0], n[:0], Hq, Hkv, D).shape == (0, Hq * D)
     scratch = torch.empty(K.kv4_scratch_size(3, D) + 4, device="cuda")
@@ -246,9 +272,15 @@ def test_decode_of_odd_views(native_lib):
     for bad in ((0, 0), (9, 0), (2, 5), (1, -1)):
         with pytest.raises(ValueError):
             K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, plan=bad)
-    for bad in (q.float(), q.half(), q.cpu()):
+    for bad in (q.float(), q.half(), q.cpu(), q.clone().requires_grad_()):
         with pytest.raises(ValueError):
             K.kv4_paged_decode(bad, cache, table, n, Hq, Hkv, D)
+    with pytest.raises(RuntimeError):      # rows that overlap
+        K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, out=torch.zeros(1, Hq * D, dtype=torch.bfloat16, device="cuda").expand(4, -1))
+    with pytest.raises(RuntimeError):
+        K.rope_kv4_cache_write(q[:1].expand(4, -1), n, _freq(D).cuda(), torch.arange(4, device="cuda"), cache.clone(), Hq, Hkv, D)
+    with pytest.raises(RuntimeError):
+        K.kv4_cache_read(cache, n, Hkv, D, out=torch.zeros(1, 2 * Hkv * D, dtype=torch.bfloat16, device="cuda").expand(4, -1))
     with pytest.raises(ValueError):
         K.rope_kv4_cache_write(q.float(), n, _freq(D).cuda(), n, cache, Hq, Hkv, D)
     with pytest.raises(ValueError):

@@ -125,7 +125,7 @@ def test_decode_and_write_together(D, Hkv, block, window):
         got = K.kv4_paged_decode(row, cache, table, torch.tensor([t + 1], dtype=torch.int32), Hq, Hkv, D, window=window)[0].double()
         # all in 32 bits: sums over D and over n, both below 2^9 terms
         assert (got - want).abs().max() <= 2.0 ** -24 * 2 ** 9 * 8 * v.abs().max()
-    assert not K.kv4_paged_decode(row, cache, table, torch.tensor([0]), Hq, Hkv, D).any()
+    assert not K.kv4_paged_decode(row, cache, table, torch.tensor([0], dtype=torch.int32), Hq, Hkv, D).any()
 
 
 def test_refusals():
@@ -156,6 +156,11 @@ def test_refusals():
         lambda: K.kv4_paged_decode(x, cache, bt[0], ln, 4, 2, 64),
         lambda: K.kv4_paged_decode(x, cache, bt, ln[:0], 4, 2, 64),
         lambda: K.kv4_paged_decode(x, cache, bt.float(), ln, 4, 2, 64),
+        lambda: K.kv4_paged_decode(x, cache, bt.long(), ln, 4, 2, 64),
+        lambda: K.kv4_paged_decode(x, cache, bt, ln.long(), 4, 2, 64),
+        lambda: K.kv4_paged_decode(x, cache, bt, ln, 4, 2, 64, scale=math.inf),
+        lambda: K.kv4_paged_decode(x.float().requires_grad_(), cache, bt, ln, 4, 2, 64),
+        lambda: K.rope_kv4_cache_write(x.float().requires_grad_(), one, f, one, cache, 4, 2, 64),
         lambda: K.kv4_paged_decode(x, cache, bt, ln, 4, 2, 64, window=-1),
         lambda: K.kv4_paged_decode(x, cache, bt, ln, 4, 2, 64, out=torch.zeros(1, 256)),
         lambda: K.kv4_paged_decode(x, cache, bt, ln, 4, 2, 64, out=torch.zeros(2, 256).bfloat16()),
