@@ -364,11 +364,12 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D == 64 ? 4 : D == 128 ? 3 : 2)
       if constexpr (PAIR) query[NS][g][lane] = r >= 4 ? all : none;
       offset[g][lane] = make_float2(-0.5f * acc[0], -0.5f * acc[1]);
     }
-    const float unit = fminf(fmaxf(times_pow2(fabsf(p.scale) * 1.4426950408889634f, 133 - k), 1e-30f), 1e30f);
+    // (never 0, so that -inf times it stays -inf; the slack is finite, so that any score passes -inf)
+    const float unit = fminf(fmaxf(times_pow2(fabsf(p.scale) * 1.4426950408889634f, 133 - k), 0x1p-149f), 0x1p127f);
     c[0] = __shfl_sync(0xffffffffu, unit, 8 * t);
     c[1] = __shfl_sync(0xffffffffu, unit, 8 * t + 4);
-    slack[0] = K4_SLACK / c[0];
-    slack[1] = K4_SLACK / c[1];
+    slack[0] = fminf(K4_SLACK / c[0], 0x1p127f);
+    slack[1] = fminf(K4_SLACK / c[1], 0x1p127f);
   }
   __syncthreads();
 

@@ -86,14 +86,15 @@ class NativeGeneration:
             model, block_size=c["block_size"], kv_cache_tokens=c["kv_cache_tokens"],
             gpu_memory_utilization=c["gpu_memory_utilization"], max_running=c["max_running"],
             max_prefill_tokens=c["max_prefill_tokens"], max_model_len=c["max_model_len"] or 8192,
-            use_cuda_graphs=c["use_cuda_graphs"], tokenizer=tokenizer, kv_cache_dtype="int4" if self._kv_cache_dtype() == "int4" else None,
+            use_cuda_graphs=c["use_cuda_graphs"], tokenizer=tokenizer, kv_cache_dtype=self._kv_cache_dtype(),
             quantization=(c.get("native_cfg") or {}).get("precision") or (c.get("vllm_cfg") or {}).get("precision") or c.get("precision"))
         self._calls = 0
 
     def _kv_cache_dtype(self) -> str:
-        """``int4`` where the configuration asks for it; other names of the reference (fp8 and its forms) have no cache here and serve the model's type."""
+        """What the configuration asks for; the reference's names for types that have no cache here (fp8 and its forms) serve the model's type."""
         c = self.cfg
-        return str((c.get("native_cfg") or {}).get("kv_cache_dtype") or (c.get("vllm_cfg") or {}).get("kv_cache_dtype") or c.get("kv_cache_dtype"))
+        name = str((c.get("native_cfg") or {}).get("kv_cache_dtype") or (c.get("vllm_cfg") or {}).get("kv_cache_dtype") or c.get("kv_cache_dtype") or "auto")
+        return "auto" if name.startswith(("fp8", "bfloat16", "float16")) else name
 
     # lifecycle hooks of the generation contract
     def prepare_for_generation(self, *args, **kw) -> bool:

@@ -205,6 +205,17 @@ def test_decode_scales(native_lib, scale):
         K.kv4_paged_decode(q, cache, table, n, 10, 2, 64, scale=math.nan)
 
 
+@pytest.mark.parametrize("q_by,big,scale", [(2.0 ** -120, 2.0 ** 118, 0.1), (2.0 ** 104, 2.0 ** -88, 2.0 ** -16), (1.0, 2.0 ** 118, 0.0), (2.0 ** -125, 1.0, None)])
+def test_decode_of_scores_from_far_apart_factors(native_lib, q_by, big, scale):
+    """Queries, keys and scales at the ends of their type whose products are ordinary scores, or none at all."""
+    for Hq in (4, 10):
+        q, cache, table, n = _decode_case([700, 33, 1], Hq, 2, 64, 16, seed=7, big=big)
+        q = (q.double() * q_by).bfloat16()
+        for plan in ((1, 0), (4, 0), (1, 7)):
+            got = K.kv4_paged_decode(q, cache, table, n, Hq, 2, 64, scale=scale, plan=plan)
+            _check(got, q, cache, table, n, Hq, 2, 64, scale=1e-300 if scale == 0 else scale)
+
+
 @pytest.mark.parametrize("Hq", [4, 16])
 def test_a_query_that_is_not_finite_spoils_its_head_alone(native_lib, Hq):
     q, cache, table, n = _decode_case([50, 300], Hq, 2, 128, 16, seed=2)

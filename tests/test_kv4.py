@@ -267,3 +267,6 @@ def test_engine_memory_and_refusals():
     cfg = dict(block_size=16, kv_cache_tokens=256, max_running=4, max_model_len=64, use_cuda_graphs=False)
     assert NativeGeneration(model, dict(cfg, kv_cache_dtype="int4")).engine.kv4 and NativeGeneration(model, dict(cfg, vllm_cfg=dict(kv_cache_dtype="int4"))).engine.kv4
     assert not NativeGeneration(model, dict(cfg, vllm_cfg=dict(kv_cache_dtype="fp8"))).engine.kv4 and not NativeGeneration(model, cfg).engine.kv4
+    for bad in (dict(kv_cache_dtype="int8"), dict(vllm_cfg=dict(kv_cache_dtype="int"))):
+        with pytest.raises(ValueError):
+            NativeGeneration(model, {**cfg, **bad})
