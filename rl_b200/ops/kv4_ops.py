@@ -239,18 +239,18 @@ def kv4_plan(B: int, Hq: int, Hkv: int, D: int, max_len: int, sm_count: int = 14
     """How decode attention over the 4-bit cache is cut up: (cluster, 0): a cluster of CTAs per sequence and key/value head (with up to eight query
     heads), or (1, n): n CTAs, as many as the device holds, share all tokens evenly, and a second kernel joins what they cut through.
 
-    Sharing costs some 4 us and pays off for sequences of 3200 tokens and more (8 KV heads of 128, four query heads each, us in a graph, one CTA each / shared: 64
-    sequences of 16000 tokens 259 / 222, of 4000 73 / 70, of 1280 30 / 34; 16 of 4000 29 / 27, of 1000 11 / 16), where there are no more than two CTAs for each that
-    the device holds (128 of 4000: 118 / 125). Few sequences are cut into a cluster of at least eight steps of 32 tokens per CTA, one CTA on most SMs
-    (us with one, four, eight CTAs: one sequence of 1000 tokens 9.7, 7.0, 6.6, of 4000 27, 12, 9.4 and shared 14; four of 4000 28, 14, 14 and shared 16; 16 of 1000
-    11, 18, 24)."""
+    A cluster of twice the CTAs is taken while they run at once and keep 12 steps of 32 tokens each, or 24 where some SMs get two (us in a graph with one, two,
+    four, eight CTAs: one sequence of 1000 tokens with 8 KV heads of 128 9.7, 8.0, 7.0, 6.6; 12 of 600 7.2, 8.3, 8.1, 14.6; 26 of 2400 with 4 heads
+    21.1, 17.7, 15.5; 48 of 2400 26.7, 22.5, 28.7). Sharing has its search and its join, some 5 us, and pays off from 50 steps per CTA on (8 heads of 128, best cluster /
+    shared: one sequence of 4800 tokens 9.7 / 10.7, of 19200 20.8 / 18.6, of 40000 36 / 23; 64 of 4000 67 / 67, of 16000 259 / 222), where there are at most two CTAs for each that
+    the device holds (128 of 4000: 112 / 120). Of 732 calls with 8 to 384 sequences times heads the mean is 1.1 % above the best of the five choices, the worst 20 %."""
     segments, steps = max(1, B) * Hkv * -(-(Hq // Hkv) // 8), -(-max_len // 32)
-    slots = (3 if D > 64 else 4) * sm_count if D <= 128 else 2 * sm_count
-    if steps >= 100 and segments < 2 * slots and (steps >= 400 or steps * segments >= 10000) and segments * (steps + 2) < 2**30:
-        return 1, slots
+    slots = (4 if D == 64 else 3 if D == 128 else 2) * sm_count
     cluster = 1
-    while cluster < MAX_CLUSTER and 2 * cluster * segments <= 200 and 16 * cluster <= steps:
+    while cluster < MAX_CLUSTER and 2 * cluster * segments <= slots and steps >= cluster * (12 if 2 * cluster * segments <= 200 else 24):
         cluster *= 2
+    if steps >= max(100, 50 * cluster) and segments < 2 * slots and segments * (steps + 2) < 2**30:
+        return 1, slots
     return cluster, 0
 
 
