@@ -1,8 +1,11 @@
 // Writing and reading the 4-bit key/value cache of the generation engine (kv4.cuh has the format).
 //
-// Both kernels move every byte once and are bound by memory: D / 16 threads take a head of a token, each eight dimensions of its lower half and the
-// eight that these pair with in the rotation, so that neither the rotation nor the unpacking needs another thread; four neighbouring threads hold
-// a group of 32 and find its largest magnitude with two shuffles.
+// Both kernels move every byte once and are bound by memory. Write: D / 16 threads take a head of a token, each eight dimensions of its lower half and the
+// eight that these pair with in the rotation, so that the rotation needs no other thread; four neighbouring threads hold a group of 32 and find its largest
+// magnitude with two shuffles. Read-back: four threads a head, each eight dimensions of every group, whose codes stand in one load.
+//
+// Measured (a graph of calls on states larger than L2): write of 15003 tokens of 32 + 2 * 8 heads of 128 62 us, 5.7 TB/s, 0.87 of what a plain copy moves (three quarters
+// of the instruction slots are used); 64 tokens 2.7 us, one 2.5 us: a launch and two dependent loads. Read-back of 32771 tokens of 8 heads of 128 29.8 us, 5.8 TB/s, 0.88; 517 of 4 of 64 2.1 us.
 //
 // The reference reaches its quantised caches through vLLM's kv_cache_dtype (nemo_rl/models/generation/vllm/config.py).
 #include "kv4.cuh"

@@ -1,6 +1,7 @@
 // Decode attention over the 4-bit key/value cache (kv4.cuh): one query token per sequence, softmax(scale q k^T) v over its cached tokens or the last
-// `window` of them. A CTA of four warps takes a sequence and one key/value head with up to eight of its query heads; or as many CTAs as the device holds
-// share all tokens evenly, so that each gets a run of whole sequences and a part of one or two, and a second kernel joins the parts.
+// `window` of them. A CTA of four warps takes a sequence and one key/value head with up to eight of its query heads. Few sequences: a cluster of up to eight CTAs
+// shares the tokens of each and adds the parts through distributed shared memory. Long ones: as many CTAs as the device holds share all tokens evenly, so that each gets
+// a run of whole sequences and a part of one or two, and a second kernel joins the parts (kv4_plan in ops/kv4_ops.py has the choice, both sides measured).
 //
 // Both products run as 16 x 8 x 16 tensor-core instructions whose 16-row operand comes from the codes in registers; the query heads are the eight columns:
 //     S^T[16 tokens, 8 heads] = K[16 tokens, dims] Q^T        O^T[16 dims, 8 heads] += V^T[16 dims, 16 tokens] P^T
@@ -12,7 +13,13 @@
 // such that a thread's registers are what it loads: no shuffle and no pass through shared memory. A thread's rows of S^T are the
 // tokens 4 (r / 2) + r % 2 and two later (r = lane / 4), so that the columns it has to hold of V^T are four consecutive tokens.
 //
-// tcgen05 would want the unpacked keys and values written to shared or tensor memory first; the unpacking is what bounds the kernel, not the products.
+// tcgen05 would want the unpacked keys and values written to shared or tensor memory first; the unpacking is what bounds the kernel, not the products (a third of
+// mma.sync's rate at long contexts): 5 of a word's instructions are its unpacking, 65 of 125 million instructions of the case below run on the integer pipe.
+//
+// Measured (a graph of calls on states larger than L2): 32 sequences of 32768 tokens, 32 query and 8 KV heads of 128: 217 us, 5.57 TB/s, 0.85 of what a plain copy moves;
+// 258 us back to back for seconds, at the board's power limit. 64 / 8 heads 241 us. 64 of 4000 67 us, 128 of 4000 112 us, 64 of 1280 27 us (two waves of CTAs), one of
+// 131072 with 40 heads 45 us, one of 4000 9.1 us, 48 of 1024 with heads of 256 30 us. Short calls are a chain of latencies: length, page, keys, a step's products and softmax
+// (some 0.8 us a step of a warp alone on its scheduler, however many steps are on their way), the join.
 //
 // The reference's counterpart is the paged attention behind vLLM's kv_cache_dtype (nemo_rl/models/generation/vllm/config.py).
 #include "kv4.cuh"
