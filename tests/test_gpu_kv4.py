@@ -52,6 +52,12 @@ def test_write_is_exact(native_lib, T, D, Hq, Hkv, block):
     assert torch.equal(back.cpu(), K.kv4_cache_read(ref, slots, Hkv, D))
 
 
+@pytest.mark.parametrize("T,D,Hq,Hkv,block", [(2003, 64, 32, 4, 32), (1001, 128, 32, 8, 64), (1333, 128, 28, 4, 16), (701, 256, 20, 10, 16)])
+def test_write_of_more_rows_than_the_device_holds_threads(native_lib, T, D, Hq, Hkv, block):
+    """Blocks of several whole rows, the last one short."""
+    test_write_is_exact(native_lib, T, D, Hq, Hkv, block)
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_write_of_special_values(native_lib, D):
     T, Hq, Hkv, block = 12, 1, 1, 16
