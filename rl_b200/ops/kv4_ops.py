@@ -239,18 +239,19 @@ def kv4_plan(B: int, Hq: int, Hkv: int, D: int, max_len: int, sm_count: int = 14
     """How decode attention over the 4-bit cache is cut up: (cluster, 0): a cluster of CTAs per sequence and key/value head (with up to eight query
     heads), or (1, n): n CTAs, as many as the device holds, share all tokens evenly, and a second kernel joins what they cut through.
 
-    A cluster of twice the CTAs is taken while they run at once and keep 12 steps of 32 tokens each, or 24 where some SMs get two (us in a graph with one, two,
-    four, eight CTAs: one sequence of 1000 tokens with 8 KV heads of 128 9.7, 8.0, 7.0, 6.6; 12 of 600 7.2, 8.3, 8.1, 14.6; 26 of 2400 with 4 heads
-    21.1, 17.7, 15.5; 48 of 2400 26.7, 22.5, 28.7). Sharing has its search and its join, some 5 us, and pays off from 50 steps per CTA on (8 heads of 128, best cluster /
-    shared: one sequence of 4800 tokens 9.7 / 10.7, of 19200 20.8 / 18.6, of 40000 36 / 23; 64 of 4000 67 / 67, of 16000 259 / 222), where there are at most two CTAs for each that
-    the device holds (128 of 4000: 112 / 120). Of 732 calls with 8 to 384 sequences times heads the mean is 1.1 % above the best of the five choices, the worst 20 %."""
+    A cluster of twice the CTAs is taken while they run at once and keep 12 steps of 32 tokens each, and a few more where some SMs get two (us in a graph with one,
+    two, four, eight CTAs: one sequence of 1200 tokens with 8 KV heads of 128 10.6, 8.6, 7.3, 7.1; 12 of 600 7.3, 8.3, 8.0, 14.5; 26 of 2400 with 4 heads
+    21.0, 17.8, 15.6; 48 of 2400 26.6, 22.5, 28.5). Sharing has its search and its join, some 5 us, and pays off from 50 steps per CTA on (8 heads of 128, best cluster /
+    shared: one sequence of 4800 tokens 9.7 / 10.7, of 40000 36 / 23; 64 of 4000 71 / 67, of 16000 255 / 214), where there are at most two CTAs for each that
+    the device holds (128 of 4000: 112 / 120); with two CTAs an SM where they would get less than 20 steps otherwise (one of 19200: 15.9, all places 18.8). Of 732
+    calls with 8 to 384 sequences times heads the mean is 1.0 % above the best of five choices, the worst 20 %."""
     segments, steps = max(1, B) * Hkv * -(-(Hq // Hkv) // 8), -(-max_len // 32)
     slots = (4 if D == 64 else 3 if D == 128 else 2) * sm_count
     cluster = 1
-    while cluster < MAX_CLUSTER and 2 * cluster * segments <= slots and steps >= cluster * (12 if 2 * cluster * segments <= 200 else 24):
+    while cluster < MAX_CLUSTER and 2 * cluster * segments <= slots and steps >= 12 * cluster + (8 if 2 * cluster * segments > sm_count else 0):
         cluster *= 2
     if steps >= max(100, 50 * cluster) and segments < 2 * slots and segments * (steps + 2) < 2**30:
-        return 1, slots
+        return 1, 2 * sm_count if segments * steps < 20 * slots else slots
     return cluster, 0
 
 
