@@ -36,6 +36,11 @@ constexpr int K4_STEP = 32;      // tokens a warp takes at a time: twice the 16 
 constexpr int K4_CLUSTER = 8;    // CTAs of a cluster at most
 constexpr int K4_FOLD = 16;      // steps between two corrections of the sums
 constexpr float K4_SLACK = 8.f;  // how far (in powers of two) a score may pass the running maximum before the sums are rescaled: weights stay below 2^8
+// Weights are held 2^lift times as large, so that their products with the largest of the values' scales seen so far start near 2^88. Above, 28 powers of two are left until the
+// next change of the lift, and K4_SLACK: products stay below 2^125, of bf16's 2^128. Below, a product of 2^-9 is the least whose eight bits all count in 32 bits (a code's unit
+// is 2^-133, the least number 2^-149): weight times scale may be 2^-97 of the largest scale, and by the lift's end of 92 2^-101 (no scale is below 2^-103). That end is there for
+// the denominator: lifted weights of 2^27 tokens have a sum.
+constexpr int K4_LIFT = 88, K4_ROOM = 28, K4_MOST = 92;
 
 struct K4Params {
   const __nv_bfloat16* q;
@@ -381,8 +386,7 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D == 64 ? 4 : D == 128 ? 3 : 2)
   __syncthreads();
 
   float o[2 * G][4], z[G / 2][4], top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
-  // Weights are held 2^lift times as large, so that their products with the values' scales lie near 2^40 and keep clear of the ends of 32 bits (times 2^-133) and of
-  // bf16. limit: the largest scale, in bf16 bits in both halves, for which that holds.
+  // limit: the largest scale, in bf16 bits in both halves, that the lift is good for.
   float lift = 0.f, ref[2] = {0.f, 0.f};      // ref: what is added to a score's power of two
   uint32_t limit = 0u;
 #pragma unroll
@@ -461,7 +465,7 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D == 64 ? 4 : D == 128 ? 3 : 2)
 #pragma unroll
       for (int g = 0; g < G / 2; ++g) widest = __vmaxu2(widest, __vmaxu2(va[h][g], vb[h][g]));
     if (__any_sync(0xffffffffu, m0 > top[0] + slack[0] || m1 > top[1] + slack[1] || widest != limit)) {
-      float f[2] = {1.f, 1.f};
+      float f[2] = {1.f, 1.f}, rise = 1.f;
       uint32_t most = 0u, lost = 0u;      // the largest scale; groups with one that is not finite, which are NaN from here on (and count as zeros, for z's sake)
 #pragma unroll
       for (int h = 0; h < NS; ++h)
@@ -489,10 +493,10 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D == 64 ? 4 : D == 128 ? 3 : 2)
       }
       if (most > (limit & 0xffffu)) {
         const int e = static_cast<int>(most >> 7) - 127;
-        const float to = static_cast<float>(max(-100, min(96, 40 - e)));
-        f[0] = f[1] = exp2_fast(to - lift);
-        lift = to;
-        limit = static_cast<uint32_t>(min(254, max(1, e + 40 + 127))) << 7;
+        const int to = min(K4_MOST, K4_LIFT - e);      // -39 to 92
+        rise = times_pow2(1.f, to - static_cast<int>(lift));      // 2^-131 at least, exactly: no token leaves the denominator when far larger values come
+        lift = static_cast<float>(to);
+        limit = static_cast<uint32_t>(min(254, max(1, e + K4_ROOM + 127))) << 7;
         limit |= limit << 16;
       }
 #pragma unroll
@@ -502,11 +506,12 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D == 64 ? 4 : D == 128 ? 3 : 2)
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
         if (m > top[h]) {
-          f[h] *= exp2_fast((top[h] - m) * c[h]);      // (0 for the first)
+          f[h] = exp2_fast((top[h] - m) * c[h]);      // (0 for the first)
           top[h] = m;
         }
         ref[h] = top[h] == -INFINITY ? 0.f : fmaf(-top[h], c[h], lift);
-        sum[h] *= f[h];
+        sum[h] = sum[h] * f[h] * rise;
+        f[h] *= rise;
 #pragma unroll
         for (int j = 0; j < 2 * G; ++j) {
           o[j][h] *= f[h];
@@ -556,7 +561,9 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D == 64 ? 4 : D == 128 ? 3 : 2)
   fold<G>(o, z);
 
   // The warps' parts (and, where four heads have two columns each, the columns') are brought to one reference and added: columns 2 t and 2 t + 1, dimensions
-  // 32 g + 4 r .. + 3 of each lane.
+  // 32 g + 4 r .. + 3 of each lane. Tops are less the lift here, and lifts differ by up to 131. So a factor between parts, which 32 bits may
+  // not hold, is applied as its root, twice: a part of tiny values keeps its share of the denominator beside one of huge values. Sums leave in 2^64 of the lifted values' unit, in
+  // which alone they could pass the end of 32 bits.
   constexpr int PARTS = PAIR ? 2 * K4_WARPS : K4_WARPS;
   auto part_of = [&](int head, int i) -> float2 { return PAIR ? ml[i >> 1][head + 4 * (i & 1)] : ml[i][head]; };
 #pragma unroll
@@ -577,11 +584,11 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D == 64 ? 4 : D == 128 ? 3 : 2)
 #pragma unroll
     for (int i = 1; i < PARTS; ++i) m = fmaxf(m, part_of(head, i).x);
     // (a part without a finite score has no tokens, or NaN, which is to stay)
-    const float f = top[h] == -INFINITY ? 1.f : exp2_fast(top[h] - m), f0 = f * 0x1p67f, f1 = f * 0x1p63f;
+    const float root = top[h] == -INFINITY ? 1.f : exp2_fast(0.5f * (top[h] - m)), f = root * 0x1p34f, f0 = root * 0x1p35f, f1 = root * 0x1p31f;
 #pragma unroll
     for (int g = 0; g < G; ++g)
       *reinterpret_cast<float4*>(red + (warp * 8 + column) * ROW + 32 * g + 4 * r) =
-          make_float4(o[2 * g][h] * 0x1p66f * f0, o[2 * g][h + 2] * 0x1p66f * f1, o[2 * g + 1][h] * 0x1p66f * f0, o[2 * g + 1][h + 2] * 0x1p66f * f1);
+          make_float4(o[2 * g][h] * f * f0, o[2 * g][h + 2] * f * f1, o[2 * g + 1][h] * f * f0, o[2 * g + 1][h + 2] * f * f1);
   }
   __syncthreads();
   float* joined = red + K4_WARPS * 8 * ROW;
@@ -594,7 +601,8 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D == 64 ? 4 : D == 128 ? 3 : 2)
 #pragma unroll
     for (int w = 0; w < PARTS; ++w) {
       const float2 part = part_of(head, w);
-      l += part.y * (part.x == -INFINITY ? 1.f : exp2_fast(part.x - m));
+      const float root = part.x == -INFINITY ? 1.f : exp2_fast(0.5f * (part.x - m));
+      l += part.y * root * root;
       const float4 v = *reinterpret_cast<const float4*>(red + (PAIR ? (w >> 1) * 8 + head + 4 * (w & 1) : w * 8 + head) * ROW + d);
       acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
     }
@@ -602,7 +610,7 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D == 64 ? 4 : D == 128 ? 3 : 2)
       *reinterpret_cast<float4*>(joined + head * D + d) = acc;
       if (d == 0) joined_ml[head] = make_float2(m, l);
     } else if (count == span.steps) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = l == 0.f ? 0.f : 0x1p64f / l;
       *reinterpret_cast<uint2*>(p.out + static_cast<long long>(b) * p.out_stride + static_cast<long long>(head0 + head) * D + d) =
           make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
     } else {      // a part: of a sequence that began in an earlier CTA, or of one that begins here
@@ -628,16 +636,16 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D == 64 ? 4 : D == 128 ? 3 : 2)
 #pragma unroll
       for (int c = 0; c < K4_CLUSTER; ++c)
         if (c < p.cluster) {
-          const float f = parts[c].x == -INFINITY ? 1.f : exp2_fast(parts[c].x - m);
+          const float root = parts[c].x == -INFINITY ? 1.f : exp2_fast(0.5f * (parts[c].x - m));
           const uint32_t from = mapa_shared(sums_at + (head * D + d) * 4, c);
           const float2 u = ld_cluster2(from), v = ld_cluster2(from + 8);
-          l = fmaf(parts[c].y, f, l);
-          acc.x = fmaf(u.x, f, acc.x);
-          acc.y = fmaf(u.y, f, acc.y);
-          acc.z = fmaf(v.x, f, acc.z);
-          acc.w = fmaf(v.y, f, acc.w);
+          l = fmaf(parts[c].y * root, root, l);
+          acc.x = fmaf(u.x * root, root, acc.x);
+          acc.y = fmaf(u.y * root, root, acc.y);
+          acc.z = fmaf(v.x * root, root, acc.z);
+          acc.w = fmaf(v.y * root, root, acc.w);
         }
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = l == 0.f ? 0.f : 0x1p64f / l;
       *reinterpret_cast<uint2*>(p.out + static_cast<long long>(b) * p.out_stride + static_cast<long long>(head0 + head) * D + d) =
           make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
     }
@@ -693,16 +701,16 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const K4Params p) {
   for (int i = FEW ? warp : 0; i < n; i += BY) {
     const long long from = part(i);
     const float2 w = p.part_ml[from];
-    const float f = w.x == -INFINITY ? 1.f : exp2_fast(w.x - m);      // (a part without a finite score has no tokens, or NaN)
-    l += w.y * f;
+    const float root = w.x == -INFINITY ? 1.f : exp2_fast(0.5f * (w.x - m));      // (a part without a finite score has no tokens, or NaN)
+    l += w.y * root * root;
 #pragma unroll
     for (int v = 0; v < V; ++v)
       if (lane + 32 * v < D / 4) {
         const float4 o = reinterpret_cast<const float4*>(p.part_o + from * D)[lane + 32 * v];
-        acc[v].x = fmaf(o.x, f, acc[v].x);
-        acc[v].y = fmaf(o.y, f, acc[v].y);
-        acc[v].z = fmaf(o.z, f, acc[v].z);
-        acc[v].w = fmaf(o.w, f, acc[v].w);
+        acc[v].x = fmaf(o.x * root, root, acc[v].x);
+        acc[v].y = fmaf(o.y * root, root, acc[v].y);
+        acc[v].z = fmaf(o.z * root, root, acc[v].z);
+        acc[v].w = fmaf(o.w * root, root, acc[v].w);
       }
   }
   if constexpr (FEW) {
@@ -716,7 +724,7 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const K4Params p) {
 #pragma unroll
     for (int q = 0; q < 8; ++q) l += reds[q];
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = l == 0.f ? 0.f : 0x1p64f / l;
   __nv_bfloat16* out = p.out + job.z * p.out_stride + static_cast<long long>(kvh * p.G + chunk * 8 + head) * D;
 #pragma unroll
   for (int v = 0; v < V; ++v) {

@@ -267,7 +267,10 @@ def kv4_paged_decode(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
     ``seq_lens`` [B] int32 tokens in the pages that ``block_table`` [B, pages] int32 names, of which ``window`` > 0 leaves the last ``window``. A
     sequence without tokens gives zeros. ``plan``: (cluster, num_ctas): a cluster of up to eight CTAs per sequence and key/value head, or with (1, n) n CTAs
     that share all tokens evenly (None: :func:`kv4_plan` for the table's width); ``scratch``: float32 tensor of :func:`kv4_scratch_size` elements, for callers that
-    keep their own (one call at a time). Returns [B, Hq D]."""
+    keep their own (one call at a time). Returns [B, Hq D].
+
+    Scores and sums are in 32 bits, a weight times a value's scale is rounded to bf16. A token's share of a group of 32 dimensions keeps these eight bits where weight times
+    scale (weights: 1 for the largest) is at least 2^-100 and 2^-80 of the head's largest scale in that sequence."""
     block = block_size_of(cache, Hkv, D)
     device, width = q.device, Hq * D
     if Hq < 1 or Hq % Hkv or q.dim() != 2 or q.shape[1] < width:

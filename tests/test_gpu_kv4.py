@@ -222,6 +222,48 @@ def test_decode_of_scores_from_far_apart_factors(native_lib, q_by, big, scale):
             _check(got, q, cache, table, n, Hq, 2, 64, scale=1e-300 if scale == 0 else scale)
 
 
+def _with_value_scales(cache, table, lens, D, power):
+    """The cache with the values' scales of each sequence's token t times 2^power(t) ([tokens] or [tokens, groups])."""
+    kc, vc, ks, vs = K._unpack_pages(cache, D)
+    block, s = kc.shape[2], vs.double()
+    for b, n in enumerate(lens):
+        t = torch.arange(n, device="cuda")
+        s[table[b, t // block].long(), :, t % block] *= 2.0 ** power(t).double().reshape(n, 1, -1)
+    assert (s.abs() < 2.0 ** 124).all() and (s[s > 0] > 2.0 ** -100).all()
+    return K._pack_pages(kc, vc, ks, s.to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("low,high", [(-60, 75), (-94, 118), (0, 100)])
+@pytest.mark.parametrize("D,Hq", [(64, 4), (64, 10), (128, 4), (128, 10), (256, 2), (256, 16)])
+def test_decode_of_values_from_far_apart_scales(native_lib, D, Hq, low, high):
+    """Tokens of tiny values keep their weight beside tokens of huge ones: within a warp, between warps, clusters' CTAs and shared parts. Queries of zeros
+    give every token the same weight, so that each that is left out of the denominator shows."""
+    lens = [700, 33, 300]
+    q, cache, table, n = _decode_case(lens, Hq, 2, D, 16, seed=11)
+    orders = [lambda t, cut=cut: t >= cut for cut in (16, 32, 128, 350)]
+    orders += [lambda t: t < 350, lambda t: t // 32 % 2 == 1, lambda t: t == 290]
+    for order in orders:
+        c = _with_value_scales(cache, table, lens, D, lambda t: torch.where(order(t), high, low))
+        for x in (q, torch.zeros_like(q)):
+            for plan in ((1, 0), (4, 0), (1, 7), (1, 1)):
+                _check(K.kv4_paged_decode(x, c, table, n, Hq, 2, D, plan=plan), x, c, table, n, Hq, 2, D)
+    assert L.check_status() == 0
+
+
+@pytest.mark.parametrize("D,Hq", [(64, 4), (64, 10), (128, 4), (128, 10), (256, 2), (256, 16)])
+def test_decode_of_groups_far_below_the_largest(native_lib, D, Hq):
+    """A group of dimensions whose scales lie 2^-80 times the head's largest and above keeps its bits; sequences of one token to some steps a warp, also of tiny values."""
+    lens, G = [700, 33, 1, 300], D // 32
+    q, cache, table, n = _decode_case(lens, Hq, 2, D, 16, seed=12)
+    for powers in ([0, -79], [-40, 0], [118, 40], [-15, -94], [-94, -90], [0, -60, -79, -20]):
+        power = torch.tensor((powers * G)[:G], device="cuda")
+        c = _with_value_scales(cache, table, lens, D, lambda t: power.expand(len(t), G))
+        for x in (q, torch.zeros_like(q)):
+            for plan in ((1, 0), (4, 0), (1, 7)):
+                _check(K.kv4_paged_decode(x, c, table, n, Hq, 2, D, plan=plan), x, c, table, n, Hq, 2, D)
+    assert L.check_status() == 0
+
+
 @pytest.mark.parametrize("Hq", [4, 16])
 def test_a_query_that_is_not_finite_spoils_its_head_alone(native_lib, Hq):
     q, cache, table, n = _decode_case([50, 300], Hq, 2, 128, 16, seed=2)
