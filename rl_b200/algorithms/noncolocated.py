@@ -193,7 +193,7 @@ def _numel(shape) -> int:
 def build_generation_rank(cfg: dict, tokenizer, model_cfg=None, device=None):
     """The model and engine of a generation rank: the policy's architecture with uninitialised weights (the trainer's
     first broadcast fills them) behind the ordinary generation facade."""
-    from rl_b200.engine.generation import NativeGeneration
+    from rl_b200.engine.generation import NativeGeneration, kv_cache_dtype_of
     from rl_b200.models.config import ModelConfig, preset
     from rl_b200.models.transformer import build_model
 
@@ -213,6 +213,7 @@ def build_generation_rank(cfg: dict, tokenizer, model_cfg=None, device=None):
     for k in ("gpu_memory_utilization", "max_model_len", "block_size", "kv_cache_tokens", "max_running", "use_cuda_graphs", "decode_window"):
         if k in native_cfg:
             merged[k] = native_cfg[k]
+    merged["kv_cache_dtype"] = kv_cache_dtype_of(g)
     merged.setdefault("max_model_len", pcfg["max_total_sequence_length"])
     return NativeGeneration(model, merged, tokenizer)
 

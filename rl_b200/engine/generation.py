@@ -52,6 +52,13 @@ def configure_generation_config(cfg: Optional[dict], tokenizer=None, is_eval: bo
     return out
 
 
+def kv_cache_dtype_of(cfg: dict) -> str:
+    """What a generation section asks to hold keys and values in, its ``native_cfg`` and ``vllm_cfg`` before the section itself; the reference's names for types that have no
+    cache here (fp8 and its forms) serve the model's type."""
+    name = str((cfg.get("native_cfg") or {}).get("kv_cache_dtype") or (cfg.get("vllm_cfg") or {}).get("kv_cache_dtype") or cfg.get("kv_cache_dtype") or "auto")
+    return "auto" if name.startswith(("fp8", "bfloat16", "float16")) else name
+
+
 def verify_right_padding(data: BatchedDataDict, pad_value: int = 0) -> tuple[bool, str]:
     """Checks that every row of ``input_ids`` holds its tokens first and padding last."""
     ids = data["input_ids"]
@@ -86,15 +93,9 @@ class NativeGeneration:
             model, block_size=c["block_size"], kv_cache_tokens=c["kv_cache_tokens"],
             gpu_memory_utilization=c["gpu_memory_utilization"], max_running=c["max_running"],
             max_prefill_tokens=c["max_prefill_tokens"], max_model_len=c["max_model_len"] or 8192,
-            use_cuda_graphs=c["use_cuda_graphs"], tokenizer=tokenizer, kv_cache_dtype=self._kv_cache_dtype(),
+            use_cuda_graphs=c["use_cuda_graphs"], tokenizer=tokenizer, kv_cache_dtype=kv_cache_dtype_of(c),
             quantization=(c.get("native_cfg") or {}).get("precision") or (c.get("vllm_cfg") or {}).get("precision") or c.get("precision"))
         self._calls = 0
-
-    def _kv_cache_dtype(self) -> str:
-        """What the configuration asks for; the reference's names for types that have no cache here (fp8 and its forms) serve the model's type."""
-        c = self.cfg
-        name = str((c.get("native_cfg") or {}).get("kv_cache_dtype") or (c.get("vllm_cfg") or {}).get("kv_cache_dtype") or c.get("kv_cache_dtype") or "auto")
-        return "auto" if name.startswith(("fp8", "bfloat16", "float16")) else name
 
     # lifecycle hooks of the generation contract
     def prepare_for_generation(self, *args, **kw) -> bool:

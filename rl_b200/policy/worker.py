@@ -542,15 +542,16 @@ class PolicyWorker:
     # ------------------------------------------------------------------ generation (colocated, shared weights)
     def build_generation(self, gen_cfg: Optional[dict] = None):
         """Creates the colocated generation engine over this worker's own weight buffers."""
-        from rl_b200.engine.generation import NativeGeneration
+        from rl_b200.engine.generation import NativeGeneration, kv_cache_dtype_of
 
         g = dict(self.cfg.get("generation") or {})
         g.update(gen_cfg or {})
         native_cfg = dict(g.get("native_cfg") or g.get("vllm_cfg") or {})
         merged = {k: v for k, v in g.items() if k not in ("native_cfg", "vllm_cfg", "colocated", "sglang_cfg")}
-        for k in ("gpu_memory_utilization", "max_model_len", "block_size", "kv_cache_tokens", "max_running", "use_cuda_graphs", "kv_cache_dtype"):
+        for k in ("gpu_memory_utilization", "max_model_len", "block_size", "kv_cache_tokens", "max_running", "use_cuda_graphs"):
             if k in native_cfg:
                 merged[k] = native_cfg[k]
+        merged["kv_cache_dtype"] = kv_cache_dtype_of(g)
         if native_cfg.get("enforce_eager"):
             merged["use_cuda_graphs"] = False
         merged.setdefault("max_model_len", self.cfg["max_total_sequence_length"])

@@ -270,3 +270,20 @@ def test_engine_memory_and_refusals():
     for bad in (dict(kv_cache_dtype="int8"), dict(vllm_cfg=dict(kv_cache_dtype="int"))):
         with pytest.raises(ValueError):
             NativeGeneration(model, {**cfg, **bad})
+
+
+def _generation_rank(generation):
+    from rl_b200.algorithms.noncolocated import build_generation_rank
+    from rl_b200.models.config import ModelConfig
+
+    mc = ModelConfig(vocab_size=97, hidden_size=64, intermediate_size=96, num_hidden_layers=1, num_attention_heads=2, num_key_value_heads=1, head_dim=64, torch_dtype="float32")
+    g = dict(block_size=16, kv_cache_tokens=64, max_running=2, use_cuda_graphs=False, **generation)
+    return build_generation_rank(dict(policy=dict(precision="float32", max_total_sequence_length=64, generation=g)), None, mc, torch.device("cpu")).engine
+
+
+@pytest.mark.parametrize("section", [None, "vllm_cfg", "native_cfg"])
+def test_generation_ranks_read_every_section(section):
+    """A rank of its own for generation holds its cache as the section, ``vllm_cfg`` or ``native_cfg`` says."""
+    for name in ("int4", "auto"):
+        asked = dict(kv_cache_dtype=name)
+        assert _generation_rank({section: asked} if section else asked).kv4 == (name == "int4")
