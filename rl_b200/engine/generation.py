@@ -53,9 +53,10 @@ def configure_generation_config(cfg: Optional[dict], tokenizer=None, is_eval: bo
 
 
 def kv_cache_dtype_of(cfg: dict) -> str:
-    """What a generation section asks to hold keys and values in, its ``native_cfg`` and ``vllm_cfg`` before the section itself; the reference's names for types that have no
-    cache here (fp8 and its forms) serve the model's type."""
-    name = str((cfg.get("native_cfg") or {}).get("kv_cache_dtype") or (cfg.get("vllm_cfg") or {}).get("kv_cache_dtype") or cfg.get("kv_cache_dtype") or "auto")
+    """What a generation section asks to hold keys and values in: the first of its ``native_cfg``, its ``vllm_cfg`` and the section itself that names a type (``auto``, the
+    reference's default, names none); the reference's names for types that have no cache here (fp8 and its forms) serve the model's type."""
+    names = (str((section or {}).get("kv_cache_dtype") or "auto") for section in (cfg.get("native_cfg"), cfg.get("vllm_cfg"), cfg))
+    name = next((n for n in names if n != "auto"), "auto")
     return "auto" if name.startswith(("fp8", "bfloat16", "float16")) else name
 
 

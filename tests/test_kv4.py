@@ -287,3 +287,21 @@ def test_generation_ranks_read_every_section(section):
     for name in ("int4", "auto"):
         asked = dict(kv_cache_dtype=name)
         assert _generation_rank({section: asked} if section else asked).kv4 == (name == "int4")
+
+
+@pytest.mark.parametrize("section", ["vllm_cfg", "native_cfg"])
+@pytest.mark.parametrize("unset", ["auto", None])
+def test_auto_in_a_subsection_asks_for_nothing(section, unset):
+    """``auto`` there, the reference's default, leaves the choice to the section itself."""
+    from rl_b200.engine.generation import NativeGeneration
+    from rl_b200.policy.worker import PolicyWorker
+
+    asked = {"kv_cache_dtype": "int4", section: dict(kv_cache_dtype=unset)}
+    assert _generation_rank(asked).kv4
+    cfg = dict(block_size=16, kv_cache_tokens=256, max_running=4, max_model_len=64, use_cuda_graphs=False, **asked)
+    assert NativeGeneration(_model(), cfg).engine.kv4
+    both = dict(native_cfg=dict(kv_cache_dtype="auto"), vllm_cfg=dict(kv_cache_dtype="int4"))
+    assert _generation_rank(both).kv4
+    p = PolicyWorker(dict(precision="float32", train_global_batch_size=2, train_micro_batch_size=2, max_total_sequence_length=64,
+                          optimizer=dict(name="torch.optim.AdamW", kwargs=dict(lr=1e-4)), generation=cfg), model_cfg=_model().cfg, device="cpu", init_reference_model=False, seed=3)
+    assert p.build_generation().engine.kv4
