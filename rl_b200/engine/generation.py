@@ -52,12 +52,16 @@ def configure_generation_config(cfg: Optional[dict], tokenizer=None, is_eval: bo
     return out
 
 
+MODEL_TYPES = ("bfloat16", "bf16", "float16", "fp16", "half", "float32", "fp32", "float")
+
+
 def kv_cache_dtype_of(cfg: dict) -> str:
     """What a generation section asks to hold keys and values in: the first of its ``native_cfg``, its ``vllm_cfg`` and the section itself that names a type (``auto``, the
-    reference's default, names none); the reference's names for types that have no cache here (fp8 and its forms) serve the model's type."""
+    reference's default, names none); names of types that have no cache here (fp8 and its forms, 16 and 32
+    bits) serve the model's type."""
     names = (str((section or {}).get("kv_cache_dtype") or "auto") for section in (cfg.get("native_cfg"), cfg.get("vllm_cfg"), cfg))
     name = next((n for n in names if n != "auto"), "auto")
-    return "auto" if name.startswith(("fp8", "bfloat16", "float16")) else name
+    return "auto" if name in MODEL_TYPES or name.startswith("fp8") else name
 
 
 def verify_right_padding(data: BatchedDataDict, pad_value: int = 0) -> tuple[bool, str]:

@@ -305,3 +305,17 @@ def test_auto_in_a_subsection_asks_for_nothing(section, unset):
     p = PolicyWorker(dict(precision="float32", train_global_batch_size=2, train_micro_batch_size=2, max_total_sequence_length=64,
                           optimizer=dict(name="torch.optim.AdamW", kwargs=dict(lr=1e-4)), generation=cfg), model_cfg=_model().cfg, device="cpu", init_reference_model=False, seed=3)
     assert p.build_generation().engine.kv4
+
+
+@pytest.mark.parametrize("name", ["auto", "bfloat16", "bf16", "float16", "fp16", "half", "float32", "fp32", "float", "fp8", "fp8_e4m3", "fp8_e5m2"])
+def test_names_of_the_models_type(name):
+    """Every name of a type without a 4-bit cache serves the model's type, as before there was one; a name that nobody knows is refused."""
+    from rl_b200.engine.generation import kv_cache_dtype_of
+
+    for section in (None, "vllm_cfg", "native_cfg"):
+        asked = dict(kv_cache_dtype=name)
+        assert not _generation_rank({section: asked} if section else asked).kv4
+    for unknown in ("int8", "bfloat", "bf16x", "INT4 "):
+        assert kv_cache_dtype_of(dict(kv_cache_dtype=unknown)) == unknown
+        with pytest.raises(ValueError):
+            _generation_rank(dict(kv_cache_dtype=unknown))
