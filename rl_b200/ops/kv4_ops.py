@@ -88,8 +88,19 @@ def _aligned(t: torch.Tensor) -> bool:
 
 
 def _apart(t: torch.Tensor, width: int) -> bool:
-    """Whether the rows that are written do not overlap (copying to rows that do is refused by PyTorch)."""
-    return t.shape[0] < 2 or t.stride(0) >= width
+    """Whether rows that lie one after the other are written, none of which reaches into the next."""
+    stride = t.stride()
+    return stride[1] == 1 and (t.shape[0] < 2 or stride[0] >= width)
+
+
+def _refuse_overlap(t: torch.Tensor, width: int) -> None:
+    """Refuses rows that are written where two numbers have one place: numbers (i, j) and (k, l) with (i - k) a = (l - j) b for the strides a and b, first at b / g rows and a / g
+    columns with g the greatest common divisor."""
+    a, b = t.stride()
+    n = t.shape[0]
+    g = math.gcd(a, b)
+    if (n > b // g and width > a // g) if a and b else (n > 1 and not a) or (width > 1 and not b):
+        raise RuntimeError(f"rows {n} x {width} with strides ({a}, {b}) share places: nothing is written to rows that overlap")
 
 
 def _no_gradient(t: torch.Tensor) -> None:
@@ -183,7 +194,10 @@ def rope_kv4_cache_write(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: t
     if torch.cuda.current_device() != index:      # kernels go to the current stream of the tensors' device, whichever device is current
         with torch.cuda.device(qkv.device):
             return rope_kv4_cache_write(qkv, positions, inv_freq, slots, cache, Hq, Hkv, D)
-    rows = qkv if _aligned(qkv) and _apart(qkv, qkv.shape[1]) else qkv.clone(memory_format=torch.contiguous_format)      # (rows that do not start on 16 bytes: turned in a copy)
+    rows = qkv
+    if not (_aligned(qkv) and _apart(qkv, qkv.shape[1])):      # rows that do not start on 16 bytes: turned in a copy
+        _refuse_overlap(qkv, qkv.shape[1])
+        rows = qkv.clone(memory_format=torch.contiguous_format)
     inv_freq = inv_freq.contiguous()
     call("rlb_rope_kv4_cache_write", rows.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), slots.data_ptr(), cache.data_ptr(), T, Hq, Hkv, D, block,
          rows.stride(0), cache.shape[0], _L.status_word(qkv.device).data_ptr(), _raw_stream(index))
@@ -211,6 +225,8 @@ def kv4_cache_read(cache: torch.Tensor, slots: torch.Tensor, Hkv: int, D: int, *
         raise ValueError(f"out {tuple(out.shape)} has no room for {n} rows of {width}")
     else:
         _same_device(device, out)
+        if not _apart(out, width):
+            _refuse_overlap(out, width)
     if not use_native(cache):
         kc, vc, ks, vs = _unpack_pages(cache[(slots // block).clamp(min=0)], D)      # [n, Hkv, block, ...]
         ar, off = torch.arange(n, device=device), slots.clamp(min=0) % block
@@ -295,6 +311,8 @@ def kv4_paged_decode(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
         raise ValueError(f"out is {q.dtype} [{B}, {width}], not {out.dtype} {tuple(out.shape)}")
     else:
         _same_device(device, out)
+        if not _apart(out, width):
+            _refuse_overlap(out, width)
     if not use_native(q):
         for b in range(B):
             n = int(seq_lens[b])

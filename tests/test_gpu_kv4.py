@@ -104,6 +104,37 @@ def test_write_and_read_of_odd_views(native_lib):
     assert L.check_status() == 0
 
 
+def test_rows_that_overlap_are_refused_before_anything_is_written(native_lib):
+    """Rows that share places by any strides; the cache and the rows stay as they were. Views whose rows interleave without sharing a place are served."""
+    T, Hq, Hkv, D, block = 4, 2, 1, 64, 16
+    W, Wkv = 4 * D, 2 * D
+    pos, freq, slots = torch.arange(T).cuda(), _freq(D).cuda(), torch.arange(T).cuda()
+    held = torch.randint(0, 255, (2, Hkv, K.kv4_page_bytes(block, D)), dtype=torch.uint8).cuda()
+    held[..., block * D :].view(torch.bfloat16).fill_(0.5)
+    mem = _rows(1, Hq, Hkv, 16 * D).cuda().flatten()
+    q, table, n = _rows(T, Hq, Hkv, D).cuda(), torch.zeros((T, 1), dtype=torch.int32, device="cuda"), torch.full((T,), 9, dtype=torch.int32, device="cuda")
+    for strides in ((0, 1), (8, 1), (1, 1), (W - 8, 1), (W, 2), (3, 2), (W, 0)):
+        cache, was = held.clone(), mem.clone()
+        with pytest.raises(RuntimeError):
+            K.rope_kv4_cache_write(mem.as_strided((T, W), strides), pos, freq, slots, cache, Hq, Hkv, D)
+        assert torch.equal(cache, held) and torch.equal(mem, was)
+    for strides in ((0, 1), (8, 1), (Wkv - 4, 1), (Wkv, 2), (Wkv, 0)):
+        for call in (lambda out: K.kv4_cache_read(held, slots, Hkv, D, out=out), lambda out: K.kv4_paged_decode(q, held, table, n, Hq, Hkv, D, out=out)):
+            was = mem.clone()
+            with pytest.raises(RuntimeError):
+                call(mem.as_strided((T, Wkv), strides))
+            assert torch.equal(mem, was)
+    ref = K.kv4_cache(2, Hkv, block, D, "cuda")
+    want = K.rope_kv4_cache_write(q.clone(), pos, freq, slots, ref, Hq, Hkv, D)
+    for strides in ((1, T), (3 * W - 1, 3), (1, 2 * T + 1)):
+        view, cache = torch.zeros(4 * T * W, dtype=torch.bfloat16, device="cuda").as_strided((T, W), strides), torch.zeros_like(ref)
+        view.copy_(q)
+        assert K.rope_kv4_cache_write(view, pos, freq, slots, cache, Hq, Hkv, D) is view and torch.equal(view, want) and torch.equal(cache, ref)
+    one = mem.as_strided((1, W), (0, 1))      # one row overlaps with none
+    assert K.rope_kv4_cache_write(one, pos[:1], freq, slots[:1], cache, Hq, Hkv, D) is one
+    assert L.check_status() == 0
+
+
 def test_bad_slots_are_reported_and_skipped(native_lib):
     T, Hq, Hkv, D, block = 3, 2, 1, 128, 16
     rows, slots = _rows(T, Hq, Hkv, D), torch.tensor([32, 5, 10**12])

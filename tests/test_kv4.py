@@ -319,3 +319,15 @@ def test_names_of_the_models_type(name):
         assert kv_cache_dtype_of(dict(kv_cache_dtype=unknown)) == unknown
         with pytest.raises(ValueError):
             _generation_rank(dict(kv_cache_dtype=unknown))
+
+
+def test_outputs_whose_rows_overlap_are_refused():
+    T, Hq, Hkv, D, block = 4, 2, 1, 64, 16
+    cache, slots, mem = K.kv4_cache(2, Hkv, block, D, "cpu"), torch.arange(T), torch.zeros(4 * T * 2 * D)
+    q, table, n = _rows(T, Hq, Hkv, D).float(), torch.zeros((T, 1), dtype=torch.int32), torch.full((T,), 9, dtype=torch.int32)
+    for strides in ((0, 1), (8, 1), (2 * D - 4, 1), (2 * D, 2), (2 * D, 0)):
+        for call in (lambda out: K.kv4_cache_read(cache, slots, Hkv, D, out=out), lambda out: K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, out=out)):
+            with pytest.raises(RuntimeError):
+                call(mem.as_strided((T, 2 * D), strides))
+    for strides in ((1, T), (2 * D, 1), (6 * D - 1, 3)):
+        assert K.kv4_cache_read(cache, slots, Hkv, D, out=mem.as_strided((T, 2 * D), strides)).shape == (T, 2 * D)
