@@ -275,7 +275,8 @@ __global__ void __launch_bounds__(K4_WARPS * 32, D == 64 ? 4 : D == 128 ? 3 : 2)
     b = found[0];
     at = found[1];
   } else {
-    b = blockIdx.y;
+    b = blockIdx.z * gridDim.y + blockIdx.y;
+    if (static_cast<uint32_t>(b) >= static_cast<uint32_t>(p.B)) return;      // (with the whole cluster)
     hc = blockIdx.x / p.cluster;
     at = 0;
   }
@@ -760,7 +761,8 @@ int launch_decode(const K4Params& p, cudaStream_t stream) {
   }
   const int all_heads = p.Hkv * p.chunks;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = p.num_ctas ? dim3(p.num_ctas) : dim3(all_heads * p.cluster, p.B);
+  constexpr int MOST = 65535;      // of a grid in its second and third direction
+  cfg.gridDim = p.num_ctas ? dim3(p.num_ctas) : dim3(all_heads * p.cluster, p.B < MOST ? p.B : MOST, (p.B - 1) / MOST + 1);
   cfg.blockDim = dim3(K4_WARPS * 32);
   cfg.dynamicSmemBytes = k4_smem<D>();
   cfg.stream = stream;
@@ -816,7 +818,7 @@ RLB_API int rlb_kv4_paged_decode(const void* q, long long q_stride, const void* 
   const int group = Hq / Hkv, chunks = (group + 7) / 8;
   if (cluster < 1 || cluster > K4_CLUSTER || (num_ctas && cluster != 1)) return -3;
   if (num_ctas < 0 || (num_ctas && (!part_o || !part_ml || ((reinterpret_cast<uintptr_t>(part_o) | reinterpret_cast<uintptr_t>(part_ml)) & 15)))) return -3;
-  if (static_cast<long long>(max_blocks) * block_size > 0x7fff0000ll || (!num_ctas && B > 65535) ||
+  if (static_cast<long long>(max_blocks) * block_size > 0x7fff0000ll ||
       (num_ctas && static_cast<long long>(B) * Hkv * chunks * (static_cast<long long>(max_blocks) * block_size / K4_STEP + 2) + num_ctas > 0x7fffffffll) || static_cast<long long>(B) * Hkv * chunks > 0x7fffffffll || static_cast<long long>(Hkv) * chunks * cluster > 0x7fffffffll ||
       num_blocks * Hkv > 0x7fffffffll)
     return -4;

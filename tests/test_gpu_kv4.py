@@ -395,6 +395,28 @@ def test_bad_pages_and_lengths_are_reported(native_lib):
         _check(got[:1], q, cache, table, n, Hq, Hkv, D)
 
 
+@pytest.mark.parametrize("plan", [None, (1, 0), (2, 0), (1, 444)])
+def test_decode_of_more_rows_than_a_grid_has_in_one_direction(native_lib, plan):
+    """70001 sequences: the rows of the same call in two halves."""
+    B, Hq, Hkv, D, block = 70001, 2, 1, 64, 16
+    cache = _pool(40, Hkv, D, block, 4)
+    g = torch.Generator().manual_seed(1)
+    n = torch.randint(0, 100, (B,), generator=g).int().cuda()
+    table = torch.randint(0, 40, (B, 7), generator=g).int().cuda()
+    q = torch.randn(B, Hq * D, generator=g).bfloat16().cuda()
+    got = K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, plan=plan)
+    half = B // 2
+    want = torch.cat([K.kv4_paged_decode(q[r], cache, table[r], n[r], Hq, Hkv, D, plan=plan or (1, 0)) for r in (slice(0, half), slice(half, B))])
+    if plan and plan[1]:      # other shares, so other parts: on both sides half a step of the result and half a step of each token's share, neither above the largest value
+        for r in (slice(0, 50), slice(B - 50, B)):
+            _check(got[r], q[r], cache, table[r], n[r], Hq, Hkv, D)
+        largest = K._unpack_pages(cache, D)[3].float().max() * 7.5
+        assert ((got.float() - want.float()).abs() <= 4.1 * 2.0 ** -8 * largest).all()
+    else:
+        assert torch.equal(got, want)
+    assert L.check_status() == 0
+
+
 def test_places_beyond_32_bits(native_lib):
     """A cache of more than 4 GiB: pages at its far end."""
     Hq, Hkv, D, block = 8, 8, 128, 128
