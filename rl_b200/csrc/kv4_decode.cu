@@ -818,9 +818,9 @@ RLB_API int rlb_kv4_paged_decode(const void* q, long long q_stride, const void* 
   const int group = Hq / Hkv, chunks = (group + 7) / 8;
   if (cluster < 1 || cluster > K4_CLUSTER || (num_ctas && cluster != 1)) return -3;
   if (num_ctas < 0 || (num_ctas && (!part_o || !part_ml || ((reinterpret_cast<uintptr_t>(part_o) | reinterpret_cast<uintptr_t>(part_ml)) & 15)))) return -3;
-  if (static_cast<long long>(max_blocks) * block_size > 0x7fff0000ll ||
-      (num_ctas && static_cast<long long>(B) * Hkv * chunks * (static_cast<long long>(max_blocks) * block_size / K4_STEP + 2) + num_ctas > 0x7fffffffll) || static_cast<long long>(B) * Hkv * chunks > 0x7fffffffll || static_cast<long long>(Hkv) * chunks * cluster > 0x7fffffffll ||
-      num_blocks * Hkv > 0x7fffffffll)
+  const long long room = static_cast<long long>(max_blocks) * block_size, visible = window && window < room ? window : room, segments = static_cast<long long>(B) * Hkv * chunks;
+  if (room > 0x7fff0000ll || segments > 0x7fffffffll || (num_ctas && segments * (visible / K4_STEP + 2) + num_ctas > 0x7fffffffll) ||
+      static_cast<long long>(Hkv) * chunks * cluster > 0x7fffffffll || num_blocks * Hkv > 0x7fffffffll)
     return -4;
   const K4Params p{static_cast<const __nv_bfloat16*>(q), q_stride, static_cast<const uint8_t*>(cache), num_blocks, block_table, table_stride, max_blocks, seq_lens, Hkv, group, chunks,
                    block_size, window, scale, B, num_ctas, cluster, part_o, reinterpret_cast<float2*>(part_ml), reinterpret_cast<int4*>(part_ml + static_cast<long long>(num_ctas) * 32),

@@ -32,6 +32,7 @@ GROUP = 32
 TINY = 2.0 ** -100
 MAX_BLOCK = 65536
 MAX_CLUSTER = 8
+MAX_TOKENS = 0x7FFF0000      # of a sequence: places are 32-bit numbers, with room for the steps that are requested ahead
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else lambda index: torch.cuda.current_stream(index).cuda_stream
 
 
@@ -300,6 +301,9 @@ def kv4_paged_decode(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
     pages = block_table.shape[1]
     if block_table.shape[0] != B or seq_lens.shape != (B,) or block_table.dtype is not torch.int32 or seq_lens.dtype is not torch.int32:
         raise ValueError(f"block_table is int32 [{B}, pages] and seq_lens int32 [{B}], not {block_table.dtype} {tuple(block_table.shape)} and {seq_lens.dtype} {tuple(seq_lens.shape)}")
+    room = pages * block
+    if room > MAX_TOKENS:
+        raise ValueError(f"block_table has room for {room} tokens a sequence, the kernels count to {MAX_TOKENS}")
     _no_gradient(q)
     table = block_table if block_table.stride(1) == 1 else block_table.contiguous()      # (rows of a wider table are read where they are)
     lens = seq_lens.contiguous()
@@ -328,11 +332,13 @@ def kv4_paged_decode(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
     if q.dtype is not BF16:
         raise ValueError(f"the 4-bit cache takes bf16 queries, not {q.dtype}")
     if plan is None:
-        plan = kv4_plan(B, Hq, Hkv, D, min(pages * block, window) if window else pages * block)
+        plan = kv4_plan(B, Hq, Hkv, D, min(room, window) if window else room)
     cluster, num_ctas = plan
     if not 1 <= cluster <= MAX_CLUSTER or num_ctas < 0 or (num_ctas and cluster != 1):
         raise ValueError(f"plan {plan} is neither (1 to {MAX_CLUSTER}, 0) nor (1, CTAs)")
     if num_ctas:
+        if B * Hkv * -(-(Hq // Hkv) // 8) * ((min(room, window) if window else room) // 32 + 2) + num_ctas > 0x7FFFFFFF:
+            raise ValueError(f"plan {plan} shares more steps than it can count: take a cluster, or a window or a narrower block_table")
         size = kv4_scratch_size(num_ctas, D)
         if scratch is None:
             scratch = torch.empty(size, dtype=torch.float32, device=device)

@@ -417,6 +417,25 @@ def test_decode_of_more_rows_than_a_grid_has_in_one_direction(native_lib, plan):
     assert L.check_status() == 0
 
 
+def test_decode_window_over_a_very_wide_table(native_lib):
+    """A table with room for 2^31 tokens a sequence, of which a window is visible: planned and shared by the window. What no plan can share is refused by name."""
+    B, Hq, Hkv, D, block, window = 8, 8, 8, 64, 65536, 16384
+    cache = _pool(9, Hkv, D, block, 5)
+    table = torch.zeros((B, 32767), dtype=torch.int32, device="cuda")
+    table[:, 0] = torch.arange(8)
+    n = torch.tensor([20000, 16384, 16385, 1, 0, 65000, 30000, 16500], dtype=torch.int32, device="cuda")
+    q = _rows(B, Hq, Hkv, D).cuda()
+    assert K.kv4_plan(B, Hq, Hkv, D, window)[1] > 0
+    for plan in (None, (1, 100), (4, 0)):
+        _check(K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, window=window, plan=plan), q, cache, table, n, Hq, Hkv, D, window)
+    _check(K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D), q, cache, table, n, Hq, Hkv, D)
+    assert L.check_status() == 0
+    with pytest.raises(ValueError):
+        K.kv4_paged_decode(q, cache, table, n, Hq, Hkv, D, plan=(1, 444))
+    with pytest.raises(ValueError):
+        K.kv4_paged_decode(q, cache, torch.zeros((B, 32768), dtype=torch.int32, device="cuda"), n, Hq, Hkv, D)
+
+
 def test_places_beyond_32_bits(native_lib):
     """A cache of more than 4 GiB: pages at its far end."""
     Hq, Hkv, D, block = 8, 8, 128, 128
