@@ -15,10 +15,26 @@
 
 #include "common.cuh"
 
+#include <atomic>
+
 namespace rlb {
 
 constexpr int KV4_GROUP = 32;
 constexpr int KV4_MAX_BLOCK = 65536;      // places within a page are 32-bit offsets
+
+// The current device (by which launchers keep what they have asked for) and its multiprocessors.
+constexpr int KV4_DEVICES = 64;
+inline cudaError_t kv4_device(int& dev, int& sms) {
+  static std::atomic<int> known[KV4_DEVICES];
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= KV4_DEVICES) return cudaErrorInvalidDevice;
+  sms = known[dev].load();
+  if (sms) return cudaSuccess;
+  const cudaError_t asked = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (asked == cudaSuccess) known[dev].store(sms);
+  return asked;
+}
 
 template <int D>
 struct Kv4Page {

@@ -269,7 +269,10 @@ template <int D>
 int launch_write(void* qkv, const int* pos, const float* inv_freq, const long long* slots, void* cache, long long T, int Hq, int Hkv, int block_size, long long row_stride,
                  long long num_blocks, int* status, cudaStream_t stream) {
   const int heads = Hq + 2 * Hkv, per_head = D / 16;
-  const bool many = T * heads * per_head > 148 * 2048;      // more than the device holds threads: whole rows, some tokens a block (15003 tokens of 32 + 2 * 8 heads of 128, us with 2, 4, 8: 62, 64, 69; 32 + 2 * 4 of 64: 31, 29, 30)
+  int dev = 0, sms = 0;
+  const cudaError_t e = kv4_device(dev, sms);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const bool many = T * heads * per_head > static_cast<long long>(sms) * 2048;      // more than the device holds threads: whole rows, some tokens a block (15003 tokens of 32 + 2 * 8 heads of 128, us with 2, 4, 8: 62, 64, 69; 32 + 2 * 4 of 64: 31, 29, 30; 16 + 2 * 8 of 256 with 1, 2, 4: 2500 tokens 20.0, 17.7, 18.7, 16000 104, 89, 87)
   const int rows = many ? (D == 64 ? 4 : 2) : 1, per_block = many ? heads : 128 / per_head;
   const int per_row = heads * per_head, times = (per_row + 255) / 256, threads = many ? ((per_row + times - 1) / times + 31) / 32 * 32 : 128;
   const dim3 grid(static_cast<unsigned>((T + rows - 1) / rows), static_cast<unsigned>((heads + per_block - 1) / per_block));

@@ -26,8 +26,6 @@
 
 #include <math.h>
 
-#include <atomic>
-
 namespace {
 using namespace rlb;
 
@@ -745,19 +743,18 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const K4Params p) {
 }
 
 // Shared memory of which an SM (227 KB) has room for `per_sm` CTAs, and no more.
-constexpr int K4_SMS = 148;
 constexpr int k4_room(int per_sm) { return (per_sm == 1 ? 116 : per_sm == 2 ? 77 : 58) * 1024; }
 
 template <int D, bool PAIR>
 int launch_decode(const K4Params& p, cudaStream_t stream) {
   static std::atomic<unsigned long long> ready{0};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  int dev = 0, sms = 0;
+  cudaError_t e = kv4_device(dev, sms);
   if (e != cudaSuccess) return static_cast<int>(e);
-  if (!(ready.load() >> (dev & 63) & 1)) {
+  if (!(ready.load() >> dev & 1)) {
     e = cudaFuncSetAttribute(kv4_decode_kernel<D, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, k4_room(1));
     if (e != cudaSuccess) return static_cast<int>(e);
-    ready.fetch_or(1ull << (dev & 63));
+    ready.fetch_or(1ull << dev);
   }
   const int all_heads = p.Hkv * p.chunks;
   cudaLaunchConfig_t cfg = {};
@@ -784,15 +781,15 @@ int launch_decode(const K4Params& p, cudaStream_t stream) {
   // so much shared memory that only as many fit an SM as have to (37 sequences of 2048 tokens, 8 heads of 128: 27.3 -> 22.0 us; 96 of 3001, 2 heads of 64 in
   // clusters of two: 21.7 -> 18.7), where that leaves the clusters their places: those of eight do not fill the SMs.
   const long long clusters = p.num_ctas ? p.num_ctas : static_cast<long long>(all_heads) * p.B;
-  static std::atomic<int> held[K4_CLUSTER + 1][4];      // clusters that run at once with so many CTAs on an SM, plus one (0: not asked yet)
+  static std::atomic<int> held[KV4_DEVICES][K4_CLUSTER + 1][4];      // clusters that run at once with so many CTAs on an SM, plus one (0: not asked yet)
   for (int per_sm = 1; per_sm < 4 && k4_room(per_sm) > k4_smem<D>(); ++per_sm) {
-    if (static_cast<long long>(K4_SMS) * per_sm < clusters * p.cluster) continue;
-    int most = p.cluster == 1 ? K4_SMS * per_sm + 1 : held[p.cluster][per_sm].load();
+    if (static_cast<long long>(sms) * per_sm < clusters * p.cluster) continue;
+    int most = p.cluster == 1 ? sms * per_sm + 1 : held[dev][p.cluster][per_sm].load();
     cfg.dynamicSmemBytes = k4_room(per_sm);
     if (!most) {
       e = cudaOccupancyMaxActiveClusters(&most, kv4_decode_kernel<D, PAIR>, &cfg);
       if (e != cudaSuccess) return static_cast<int>(e);
-      held[p.cluster][per_sm].store(++most);
+      held[dev][p.cluster][per_sm].store(++most);
     }
     if (clusters < most) break;
     cfg.dynamicSmemBytes = k4_smem<D>();
