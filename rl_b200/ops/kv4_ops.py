@@ -256,7 +256,7 @@ def kv4_plan(B: int, Hq: int, Hkv: int, D: int, max_len: int, sm_count: int = 14
     """How decode attention over the 4-bit cache is cut up: (cluster, 0): a cluster of CTAs per sequence and key/value head (with up to eight query
     heads), or (1, n): n CTAs, as many as the device holds, share all tokens evenly, and a second kernel joins what they cut through.
 
-    A cluster of twice the CTAs is taken while they run at once and keep 12 steps of 32 tokens each, and a few more where some SMs get two (us in a graph with one,
+    A cluster of twice the CTAs is taken while they run at once and keep six steps of 32 tokens each, eight more in all where some SMs get two (us in a graph with one,
     two, four, eight CTAs: one sequence of 1200 tokens with 8 KV heads of 128 10.6, 8.6, 7.3, 7.1; 12 of 600 7.3, 8.3, 8.0, 14.5; 26 of 2400 with 4 heads
     21.0, 17.8, 15.6; 48 of 2400 26.6, 22.5, 28.5). Sharing has its search and its join, some 5 us, and pays off from 50 steps per CTA on (8 heads of 128, best cluster /
     shared: one sequence of 4800 tokens 9.7 / 10.7, of 40000 36 / 23; 64 of 4000 71 / 67, of 16000 255 / 214), where there are at most two CTAs for each that

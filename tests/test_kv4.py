@@ -331,3 +331,15 @@ def test_outputs_whose_rows_overlap_are_refused():
                 call(mem.as_strided((T, 2 * D), strides))
     for strides in ((1, T), (2 * D, 1), (6 * D - 1, 3)):
         assert K.kv4_cache_read(cache, slots, Hkv, D, out=mem.as_strided((T, 2 * D), strides)).shape == (T, 2 * D)
+
+
+def test_plan_at_its_thresholds():
+    """Twice the CTAs from six steps of 32 tokens for each on, eight steps more where some multiprocessors get two of them, and only while all run at once."""
+    for cluster, steps in ((2, 12), (4, 24), (8, 48)):
+        assert K.kv4_plan(1, 32, 8, 128, 32 * steps) == (cluster, 0) and K.kv4_plan(1, 32, 8, 128, 32 * steps - 31) == (cluster, 0)
+        assert K.kv4_plan(1, 32, 8, 128, 32 * (steps - 1)) == (cluster // 2, 0)
+    for B, Hkv, D in ((1, 1, 64), (3, 2, 128), (20, 4, 64), (40, 8, 128), (12, 8, 256), (9, 3, 256)):
+        slots = {64: 4, 128: 3, 256: 2}[D] * 148
+        for n in range(1, 3000, 31):
+            cluster, ctas = K.kv4_plan(B, Hkv, Hkv, D, n)
+            assert cluster == 1 or (ctas == 0 and -(-n // 32) >= 6 * cluster + (8 if B * Hkv * cluster > 148 else 0) and B * Hkv * cluster <= slots)
