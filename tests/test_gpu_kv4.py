@@ -593,3 +593,32 @@ def test_generation_by_configuration(native_lib):
     assert L.check_status() == 0 and (out["generation_lengths"] == 24).all()
     assert 0 < err.mean().item() < 0.3 and err.max().item() < 2.0      # the bounds of the other quantised rollouts
     assert gen.engine.kv_cache_bytes() * 32 == 2 * 2 * gen.engine.num_blocks * 2 * 64 * 128 * 2 * 9
+
+
+@pytest.mark.parametrize("kind", ["hybrid", "experts"])
+def test_engine_of_hybrid_and_expert_models(native_lib, kind):
+    """Attention blocks between others, and expert layers: by graphs and without the same tokens, near the log-probabilities of the model's own pass (the bounds of the other
+    quantised rollouts)."""
+    from rl_b200.engine.engine import SamplingParams
+    from rl_b200.models.config import preset
+    from rl_b200.models.transformer import PackedBatch, build_model
+
+    if kind == "hybrid":
+        mc = preset("tiny-nemotron-h", vocab_size=4096, hidden_size=512, intermediate_size=1024, head_dim=128, num_attention_heads=4, num_key_value_heads=2)
+    else:
+        mc = preset("tiny-llama-oracle", num_experts=8, num_experts_per_tok=2, moe_intermediate_size=128, norm_topk_prob=True, hidden_size=256, num_attention_heads=2,
+                    num_key_value_heads=1, head_dim=128, vocab_size=2048)
+    model = build_model(mc, device="cuda", dtype=torch.bfloat16, seed=7)
+    g = torch.Generator().manual_seed(0)
+    prompts = [torch.randint(1, mc.vocab_size, (n,), generator=g).tolist() for n in (9, 170, 5, 30)]
+    runs = [_engine(model, use_cuda_graphs=graphs).generate(prompts, SamplingParams(max_new_tokens=24, stop_token_ids=[], seed=3, temperature=1.0)) for graphs in (True, False)]
+    assert L.check_status() == 0
+    assert sum(a.out_tokens == b.out_tokens for a, b in zip(*runs)) >= 3      # (the few-token expert layer's sums may split a tie)
+    gaps = []
+    for r in runs[0]:
+        seq = torch.tensor([r.prompt + r.out_tokens], device="cuda")
+        with torch.no_grad():
+            lp, _ = model.next_token_logprobs(PackedBatch.from_padded(seq, torch.tensor([seq.shape[1]], device="cuda")), temperature=1.0)
+        gaps.append((lp[len(r.prompt) :].float().cpu() - torch.tensor(r.out_logprobs)).abs())
+    gaps = torch.cat(gaps)
+    assert 0 < gaps.mean() < 0.3 and gaps.max() < 2.0, (gaps.mean(), gaps.max())

@@ -333,6 +333,116 @@ def test_outputs_whose_rows_overlap_are_refused():
         assert K.kv4_cache_read(cache, slots, Hkv, D, out=mem.as_strided((T, 2 * D), strides)).shape == (T, 2 * D)
 
 
+# ------------------------------------------------------------------------------------------- the engine's other paths, against a cache of the model's type that holds what 4 bits hold
+def held_write(qkv, positions, inv_freq, slots, k_cache, v_cache, Hq, Hkv, D):
+    """The write of the model's type's cache, with what the 4-bit cache would keep in the place of keys and values."""
+    T = qkv.shape[0]
+    out = qkv.clone()
+    out[:, : (Hq + Hkv) * D] = K._rotate_ref(qkv[:, : (Hq + Hkv) * D].reshape(T, Hq + Hkv, D), positions, inv_freq).reshape(T, -1)
+    kv = K._values(*K.quantize_ref(out[:, Hq * D :].reshape(T, 2, Hkv, D))).to(k_cache.dtype)
+    ok = slots >= 0
+    page, off = slots[ok] // k_cache.shape[2], slots[ok] % k_cache.shape[2]
+    k_cache[page, :, off], v_cache[page, :, off] = kv[ok, 0], kv[ok, 1]
+    return out
+
+
+def _against_held(monkeypatch, model, prompts, sp, **kw):
+    """Runs both engines. Log-probabilities agree for as long as both sample the same tokens (float32, sums in other orders: a value may fall on the other side of its code's border,
+    one level of one value), which is most of the way. Returns the 4-bit engine."""
+    from rl_b200.ops import engine_ops as E
+
+    eng = _engine(model, **kw)
+    got = eng.generate(prompts, sp)
+    with monkeypatch.context() as m:
+        m.setattr(E, "rope_kv_cache_write", held_write)
+        want = _engine(model, kv_cache_dtype="auto", **kw).generate(prompts, sp)
+    compared = 0
+    for a, b in zip(got, want):
+        assert len(a.out_tokens) == len(b.out_tokens) == sp.max_new_tokens
+        same = next((i for i, (x, y) in enumerate(zip(a.out_tokens, b.out_tokens)) if x != y), len(a.out_tokens))
+        compared += same
+        gap = (torch.tensor(a.out_logprobs[:same]) - torch.tensor(b.out_logprobs[:same])).abs()
+        assert same == 0 or gap.max() < 5e-3, gap
+    assert compared * 2 > sp.max_new_tokens * len(prompts), compared
+    return eng
+
+
+def _louder(model):
+    with torch.no_grad():
+        for n, p in model.named_parameters():
+            if p.dim() >= 2 and "conv" not in n:
+                p.mul_(3.0)
+    return model
+
+
+def test_engine_prefills_again_what_lost_its_pages(monkeypatch):
+    """A cache so small that sequences are preempted and come back: prompt and generated tokens are prefilled again into other pages."""
+    from rl_b200.engine.engine import SamplingParams
+
+    prompts = [[(5 * i) % 90 + 1 for i in range(21)], [3] * 20, [4] * 30]
+    for temperature in (0.0, 0.8):
+        eng = _against_held(monkeypatch, _model(), prompts, SamplingParams(max_new_tokens=40, stop_token_ids=[], seed=3, temperature=temperature), num_blocks=9)
+        assert eng.sched.num_preemptions > 0
+
+
+def test_engine_serves_hybrid_models_on_the_4_bit_cache(monkeypatch):
+    """Nemotron-H blocks: the attention blocks' keys and values in 4 bits, no rotation, prompts whole and in portions."""
+    from rl_b200.engine.engine import SamplingParams
+
+    model = _louder(_model(model_type="nemotron_h", layers_block_type=["mamba", "mlp", "attention", "mamba", "moe", "attention"], num_hidden_layers=6, mamba_num_heads=4, mamba_head_dim=8,
+                           ssm_state_size=8, mamba_n_groups=2, mamba_chunk_size=4, use_rope=False, mlp_gated=False, hidden_act="relu2", num_experts=4, num_experts_per_tok=2,
+                           moe_intermediate_size=16, n_shared_experts=1, moe_shared_expert_intermediate_size=24, scoring_func="sigmoid"))
+    prompts = [[1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11] * 3, [9, 8, 7], [11] * 9, [5, 4, 3, 2, 1, 2, 3, 4, 5, 6, 7, 8, 9]]
+    for kw in (dict(), dict(max_prefill_tokens=16)):
+        eng = _against_held(monkeypatch, model, prompts, SamplingParams(max_new_tokens=10, stop_token_ids=[], seed=3, temperature=0.8), **kw)
+        assert eng.hybrid and sum(c is not None for c in eng.k_cache) == 2
+
+
+def test_engine_serves_expert_models_on_the_4_bit_cache(monkeypatch):
+    from rl_b200.engine.engine import SamplingParams
+
+    model = _model(model_type="qwen3_moe", qk_norm=True, num_hidden_layers=3, num_experts=8, num_experts_per_tok=2, moe_intermediate_size=16)
+    prompts = [[1, 2, 3, 4, 5, 6, 7, 8, 9] * 3, [9, 8, 7], [1, 2, 3, 4, 5, 6, 7, 8, 9] * 3]
+    for kw in (dict(), dict(max_prefill_tokens=16)):
+        _against_held(monkeypatch, model, prompts, SamplingParams(max_new_tokens=12, stop_token_ids=[], seed=3, temperature=0.8), **kw)
+
+
+_TENSOR_PARALLEL = dict(precision="float32", train_global_batch_size=4, train_micro_batch_size=2, max_total_sequence_length=96,
+                        optimizer=dict(name="torch.optim.AdamW", kwargs=dict(lr=1e-3)),
+                        generation=dict(max_new_tokens=12, temperature=1.0, stop_token_ids=[], kv_cache_tokens=2048, block_size=16, max_running=8, kv_cache_dtype="int4"))
+
+
+def _served(ranks):
+    from rl_b200.distributed.batched_data_dict import BatchedDataDict
+    from rl_b200.models.config import preset
+    from rl_b200.policy.worker import PolicyWorker
+
+    w = PolicyWorker(dict(_TENSOR_PARALLEL, parallel=dict(tensor_parallel_size=ranks)), model_cfg=preset("tiny-llama-oracle", torch_dtype="float32"), init_reference_model=False, seed=4)
+    gen = w.build_generation()
+    assert gen.engine.kv4 and gen.engine.hkv * ranks == w.model_cfg.num_key_value_heads
+    gen.prepare_for_generation()
+    ids = torch.randint(1, 2048, (3, 40), generator=torch.Generator().manual_seed(20))
+    out = gen.generate(BatchedDataDict(input_ids=ids, input_lengths=torch.full((3,), 40)), greedy=True)
+    return out["output_ids"].tolist(), out["logprobs"].tolist()
+
+
+def _served_by_two(rank, world):
+    return _served(world)
+
+
+def test_tensor_parallel_engine_on_the_4_bit_cache():
+    """Two ranks, each with half of the key/value heads in 4 bits: the tokens and log-probabilities of one rank."""
+    from test_parallel_cpu import _spawn
+
+    from rl_b200.parallel.state import reset_parallel
+
+    got = _spawn(_served_by_two, 2)
+    reset_parallel()
+    ids, lp = _served(1)
+    assert got[0][0] == got[1][0] == ids
+    assert (torch.tensor(got[0][1]) - torch.tensor(lp)).abs().max() < 5e-3
+
+
 def test_plan_at_its_thresholds():
     """Twice the CTAs from six steps of 32 tokens for each on, eight steps more where some multiprocessors get two of them, and only while all run at once."""
     for cluster, steps in ((2, 12), (4, 24), (8, 48)):
