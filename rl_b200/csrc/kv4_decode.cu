@@ -17,7 +17,7 @@
 // mma.sync's rate at long contexts): 5 of a word's instructions are its unpacking, 65 of 125 million instructions of the case below run on the integer pipe.
 //
 // Measured (a graph of calls on states larger than L2): 32 sequences of 32768 tokens, 32 query and 8 KV heads of 128: 217 us, 5.57 TB/s, 0.85 of what a plain copy moves;
-// 258 us back to back for seconds, at the board's power limit. 64 / 8 heads 241 us. 64 of 4000 67 us, 128 of 4000 112 us, 64 of 1280 27 us (two waves of CTAs), one of
+// 258 us back to back for seconds, at the board's power limit. 64 / 8 heads 242 us. 64 of 4000 67 us, 128 of 4000 113 us, 64 of 1280 27 us (two waves of CTAs), one of
 // 131072 with 40 heads 45 us, one of 4000 9.1 us, 48 of 1024 with heads of 256 30 us. Short calls are a chain of latencies: length, page, keys, a step's products and softmax
 // (some 0.8 us a step of a warp alone on its scheduler, however many steps are on their way), the join.
 //

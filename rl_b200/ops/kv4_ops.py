@@ -164,7 +164,9 @@ def rope_kv4_cache_write(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: t
                          Hq: int, Hkv: int, D: int) -> torch.Tensor:
     """Rotary embedding of the q and k heads of fused rows [T, (Hq + 2 Hkv) D] (in place on CUDA) and the write of the rotated k and of v into the
     4-bit ``cache``, in one launch; returns the rotated fused rows. ``slots`` [T]: block * block_size + offset of each token (negative: rotate only);
-    the slots of one call differ from each other. The angles are taken in 64 bits, whatever the position."""
+    the slots of one call differ from each other. The angles are taken in 64 bits, whatever the (32-bit) position; the policy's own passes and the write of a bf16 cache take them in
+    32 bits (``elementwise.cu``, ``paged_attention.cu``), which is half a unit in the last place of the angle away: 0.001 near position 32768, 0.004 near 131072, on the pairs that turn
+    fastest."""
     block = block_size_of(cache, Hkv, D)
     if qkv.dim() != 2 or Hq < 0 or qkv.shape[1] != (Hq + 2 * Hkv) * D:
         raise ValueError(f"qkv is [T, {(Hq + 2 * Hkv) * D}], not {tuple(qkv.shape)}")
