@@ -307,6 +307,7 @@ def kv4_paged_decode(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
     if room > MAX_TOKENS:
         raise ValueError(f"block_table has room for {room} tokens a sequence, the kernels count to {MAX_TOKENS}")
     _no_gradient(q)
+    window = min(window, MAX_TOKENS)      # (no sequence is longer, and the kernels count in 32 bits)
     table = block_table if block_table.stride(1) == 1 else block_table.contiguous()      # (rows of a wider table are read where they are)
     lens = seq_lens.contiguous()
     if scale is None:

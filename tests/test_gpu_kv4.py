@@ -436,6 +436,15 @@ def test_decode_window_over_a_very_wide_table(native_lib):
         K.kv4_paged_decode(q, cache, torch.zeros((B, 32768), dtype=torch.int32, device="cuda"), n, Hq, Hkv, D)
 
 
+@pytest.mark.parametrize("window", [2**31 - 1, 2**31 + 7, 2**32, 2**32 + 5, 2**40 + 1])
+def test_decode_of_windows_beyond_32_bits(native_lib, window):
+    """A window wider than any sequence leaves everything."""
+    q, cache, table, n = _decode_case([1, 17, 100, 0, 1000, 333, 16], 4, 2, 64, 32, seed=3)
+    for plan in ((1, 0), (2, 0), (1, 3)):
+        assert torch.equal(K.kv4_paged_decode(q, cache, table, n, 4, 2, 64, window=window, plan=plan), K.kv4_paged_decode(q, cache, table, n, 4, 2, 64, plan=plan))
+    assert L.check_status() == 0
+
+
 def test_places_beyond_32_bits(native_lib):
     """A cache of more than 4 GiB: pages at its far end."""
     Hq, Hkv, D, block = 8, 8, 128, 128
