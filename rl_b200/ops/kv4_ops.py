@@ -32,6 +32,7 @@ GROUP = 32
 TINY = 2.0 ** -100
 MAX_BLOCK = 65536
 MAX_CLUSTER = 8
+MAX_SCALE = torch.finfo(torch.float32).max
 MAX_TOKENS = 0x7FFF0000      # of a sequence: places are 32-bit numbers, with room for the steps that are requested ahead
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else lambda index: torch.cuda.current_stream(index).cuda_stream
 
@@ -294,8 +295,8 @@ def kv4_paged_decode(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
     device, width = q.device, Hq * D
     if Hq < 1 or Hq % Hkv or q.dim() != 2 or q.shape[1] < width:
         raise ValueError(f"q is [B, {width}] with {Hq} heads, a multiple of {Hkv}, not {tuple(q.shape)}")
-    if window < 0 or (scale is not None and not math.isfinite(scale)):
-        raise ValueError(f"window {window} is negative, or scale {scale} not a number")
+    if window < 0 or (scale is not None and not abs(scale) <= MAX_SCALE):
+        raise ValueError(f"window {window} is negative, or scale {scale} not a number of 32 bits")
     B = q.shape[0]
     _same_device(device, cache, block_table, seq_lens)
     if block_table.dim() != 2:

@@ -453,3 +453,12 @@ def test_plan_at_its_thresholds():
         for n in range(1, 3000, 31):
             cluster, ctas = K.kv4_plan(B, Hkv, Hkv, D, n)
             assert cluster == 1 or (ctas == 0 and -(-n // 32) >= 6 * cluster + (8 if B * Hkv * cluster > 148 else 0) and B * Hkv * cluster <= slots)
+
+
+def test_scales_beyond_32_bits_are_refused():
+    """The kernels take the scale in 32 bits, where these would be infinite."""
+    cache, q = K.kv4_cache(1, 1, 16, 64, "cpu"), _rows(1, 1, 1, 64)
+    for scale in (1e39, -1e300, math.inf, math.nan):
+        with pytest.raises(ValueError):
+            K.kv4_paged_decode(q, cache, torch.zeros((1, 1), dtype=torch.int32), torch.ones(1, dtype=torch.int32), 1, 1, 64, scale=scale)
+    assert K.kv4_paged_decode(q, cache, torch.zeros((1, 1), dtype=torch.int32), torch.ones(1, dtype=torch.int32), 1, 1, 64, scale=3e38).shape == (1, 64)
