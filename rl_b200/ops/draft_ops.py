@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from functools import lru_cache
 from typing import Optional, Sequence
 
 import torch
@@ -29,7 +30,7 @@ _P, _I, _LL, _F = _L.P, _L.I, _L.L, _L.F
 _L.register("rlb_tree_rows", [_P, _P, _P, _P, _LL, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P])
 _L.register("rlb_kv_keep", [_P, _I, _P, _LL, _I, _I, _I, _I, _I, _P, _P, _I, _P, _I, _P, _P])
 _L.register("rlb_verify_drafts", [_P, _LL, _P, _LL, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, C.c_double, _I, _P, _P, _P, _P, _P, _P])
-_L.register("rlb_tree_decode", [_P, _LL, _P, _P, _I, _I, _P, _LL, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _LL, _P, _I, _F, _P, _LL, _P, _P])
+_L.register("rlb_tree_decode", [_P, _LL, _P, _P, _I, _I, _P, _LL, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _LL, _P, _I, _F, _I, _I, _P, _P, _P, _LL, _P, _P])
 
 BF16 = torch.bfloat16
 HEAD_DIMS = (64, 128)
@@ -144,20 +145,37 @@ def _tree_decode_ref(q, k_cache, v_cache, table, ctx, spans, Hq, Hkv, D, masks, 
     return out
 
 
+@lru_cache(maxsize=4096)
+def tree_plan(B: int, Hq: int, Hkv: int, max_rows: int, max_len: int, sm_count: int = 148) -> int:
+    """CTAs that share all tiles of 64 keys evenly in :func:`tree_paged_decode`, or 0: a CTA for each sequence, key/value head and block of 128 / (Hq / Hkv) rows."""
+    units, tiles = B * Hkv * -(-max_rows // (128 // (Hq // Hkv))), -(-max_len // 64)
+    return 0 if tiles <= 4 or units >= 6 * sm_count else 2 * sm_count
+
+
+def tree_scratch_size(ctas: int, Hq: int, Hkv: int, D: int, max_rows: int) -> int:
+    """Floats of the scratch tensor of :func:`tree_paged_decode` with this many CTAs."""
+    return 2 * ctas * min(max_rows, 128 // (Hq // Hkv)) * (Hq // Hkv) * (D + 2)
+
+
 def tree_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, ctx_lens: torch.Tensor, cu_rows: torch.Tensor,
                       Hq: int, Hkv: int, D: int, *, max_rows: int, masks: Optional[torch.Tensor] = None, scale: Optional[float] = None, window: int = 0,
-                      positions: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                      positions: Optional[torch.Tensor] = None, plan: Optional[int] = None, scratch: Optional[torch.Tensor] = None,
+                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of the trees' rows, ``q`` [T, >= Hq D] (rows may be strided: the fused rows do), against the paged cache [blocks, Hkv, block size, D], which holds their own
     keys and values behind the context. A row sees the whole context of its sequence and the tree rows whose bits ``masks`` (as :func:`tree_rows` gives them; any bits
     do) has set; without ``masks`` the rows up to itself, which is a chain. ``window`` > 0: of these only keys whose position is less than ``window`` before the row's own
     (sliding-window layers): ``positions`` [T] int32 has the rows' (from the context's end on), a context place's is its number. A row that sees nothing gives zeros. Rows of no sequence are left as
-    they are in ``out`` (a new ``out`` has no values there). Heads of 64 and 128, pages of a multiple of 16 tokens. Returns [T, Hq D]."""
+    they are in ``out`` (a new ``out`` has no values there). Heads of 64 and 128, at most 128 query heads to a key/value head, pages of a multiple of 16 tokens. ``plan``: CTAs that
+    share the keys (None: :func:`tree_plan` for the table's width); ``scratch``: float32 tensor of :func:`tree_scratch_size` elements, for callers that keep their own (one call at a
+    time). Returns [T, Hq D].
+
+    Scores, maxima and sums are in 32 bits, weights are rounded to bf16 before they meet the values."""
     B = _rows_of(cu_rows, max_rows)
     width, device = Hq * D, q.device
     if D not in HEAD_DIMS:
         raise ValueError(f"heads of {HEAD_DIMS} dimensions, not {D}")
-    if Hkv < 1 or Hq < 1 or Hq % Hkv or q.dim() != 2 or q.shape[1] < width:
-        raise ValueError(f"q is [T, {width}] with {Hq} heads, a multiple of {Hkv}, not {tuple(q.shape)}")
+    if Hkv < 1 or Hq < 1 or Hq % Hkv or Hq // Hkv > 128 or q.dim() != 2 or q.shape[1] < width:
+        raise ValueError(f"q is [T, {width}] with {Hq} heads, 1 to 128 times {Hkv}, not {tuple(q.shape)}")
     T = q.shape[0]
     if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1] != Hkv or k_cache.shape[3] != D or not k_cache.is_contiguous() or not v_cache.is_contiguous():
         raise ValueError(f"the caches are contiguous [blocks, {Hkv}, block size, {D}], not {tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
@@ -193,12 +211,28 @@ def tree_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         return _tree_decode_ref(q, k_cache, v_cache, table, ctx, _spans(cu, T, max_rows), Hq, Hkv, D, masks, positions, window, scale, out)
     if q.dtype is not BF16:
         raise ValueError(f"the kernels take bf16 queries and caches, not {q.dtype}")
+    if (k_cache.data_ptr() | v_cache.data_ptr()) % 16 or k_cache.shape[0] * Hkv * block > 0x7FFFFFFE or B > 65535 or Hkv * -(-max_rows // (128 // (Hq // Hkv))) > 65535:
+        raise ValueError(f"caches {tuple(k_cache.shape)} start on 16 bytes and have less than 2^31 - 1 places of all heads, for at most 65535 sequences, and units of a sequence")
+    room = table.shape[1] * block
+    if plan is None:
+        plan = tree_plan(B, Hq, Hkv, max_rows, min(room, window + max_rows) if window else room)
+    elif plan < 0 or plan > 65535:
+        raise ValueError(f"plan is 0 to 65535 CTAs, not {plan}")
+    sums = parts = None
+    if plan:
+        size = tree_scratch_size(plan, Hq, Hkv, D, max_rows)
+        if scratch is None:
+            scratch = torch.empty(size, dtype=torch.float32, device=device)
+        elif scratch.dtype is not torch.float32 or not scratch.is_contiguous() or scratch.numel() < size or scratch.data_ptr() % 16 or scratch.device != device:
+            raise ValueError(f"scratch is a contiguous float32 tensor of {size} elements on {device} that starts on 16 bytes")
+        parts = scratch.data_ptr()
+        sums = parts + size // (D + 2) * D * 4
     with torch.cuda.device(device):
         if q.stride(1) != 1 or q.stride(0) % 8 or q.data_ptr() % 16:      # rows that do not start on 16 bytes
             q = q[:, :width].clone(memory_format=torch.contiguous_format)
         call("rlb_tree_decode", q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], block, table.data_ptr(), table.stride(0), table.shape[1],
              ctx.data_ptr(), cu.data_ptr(), B, T, max_rows, Hq, Hkv, D, _L.ptr(masks), masks.stride(0) if masks is not None else 0, _L.ptr(positions) if window else None,
-             window, scale, out.data_ptr(), out.stride(0), _L.status_word(device).data_ptr(), _raw_stream(device.index))
+             window, scale, plan, 4, parts, sums, out.data_ptr(), out.stride(0), _L.status_word(device).data_ptr(), _raw_stream(device.index))
     return out
 
 
