@@ -123,14 +123,15 @@ keep_kernel(const __grid_constant__ KeepCaches caches, const int* __restrict__ t
 
 // ------------------------------------------------------------------------------------------------ verification
 // p = softmax(l / T) of a node, in 64 bits throughout: the last token is the first whose running sum passes a given number, and with 32 bits the running sums of a flat
-// distribution over 10^5 tokens would be off by as much as a token has. A weight is e = 2^((l - m) log2(e) / T), taken as 2^(k / 256) from a table times a polynomial of third degree
-// in the rest r, |r| <= 1 / 512, whose error is (r ln 2)^4 / 24 < 1.5e-13: ten instructions of the 64-bit pipe, which has half the rate of the 32-bit one.
+// distribution over 10^5 tokens would be off by as much as a token has. A weight is 2^(l c - N), c = log2(e) / T, with a whole number N next to the largest l c that a warp has met first: so
+// sums of several warps are joined by their exponents. l c - N is cut into 256ths, a table's entry, and a rest r, |r| <= 1 / 512, for which a polynomial of third degree is off by
+// (r ln 2)^4 / 24 < 1.5e-13. Eight instructions of the 64-bit pipe and some ten others a logit.
 //
 // A cluster of CTAs has a sequence. It walks down the accepted rows and reads the logits of these rows alone, which is what the operator cannot do without: each warp has a range
-// of tokens and leaves its sum in every CTA's shared memory; all CTAs come to the same decision. The ranges' sums say in which range the last token lies, whose warp
-// goes through it once more. Where tokens have been rejected the sums are taken again first: with draft logits all of them, otherwise the ranges that a rejected token was in.
+// of tokens and leaves its sum in every CTA's shared memory; all CTAs come to the same decision. The ranges' sums say in which range the last token lies, whose CTA
+// goes through it once more. With draft logits the sums are taken again behind a rejection; without, the rejected tokens' weights are taken off their ranges.
 //
-// Bound by the 64-bit pipe and, for few sequences, by latency: the row, the exchange and the decision one after another.
+// Bound by the instructions' rate and, for few sequences, by latency: the row, the exchange and the decision one after another (a 64-bit instruction takes 18 cycles).
 struct VerifyArgs {
   const void* logits;
   const void* draft;      // null: children are taken without chance
@@ -150,9 +151,12 @@ struct VerifyArgs {
 };
 
 constexpr int DV_THREADS = 512, DV_WARPS = DV_THREADS / 32, DV_CLUSTER = 8, DV_PARTS = DV_WARPS * DV_CLUSTER;
+constexpr int DV_ELEMS = 8;      // logits a lane has at a time
 constexpr int EXP_STEPS = 256;
 constexpr double LOG2E = 1.4426950408889634074, LN2 = 0.69314718055994530942;
+constexpr double MAGIC = 6755399441055744.0 / EXP_STEPS;      // 1.5 * 2^52 / 256: a sum with it has the nearest number of 256ths in its low word
 constexpr float F_MAX = 3.402823466e38f;
+constexpr float COLDEST = 1.17549435e-38f;      // temperatures below are greedy
 
 // NaN weighs nothing, +inf as much as the largest number.
 __device__ __forceinline__ float usable(float x) { return fminf(fmaxf(x, -INFINITY), F_MAX); }
@@ -161,42 +165,75 @@ __device__ __forceinline__ double warp_sum_d(double v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+__device__ __forceinline__ float warp_top(float x) {      // largest of the warp's numbers, none of them NaN
+  const int u = __float_as_int(x), m = __reduce_max_sync(0xffffffffu, u < 0 ? u ^ 0x7fffffff : u);
+  return __int_as_float(m < 0 ? m ^ 0x7fffffff : m);
+}
+// x in 64 bits times 2^-896, by its bits (the conversion instruction gives one lane a cycle).
+__device__ __forceinline__ double lowered(float x) {
+  const int u = __float_as_int(x);
+  return __hiloint2double((u >> 3) & 0x8fffffff, u << 29);
+}
+// 2^z of |z| <= 1022 as table entry, rest and exponent: `t` is z + MAGIC, `r` what z has over its 256ths.
+__device__ __forceinline__ double power(const double* table, double t, double r) {
+  const int k = __double2loint(t);
+  const double p = r * (LN2 + r * (LN2 * LN2 / 2 + r * (LN2 * LN2 * LN2 / 6)));
+  const double f = table[k & (EXP_STEPS - 1)];
+  const double s = __hiloint2double(__double2hiint(f) + (k & ~(EXP_STEPS - 1)) * (0x100000 / EXP_STEPS), __double2loint(f));
+  return fma(s, p, s);
+}
+// log2 of a sum: 32 bits, then one step on 2^-l s = 1 + d.
+__device__ __forceinline__ double log2_of(const double* table, double s) {
+  const int hi = __double2hiint(s), e = (hi >> 20) - 1023;
+  const double f = __hiloint2double((hi & 0xfffff) | 0x3ff00000, __double2loint(s));
+  const double l = static_cast<double>(__log2f(static_cast<float>(f))), t = MAGIC - l, d = fma(f, power(table, t, -l - (t - MAGIC)), -1.0);
+  return e + (l + (d - d * d * 0.5 + d * d * d * (1.0 / 3)) * LOG2E);
+}
 
-// Weights relative to the logit m. Logits below `low` weigh nothing (2^-1000 of m's), those above `high` would pass 2^800.
-struct Scale {
-  double m;
-  float low, high;
-  // octave: the difference of logits that doubles a weight
-  __device__ __forceinline__ void set(float top, double octave) {
-    m = static_cast<double>(top);
-    low = fmaxf(fminf(__double2float_ru(m - 1000.0 * octave), top), -F_MAX);
-    high = fmaxf(__double2float_rd(m + 800.0 * octave), top);
+struct Temperature {
+  double c;            // log2(e) / T * 2^896
+  float far, near;     // differences of logits that make 2^1000 (rounded down) and 2^800
+};
+// Weights relative to 2^N, N = rint(top c).
+struct Frame {
+  double add;          // MAGIC - N
+  float top, low;      // logits below `low` weigh nothing (2^-1000 of top's)
+  int kind;            // 0: what is below `low` may be taken as `low` in a sum; 1: it may not; 2: so far apart are the logits (top c beyond 2^42) that top's equals alone have weight
+  __device__ __forceinline__ void set(float x, const Temperature& q) {
+    top = x;
+    low = fmaxf(fminf(__fsub_ru(x, q.far), x), -F_MAX);
+    const double m = lowered(x) * q.c, n = (m + 256 * MAGIC) - 256 * MAGIC;
+    add = MAGIC - n;
+    kind = !(fabs(m) < 0x1p42) ? 2 : low >= x || low <= -F_MAX ? 1 : 0;
+  }
+  __device__ __forceinline__ double near(const double* table, double c, float x) const {
+    const double v = lowered(x), t = fma(v, c, add);
+    return power(table, t, fma(v, c, add - t));
   }
   __device__ __forceinline__ double operator()(const double* table, double c, float x) const {
-    const double z = (static_cast<double>(x) - m) * c;
-    const double magic = 6755399441055744.0 / EXP_STEPS;      // 1.5 * 2^52 / 256: the sum's low word is the nearest number of 256ths
-    const double t = z + magic, r = z - (t - magic);
-    const int k = __double2loint(t);
-    const double p = r * (LN2 + r * (LN2 * LN2 / 2 + r * (LN2 * LN2 * LN2 / 6)));
-    const double f = table[k & (EXP_STEPS - 1)];
-    const bool none = !(x >= low);
-    const double s = __hiloint2double(none ? 0 : __double2hiint(f) + (k >> 8 << 20), none ? 0 : __double2loint(f));
-    return none ? 0.0 : fma(s, p, s);
+    return !(x >= low) ? 0.0 : kind == 2 ? (x == top ? 1.0 : 0.0) : near(table, c, x);
+  }
+  // 2^(N - N') of another frame, of whose top less than 2^-1000 of this one's counts as nothing
+  __device__ __forceinline__ double over(const Frame& o) const {
+    if (top == -INFINITY) return 0.0;
+    if (o.kind == 2 || kind == 2) return top == o.top ? 1.0 : 0.0;
+    const double d = o.add - add;
+    return d < -1000.0 ? 0.0 : __hiloint2double((1023 + __double2loint(d + 256 * MAGIC)) << 20, 0);
   }
 };
 
 __device__ __forceinline__ void push_d(uint32_t addr, double v) { asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory"); }
 
-struct Part {      // of a warp's range
-  double m, sum;      // sum of weights relative to m (-inf: none)
-  double dm, dsum;    // of the draft's
+struct Part {      // of a warp's range: sums of weights relative to the frames of m and dm (-inf: none)
+  double sum, dsum;
+  float m, dm;
   float peak;
   int at;
 };
 
-template <typename T, int ELEMS>      // logits a lane has at a time
+template <typename T>
 struct RowLogits {
-  static constexpr int VEC = 16 / sizeof(T), LOADS = ELEMS / VEC;
+  static constexpr int VEC = 16 / sizeof(T), LOADS = DV_ELEMS / VEC;
   const T* p;
   int V;
   int shift;      // elements before the row's first that its first group of 16 bytes has
@@ -204,83 +241,101 @@ struct RowLogits {
   // group g: elements g * VEC - shift and on; those outside of the row are -inf
   __device__ __forceinline__ uint4 load(int g, int g1) const {
     const int e = g * VEC - shift;
+    if (g < g1 && vec && e >= 0 && e + VEC <= V) return __ldg(reinterpret_cast<const uint4*>(p + e));
+    return edge(p, e, g < g1 ? V : 0);
+  }
+  static __device__ __noinline__ uint4 edge(const T* p, int e, int V) {
     uint4 v;
     uint32_t* w = &v.x;
-    if (g < g1 && vec && e >= 0 && e + VEC <= V) return __ldg(reinterpret_cast<const uint4*>(p + e));
     if (sizeof(T) == 4) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = g < g1 && e + i >= 0 && e + i < V ? reinterpret_cast<const uint32_t*>(p)[e + i] : 0xff800000u;
+      for (int i = 0; i < 4; ++i) w[i] = e + i >= 0 && e + i < V ? reinterpret_cast<const uint32_t*>(p)[e + i] : 0xff800000u;
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int a = e + 2 * i;
-        const uint32_t lo = g < g1 && a >= 0 && a < V ? reinterpret_cast<const uint16_t*>(p)[a] : 0xff80u;
-        const uint32_t hi = g < g1 && a + 1 >= 0 && a + 1 < V ? reinterpret_cast<const uint16_t*>(p)[a + 1] : 0xff80u;
+        const uint32_t lo = a >= 0 && a < V ? reinterpret_cast<const uint16_t*>(p)[a] : 0xff80u;
+        const uint32_t hi = a + 1 >= 0 && a + 1 < V ? reinterpret_cast<const uint16_t*>(p)[a + 1] : 0xff80u;
         w[i] = lo | hi << 16;
       }
     }
     return v;
   }
-  static __device__ __forceinline__ float element(const uint4& v, int i) {
+  static __device__ __forceinline__ float raw(const uint4& v, int i) {
     const uint32_t* w = &v.x;
-    return usable(sizeof(T) == 4 ? __uint_as_float(w[i]) : __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16));
+    return sizeof(T) == 4 ? __uint_as_float(w[i]) : __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+  }
+  static __device__ __forceinline__ float element(const uint4& v, int i) { return usable(raw(v, i)); }
+  static __device__ __noinline__ double seldom(uint4 v, Frame f, const double* table, double c) {      // a group's weights in frames of the other kinds
+    double t = 0.0;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) t += f(table, c, element(v, i));
+    return t;
   }
   __device__ __forceinline__ float at(int i) const { return usable(static_cast<float>(p[i])); }
+};
+
+struct RowSum {      // what the first warp makes of the parts
+  Frame p, q;
+  double inv, dinv, sum;      // reciprocals of the sums (0: no logit above -inf), the sum
+  int best;
 };
 
 template <typename T, bool DRAFT>
 __global__ void __launch_bounds__(DV_THREADS, 2)
 verify_kernel(const VerifyArgs a) {
-  using Row = RowLogits<T, DRAFT ? 8 : 16>;
-  constexpr int VEC = Row::VEC, LOADS = Row::LOADS;
+  using Row = RowLogits<T>;
+  constexpr int VEC = Row::VEC, LOADS = Row::LOADS, STEP = 32 * LOADS;
   __shared__ double table[EXP_STEPS];
   __shared__ Part parts[2][DV_PARTS];      // of all warps of the cluster, by turns
+  __shared__ double share[DV_PARTS], pieces[DV_WARPS];      // the ranges' probabilities; sums of a range's pieces
+  __shared__ RowSum row;
   __shared__ int up[DR_ROWS], tok[DR_ROWS], gone[DR_ROWS];
   __shared__ float num[DR_ROWS], lz[DR_ROWS], ld[DR_ROWS];      // numbers, logits of the children's tokens in their parent's rows
-  __shared__ double left[DR_ROWS + 1];                          // what is left to be given after so many rejections
+  __shared__ double left[DR_ROWS + 1], grow[DR_ROWS + 1];       // what is left to be given after so many rejections, and its reciprocal
+  __shared__ double chosen[DR_ROWS], sums[DR_ROWS];             // of each accepted step: l c - N of its token, the sum of weights
   __shared__ int verdict, tried, turned_down;
-  __shared__ double share[DV_PARTS];      // the ranges' probabilities
-  __shared__ double row_top, row_sum, row_inv, draft_top, draft_inv;
-  __shared__ int row_best;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t ctas;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
   const int rank = static_cast<int>(cluster_ctarank()), b = blockIdx.x / ctas, W = static_cast<int>(ctas) * DV_WARPS, me = rank * DV_WARPS + warp;
-  if (tid < EXP_STEPS) table[tid] = exp2(static_cast<double>(tid) / EXP_STEPS);
+  if (tid < EXP_STEPS) {      // 2^(i / 256) by exp's series, 0.7^18 / 18! < 3e-19
+    const double y = tid * (LN2 / EXP_STEPS);
+    double v = 1.0;
+#pragma unroll
+    for (int i = 17; i > 0; --i) v = fma(v, y * (1.0 / i), 1.0);
+    table[tid] = v;
+  }
+  __syncthreads();
   pdl_sync();
   const TreeSpan s = tree_span(a.cu, b, a.T, a.max_rows, a.status, tid == 0 && rank == 0);
   const long long out = static_cast<long long>(b) * a.steps;
   int count = 0;
   if (s.n > 0) {
-    for (int j = tid; j < s.n; j += DV_THREADS) {
-      up[j] = j ? a.parents[s.lo + j] : -1;
-      tok[j] = a.tokens[s.lo + j];
-      num[j] = a.uniforms[s.lo + j];
-    }
     const float given = a.temps ? a.temps[b] : static_cast<float>(a.temp);
-    const bool cold = a.greedy || !(given > 0.f);
-    const double temp = !(given > 0.f) ? 1.0 : a.temps ? static_cast<double>(given) : a.temp, c = LOG2E / temp, octave = 1.0 / c;
-    int turn = 0;
-    cluster_arrive();      // (all CTAs of the cluster run before one writes into another's memory)
-    cluster_wait();
+    const bool cold = a.greedy || !(given >= COLDEST);
+    const double temp = !(given >= COLDEST) ? 1.0 : a.temps ? static_cast<double>(given) : a.temp;
+    const Temperature tp{LOG2E / temp * 0x1p896, __double2float_rd(1000 * LN2 * temp), __double2float_rd(800 * LN2 * temp)};
+    const int groups_per = (a.V + 2 * VEC - 2) / VEC / W + 1;      // groups of a range, whatever the row's alignment
+    int turn = 0, node = 0;
+    bool started = false;
+    cluster_arrive();
 
-    auto exchange = [&](double m, double sum, double dm, double dsum, float peak, int at) {      // this warp's part to all CTAs
+    auto exchange = [&](double sum, double dsum, float m, float dm, float peak, int at) {      // this warp's part to all CTAs
       turn ^= 1;
+      if (!started) cluster_wait();      // (all CTAs of the cluster run before one writes into another's memory)
+      started = true;
       if (lane < static_cast<int>(ctas)) {
         Part* p = &parts[turn][me];
-        push_d(mapa_shared(smem_u32(&p->m), lane), m);
         push_d(mapa_shared(smem_u32(&p->sum), lane), sum);
-        if (DRAFT) {
-          push_d(mapa_shared(smem_u32(&p->dm), lane), dm);
-          push_d(mapa_shared(smem_u32(&p->dsum), lane), dsum);
-        }
-        push_d(mapa_shared(smem_u32(&p->peak), lane), __hiloint2double(at, __float_as_int(peak)));
+        if (DRAFT) push_d(mapa_shared(smem_u32(&p->dsum), lane), dsum);
+        push_d(mapa_shared(smem_u32(&p->m), lane), __hiloint2double(__float_as_int(dm), __float_as_int(m)));
+        if (cold) push_d(mapa_shared(smem_u32(&p->peak), lane), __hiloint2double(at, __float_as_int(peak)));
       }
       cluster_arrive();
       cluster_wait();
     };
 
-    int node = 0;
     while (true) {
       Row z{static_cast<const T*>(a.logits) + (s.lo + node) * a.ld, a.V, 0, true}, d{};
       z.shift = static_cast<int>(reinterpret_cast<uintptr_t>(z.p) % 16 / sizeof(T));
@@ -288,64 +343,85 @@ verify_kernel(const VerifyArgs a) {
         d = Row{static_cast<const T*>(a.draft) + (s.lo + node) * a.ld_draft, a.V, z.shift, false};
         d.vec = reinterpret_cast<uintptr_t>(d.p) % 16 / sizeof(T) == z.shift;
       }
-      const int groups = (a.V + z.shift + VEC - 1) / VEC, per = (groups + W - 1) / W, g0 = min(groups, me * per), g1 = min(groups, g0 + per);
-      for (int j = tid; j < s.n; j += DV_THREADS)
-        if (j > node && up[j] == node && tok[j] >= 0 && tok[j] < a.V) {
-          lz[j] = z.at(tok[j]);
-          if (DRAFT) ld[j] = d.at(tok[j]);
+      const int groups = (a.V + z.shift + VEC - 1) / VEC, g0 = min(groups, me * groups_per), g1 = min(groups, g0 + groups_per);
+      uint4 vz[LOADS], vd[DRAFT ? LOADS : 1];      // the groups of the next step
+      auto fetch = [&](int g) {
+        if (z.vec && (!DRAFT || d.vec) && g * VEC >= z.shift && g + STEP <= g1 && (g + STEP) * VEC - z.shift <= a.V) {      // all inside
+          const int e = (g + lane) * VEC - z.shift;
+#pragma unroll
+          for (int u = 0; u < LOADS; ++u) {
+            vz[u] = __ldg(reinterpret_cast<const uint4*>(z.p + e) + u * 32);
+            if (DRAFT) vd[u] = __ldg(reinterpret_cast<const uint4*>(d.p + e) + u * 32);
+          }
+          return;
         }
-      // the range's groups, LOADS of them a lane at a time, the next ones on their way
-      auto each = [&](auto&& fn) {
-        uint4 vz[LOADS], vd[DRAFT ? LOADS : 1];
-        auto fetch = [&](int g) {
 #pragma unroll
-          for (int u = 0; u < LOADS; ++u) {
-            vz[u] = z.load(g + u * 32 + lane, g1);
-            if (DRAFT) vd[u] = d.load(g + u * 32 + lane, g1);
-          }
-        };
-        fetch(g0);
-        for (int g = g0; g < g1; g += 32 * LOADS) {
-          uint4 wz[LOADS], wd[DRAFT ? LOADS : 1];
-#pragma unroll
-          for (int u = 0; u < LOADS; ++u) {
-            wz[u] = vz[u];
-            if (DRAFT) wd[u] = vd[u];
-          }
-          if (g + 32 * LOADS < g1) fetch(g + 32 * LOADS);
-          if (!fn(g, wz, wd)) break;
+        for (int u = 0; u < LOADS; ++u) {
+          vz[u] = z.load(g + u * 32 + lane, g1);
+          if (DRAFT) vd[u] = d.load(g + u * 32 + lane, g1);
         }
       };
+      if (g0 < g1) fetch(g0);
+      if (count == 0)
+        for (int j = tid; j < s.n; j += DV_THREADS) {
+          up[j] = j ? a.parents[s.lo + j] : -1;
+          tok[j] = a.tokens[s.lo + j];
+          num[j] = a.uniforms[s.lo + j];
+        }
+      const bool child = tid > node && tid < s.n && up[tid] == node && tok[tid] >= 0 && tok[tid] < a.V;
+      float own_z = 0.f, own_d = 0.f;
+      if (child) {
+        own_z = z.at(tok[tid]);
+        if (DRAFT) own_d = d.at(tok[tid]);
+      }
       // ---------------------------------------------------------------- the sums of the row
       float peak = -INFINITY;
       int at = 0x7fffffff;
+      Frame f, fd;
+      f.top = fd.top = -INFINITY;
+      float high = -INFINITY, dhigh = -INFINITY;
       double sum = 0.0, dsum = 0.0;
-      Scale sc, dsc;
-      sc.m = dsc.m = -INFINITY;
-      sc.high = dsc.high = -INFINITY;
-      auto add = [&](Scale& q, double& total, const uint4 (&v)[LOADS]) {
+      auto add = [&](Frame& q, float& high, double& total, const uint4 (&v)[LOADS]) {
         float top = -INFINITY;
 #pragma unroll
         for (int u = 0; u < LOADS; ++u)
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) top = fmaxf(top, Row::element(v[u], i));
-        if (__any_sync(0xffffffffu, top > q.high)) {      // the first numbers, or far larger ones
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const double before = q.m;
-          q.set(top, octave);
-          total = before == -INFINITY ? 0.0 : total * exp2((before - q.m) * c);
+          for (int i = 0; i < VEC; ++i) top = fmaxf(top, Row::raw(v[u], i));
+        if (__any_sync(0xffffffffu, top > high)) {      // the first numbers, or some 2^800 times as heavy ones: what was there is nothing beside them
+          top = fminf(warp_top(top), F_MAX);
+          if (top > q.top) {
+            q.set(top, tp);
+            total = 0.0;
+            high = fmaxf(__fadd_rd(top, tp.near), top);
+          }
         }
-        if (q.m == -INFINITY) return;
+        if (q.top == -INFINITY) return;
+        if (q.kind != 0 || high >= F_MAX) {      // (F_MAX: there may be +inf)
+#pragma unroll
+          for (int u = 0; u < LOADS; ++u) total += Row::seldom(v[u], q, table, tp.c);
+          return;
+        }
+        double even = 0.0, odd = 0.0;      // what is below `low`, and what is not a number, is taken as 2^-1000
 #pragma unroll
         for (int u = 0; u < LOADS; ++u)
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) total += q(table, c, Row::element(v[u], i));
+          for (int i = 0; i < VEC; i += 2) {
+            even += q.near(table, tp.c, fmaxf(Row::raw(v[u], i), q.low));
+            odd += q.near(table, tp.c, fmaxf(Row::raw(v[u], i + 1), q.low));
+          }
+        total += even + odd;
       };
-      each([&](int g, const uint4 (&wz)[LOADS], const uint4 (&wd)[DRAFT ? LOADS : 1]) {
-        add(sc, sum, wz);
+      for (int g = g0; g < g1; g += STEP) {
+        uint4 wz[LOADS], wd[LOADS];
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+          wz[u] = vz[u];
+          if (DRAFT) wd[u] = vd[DRAFT ? u : 0];
+        }
+        if (g + STEP < g1) fetch(g + STEP);
+        add(f, high, sum, wz);
         if (DRAFT) {
-          if (!cold) add(dsc, dsum, reinterpret_cast<const uint4(&)[LOADS]>(wd));
+          if (!cold) add(fd, dhigh, dsum, wd);
         }
         if (cold) {
 #pragma unroll
@@ -359,8 +435,7 @@ verify_kernel(const VerifyArgs a) {
               }
             }
         }
-        return true;
-      });
+      }
       sum = warp_sum_d(sum);
       if (DRAFT) dsum = warp_sum_d(dsum);
       if (cold) {
@@ -374,102 +449,92 @@ verify_kernel(const VerifyArgs a) {
           }
         }
       }
-      exchange(sc.m, sum, dsc.m, dsum, peak, at);
+      if (child) {
+        lz[tid] = own_z;
+        if (DRAFT) ld[tid] = own_d;
+      }
+      exchange(sum, dsum, f.top, fd.top, peak, at);
       // the first warp joins the parts: lane i has four of them, in their order
       if (warp == 0) {
-        const Part* got = parts[turn];
-        double mine[4], top = -INFINITY, dtop = -INFINITY, all = 0.0, dall = 0.0;
+        const Part* got = &parts[turn][lane * 4];
+        auto join = [&](Frame& whole, bool second, double& all, double (&mine)[4]) {
+          float m[4], top = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int w = lane * 4 + k;
-          if (w >= W) continue;
-          top = fmax(top, got[w].m);
-          if (DRAFT) dtop = fmax(dtop, got[w].dm);
-        }
+          for (int k = 0; k < 4; ++k) {
+            m[k] = lane * 4 + k < W ? (second ? got[k].dm : got[k].m) : -INFINITY;
+            top = fmaxf(top, m[k]);
+          }
+          whole.set(warp_top(top), tp);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-          if (DRAFT) dtop = fmax(dtop, __shfl_xor_sync(0xffffffffu, dtop, o));
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int w = lane * 4 + k;
-          mine[k] = w < W && got[w].m > -INFINITY ? got[w].sum * exp2((got[w].m - top) * c) : 0.0;
-          all += mine[k];
-          if (DRAFT) dall += w < W && got[w].dm > -INFINITY ? got[w].dsum * exp2((got[w].dm - dtop) * c) : 0.0;
-        }
-        all = warp_sum_d(all);
-        if (DRAFT) dall = warp_sum_d(dall);
-        const double inv = top > -INFINITY ? 1.0 / all : 0.0;
+          for (int k = 0; k < 4; ++k) {
+            Frame one;
+            one.set(m[k], tp);
+            const double w = one.over(whole);
+            mine[k] = w > 0.0 ? w * (second ? got[k].dsum : got[k].sum) : 0.0;
+          }
+          all = warp_sum_d((mine[0] + mine[1]) + (mine[2] + mine[3]));
+        };
+        Frame p, q;
+        double mine[4], all, dall = 0.0;
+        if (DRAFT) join(q, true, dall, mine);
+        join(p, false, all, mine);
+        const double inv = p.top > -INFINITY ? 1.0 / all : 0.0;
 #pragma unroll
         for (int k = 0; k < 4; ++k) share[lane * 4 + k] = mine[k] * inv;
         if (lane == 0) {
-          row_top = top;
-          row_sum = all;
-          row_inv = inv;
+          row.p = p;
+          row.inv = inv;
+          row.sum = all;
           if (DRAFT) {
-            draft_top = dtop;
-            draft_inv = dtop > -INFINITY ? 1.0 / dall : 0.0;
+            row.q = q;
+            row.dinv = q.top > -INFINITY && !cold ? 1.0 / dall : 0.0;
           }
-          int best = 0x7fffffff;
           if (cold) {
             float x = -INFINITY;
+            row.best = 0;
             for (int w = 0; w < W; ++w)
-              if (got[w].peak > x) {      // (parts lie in the tokens' order)
-                x = got[w].peak;
-                best = got[w].at;
+              if (parts[turn][w].peak > x) {      // (parts lie in the tokens' order)
+                x = parts[turn][w].peak;
+                row.best = parts[turn][w].at;
               }
           }
-          row_best = best;
-          left[0] = 1.0;
+          left[0] = grow[0] = 1.0;
           tried = node;
           turned_down = 0;
         }
+        __syncwarp();
       }
-      __syncthreads();
-      const double top = row_top, inv = row_inv, dinv = DRAFT ? draft_inv : 0.0;
-      const bool some = top > -INFINITY;      // a row without a number above -inf has no probabilities
-      Scale p, q;      // of the whole row
-      p.set(static_cast<float>(some ? top : 0.0), octave);
-      if (DRAFT) q.set(static_cast<float>(dinv > 0.0 ? draft_top : 0.0), octave);
       // what is left of the probability of a token after `r` rejections, from its logits
-      int rejected = 0;
       auto rest = [&](int i, float x, float y, int r) {
-        double w = p(table, c, x) * inv;
+        double w = row.p(table, tp.c, x) * row.inv;
         if (DRAFT) {
           if (r > 0) {
-            const double g = q(table, c, y) * dinv;
-            for (int k = 0; k < r; ++k) w = fmax(w / left[k] - g, 0.0);
+            const double g = row.q(table, tp.c, y) * row.dinv;
+            for (int k = 0; k < r; ++k) w = fmax(w * grow[k] - g, 0.0);
           }
         } else {
           for (int k = 0; k < r; ++k) w = gone[k] == i ? 0.0 : w;
         }
         return w;
       };
-      auto sum_rest = [&](int r) {      // over this warp's range
+      auto sum_rest = [&](int g0, int g1, int r) {
         double v = 0.0;
-        each([&](int g, const uint4 (&wz)[LOADS], const uint4 (&wd)[DRAFT ? LOADS : 1]) {
+        for (int g = g0; g < g1; g += 32) {
+          const uint4 x = z.load(g + lane, g1), y = DRAFT ? d.load(g + lane, g1) : x;
 #pragma unroll
-          for (int u = 0; u < LOADS; ++u)
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) v += rest((g + u * 32 + lane) * VEC - z.shift + i, Row::element(wz[u], i), DRAFT ? Row::element(wd[DRAFT ? u : 0], i) : 0.f, r);
-          return true;
-        });
+          for (int i = 0; i < VEC; ++i) v += rest((g + lane) * VEC - z.shift + i, Row::element(x, i), Row::element(y, i), r);
+        }
         return warp_sum_d(v);
       };
       double mine[4], total = 0.0;
       auto take = [&](double v) {      // this warp's part of new sums; the parts and the whole sum of all
-        exchange(0.0, v, 0.0, 0.0, 0.f, 0);
-        total = 0.0;
+        exchange(v, 0.0, 0.f, 0.f, 0.f, 0);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          mine[k] = lane * 4 + k < W ? parts[turn][lane * 4 + k].sum : 0.0;
-          total += mine[k];
-        }
-        total = warp_sum_d(total);
+        for (int k = 0; k < 4; ++k) mine[k] = lane * 4 + k < W ? parts[turn][lane * 4 + k].sum : 0.0;
+        total = warp_sum_d((mine[0] + mine[1]) + (mine[2] + mine[3]));
       };
       // ---------------------------------------------------------------- the children
-      int next = -1;
+      int next = -1, rejected = 0;
       while (true) {
         if (tid == 0) {      // verdict: an accepted row, -1 none, -2 one rejected after which the sums are taken again
           int v = -1, j = tried + 1, r = rejected;
@@ -477,12 +542,12 @@ verify_kernel(const VerifyArgs a) {
             if (up[j] != node) continue;
             const int t = tok[j];
             if (cold) {
-              if (some && t == row_best) v = j;
+              if (row.inv > 0.0 && t == row.best) v = j;
               continue;
             }
             if (t < 0 || t >= a.V) continue;      // has no probability, and is none of the draft's
             const double w = rest(t, lz[j], DRAFT ? ld[j] : 0.f, r);
-            const double g = DRAFT ? q(table, c, ld[j]) * dinv : 1.0;
+            const double g = DRAFT ? row.q(table, tp.c, ld[j]) * row.dinv : 1.0;
             if (static_cast<double>(num[j]) * g * left[r] < w) {
               v = j;
             } else if (DRAFT) {
@@ -505,50 +570,64 @@ verify_kernel(const VerifyArgs a) {
           break;
         }
         ++rejected;
-        take(sum_rest(rejected));
-        if (tid == 0) left[rejected] = total;
+        take(sum_rest(g0, g1, rejected));
+        if (tid == 0) {
+          left[rejected] = total;
+          grow[rejected] = 1.0 / total;
+        }
         __syncthreads();
         if (!(total > 0.0)) break;
       }
       // ---------------------------------------------------------------- the token
-      const auto logprob = [&](float x) { return some ? static_cast<float>((static_cast<double>(x) - top) / temp - log(row_sum)) : -INFINITY; };
+      const bool some = row.inv > 0.0;      // a row without a number above -inf has no probabilities
+      auto depth = [&](float x) { return row.p.kind == 2 ? 0.0 : fma(lowered(x), tp.c, row.p.add - MAGIC); };      // l c - N
       if (rank == 0 && tid == 0) a.out_rows[out + count] = node;
       if (next >= 0) {
         if (rank == 0 && tid == 0) {
           a.out_tokens[out + count] = tok[next];
-          a.out_logprobs[out + count] = logprob(lz[next]);
+          chosen[count] = depth(lz[next]);
+          sums[count] = row.sum;
         }
         ++count;
         node = next;
-        __syncthreads();      // (the rejections of this row have been read)
+        __syncthreads();      // (this row's numbers have been read)
         continue;
       }
+      auto put = [&](int t, float x) {
+        a.out_tokens[out + count] = t;
+        a.out_logprobs[out + count] = some ? static_cast<float>((depth(x) - log2_of(table, row.sum)) * LN2) : -INFINITY;
+      };
       if (cold || !some) {
-        if (rank == 0 && tid == 0) {
-          const int t = some ? row_best : 0;
-          a.out_tokens[out + count] = t;
-          a.out_logprobs[out + count] = logprob(some ? z.at(t) : 0.f);
-        }
+        if (rank == 0 && tid == 0) put(some ? row.best : 0, some ? z.at(row.best) : 0.f);
         ++count;
         break;
       }
       if (!DRAFT && rejected > 0) {      // without the rejected tokens
-        bool hit = false;
-        for (int k = 0; k < rejected; ++k) {
-          const int g = (gone[k] + z.shift) / VEC;
-          hit |= g >= g0 && g < g1;
+        if (left[rejected] >= 1.0 / 1024) {      // their weights are taken off their ranges' sums, of which no more than ten bits are lost
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mine[k] = share[lane * 4 + k];
+          for (int r = 0; r < rejected; ++r) {
+            const int w = (gone[r] + z.shift) / VEC / groups_per;
+            const double off = left[r] - left[r + 1];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (w == lane * 4 + k) mine[k] = fmax(mine[k] - off, 0.0);
+          }
+          total = warp_sum_d((mine[0] + mine[1]) + (mine[2] + mine[3]));
+        } else {
+          bool hit = false;
+          for (int k = 0; k < rejected; ++k) {
+            const int g = (gone[k] + z.shift) / VEC;
+            hit |= g >= g0 && g < g1;
+          }
+          take(hit ? sum_rest(g0, g1, rejected) : share[me]);
         }
-        take(hit ? sum_rest(rejected) : share[me]);
       }
       if (rejected == 0 || !(total > 0.0)) {      // (nothing is left: from p itself)
         rejected = 0;
-        total = 0.0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          mine[k] = share[lane * 4 + k];
-          total += mine[k];
-        }
-        total = warp_sum_d(total);
+        for (int k = 0; k < 4; ++k) mine[k] = share[lane * 4 + k];
+        total = warp_sum_d((mine[0] + mine[1]) + (mine[2] + mine[3]));
       }
       const double aim = static_cast<double>(num[0]) * total;
       double run = (mine[0] + mine[1]) + (mine[2] + mine[3]);
@@ -578,19 +657,36 @@ verify_kernel(const VerifyArgs a) {
         start = __shfl_sync(0xffffffffu, start, l);
       } else {      // a number of 1 and more, or none: the last token that has a share
         owner = __shfl_sync(0xffffffffu, last, 31 - __clz(any));
-        start = 0.0;
       }
-      if (me == owner) {
-        int hit = -1, end = 0;
-        each([&](int g, const uint4 (&wz)[LOADS], const uint4 (&wd)[DRAFT ? LOADS : 1]) {
-#pragma unroll 1
-          for (int u = 0; u < LOADS; ++u) {
-            const int e = (g + u * 32 + lane) * VEC - z.shift;
-            const uint4 x = wz[u], y = wd[DRAFT ? u : 0];
+      if (rank == owner / DV_WARPS) {      // the range once more, by all warps of its CTA
+        const int r0 = min(groups, owner * groups_per), r1 = min(groups, r0 + groups_per), piece = (r1 - r0 + DV_WARPS - 1) / DV_WARPS;
+        const int q0 = min(r1, r0 + warp * piece), q1 = min(r1, q0 + piece);
+        const double own = sum_rest(q0, q1, rejected);
+        if (lane == 0) pieces[warp] = own;
+        __syncthreads();
+        int mover = -1, filled = -1;
+        double from = start;
+        for (int w = 0; w < DV_WARPS; ++w) {
+          const double v = pieces[w];
+          if (v > 0.0) {
+            filled = w;
+            if (mover < 0 && over && from + v > aim) {
+              mover = w;
+              start = from;
+            }
+          }
+          from += v;
+        }
+        const bool inside = mover >= 0;      // (otherwise the last that has a share)
+        if (warp == (inside ? mover : filled)) {
+          int hit = -1, end = 0;
+          for (int g = q0; g < q1 && hit < 0; g += 32) {
+            const int e = (g + lane) * VEC - z.shift;
+            const uint4 x = z.load(g + lane, q1), y = DRAFT ? d.load(g + lane, q1) : x;
             double w[VEC], own = 0.0;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-              w[i] = rest(e + i, Row::element(x, i), DRAFT ? Row::element(y, i) : 0.f, rejected);
+              w[i] = rest(e + i, Row::element(x, i), Row::element(y, i), rejected);
               own += w[i];
             }
             double sofar = own;
@@ -608,23 +704,16 @@ verify_kernel(const VerifyArgs a) {
               at_lane += w[i];
               if (w[i] > 0.0) {
                 has = e + i;
-                if (pass < 0 && over && at_lane > aim) pass = e + i;
+                if (pass < 0 && inside && at_lane > aim) pass = e + i;
               }
             }
             const unsigned passed = __ballot_sync(0xffffffffu, pass >= 0), there = __ballot_sync(0xffffffffu, has >= 0);
             if (there) end = __shfl_sync(0xffffffffu, has, 31 - __clz(there));
-            if (passed) {
-              hit = __shfl_sync(0xffffffffu, pass, __ffs(passed) - 1);
-              return false;
-            }
+            if (passed) hit = __shfl_sync(0xffffffffu, pass, __ffs(passed) - 1);
             start += __shfl_sync(0xffffffffu, sofar, 31);
           }
-          return true;
-        });
-        if (hit < 0) hit = end;
-        if (lane == 0) {
-          a.out_tokens[out + count] = hit;
-          a.out_logprobs[out + count] = logprob(z.at(hit));
+          if (hit < 0) hit = end;
+          if (lane == 0) put(hit, z.at(hit));
         }
       }
       ++count;
@@ -633,6 +722,8 @@ verify_kernel(const VerifyArgs a) {
   }
   if (rank == 0) {
     if (tid == 0) a.out_counts[b] = count;
+    __syncthreads();
+    for (int i = tid; i < count - 1; i += DV_THREADS) a.out_logprobs[out + i] = static_cast<float>((chosen[i] - log2_of(table, sums[i])) * LN2);
     for (int i = count + tid; i < a.steps; i += DV_THREADS) {
       a.out_tokens[out + i] = -1;
       a.out_rows[out + i] = -1;

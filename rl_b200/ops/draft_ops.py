@@ -35,6 +35,7 @@ _L.register("rlb_tree_decode", [_P, _LL, _P, _P, _I, _I, _P, _LL, _I, _P, _P, _I
 BF16 = torch.bfloat16
 HEAD_DIMS = (64, 128)
 MAX_ROWS = 256
+COLDEST = torch.finfo(torch.float32).tiny
 MAX_TOKENS = 0x7FFF0000      # of a sequence: places are 32-bit numbers
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else lambda index: torch.cuda.current_stream(index).cuda_stream
 
@@ -253,8 +254,8 @@ def _verify_ref(logits, tokens, parents, spans, uniforms, draft, temps, greedy, 
     got_tokens, got_counts, got_rows, got_logprobs = out
     V = logits.shape[1]
     for b, (lo, n) in enumerate(spans):
-        cold = greedy or not temps[b] > 0
-        temp = temps[b] if temps[b] > 0 else 1.0
+        warm = torch.tensor(temps[b], dtype=torch.float32) >= COLDEST
+        cold, temp = greedy or not warm, temps[b] if warm else 1.0
         node, step = 0, 0
         while n:
             p, logp = _weights(logits[lo + node], temp)
@@ -308,7 +309,7 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Ten
                   max_steps: Optional[int] = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """Accepts drafted tokens so that what is kept is distributed as the target's own samples. ``logits`` [T, V] (bf16 or fp32) of every row's next token, ``tokens`` [T] int32
     the rows' own tokens, ``uniforms`` [T] fp32 in [0, 1): a drafted row's number decides on it, row 0's draws the last token. ``temperature``, ``temps`` [B] fp32 and
-    ``greedy`` as in :func:`rl_b200.ops.engine_ops.sample`.
+    ``greedy`` as in :func:`rl_b200.ops.engine_ops.sample` (temperatures below 2^-126 are greedy too).
 
     From row 0 on, with p the target's probabilities at the node and w = p, Z = 1: the node's children are tried in order of their rows. Child c with token x and number u is
     accepted if u Z q(x) < w(x), and is the next node. Otherwise, with ``draft_logits`` [T, V] (the logits, at the same temperature, that a row's children were drawn from,
