@@ -165,6 +165,11 @@ __device__ __forceinline__ double warp_sum_d(double v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {      // of those that are numbers
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ float warp_top(float x) {      // largest of the warp's numbers, none of them NaN
   const int u = __float_as_int(x), m = __reduce_max_sync(0xffffffffu, u < 0 ? u ^ 0x7fffffff : u);
   return __int_as_float(m < 0 ? m ^ 0x7fffffff : m);
@@ -178,8 +183,8 @@ __device__ __forceinline__ double lowered(float x) {
 __device__ __forceinline__ double power(const double* table, double t, double r) {
   const int k = __double2loint(t);
   const double p = r * (LN2 + r * (LN2 * LN2 / 2 + r * (LN2 * LN2 * LN2 / 6)));
-  const double f = table[k & (EXP_STEPS - 1)];
-  const double s = __hiloint2double(__double2hiint(f) + (k & ~(EXP_STEPS - 1)) * (0x100000 / EXP_STEPS), __double2loint(f));
+  const double f = table[k & (EXP_STEPS - 1)];      // without what its index adds to the exponent below
+  const double s = __hiloint2double(__double2hiint(f) + k * (0x100000 / EXP_STEPS), __double2loint(f));
   return fma(s, p, s);
 }
 // log2 of a sum: 32 bits, then one step on 2^-l s = 1 + d.
@@ -192,9 +197,9 @@ __device__ __forceinline__ double log2_of(const double* table, double s) {
 
 struct Temperature {
   double c;            // log2(e) / T * 2^896
-  float far, near;     // differences of logits that make 2^1000 (rounded down) and 2^800
+  float far, near;     // differences of logits that make 2^1000 and 2^60, rounded down
 };
-// Weights relative to 2^N, N = rint(top c).
+// Weights relative to 2^N, N = rint(top c). A logit that is less than 2^-1000 of the row's largest weighs nothing.
 struct Frame {
   double add;          // MAGIC - N
   float top, low;      // logits below `low` weigh nothing (2^-1000 of top's)
@@ -206,6 +211,18 @@ struct Frame {
     add = MAGIC - n;
     kind = !(fabs(m) < 0x1p42) ? 2 : low >= x || low <= -F_MAX ? 1 : 0;
   }
+  // `v` in a frame with a larger N
+  static __device__ __forceinline__ double moved(double v, double add, double larger) {
+    const double d = larger - add;
+    return static_cast<uint32_t>(__double2hiint(d)) <= 0xc090e000u ? v * __hiloint2double((1123 + __double2loint(d + 256 * MAGIC)) << 20, 0) * 0x1p-100 : 0.0;      // (-1080)
+  }
+  __device__ __forceinline__ void move(float x, const Temperature& q, double& total) {
+    const double before = add;
+    const bool first = top == -INFINITY;
+    set(x, q);
+    total = first ? 0.0 : moved(total, before, add);
+  }
+  __device__ __forceinline__ double depth(double c, float x) const { return kind == 2 ? 0.0 : fma(lowered(x), c, add - MAGIC); }      // x c - N
   __device__ __forceinline__ double near(const double* table, double c, float x) const {
     const double v = lowered(x), t = fma(v, c, add);
     return power(table, t, fma(v, c, add - t));
@@ -213,22 +230,14 @@ struct Frame {
   __device__ __forceinline__ double operator()(const double* table, double c, float x) const {
     return !(x >= low) ? 0.0 : kind == 2 ? (x == top ? 1.0 : 0.0) : near(table, c, x);
   }
-  // 2^(N - N') of another frame, of whose top less than 2^-1000 of this one's counts as nothing
-  __device__ __forceinline__ double over(const Frame& o) const {
-    if (top == -INFINITY) return 0.0;
-    if (o.kind == 2 || kind == 2) return top == o.top ? 1.0 : 0.0;
-    const double d = o.add - add;
-    return d < -1000.0 ? 0.0 : __hiloint2double((1023 + __double2loint(d + 256 * MAGIC)) << 20, 0);
-  }
 };
 
 __device__ __forceinline__ void push_d(uint32_t addr, double v) { asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory"); }
 
-struct Part {      // of a warp's range: sums of weights relative to the frames of m and dm (-inf: none)
-  double sum, dsum;
-  float m, dm;
-  float peak;
-  int at;
+struct Part {      // of a warp's range, target and draft: sum of weights in its frame, the frame's MAGIC - N and logit (-inf: none)
+  double sum, add;
+  float m, peak;   // the range's largest logit
+  int at, none;    // and its place, where that is asked for
 };
 
 template <typename T>
@@ -275,10 +284,9 @@ struct RowLogits {
   __device__ __forceinline__ float at(int i) const { return usable(static_cast<float>(p[i])); }
 };
 
-struct RowSum {      // what the first warp makes of the parts
-  Frame p, q;
-  double inv, dinv, sum;      // reciprocals of the sums (0: no logit above -inf), the sum
-  int best;
+struct RowSum {      // of all parts
+  Frame f;
+  double inv, sum;      // the sum's reciprocal (0: no logit above -inf)
 };
 
 template <typename T, bool DRAFT>
@@ -287,9 +295,10 @@ verify_kernel(const VerifyArgs a) {
   using Row = RowLogits<T>;
   constexpr int VEC = Row::VEC, LOADS = Row::LOADS, STEP = 32 * LOADS;
   __shared__ double table[EXP_STEPS];
-  __shared__ Part parts[2][DV_PARTS];      // of all warps of the cluster, by turns
+  __shared__ Part parts[2][1 + DRAFT][DV_PARTS];      // of all warps of the cluster, by turns
   __shared__ double share[DV_PARTS], pieces[DV_WARPS];      // the ranges' probabilities; sums of a range's pieces
-  __shared__ RowSum row;
+  __shared__ RowSum row[1 + DRAFT];
+  __shared__ int row_best;
   __shared__ int up[DR_ROWS], tok[DR_ROWS], gone[DR_ROWS];
   __shared__ float num[DR_ROWS], lz[DR_ROWS], ld[DR_ROWS];      // numbers, logits of the children's tokens in their parent's rows
   __shared__ double left[DR_ROWS + 1], grow[DR_ROWS + 1];       // what is left to be given after so many rejections, and its reciprocal
@@ -304,34 +313,41 @@ verify_kernel(const VerifyArgs a) {
     double v = 1.0;
 #pragma unroll
     for (int i = 17; i > 0; --i) v = fma(v, y * (1.0 / i), 1.0);
-    table[tid] = v;
+    table[tid] = __hiloint2double(__double2hiint(v) - tid * (0x100000 / EXP_STEPS), __double2loint(v));
   }
   __syncthreads();
   pdl_sync();
   const TreeSpan s = tree_span(a.cu, b, a.T, a.max_rows, a.status, tid == 0 && rank == 0);
   const long long out = static_cast<long long>(b) * a.steps;
-  int count = 0;
+  int count = 0, drawn = -1;      // the last token, of the thread that has it
+  float drawn_z = 0.f;
+  double depth_c = 0.0;
   if (s.n > 0) {
     const float given = a.temps ? a.temps[b] : static_cast<float>(a.temp);
     const bool cold = a.greedy || !(given >= COLDEST);
     const double temp = !(given >= COLDEST) ? 1.0 : a.temps ? static_cast<double>(given) : a.temp;
-    const Temperature tp{LOG2E / temp * 0x1p896, __double2float_rd(1000 * LN2 * temp), __double2float_rd(800 * LN2 * temp)};
+    const Temperature tp{LOG2E / temp * 0x1p896, __double2float_rd(1000 * LN2 * temp), __double2float_rd(60 * LN2 * temp)};
     const int groups_per = (a.V + 2 * VEC - 2) / VEC / W + 1;      // groups of a range, whatever the row's alignment
+    depth_c = tp.c;
     int turn = 0, node = 0;
     bool started = false;
     cluster_arrive();
 
-    auto exchange = [&](double sum, double dsum, float m, float dm, float peak, int at) {      // this warp's part to all CTAs
+    auto begin = [&]() {
       turn ^= 1;
       if (!started) cluster_wait();      // (all CTAs of the cluster run before one writes into another's memory)
       started = true;
+    };
+    auto push = [&](int which, double sum, double add, float m, int at, float peak) {      // this warp's part to all CTAs
       if (lane < static_cast<int>(ctas)) {
-        Part* p = &parts[turn][me];
-        push_d(mapa_shared(smem_u32(&p->sum), lane), sum);
-        if (DRAFT) push_d(mapa_shared(smem_u32(&p->dsum), lane), dsum);
-        push_d(mapa_shared(smem_u32(&p->m), lane), __hiloint2double(__float_as_int(dm), __float_as_int(m)));
-        if (cold) push_d(mapa_shared(smem_u32(&p->peak), lane), __hiloint2double(at, __float_as_int(peak)));
+        const uint32_t p = mapa_shared(smem_u32(&parts[turn][which][me]), lane);
+        push_d(p, sum);
+        push_d(p + 8, add);
+        push_d(p + 16, __hiloint2double(__float_as_int(peak), __float_as_int(m)));
+        if (cold) push_d(p + 24, __hiloint2double(0, at));
       }
+    };
+    auto end = [&]() {
       cluster_arrive();
       cluster_wait();
     };
@@ -345,7 +361,7 @@ verify_kernel(const VerifyArgs a) {
       }
       const int groups = (a.V + z.shift + VEC - 1) / VEC, g0 = min(groups, me * groups_per), g1 = min(groups, g0 + groups_per);
       uint4 vz[LOADS], vd[DRAFT ? LOADS : 1];      // the groups of the next step
-      auto fetch = [&](int g) {
+      auto fetch = [&](int g, int g1) {
         if (z.vec && (!DRAFT || d.vec) && g * VEC >= z.shift && g + STEP <= g1 && (g + STEP) * VEC - z.shift <= a.V) {      // all inside
           const int e = (g + lane) * VEC - z.shift;
 #pragma unroll
@@ -361,7 +377,7 @@ verify_kernel(const VerifyArgs a) {
           if (DRAFT) vd[u] = d.load(g + u * 32 + lane, g1);
         }
       };
-      if (g0 < g1) fetch(g0);
+      if (g0 < g1) fetch(g0, g1);
       if (count == 0)
         for (int j = tid; j < s.n; j += DV_THREADS) {
           up[j] = j ? a.parents[s.lo + j] : -1;
@@ -375,23 +391,23 @@ verify_kernel(const VerifyArgs a) {
         if (DRAFT) own_d = d.at(tok[tid]);
       }
       // ---------------------------------------------------------------- the sums of the row
-      float peak = -INFINITY;
+      float peak = -INFINITY;      // the largest that a lane has met first
       int at = 0x7fffffff;
       Frame f, fd;
       f.top = fd.top = -INFINITY;
-      float high = -INFINITY, dhigh = -INFINITY;
+      float high = -INFINITY, dhigh = -INFINITY, most = -INFINITY, dmost = -INFINITY;
       double sum = 0.0, dsum = 0.0;
-      auto add = [&](Frame& q, float& high, double& total, const uint4 (&v)[LOADS]) {
+      auto add = [&](Frame& q, float& high, float& most, double& total, const uint4 (&v)[LOADS]) {
         float top = -INFINITY;
 #pragma unroll
         for (int u = 0; u < LOADS; ++u)
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) top = fmaxf(top, Row::raw(v[u], i));
-        if (__any_sync(0xffffffffu, top > high)) {      // the first numbers, or some 2^800 times as heavy ones: what was there is nothing beside them
+          for (int i = 0; i < VEC; i += 2) top = max3(top, Row::raw(v[u], i), Row::raw(v[u], i + 1));
+        most = fmaxf(most, top);
+        if (__any_sync(0xffffffffu, top > high)) {      // the first numbers, or some that weigh 2^60 and more
           top = fminf(warp_top(top), F_MAX);
           if (top > q.top) {
-            q.set(top, tp);
-            total = 0.0;
+            q.move(top, tp, total);
             high = fmaxf(__fadd_rd(top, tp.near), top);
           }
         }
@@ -418,10 +434,10 @@ verify_kernel(const VerifyArgs a) {
           wz[u] = vz[u];
           if (DRAFT) wd[u] = vd[DRAFT ? u : 0];
         }
-        if (g + STEP < g1) fetch(g + STEP);
-        add(f, high, sum, wz);
+        if (g + STEP < g1) fetch(g + STEP, g1);
+        add(f, high, most, sum, wz);
         if (DRAFT) {
-          if (!cold) add(fd, dhigh, dsum, wd);
+          if (!cold) add(fd, dhigh, dmost, dsum, wd);
         }
         if (cold) {
 #pragma unroll
@@ -453,84 +469,117 @@ verify_kernel(const VerifyArgs a) {
         lz[tid] = own_z;
         if (DRAFT) ld[tid] = own_d;
       }
-      exchange(sum, dsum, f.top, fd.top, peak, at);
-      // the first warp joins the parts: lane i has four of them, in their order
-      if (warp == 0) {
-        const Part* got = &parts[turn][lane * 4];
-        auto join = [&](Frame& whole, bool second, double& all, double (&mine)[4]) {
-          float m[4], top = -INFINITY;
+      begin();
+      push(0, sum, f.add, f.top, at, fminf(warp_top(most), F_MAX));
+      if (DRAFT) push(1, dsum, fd.add, fd.top, 0, fminf(warp_top(dmost), F_MAX));
+      end();
+      // a warp joins the target's parts, another the draft's: lane i has four of them, in their order
+      if (warp < 1 + DRAFT) {
+        const Part* got = &parts[turn][warp][lane * 4];
+        RowSum& to = row[warp];
+        float m[4], top = -INFINITY;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            m[k] = lane * 4 + k < W ? (second ? got[k].dm : got[k].m) : -INFINITY;
-            top = fmaxf(top, m[k]);
-          }
-          whole.set(warp_top(top), tp);
+        for (int k = 0; k < 4; ++k) {
+          m[k] = lane * 4 + k < W ? got[k].peak : -INFINITY;
+          top = fmaxf(top, m[k]);
+        }
+        Frame whole;
+        whole.set(warp_top(top), tp);
+        double v[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            Frame one;
-            one.set(m[k], tp);
-            const double w = one.over(whole);
-            mine[k] = w > 0.0 ? w * (second ? got[k].dsum : got[k].sum) : 0.0;
-          }
-          all = warp_sum_d((mine[0] + mine[1]) + (mine[2] + mine[3]));
-        };
-        Frame p, q;
-        double mine[4], all, dall = 0.0;
-        if (DRAFT) join(q, true, dall, mine);
-        join(p, false, all, mine);
-        const double inv = p.top > -INFINITY ? 1.0 / all : 0.0;
+        for (int k = 0; k < 4; ++k) {      // of rows with one logit far above the others the parts that have it
+          v[k] = !(m[k] >= whole.low) ? 0.0 : whole.kind == 2 ? (m[k] == whole.top ? got[k].sum : 0.0) : Frame::moved(got[k].sum, got[k].add, whole.add);
+        }
+        const double all = warp_sum_d((v[0] + v[1]) + (v[2] + v[3])), inv = whole.top > -INFINITY && !(cold && warp) ? 1.0 / all : 0.0;
+        if (warp == 0)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) share[lane * 4 + k] = mine[k] * inv;
+          for (int k = 0; k < 4; ++k) share[lane * 4 + k] = v[k] * inv;
         if (lane == 0) {
-          row.p = p;
-          row.inv = inv;
-          row.sum = all;
-          if (DRAFT) {
-            row.q = q;
-            row.dinv = q.top > -INFINITY && !cold ? 1.0 / dall : 0.0;
+          to.f = whole;
+          to.inv = inv;
+          to.sum = all;
+          if (warp == 0) {
+            if (cold) {
+              float x = -INFINITY;
+              row_best = 0;
+              for (int w = 0; w < W; ++w)
+                if (parts[turn][0][w].peak > x) {      // (parts lie in the tokens' order)
+                  x = parts[turn][0][w].peak;
+                  row_best = parts[turn][0][w].at;
+                }
+            }
+            left[0] = grow[0] = 1.0;
+            tried = node;
+            turned_down = 0;
           }
-          if (cold) {
-            float x = -INFINITY;
-            row.best = 0;
-            for (int w = 0; w < W; ++w)
-              if (parts[turn][w].peak > x) {      // (parts lie in the tokens' order)
-                x = parts[turn][w].peak;
-                row.best = parts[turn][w].at;
-              }
-          }
-          left[0] = grow[0] = 1.0;
-          tried = node;
-          turned_down = 0;
         }
         __syncwarp();
       }
+      if (DRAFT) __syncthreads();
       // what is left of the probability of a token after `r` rejections, from its logits
       auto rest = [&](int i, float x, float y, int r) {
-        double w = row.p(table, tp.c, x) * row.inv;
+        double w = row[0].f(table, tp.c, x) * row[0].inv;
         if (DRAFT) {
           if (r > 0) {
-            const double g = row.q(table, tp.c, y) * row.dinv;
-            for (int k = 0; k < r; ++k) w = fmax(w * grow[k] - g, 0.0);
+            const double g = row[DRAFT].f(table, tp.c, y) * row[DRAFT].inv;
+            for (int k = 0; k < r; ++k) w = fmax(fma(w, grow[k], -g), 0.0);
           }
         } else {
           for (int k = 0; k < r; ++k) w = gone[k] == i ? 0.0 : w;
         }
         return w;
       };
+      const bool simple = DRAFT && row[0].f.kind == 0 && row[DRAFT].f.kind == 0 && row[0].f.top < 0.5f * F_MAX && row[DRAFT].f.top < 0.5f * F_MAX;
       auto sum_rest = [&](int g0, int g1, int r) {
         double v = 0.0;
-        for (int g = g0; g < g1; g += 32) {
-          const uint4 x = z.load(g + lane, g1), y = DRAFT ? d.load(g + lane, g1) : x;
+        if (simple) {      // as in the row's own sums
+          const Frame p = row[0].f, q = row[DRAFT].f;
+          const double inv = row[0].inv, dinv = row[DRAFT].inv;
+          if (g0 < g1) fetch(g0, g1);
+          for (int g = g0; g < g1; g += STEP) {
+            uint4 wz[LOADS], wd[LOADS];
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) v += rest((g + lane) * VEC - z.shift + i, Row::element(x, i), Row::element(y, i), r);
+            for (int u = 0; u < LOADS; ++u) {
+              wz[u] = vz[u];
+              wd[u] = vd[DRAFT ? u : 0];
+            }
+            if (g + STEP < g1) fetch(g + STEP, g1);
+#pragma unroll
+            for (int u = 0; u < LOADS; ++u)
+#pragma unroll
+              for (int i = 0; i < VEC; ++i) {
+                double w = p.near(table, tp.c, fmaxf(Row::raw(wz[u], i), p.low)) * inv;
+                const double e = q.near(table, tp.c, fmaxf(Row::raw(wd[u], i), q.low)) * dinv;
+                for (int k = 0; k < r; ++k) w = fmax(fma(w, grow[k], -e), 0.0);
+                v += w;
+              }
+          }
+          return warp_sum_d(v);
+        }
+        uint4 x = z.load(g0 + lane, g1), y = DRAFT ? d.load(g0 + lane, g1) : x;
+        for (int g = g0; g < g1; g += 32) {
+          const uint4 xx = x, yy = y;
+          if (g + 32 < g1) {
+            x = z.load(g + 32 + lane, g1);
+            y = DRAFT ? d.load(g + 32 + lane, g1) : x;
+          }
+          double even = 0.0, odd = 0.0;
+#pragma unroll
+          for (int i = 0; i < VEC; i += 2) {
+            even += rest((g + lane) * VEC - z.shift + i, Row::element(xx, i), Row::element(yy, i), r);
+            odd += rest((g + lane) * VEC - z.shift + i + 1, Row::element(xx, i + 1), Row::element(yy, i + 1), r);
+          }
+          v += even + odd;
         }
         return warp_sum_d(v);
       };
       double mine[4], total = 0.0;
       auto take = [&](double v) {      // this warp's part of new sums; the parts and the whole sum of all
-        exchange(v, 0.0, 0.f, 0.f, 0.f, 0);
+        begin();
+        push(0, v, 0.0, 0.f, 0, 0.f);
+        end();
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mine[k] = lane * 4 + k < W ? parts[turn][lane * 4 + k].sum : 0.0;
+        for (int k = 0; k < 4; ++k) mine[k] = lane * 4 + k < W ? parts[turn][0][lane * 4 + k].sum : 0.0;
         total = warp_sum_d((mine[0] + mine[1]) + (mine[2] + mine[3]));
       };
       // ---------------------------------------------------------------- the children
@@ -542,12 +591,12 @@ verify_kernel(const VerifyArgs a) {
             if (up[j] != node) continue;
             const int t = tok[j];
             if (cold) {
-              if (row.inv > 0.0 && t == row.best) v = j;
+              if (row[0].inv > 0.0 && t == row_best) v = j;
               continue;
             }
             if (t < 0 || t >= a.V) continue;      // has no probability, and is none of the draft's
             const double w = rest(t, lz[j], DRAFT ? ld[j] : 0.f, r);
-            const double g = DRAFT ? row.q(table, tp.c, ld[j]) * row.dinv : 1.0;
+            const double g = DRAFT ? row[DRAFT].f(table, tp.c, ld[j]) * row[DRAFT].inv : 1.0;
             if (static_cast<double>(num[j]) * g * left[r] < w) {
               v = j;
             } else if (DRAFT) {
@@ -579,26 +628,24 @@ verify_kernel(const VerifyArgs a) {
         if (!(total > 0.0)) break;
       }
       // ---------------------------------------------------------------- the token
-      const bool some = row.inv > 0.0;      // a row without a number above -inf has no probabilities
-      auto depth = [&](float x) { return row.p.kind == 2 ? 0.0 : fma(lowered(x), tp.c, row.p.add - MAGIC); };      // l c - N
+      const bool some = row[0].inv > 0.0;      // a row without a number above -inf has no probabilities
       if (rank == 0 && tid == 0) a.out_rows[out + count] = node;
       if (next >= 0) {
         if (rank == 0 && tid == 0) {
           a.out_tokens[out + count] = tok[next];
-          chosen[count] = depth(lz[next]);
-          sums[count] = row.sum;
+          chosen[count] = row[0].f.depth(tp.c, lz[next]);
+          sums[count] = row[0].sum;
         }
         ++count;
         node = next;
         __syncthreads();      // (this row's numbers have been read)
         continue;
       }
-      auto put = [&](int t, float x) {
-        a.out_tokens[out + count] = t;
-        a.out_logprobs[out + count] = some ? static_cast<float>((depth(x) - log2_of(table, row.sum)) * LN2) : -INFINITY;
-      };
       if (cold || !some) {
-        if (rank == 0 && tid == 0) put(some ? row.best : 0, some ? z.at(row.best) : 0.f);
+        if (rank == 0 && tid == 0) {
+          drawn = some ? row_best : 0;
+          drawn_z = some ? z.at(drawn) : 0.f;
+        }
         ++count;
         break;
       }
@@ -713,12 +760,19 @@ verify_kernel(const VerifyArgs a) {
             start += __shfl_sync(0xffffffffu, sofar, 31);
           }
           if (hit < 0) hit = end;
-          if (lane == 0) put(hit, z.at(hit));
+          if (lane == 0) {
+            drawn = hit;
+            drawn_z = z.at(hit);
+          }
         }
       }
       ++count;
       break;
     }
+  }
+  if (drawn >= 0) {
+    a.out_tokens[out + count - 1] = drawn;
+    a.out_logprobs[out + count - 1] = row[0].inv > 0.0 ? static_cast<float>((row[0].f.depth(depth_c, drawn_z) - log2_of(table, row[0].sum)) * LN2) : -INFINITY;
   }
   if (rank == 0) {
     if (tid == 0) a.out_counts[b] = count;
@@ -734,13 +788,14 @@ verify_kernel(const VerifyArgs a) {
 
 template <typename T, bool DRAFT>
 int launch_verify(const VerifyArgs& a, int B, cudaStream_t stream) {
-  // Two CTAs to an SM. The largest cluster with which all sequences run at once.
+  // Two CTAs to an SM. The largest cluster with which all sequences run at once, or in two turns where they may go down several rows: the last sequences' rows
+  // are what the others wait for (64 trees of 17 rows: four CTAs 70 us, eight 69; 48 of 8 drawn ones 213 and 191; 64 single rows 27 and 36).
   int dev = 0, sms = 148;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return static_cast<int>(e);
   int cluster = DV_CLUSTER;
-  while (cluster > 1 && static_cast<long long>(B) * cluster > 2 * sms) cluster /= 2;
+  while (cluster > 1 && static_cast<long long>(B) * cluster > (a.steps > 1 ? 4 : 2) * sms) cluster /= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(B) * cluster);
   cfg.blockDim = dim3(DV_THREADS);

@@ -238,6 +238,11 @@ def tree_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
 
 
 # --------------------------------------------------------------------------------------- verification
+def _rounded_down(x: float) -> float:
+    f = torch.tensor(x, dtype=torch.float32)
+    return float(f) if float(f) <= x else float(torch.nextafter(f, torch.tensor(-math.inf)))
+
+
 def _weights(z: torch.Tensor, temp: float) -> tuple[torch.Tensor, torch.Tensor]:
     """Probabilities and their logarithms in 64 bits; zeros and -inf where no number is above -inf."""
     z = z.double()
@@ -245,7 +250,7 @@ def _weights(z: torch.Tensor, temp: float) -> tuple[torch.Tensor, torch.Tensor]:
     top = z.max()
     if top == -math.inf:
         return torch.zeros_like(z), z
-    e = torch.where(z == -math.inf, z, (z - top) / temp)
+    e = torch.where((z == -math.inf) | (z < top - _rounded_down(1000 * math.log(2) * temp)), -math.inf, (z - top) / temp)
     logp = e - torch.log(torch.exp(e).sum())
     return torch.exp(logp), logp
 
@@ -315,7 +320,7 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Ten
     accepted if u Z q(x) < w(x), and is the next node. Otherwise, with ``draft_logits`` [T, V] (the logits, at the same temperature, that a row's children were drawn from,
     independently), w becomes max(w / Z - q, 0) and Z its sum; without (children were taken without chance, each token once; q = 1) Z loses w(x) and x is out. Where no child
     is accepted, the last token is the first whose running sum of w passes row 0's number times the whole sum. Greedy: a child is accepted if its token has the largest logit (of equal ones the lowest), which is the last token too.
-    Logits that are not numbers weigh nothing, +inf as much as the largest number. At most ``max_steps`` tokens (None: ``max_rows``).
+    Logits that are not numbers weigh nothing, nor does what is less than 2^-1000 of the largest; +inf as much as the largest number. At most ``max_steps`` tokens (None: ``max_rows``).
 
     Returns ``tokens`` int32 [B, max_steps] (accepted ones and the last; -1 behind them), ``counts`` int32 [B], ``rows`` int32 [B, max_steps] (row 0 and the accepted rows, as :func:`kv_cache_keep`
     takes them; -1 behind them) and ``logprobs`` fp32 [B, max_steps], the tokens' logarithms of p (0 behind them; -inf where no logit is above -inf, whose token is 0). Sums are in 64 bits."""

@@ -435,3 +435,17 @@ def test_streams(native_lib):
                 got.append(S.tree_paged_decode(q, k, v, table, ctx, cu, 8, 2, 128, max_rows=18, masks=masks))
     torch.cuda.synchronize()
     assert all(torch.equal(x, want) for x in got) and L.check_status() == 0
+
+
+def test_verify_of_logits_that_grow(native_lib):
+    """Ranges whose later logits weigh far more than their first ones, up to what has no place beside them."""
+    V = 40000
+    for step in (0.01, 0.1, 30.0):
+        z = torch.arange(V).float().flip(0).reshape(2, -1).flip(0).reshape(-1) * step      # (each half falls)
+        z = torch.stack([z, z.flip(0), torch.arange(V).float() * step, torch.where(torch.arange(V) % 700 == 650, 600.0 + torch.arange(V) % 3, 0.0)])
+        tokens, parents, cu = torch.zeros(4, dtype=I32), torch.full((4,), -1, dtype=I32), torch.arange(5, dtype=I32)
+        for u in (0.0, 0.37, 0.99):
+            want = S.verify_drafts(z, tokens, parents, cu, torch.full((4,), u), max_rows=1)
+            got = S.verify_drafts(*_dev(z, tokens, parents, cu, torch.full((4,), u)), max_rows=1)
+            assert torch.equal(got[0].cpu(), want[0])
+            assert torch.allclose(got[3].cpu(), want[3], rtol=2.0**-23, atol=1e-12)
