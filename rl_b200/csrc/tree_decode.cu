@@ -25,13 +25,14 @@ using namespace rlb;
 
 constexpr int M_ROWS = 128, TILE = 64;
 constexpr int THREADS = 192;
-constexpr int TMEM_COLS = 256;      // scores of even and odd tiles at columns 0 and 64 (P in the first 32 of each), output at column 128
+constexpr int TMEM_COLS = 256;      // scores of even and odd tiles at columns 0 and 64, P and the output where Shape says
 constexpr int BAD_RING = 8;         // the producer is at most four tiles ahead of the softmax
 constexpr float RESCALE = 8.f;      // log2
 constexpr float LOG2E_F = 1.4426950408889634f;
 
+struct Cut;
 struct TreeArgs {
-  int blocks, block, pages, box;      // box: keys of a TMA box
+  int blocks, block, block_shift, pages, box;      // block_shift: of pages of a power of two, else -1; box: keys of a TMA box
   const int* table;
   long long table_ld;
   const int* ctx;
@@ -49,6 +50,7 @@ struct TreeArgs {
   const __nv_bfloat16* v;
   float* part_o;               // [2 CTAs][part_rows][D]: first and last part of a CTA; null: a CTA has a whole unit
   float2* part_ml;             // [2 CTAs][part_rows] maximum (log2) and sum
+  Cut* cuts;                   // [CTAs]
   int part_rows, least;        // least: tiles of a share at least
   int* status;
 };
@@ -59,6 +61,9 @@ struct Shape {
   static constexpr int K_STAGES = D == 128 ? 3 : 5, V_STAGES = D == 128 ? 2 : 4;
   static constexpr int Q_ATOM = M_ROWS * 128, KV_ATOM = TILE * 128;
   static constexpr int Q_BYTES = ATOMS * Q_ATOM, KV_BYTES = ATOMS * KV_ATOM;
+  // P over the scores that were read, where the output leaves no room for places of its own: the scores after next then wait for the product
+  static constexpr bool OWN_P = D == 64;
+  static constexpr int P_COL = OWN_P ? 128 : 0, P_STEP = OWN_P ? 32 : 64, O_COL = OWN_P ? 192 : 128;
   static constexpr int SMEM = Q_BYTES + (K_STAGES + V_STAGES) * KV_BYTES + 512;
 };
 
@@ -121,17 +126,12 @@ __device__ __forceinline__ long long block_scan(long long v, long long* red, lon
   }
   return before + run - v;
 }
-// Share of the tiles of all sequences that a CTA of `ctas` takes.
-__device__ __forceinline__ long long share_of(const TreeArgs& a, int ctas, long long* red, long long& total) {
-  total = 0;
-  for (int b0 = 0; b0 < a.B; b0 += blockDim.x) {
-    const int b = b0 + threadIdx.x;
-    long long all;
-    block_scan(b < a.B ? tiles_of(a, sequence(a, b)) : 0, red, all);
-    total += all;
-  }
-  return max(static_cast<long long>(a.least), (total + ctas - 1) / ctas);
-}
+// What a CTA's first part is the rest of: how many of the unit's tiles came before it (0: nothing), and of how many.
+struct Cut {
+  long long share;      // tiles of a CTA
+  int row, rows, head;  // of the output, of the unit; first head
+  int before, tiles, none;
+};
 
 struct Segment {      // what a CTA does of one unit
   Seq s;
@@ -140,28 +140,33 @@ struct Segment {      // what a CTA does of one unit
   bool whole;
 };
 struct Cursor {
-  long long left;      // tiles that this CTA still has
-  long long at;        // tile within the sequence
-  int b;
+  long long left;          // tiles that this CTA still has
+  int b, kv_head, m, t;    // sequence, unit and tile that come next
   Seq s;
   __device__ __forceinline__ bool next(const TreeArgs& a, Segment& g) {
     if (left <= 0) return false;
-    while (at >= tiles_of(a, s)) {
-      at = 0;
+    if (t == s.tiles) {
+      t = 0;
+      if (++m == s.blocks) {
+        m = 0;
+        ++kv_head;
+      }
+    }
+    while (s.blocks == 0 || kv_head == a.Hkv) {
+      kv_head = 0;
       if (++b >= a.B) return false;
       s = sequence(a, b);
     }
-    const int unit = static_cast<int>(at / s.tiles);
     g.s = s;
     g.b = b;
-    g.kv_head = unit / s.blocks;
-    g.j0 = (unit % s.blocks) * a.block_rows;
+    g.kv_head = kv_head;
+    g.j0 = m * a.block_rows;
     g.rows = min(a.block_rows, s.n - g.j0) * a.G;
-    g.t0 = static_cast<int>(at % s.tiles);
-    g.t1 = static_cast<int>(min(static_cast<long long>(s.tiles), g.t0 + left));
+    g.t0 = t;
+    g.t1 = static_cast<int>(min(static_cast<long long>(s.tiles), t + left));
     g.whole = g.t0 == 0 && g.t1 == s.tiles;
-    at += g.t1 - g.t0;
     left -= g.t1 - g.t0;
+    t = g.t1;
     return true;
   }
 };
@@ -210,9 +215,35 @@ __device__ __forceinline__ uint64_t without_pages(uint64_t v, int bad) {
 
 __device__ __forceinline__ bool not_finite(uint32_t w) { return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
 
+// Adds values that are not finite, of tiles that some row does not see as a whole, to the row that sees them: to its output, or to its part.
+template <int D>
+__device__ __noinline__ void add_special(const TreeArgs& a, const Segment g, const RowView view, int edge, __nv_bfloat16* dst, float* part) {
+  for (int t = g.t0; t < g.t1; ++t) {
+    const int k0 = (g.s.first + t) * TILE;
+    int lost = 0;
+    for (int i = 0; i < TILE && k0 + i < g.s.keys; i += 16) {
+      const int id = a.table[g.b * a.table_ld + (k0 + i) / a.block];
+      if (id < 0 || id >= a.blocks) lost |= 1 << (i >> 4);
+    }
+    if (k0 + TILE <= g.s.ctx && k0 >= edge && !lost) continue;
+    const uint64_t seen = without_pages(seen_keys(a, g.s, view, k0), lost);
+    for (int i = 0; i < TILE; ++i) {
+      if (!(seen >> i & 1)) continue;
+      const int id = a.table[g.b * a.table_ld + (k0 + i) / a.block];
+      const __nv_bfloat16* v = a.v + ((static_cast<long long>(id) * a.Hkv + g.kv_head) * a.block + (k0 + i) % a.block) * D;
+      for (int e = 0; e < D; ++e) {
+        const float x = __bfloat162float(v[e]);
+        if (fabsf(x) < INFINITY) continue;
+        if (part) part[e] += x;
+        else dst[e] = __float2bfloat16(__bfloat162float(dst[e]) + x);
+      }
+    }
+  }
+}
+
 template <int D>
 __global__ void __launch_bounds__(THREADS, 2)
-tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const TreeArgs a) {
+tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ TreeArgs a) {
   using S = Shape<D>;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* q_s = smem;
@@ -263,50 +294,75 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   pdl_sync();
 
   // ---------------------------------------------------------------- this CTA's tiles
-  Cursor first;
+  Cursor cur;
   if (a.part_o) {
-    long long total;
-    const long long share = share_of(a, gridDim.x, red, total), begin = share * blockIdx.x;
-    if (begin >= total) return;
-    long long before = 0;
+    long long total = 0, before = 0, mine = 0, all;      // of all sequences, of those before this thread's, of its own
     for (int b0 = 0; b0 < a.B; b0 += THREADS) {
       const int b = b0 + threadIdx.x;
-      const long long mine = b < a.B ? tiles_of(a, sequence(a, b)) : 0;
-      long long all;
-      const long long at = before + block_scan(mine, red, all);
-      if (begin >= at && begin < at + mine) {
-        start[0] = b;
-        start[1] = begin - at;
+      mine = b < a.B ? tiles_of(a, sequence(a, b)) : 0;
+      before = total + block_scan(mine, red, all);
+      total += all;
+    }
+    const unsigned ctas = gridDim.x;
+    const long long share = max(static_cast<long long>(a.least), total <= 0x7fffffffll ? (static_cast<unsigned>(total) + ctas - 1) / ctas : (total + ctas - 1) / ctas);
+    const long long begin = share * blockIdx.x;
+    if (begin >= total) {
+      if (threadIdx.x == 0) a.cuts[blockIdx.x].before = 0;
+      return;
+    }
+    if (a.B > THREADS) {      // the sequence that it lies in once more
+      long long sofar = 0;
+      for (int b0 = 0; b0 < a.B && sofar <= begin; b0 += THREADS) {
+        const int b = b0 + threadIdx.x;
+        mine = b < a.B ? tiles_of(a, sequence(a, b)) : 0;
+        before = sofar + block_scan(mine, red, all);
+        sofar += all;
+        if (begin >= before && begin < before + mine) start[0] = b;
+        if (begin >= before && begin < before + mine) start[1] = begin - before;
       }
-      before += all;
-      if (before > begin) break;
+    } else if (begin >= before && begin < before + mine) {
+      start[0] = threadIdx.x;
+      start[1] = begin - before;
     }
     __syncthreads();
-    first.b = static_cast<int>(start[0]);
-    first.at = start[1];
-    first.left = min(share, total - begin);
-    first.s = sequence(a, first.b);
+    cur.b = static_cast<int>(start[0]);
+    cur.s = sequence(a, cur.b);
+    const long long at = start[1];
+    const int unit = at <= 0x7fffffffll ? static_cast<int>(static_cast<unsigned>(at) / static_cast<unsigned>(cur.s.tiles)) : static_cast<int>(at / cur.s.tiles);
+    cur.t = static_cast<int>(at - static_cast<long long>(unit) * cur.s.tiles);
+    cur.kv_head = unit / cur.s.blocks;
+    cur.m = unit - cur.kv_head * cur.s.blocks;
+    cur.left = min(share, total - begin);
+    if (threadIdx.x == 0) {
+      const int j0 = cur.m * a.block_rows;
+      a.cuts[blockIdx.x] = Cut{share, cur.s.lo + j0, min(a.block_rows, cur.s.n - j0) * a.G, cur.kv_head * a.G, cur.t, cur.s.tiles, 0};
+    }
   } else {
-    first.b = blockIdx.z;
-    first.s = sequence(a, first.b);
-    if (static_cast<int>(blockIdx.x) >= first.s.blocks) return;
-    first.at = (static_cast<long long>(blockIdx.y) * first.s.blocks + blockIdx.x) * first.s.tiles;
-    first.left = first.s.tiles;
+    cur.b = blockIdx.z;
+    cur.s = sequence(a, cur.b);
+    if (static_cast<int>(blockIdx.x) >= cur.s.blocks) return;
+    cur.kv_head = blockIdx.y;
+    cur.m = blockIdx.x;
+    cur.t = 0;
+    cur.left = cur.s.tiles;
   }
   if (smem_u32(smem) & 1023u) {      // the swizzled tiles need a base of 1024 bytes; report instead of misreading
     if (threadIdx.x == 0 && a.status) atomicCAS(a.status, 0, RLB_ERR_BAD_ARG);
     return;
   }
-  if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
-    tmem_relinquish();
+  uint32_t tmem_base = 0, tmem_o = 0;
+  if (warp != 0) {      // (the loads need not wait for this)
+    if (warp == 1) {
+      tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
+      tmem_relinquish();
+    }
+    tc_fence_before();
+    asm volatile("bar.sync 1, 160;" ::: "memory");
+    tc_fence_after();
+    tmem_base = *tmem_slot;
+    tmem_o = tmem_base + S::O_COL;
   }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot, tmem_o = tmem_base + 128;
 
-  Cursor cur = first;
   Segment g;
   if (warp == 0) {
     // ------------------------------------------------------------ loads
@@ -316,6 +372,18 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     int it = 0;
     for (int unit = 0; ok && cur.next(a, g); ++unit) {
       const int* table = a.table + g.b * a.table_ld;
+      // lane i has the first row of box i of the next 32, and one more of those behind them
+      auto look = [&](int from) -> int {      // box `from` + lane of the sequence: its row in the cache, -1 without a page, -2 behind the keys
+        const long long key = (static_cast<long long>(from) + lane) * a.box;
+        if (key >= g.s.keys) return -2;
+        const int k = static_cast<int>(key), page = a.block_shift >= 0 ? k >> a.block_shift : k / a.block, id = table[page];
+        if (id < 0 || id >= a.blocks) {
+          if (a.status) atomicCAS(a.status, 0, RLB_ERR_BOUNDS);
+          return -1;
+        }
+        return (id * a.Hkv + g.kv_head) * a.block + (k - page * a.block);
+      };
+      int at = (g.s.first + g.t0) * boxes, rows = look(at), ahead = look(at + 32), used = 0;
       if (unit > 0) ok = warp_wait(q_empty, (unit - 1) & 1, abort_flag, a.status, RLB_ERR_WAIT_EMPTY);
       if (!ok) break;
       if (elect_one()) {
@@ -324,18 +392,6 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         for (int c = 0; c < S::ATOMS; ++c) tma_load_3d(smem_u32(q_s + c * S::Q_ATOM), &tmap_q, smem_u32(q_full), c * 64, g.kv_head * a.G, g.s.lo + g.j0);
       }
       __syncwarp();
-      // lane i has the first row of box i of the next 32, and one more of those behind them
-      auto look = [&](int from) -> int {      // box `from` + lane of the sequence: its row in the cache, -1 without a page, -2 behind the keys
-        const long long key = (static_cast<long long>(from) + lane) * a.box;
-        if (key >= g.s.keys) return -2;
-        const int k = static_cast<int>(key), page = k / a.block, id = table[page];
-        if (id < 0 || id >= a.blocks) {
-          if (a.status) atomicCAS(a.status, 0, RLB_ERR_BOUNDS);
-          return -1;
-        }
-        return (id * a.Hkv + g.kv_head) * a.block + (k - page * a.block);
-      };
-      int at = (g.s.first + g.t0) * boxes, rows = look(at), ahead = look(at + 32), used = 0;
       for (int t = g.t0; t < g.t1 && ok; ++t, ++it) {
         const int ks = it % S::K_STAGES, vs = it % S::V_STAGES;
         if (used == 32) {
@@ -387,7 +443,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       constexpr uint32_t idesc_s = make_idesc_bf16(M_ROWS, TILE, false, false), idesc_o = make_idesc_bf16(M_ROWS, D, false, true);
       auto scores = [&](int it, bool last_of_unit) -> bool {      // its buffer held P of tile it - 2, whose product has to be complete
         const int ks = it % S::K_STAGES;
-        if (it > 1 && !mbar_wait(smem_u32(&v_empty[(it - 2) % S::V_STAGES]), ((it - 2) / S::V_STAGES) & 1, abort_flag, a.status, RLB_ERR_WAIT_TMEM_EMPTY))
+        if (!S::OWN_P && it > 1 && !mbar_wait(smem_u32(&v_empty[(it - 2) % S::V_STAGES]), ((it - 2) / S::V_STAGES) & 1, abort_flag, a.status, RLB_ERR_WAIT_TMEM_EMPTY))
           return false;
         if (!mbar_wait(smem_u32(&k_full[ks]), (it / S::K_STAGES) & 1, abort_flag, a.status, RLB_ERR_WAIT_FULL)) return false;
         tc_fence_after();
@@ -416,7 +472,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < TILE / 16; ++kk)      // 16 keys each, 8 columns of P
-            umma_f16_ts(tmem_o, tmem_base + (it & 1) * 64 + kk * 8, make_smem_desc_sw128(smem_u32(v_s + vs * S::KV_BYTES) + kk * (16 * 128), S::KV_ATOM, 1024), idesc_o,
+            umma_f16_ts(tmem_o, tmem_base + S::P_COL + (it & 1) * S::P_STEP + kk * 8, make_smem_desc_sw128(smem_u32(v_s + vs * S::KV_BYTES) + kk * (16 * 128), S::KV_ATOM, 1024), idesc_o,
                         (t | kk) != 0 ? 1u : 0u);
           umma_commit(smem_u32(&v_empty[vs]));
         }
@@ -427,14 +483,16 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     const int quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
     // scores are compared before scaling; a negative scale turns the comparison round
+    const int own_j = r / a.G, own_h = r % a.G;
     const bool neg = a.scale_log2 < 0.f;
     const float hidden = neg ? INFINITY : -INFINITY;
     bool ok = true;
     int it = 0;
     for (int unit = 0; ok && cur.next(a, g); ++unit) {
       const bool active = quarter * 32 < g.rows;      // of the warp
-      const int j = min(g.j0 + r / a.G, g.s.n - 1);   // (rows behind the block's compute as its last one)
+      const int j = min(g.j0 + own_j, g.s.n - 1);   // (rows behind the block's compute as its last one)
       RowView view{a.masks ? a.masks + (g.s.lo + j) * a.masks_ld : nullptr, (a.max_rows + 31) >> 5, j, a.window > 0 ? max(a.positions[g.s.lo + j], g.s.ctx) : 0};
+      if (a.masks) asm volatile("prefetch.global.L1 [%0];" ::"l"(view.mask));
       int edge = 0;      // keys before it are out of some row's window
       if (a.window > 0) {
         int far = g.s.ctx;
@@ -540,7 +598,11 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             pk[16 + i] = pack_bf16x2(f0, f1);
           }
           l = l * factor + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-          tmem_st_32x32b_x32(tmem_s, pk);      // over the scores that this thread has read
+          if (S::OWN_P && it > 1 && !warp_wait(&v_empty[(it - 2) % S::V_STAGES], ((it - 2) / S::V_STAGES) & 1, abort_flag, a.status, RLB_ERR_WAIT_TMEM_EMPTY)) {
+            ok = false;
+            break;
+          }
+          tmem_st_32x32b_x32(tmem_base + S::P_COL + (it & 1) * S::P_STEP + lane_addr, pk);
           if (__any_sync(0xffffffffu, need)) {
             // O may be touched only after the previous product has completed (the next one waits for p_full)
             if (!warp_wait(&v_empty[(it - 1) % S::V_STAGES], ((it - 1) / S::V_STAGES) & 1, abort_flag, a.status, RLB_ERR_WAIT_TMEM_EMPTY)) {
@@ -571,11 +633,10 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       if (active) {
         tc_fence_after();
         const bool there = r < g.rows;
-        const int head = g.kv_head * a.G + r % a.G;
         const long long slot = (2 * static_cast<long long>(blockIdx.x) + (g.t0 == 0)) * a.part_rows + r;
-        const float inv = g.whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
         if (there && !g.whole) a.part_ml[slot] = make_float2(m_ref, l);
-        __nv_bfloat16* dst = a.out + (g.s.lo + j) * a.ldo + head * D;
+        __nv_bfloat16* dst = a.out + (g.s.lo + j) * a.ldo + (g.kv_head * a.G + own_h) * D;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
@@ -583,28 +644,6 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           tmem_ld_32x32b_x32(tmem_o + lane_addr + c * 32, o);
           tmem_ld_wait();
           if (!there) continue;
-          if (special[unit & 1] == unit) {      // what is not finite in tiles that were cut: to the rows that see it
-            for (int t = g.t0; t < g.t1; ++t) {
-              const int k0 = (g.s.first + t) * TILE;
-              int lost = 0;
-              for (int i = 0; i < TILE && k0 + i < g.s.keys; i += 16) {
-                const int id = a.table[g.b * a.table_ld + (k0 + i) / a.block];
-                if (id < 0 || id >= a.blocks) lost |= 1 << (i >> 4);
-              }
-              if (k0 + TILE <= g.s.ctx && k0 >= edge && !lost) continue;
-              const uint64_t seen = without_pages(seen_keys(a, g.s, view, k0), lost);
-              for (int i = 0; i < TILE; ++i) {
-                if (!(seen >> i & 1)) continue;
-                const int id = a.table[g.b * a.table_ld + (k0 + i) / a.block];
-                const __nv_bfloat16* v = a.v + ((static_cast<long long>(id) * a.Hkv + g.kv_head) * a.block + (k0 + i) % a.block) * D + c * 32;
-#pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                  const float x = __bfloat162float(v[e]);
-                  if (!(fabsf(x) < INFINITY)) o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
-                }
-              }
-            }
-          }
           if (!g.whole) {
             float4* to = reinterpret_cast<float4*>(a.part_o + slot * D + c * 32);
 #pragma unroll
@@ -627,6 +666,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             }
           }
         }
+        if (there && special[unit & 1] == unit) add_special<D>(a, g, view, edge, g.whole ? dst : nullptr, g.whole ? nullptr : a.part_o + slot * D);
         tc_fence_before();
       }
       __syncwarp();
@@ -641,49 +681,33 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   }
 }
 
-// Joins the parts of a unit that several CTAs had: a CTA for 8 of its rows.
+// Joins the parts of a unit that several CTAs had: a CTA for 8 of its rows, for each CTA whose first part is a unit's second.
 constexpr int JOIN_ROWS = 8;
 template <int D>
 __global__ void __launch_bounds__(JOIN_ROWS * D / 8)
-tree_join_kernel(const TreeArgs a, int ctas) {
-  __shared__ long long red[JOIN_ROWS * D / 8 / 32];
+tree_join_kernel(const TreeArgs a) {
   pdl_sync();
-  long long total;
-  const long long share = share_of(a, ctas, red, total);
-  const int b = blockIdx.z;
-  const Seq s = sequence(a, b);
-  const int unit = blockIdx.y, threads = JOIN_ROWS * D / 8;
-  if (unit >= s.blocks * a.Hkv) return;
-  const int j0 = (unit % s.blocks) * a.block_rows, rows = min(a.block_rows, s.n - j0) * a.G, r = blockIdx.x * JOIN_ROWS + threadIdx.x / (D / 8);
-  if (static_cast<int>(blockIdx.x) * JOIN_ROWS >= rows) return;
-  long long before = 0;      // tiles of the sequences before this one
-  for (int b0 = 0; b0 < b; b0 += threads) {
-    const int i = b0 + static_cast<int>(threadIdx.x);
-    long long all;
-    block_scan(i < b ? tiles_of(a, sequence(a, i)) : 0, red, all);
-    before += all;
-  }
-  const long long begin = before + static_cast<long long>(unit) * s.tiles;
-  const int c0 = static_cast<int>(begin / share), c1 = static_cast<int>((begin + s.tiles - 1) / share);
-  if (c0 == c1 || r >= rows) return;
-  auto slot = [&](int c) { return (2 * static_cast<long long>(c) + (c == c0)) * a.part_rows + r; };
-  float top = -INFINITY;
-  for (int c = c0; c <= c1; ++c) top = fmaxf(top, a.part_ml[slot(c)].x);
-  const int d = (threadIdx.x % (D / 8)) * 8;
-  float o[8] = {}, l = 0.f;
-  for (int c = c0; c <= c1; ++c) {
-    const long long i = slot(c);
+  const int c = blockIdx.y, r = blockIdx.x * JOIN_ROWS + threadIdx.x / (D / 8), d = (threadIdx.x % (D / 8)) * 8;
+  const Cut cut = a.cuts[c];
+  if (cut.before == 0 || cut.before > cut.share || r >= cut.rows) return;
+  const int last = c + static_cast<int>((cut.tiles - cut.before - 1) / cut.share);
+  float o[8] = {}, l = 0.f, top = -INFINITY;
+#pragma unroll 2
+  for (int k = c - 1; k <= last; ++k) {      // the first one is its CTA's last part, the others their CTA's first
+    const long long i = (2 * static_cast<long long>(k) + (k < c)) * a.part_rows + r;
     const float2 ml = a.part_ml[i];
-    const float w = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2f(ml.x - top);      // (a sum beside no maximum is not a number)
     const float4 x = *reinterpret_cast<const float4*>(a.part_o + i * D + d), y = *reinterpret_cast<const float4*>(a.part_o + i * D + d + 4);
-    l += ml.y * w;
-    if (w != 0.f) {
-      o[0] += x.x * w; o[1] += x.y * w; o[2] += x.z * w; o[3] += x.w * w;
-      o[4] += y.x * w; o[5] += y.y * w; o[6] += y.z * w; o[7] += y.w * w;
-    }
+    if (ml.x == -INFINITY && ml.y == 0.f) continue;      // nothing seen
+    const float m = fmaxf(top, ml.x);
+    const float f = top == -INFINITY ? 0.f : exp2f(top - m), w = ml.x == -INFINITY ? 1.f : exp2f(ml.x - m);      // (a sum beside no maximum is not a number)
+    top = m;
+    l = (f == 0.f ? 0.f : l * f) + (w == 0.f ? 0.f : ml.y * w);
+    const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int q = 0; q < 8; ++q) o[q] = (f == 0.f ? 0.f : o[q] * f) + (w == 0.f ? 0.f : v[q] * w);
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  __nv_bfloat16* dst = a.out + static_cast<long long>(s.lo + j0 + r / a.G) * a.ldo + ((unit / s.blocks) * a.G + r % a.G) * D + d;
+  __nv_bfloat16* dst = a.out + static_cast<long long>(cut.row + r / a.G) * a.ldo + (cut.head + r % a.G) * D + d;
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(o[2 * i] * inv, o[2 * i + 1] * inv);
@@ -722,24 +746,27 @@ int launch(const void* q, long long ldq, const void* k, const void* v, TreeArgs 
   const dim3 grid = ctas ? dim3(ctas) : dim3(blocks, a.Hkv, a.B);
   e = rlb_launch_pdl(tree_decode_kernel<D>, grid, dim3(THREADS), Shape<D>::SMEM, stream, tq, tk, tv, a);
   if (e != cudaSuccess || !ctas) return static_cast<int>(e);
-  const int most = a.block_rows * a.G < a.max_rows * a.G ? a.block_rows * a.G : a.max_rows * a.G;
-  return static_cast<int>(rlb_launch_pdl(tree_join_kernel<D>, dim3((most + JOIN_ROWS - 1) / JOIN_ROWS, blocks * a.Hkv, a.B), dim3(JOIN_ROWS * D / 8), 0, stream, a, ctas));
+  return static_cast<int>(rlb_launch_pdl(tree_join_kernel<D>, dim3((a.part_rows + JOIN_ROWS - 1) / JOIN_ROWS, ctas), dim3(JOIN_ROWS * D / 8), 0, stream, a));
 }
 }  // namespace
 
-// ctas > 0: so many CTAs share all tiles, at least `least` each; part_o [2 ctas, part_rows, D] and part_ml [2 ctas, part_rows, 2] fp32 with part_rows = min(max_rows, 128 / G) * G.
+// ctas > 0: so many CTAs share all tiles, at least `least` each; part_o [2 ctas, part_rows, D] and part_ml [2 ctas, part_rows, 2] fp32 with part_rows = min(max_rows, 128 / G) * G, cuts 32 bytes
+// for each CTA.
 // ctas 0: a CTA for each unit. q: rows on 16 bytes.
 RLB_API int rlb_tree_decode(const void* q, long long ldq, const void* k, const void* v, int blocks, int block, const int* table, long long table_ld, int pages,
                             const int* ctx, const int* cu, int B, int T, int max_rows, int Hq, int Hkv, int D, const int* masks, long long masks_ld,
-                            const int* positions, int window, float scale, int ctas, int least, float* part_o, float* part_ml, void* out, long long ldo, int* status,
+                            const int* positions, int window, float scale, int ctas, int least, float* part_o, float* part_ml, void* cuts, void* out, long long ldo, int* status,
                             void* stream) {
   if (D != 64 && D != 128) return -2;
   if (Hkv < 1 || Hkv > 65535 || Hq % Hkv || Hq / Hkv > M_ROWS || B > 65535 || block < 16 || block % 16 || max_rows < 1 || max_rows > 256 || ldq % 8 || least < 1) return -2;
-  if (static_cast<long long>(blocks) * Hkv * block >= 0x7fffffffll || (ctas && (!part_o || !part_ml))) return -2;
+  if (static_cast<long long>(blocks) * Hkv * block >= 0x7fffffffll || (ctas && (!part_o || !part_ml || !cuts))) return -2;
   TreeArgs a;
   a.blocks = blocks;
   a.block = block;
   a.pages = pages;
+  a.block_shift = -1;
+  for (int i = 4; i < 31; ++i)
+    if (block == 1 << i) a.block_shift = i;
   a.box = block % 64 == 0 ? 64 : block % 32 == 0 ? 32 : 16;
   a.table = table;
   a.table_ld = table_ld;
@@ -766,6 +793,7 @@ RLB_API int rlb_tree_decode(const void* q, long long ldq, const void* k, const v
   a.part_o = ctas ? part_o : nullptr;
   a.part_ml = reinterpret_cast<float2*>(part_ml);
   a.part_rows = a.q_rows * a.G;
+  a.cuts = static_cast<Cut*>(cuts);
   a.least = least;
   a.status = status;
   return D == 64 ? launch<64>(q, ldq, k, v, a, ctas, static_cast<cudaStream_t>(stream)) : launch<128>(q, ldq, k, v, a, ctas, static_cast<cudaStream_t>(stream));

@@ -30,7 +30,7 @@ _P, _I, _LL, _F = _L.P, _L.I, _L.L, _L.F
 _L.register("rlb_tree_rows", [_P, _P, _P, _P, _LL, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P])
 _L.register("rlb_kv_keep", [_P, _I, _P, _LL, _I, _I, _I, _I, _I, _P, _P, _I, _P, _I, _P, _P])
 _L.register("rlb_verify_drafts", [_P, _LL, _P, _LL, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, C.c_double, _I, _P, _P, _P, _P, _P, _P])
-_L.register("rlb_tree_decode", [_P, _LL, _P, _P, _I, _I, _P, _LL, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _LL, _P, _I, _F, _I, _I, _P, _P, _P, _LL, _P, _P])
+_L.register("rlb_tree_decode", [_P, _LL, _P, _P, _I, _I, _P, _LL, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _LL, _P, _I, _F, _I, _I, _P, _P, _P, _P, _LL, _P, _P])
 
 BF16 = torch.bfloat16
 HEAD_DIMS = (64, 128)
@@ -155,7 +155,7 @@ def tree_plan(B: int, Hq: int, Hkv: int, max_rows: int, max_len: int, sm_count: 
 
 def tree_scratch_size(ctas: int, Hq: int, Hkv: int, D: int, max_rows: int) -> int:
     """Floats of the scratch tensor of :func:`tree_paged_decode` with this many CTAs."""
-    return 2 * ctas * min(max_rows, 128 // (Hq // Hkv)) * (Hq // Hkv) * (D + 2)
+    return 2 * ctas * min(max_rows, 128 // (Hq // Hkv)) * (Hq // Hkv) * (D + 2) + 12 * ctas
 
 
 def tree_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, ctx_lens: torch.Tensor, cu_rows: torch.Tensor,
@@ -219,21 +219,22 @@ def tree_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         plan = tree_plan(B, Hq, Hkv, max_rows, min(room, window + max_rows) if window else room)
     elif plan < 0 or plan > 65535:
         raise ValueError(f"plan is 0 to 65535 CTAs, not {plan}")
-    sums = parts = None
+    parts = sums = cuts = None
     if plan:
         size = tree_scratch_size(plan, Hq, Hkv, D, max_rows)
         if scratch is None:
             scratch = torch.empty(size, dtype=torch.float32, device=device)
         elif scratch.dtype is not torch.float32 or not scratch.is_contiguous() or scratch.numel() < size or scratch.data_ptr() % 16 or scratch.device != device:
             raise ValueError(f"scratch is a contiguous float32 tensor of {size} elements on {device} that starts on 16 bytes")
-        parts = scratch.data_ptr()
-        sums = parts + size // (D + 2) * D * 4
+        cuts = scratch.data_ptr()
+        parts = cuts + 48 * plan
+        sums = parts + (size - 12 * plan) // (D + 2) * D * 4
     with torch.cuda.device(device):
         if q.stride(1) != 1 or q.stride(0) % 8 or q.data_ptr() % 16:      # rows that do not start on 16 bytes
             q = q[:, :width].clone(memory_format=torch.contiguous_format)
         call("rlb_tree_decode", q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], block, table.data_ptr(), table.stride(0), table.shape[1],
              ctx.data_ptr(), cu.data_ptr(), B, T, max_rows, Hq, Hkv, D, _L.ptr(masks), masks.stride(0) if masks is not None else 0, _L.ptr(positions) if window else None,
-             window, scale, plan, 4, parts, sums, out.data_ptr(), out.stride(0), _L.status_word(device).data_ptr(), _raw_stream(device.index))
+             window, scale, plan, 4, parts, sums, cuts, out.data_ptr(), out.stride(0), _L.status_word(device).data_ptr(), _raw_stream(device.index))
     return out
 
 
