@@ -38,7 +38,7 @@ struct TreeArgs {
   const int* ctx;
   const int* cu;
   int B, T, max_rows, Hq, Hkv, G;
-  int block_rows, q_rows;      // tree rows of a block, rows of a TMA box of queries
+  int block_rows, block_inv, q_rows;      // tree rows of a block, 65536 / that and one, rows of a TMA box of queries
   const int* masks;            // null: a row sees the rows up to itself
   long long masks_ld;
   const int* positions;        // with window > 0
@@ -100,37 +100,39 @@ __device__ __forceinline__ Seq sequence(const TreeArgs& a, int b) {
   s.ctx = min(max(a.ctx[b], 0), room);
   s.keys = s.n > 0 ? s.ctx + min(s.n, room - s.ctx) : 0;
   s.first = a.window > 0 ? max(0, s.ctx - a.window + 1) / TILE : 0;
-  s.blocks = (s.n + a.block_rows - 1) / a.block_rows;
+  s.blocks = ((s.n + a.block_rows - 1) * a.block_inv) >> 16;      // (exact: less than 384 over at most 128)
   s.tiles = max((s.keys + TILE - 1) / TILE - s.first, s.n > 0 ? 1 : 0);      // (rows without any key have a tile too, which they do not see)
   return s;
 }
-__device__ __forceinline__ long long tiles_of(const TreeArgs& a, const Seq& s) { return static_cast<long long>(s.tiles) * s.blocks * a.Hkv; }
+__device__ __forceinline__ int tiles_of(const TreeArgs& a, const Seq& s) { return s.tiles * s.blocks * a.Hkv; }      // (shared tiles are less than 2^31 in all)
 
 // Sums over the block's threads: of those before this one, and of all. `red`: a word for each warp.
-__device__ __forceinline__ long long block_scan(long long v, long long* red, long long& all) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  long long run = v;
+__device__ __forceinline__ int block_scan(int v, int* red, int& all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int run = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, run, o);
+    const int u = __shfl_up_sync(0xffffffffu, run, o);
     if (lane >= o) run += u;
   }
   __syncthreads();
   if (lane == 31) red[warp] = run;
   __syncthreads();
-  long long before = 0;
+  int before = 0;
   all = 0;
-  for (int w = 0; w < warps; ++w) {
-    if (w < warp) before += red[w];
-    all += red[w];
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    const int x = red[w];
+    if (w < warp) before += x;
+    all += x;
   }
   return before + run - v;
 }
 // What a CTA's first part is the rest of: how many of the unit's tiles came before it (0: nothing), and of how many.
 struct Cut {
-  long long share;      // tiles of a CTA
+  int share;            // tiles of a CTA
   int row, rows, head;  // of the output, of the unit; first head
-  int before, tiles, none;
+  int before, tiles, none[2];
 };
 
 struct Segment {      // what a CTA does of one unit
@@ -140,7 +142,7 @@ struct Segment {      // what a CTA does of one unit
   bool whole;
 };
 struct Cursor {
-  long long left;          // tiles that this CTA still has
+  int left;                // tiles that this CTA still has
   int b, kv_head, m, t;    // sequence, unit and tile that come next
   Seq s;
   __device__ __forceinline__ bool next(const TreeArgs& a, Segment& g) {
@@ -163,7 +165,7 @@ struct Cursor {
     g.j0 = m * a.block_rows;
     g.rows = min(a.block_rows, s.n - g.j0) * a.G;
     g.t0 = t;
-    g.t1 = static_cast<int>(min(static_cast<long long>(s.tiles), t + left));
+    g.t1 = min(s.tiles - t, left) + t;
     g.whole = g.t0 == 0 && g.t1 == s.tiles;
     left -= g.t1 - g.t0;
     t = g.t1;
@@ -263,8 +265,8 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* special = abort_flag + 1;      // [2] last even and odd unit with values that are not finite in a tile that some row does not see as a whole
   volatile int* bad = special + 2;             // [BAD_RING]
-  long long* red = reinterpret_cast<long long*>(smem + S::SMEM - 128);      // [THREADS / 32]
-  long long* start = red + THREADS / 32;                                    // [2]
+  int* red = reinterpret_cast<int*>(smem + S::SMEM - 128);      // [THREADS / 32]
+  int* start = red + THREADS / 32;                              // [2]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -296,22 +298,22 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   // ---------------------------------------------------------------- this CTA's tiles
   Cursor cur;
   if (a.part_o) {
-    long long total = 0, before = 0, mine = 0, all;      // of all sequences, of those before this thread's, of its own
+    int total = 0, before = 0, mine = 0, all;      // of all sequences, of those before this thread's, of its own
     for (int b0 = 0; b0 < a.B; b0 += THREADS) {
       const int b = b0 + threadIdx.x;
       mine = b < a.B ? tiles_of(a, sequence(a, b)) : 0;
       before = total + block_scan(mine, red, all);
       total += all;
     }
-    const unsigned ctas = gridDim.x;
-    const long long share = max(static_cast<long long>(a.least), total <= 0x7fffffffll ? (static_cast<unsigned>(total) + ctas - 1) / ctas : (total + ctas - 1) / ctas);
-    const long long begin = share * blockIdx.x;
-    if (begin >= total) {
+    const int share = max(a.least, static_cast<int>((static_cast<unsigned>(total) + gridDim.x - 1) / gridDim.x));
+    const long long from = static_cast<long long>(share) * blockIdx.x;
+    if (from >= total) {
       if (threadIdx.x == 0) a.cuts[blockIdx.x].before = 0;
       return;
     }
+    const int begin = static_cast<int>(from);
     if (a.B > THREADS) {      // the sequence that it lies in once more
-      long long sofar = 0;
+      int sofar = 0;
       for (int b0 = 0; b0 < a.B && sofar <= begin; b0 += THREADS) {
         const int b = b0 + threadIdx.x;
         mine = b < a.B ? tiles_of(a, sequence(a, b)) : 0;
@@ -325,20 +327,20 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       start[1] = begin - before;
     }
     __syncthreads();
-    cur.b = static_cast<int>(start[0]);
+    cur.b = start[0];
     cur.s = sequence(a, cur.b);
-    const long long at = start[1];
-    const int unit = at <= 0x7fffffffll ? static_cast<int>(static_cast<unsigned>(at) / static_cast<unsigned>(cur.s.tiles)) : static_cast<int>(at / cur.s.tiles);
-    cur.t = static_cast<int>(at - static_cast<long long>(unit) * cur.s.tiles);
+    const int unit = start[1] / cur.s.tiles;
+    cur.t = start[1] - unit * cur.s.tiles;
     cur.kv_head = unit / cur.s.blocks;
     cur.m = unit - cur.kv_head * cur.s.blocks;
     cur.left = min(share, total - begin);
     if (threadIdx.x == 0) {
       const int j0 = cur.m * a.block_rows;
-      a.cuts[blockIdx.x] = Cut{share, cur.s.lo + j0, min(a.block_rows, cur.s.n - j0) * a.G, cur.kv_head * a.G, cur.t, cur.s.tiles, 0};
+      a.cuts[blockIdx.x] = Cut{share, cur.s.lo + j0, min(a.block_rows, cur.s.n - j0) * a.G, cur.kv_head * a.G, cur.t, cur.s.tiles, {0, 0}};
     }
   } else {
     cur.b = blockIdx.z;
+    if (threadIdx.x == 0 && a.window == 0) asm volatile("prefetch.global.L1 [%0];" ::"l"(a.table + cur.b * a.table_ld));
     cur.s = sequence(a, cur.b);
     if (static_cast<int>(blockIdx.x) >= cur.s.blocks) return;
     cur.kv_head = blockIdx.y;
@@ -598,10 +600,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             pk[16 + i] = pack_bf16x2(f0, f1);
           }
           l = l * factor + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-          if (S::OWN_P && it > 1 && !warp_wait(&v_empty[(it - 2) % S::V_STAGES], ((it - 2) / S::V_STAGES) & 1, abort_flag, a.status, RLB_ERR_WAIT_TMEM_EMPTY)) {
-            ok = false;
-            break;
-          }
+          // (the product with what stood there has been completed: these scores were issued after it)
           tmem_st_32x32b_x32(tmem_base + S::P_COL + (it & 1) * S::P_STEP + lane_addr, pk);
           if (__any_sync(0xffffffffu, need)) {
             // O may be touched only after the previous product has completed (the next one waits for p_full)
@@ -637,7 +636,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         const float inv = l == 0.f ? 0.f : 1.f / l;
         if (there && !g.whole) a.part_ml[slot] = make_float2(m_ref, l);
         __nv_bfloat16* dst = a.out + (g.s.lo + j) * a.ldo + (g.kv_head * a.G + own_h) * D;
-#pragma unroll 1
+#pragma unroll 2
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           __syncwarp();
@@ -690,7 +689,7 @@ tree_join_kernel(const TreeArgs a) {
   const int c = blockIdx.y, r = blockIdx.x * JOIN_ROWS + threadIdx.x / (D / 8), d = (threadIdx.x % (D / 8)) * 8;
   const Cut cut = a.cuts[c];
   if (cut.before == 0 || cut.before > cut.share || r >= cut.rows) return;
-  const int last = c + static_cast<int>((cut.tiles - cut.before - 1) / cut.share);
+  const int last = c + (cut.tiles - cut.before - 1) / cut.share;
   float o[8] = {}, l = 0.f, top = -INFINITY;
 #pragma unroll 2
   for (int k = c - 1; k <= last; ++k) {      // the first one is its CTA's last part, the others their CTA's first
@@ -779,6 +778,7 @@ RLB_API int rlb_tree_decode(const void* q, long long ldq, const void* k, const v
   a.Hkv = Hkv;
   a.G = Hq / Hkv;
   a.block_rows = M_ROWS / a.G;
+  a.block_inv = 65536 / a.block_rows + 1;
   a.q_rows = a.block_rows < max_rows ? a.block_rows : max_rows;
   a.masks = masks;
   a.masks_ld = masks_ld;

@@ -219,6 +219,8 @@ def tree_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         plan = tree_plan(B, Hq, Hkv, max_rows, min(room, window + max_rows) if window else room)
     elif plan < 0 or plan > 65535:
         raise ValueError(f"plan is 0 to 65535 CTAs, not {plan}")
+    if plan and B * Hkv * -(-max_rows // (128 // (Hq // Hkv))) * ((min(room, window + max_rows) if window else room) // 64 + 2) > 0x7FFFFFFF:
+        plan = 0      # (more tiles than the kernel counts to)
     parts = sums = cuts = None
     if plan:
         size = tree_scratch_size(plan, Hq, Hkv, D, max_rows)
