@@ -38,7 +38,7 @@ struct TreeArgs {
   const int* ctx;
   const int* cu;
   int B, T, max_rows, Hq, Hkv, G;
-  int block_rows, block_inv, q_rows;      // tree rows of a block, 65536 / that and one, rows of a TMA box of queries
+  int block_rows, block_inv, group_inv, q_rows;      // tree rows of a block, 65536 / that and one, the same of G, rows of a TMA box of queries
   const int* masks;            // null: a row sees the rows up to itself
   long long masks_ld;
   const int* positions;        // with window > 0
@@ -46,7 +46,7 @@ struct TreeArgs {
   float scale_log2;
   __nv_bfloat16* out;
   long long ldo;
-  int vec;                     // rows of `out` start on 16 bytes
+  int vec;                     // rows of `out` start on 32 bytes
   const __nv_bfloat16* v;
   float* part_o;               // [2 CTAs][part_rows][D]: first and last part of a CTA; null: a CTA has a whole unit
   float2* part_ml;             // [2 CTAs][part_rows] maximum (log2) and sum
@@ -78,21 +78,33 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+// 32 bytes at once: whole sectors, although a warp's lanes write rows of their own.
+__device__ __forceinline__ void store32(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e, uint32_t f, uint32_t g, uint32_t h) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a), "r"(b), "r"(c), "r"(d), "r"(e), "r"(f), "r"(g), "r"(h) : "memory");
+}
 __device__ __forceinline__ float exp2_fast(float x) {      // relative error 2^-22
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Most waits have nothing to wait for: the rest of them is out of line (84 KB of instructions with all of it in place, for which a unit's few thousand ones that run once
+// came from the second level cache: some 6000 cycles).
+__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  return mbar_wait(bar, parity, abort_flag, status, code);
+}
+__device__ __forceinline__ bool one_wait(const uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  return mbar_try_wait(smem_u32(bar), parity) || wait_long(smem_u32(bar), parity, abort_flag, status, code);
+}
 // A whole warp waits: all of its lanes go on, or none.
 __device__ __forceinline__ bool warp_wait(const uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
-  return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, abort_flag, status, code));
+  return __all_sync(0xffffffffu, one_wait(bar, parity, abort_flag, status, code));
 }
 
 // A sequence's rows and keys, and its units' tiles.
 struct Seq {
   int lo, n, ctx, keys, first, tiles, blocks;      // first: the first tile that is in the window
 };
-__device__ __forceinline__ Seq sequence(const TreeArgs& a, int b) {
+__device__ __noinline__ Seq sequence(const TreeArgs& a, int b) {
   Seq s;
   s.lo = min(max(a.cu[b], 0), a.T);
   s.n = min(min(max(a.cu[b + 1], s.lo), a.T) - s.lo, a.max_rows);
@@ -177,15 +189,18 @@ struct Cursor {
 struct RowView {
   const int* mask;      // null: a chain
   int words, j, pos;
+  uint32_t w0, w1;      // its first two words
 };
 __device__ __forceinline__ uint64_t low_bits(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; }
-__device__ __forceinline__ uint64_t seen_keys(const TreeArgs& a, const Seq& s, const RowView& r, int k0) {
-  uint64_t v = low_bits(s.keys - k0);
-  const int base = k0 - s.ctx;      // row of the tree at bit 0
+__device__ __noinline__ uint64_t seen_keys(const TreeArgs& a, int ctx, int keys, int lo, int n, const RowView r, int k0) {
+  uint64_t v = low_bits(keys - k0);
+  const int base = k0 - ctx;      // row of the tree at bit 0
   if (base > -TILE) {
     uint64_t tree;
     const int from = max(base, 0);
-    if (r.mask) {
+    if (r.mask && from == 0) {
+      tree = r.w0 | static_cast<uint64_t>(r.w1) << 32;
+    } else if (r.mask) {
       const int w = from >> 5, sh = from & 31;
       const uint64_t w0 = w < r.words ? static_cast<uint32_t>(r.mask[w]) : 0u, w1 = w + 1 < r.words ? static_cast<uint32_t>(r.mask[w + 1]) : 0u,
                      w2 = w + 2 < r.words ? static_cast<uint32_t>(r.mask[w + 2]) : 0u;
@@ -197,11 +212,11 @@ __device__ __forceinline__ uint64_t seen_keys(const TreeArgs& a, const Seq& s, c
     v &= base < 0 ? low_bits(-base) | tree << -base : tree;
   }
   if (a.window > 0) {
-    const int behind = min(r.pos - a.window + 1, s.ctx) - k0;      // context keys before it are not in the window
+    const int behind = min(r.pos - a.window + 1, ctx) - k0;      // context keys before it are not in the window
     v &= ~low_bits(behind);
     if (base > -TILE) {
-      for (int i = max(0, -base); i < TILE && base + i < s.n; ++i)
-        if (r.pos - a.positions[s.lo + base + i] >= a.window) v &= ~(1ull << i);
+      for (int i = max(0, -base); i < TILE && base + i < n; ++i)
+        if (r.pos - a.positions[lo + base + i] >= a.window) v &= ~(1ull << i);
     }
   }
   return v;
@@ -215,6 +230,11 @@ __device__ __forceinline__ uint64_t without_pages(uint64_t v, int bad) {
   return v;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {      // of those that are numbers
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ bool not_finite(uint32_t w) { return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
 
 // Adds values that are not finite, of tiles that some row does not see as a whole, to the row that sees them: to its output, or to its part.
@@ -228,7 +248,7 @@ __device__ __noinline__ void add_special(const TreeArgs& a, const Segment g, con
       if (id < 0 || id >= a.blocks) lost |= 1 << (i >> 4);
     }
     if (k0 + TILE <= g.s.ctx && k0 >= edge && !lost) continue;
-    const uint64_t seen = without_pages(seen_keys(a, g.s, view, k0), lost);
+    const uint64_t seen = without_pages(seen_keys(a, g.s.ctx, g.s.keys, g.s.lo, g.s.n, view, k0), lost);
     for (int i = 0; i < TILE; ++i) {
       if (!(seen >> i & 1)) continue;
       const int id = a.table[g.b * a.table_ld + (k0 + i) / a.block];
@@ -241,6 +261,18 @@ __device__ __noinline__ void add_special(const TreeArgs& a, const Segment g, con
       }
     }
   }
+}
+
+// The first row of a sequence's box in the cache, -1 without a page, -2 behind the keys.
+__device__ __noinline__ int look(const TreeArgs& a, const int* table, int kv_head, int keys, int box) {
+  const long long key = static_cast<long long>(box) * a.box;
+  if (key >= keys) return -2;
+  const int k = static_cast<int>(key), page = a.block_shift >= 0 ? k >> a.block_shift : k / a.block, id = table[page];
+  if (id < 0 || id >= a.blocks) {
+    if (a.status) atomicCAS(a.status, 0, RLB_ERR_BOUNDS);
+    return -1;
+  }
+  return (id * a.Hkv + kv_head) * a.block + (k - page * a.block);
 }
 
 template <int D>
@@ -375,17 +407,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     for (int unit = 0; ok && cur.next(a, g); ++unit) {
       const int* table = a.table + g.b * a.table_ld;
       // lane i has the first row of box i of the next 32, and one more of those behind them
-      auto look = [&](int from) -> int {      // box `from` + lane of the sequence: its row in the cache, -1 without a page, -2 behind the keys
-        const long long key = (static_cast<long long>(from) + lane) * a.box;
-        if (key >= g.s.keys) return -2;
-        const int k = static_cast<int>(key), page = a.block_shift >= 0 ? k >> a.block_shift : k / a.block, id = table[page];
-        if (id < 0 || id >= a.blocks) {
-          if (a.status) atomicCAS(a.status, 0, RLB_ERR_BOUNDS);
-          return -1;
-        }
-        return (id * a.Hkv + g.kv_head) * a.block + (k - page * a.block);
-      };
-      int at = (g.s.first + g.t0) * boxes, rows = look(at), ahead = look(at + 32), used = 0;
+      int at = (g.s.first + g.t0) * boxes, rows = look(a, table, g.kv_head, g.s.keys, at + lane), ahead = -2, used = 0;
       if (unit > 0) ok = warp_wait(q_empty, (unit - 1) & 1, abort_flag, a.status, RLB_ERR_WAIT_EMPTY);
       if (!ok) break;
       if (elect_one()) {
@@ -400,7 +422,6 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           used = 0;
           at += 32;
           rows = ahead;
-          ahead = look(at + 32);
         }
         int row[4], lost = 0;
 #pragma unroll
@@ -410,6 +431,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           if (row[i] < 0) row[i] = end_row;
         }
         used += boxes;
+        const bool more = used == boxes;      // (the next ones while these are loaded)
         ok = warp_wait(&k_empty[ks], ((it / S::K_STAGES) & 1) ^ 1, abort_flag, a.status, RLB_ERR_WAIT_EMPTY);
         if (!ok) break;
         if (elect_one()) {
@@ -422,6 +444,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
               if (i < boxes) tma_load_2d(smem_u32(k_s + ks * S::KV_BYTES + c * S::KV_ATOM + i * a.box * 128), &tmap_k, smem_u32(&k_full[ks]), c * 64, row[i]);
         }
         __syncwarp();
+        if (more) ahead = look(a, table, g.kv_head, g.s.keys, at + 32 + lane);
         ok = warp_wait(&v_empty[vs], ((it / S::V_STAGES) & 1) ^ 1, abort_flag, a.status, RLB_ERR_WAIT_EMPTY);
         if (!ok) break;
         if (elect_one()) {
@@ -445,9 +468,9 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       constexpr uint32_t idesc_s = make_idesc_bf16(M_ROWS, TILE, false, false), idesc_o = make_idesc_bf16(M_ROWS, D, false, true);
       auto scores = [&](int it, bool last_of_unit) -> bool {      // its buffer held P of tile it - 2, whose product has to be complete
         const int ks = it % S::K_STAGES;
-        if (!S::OWN_P && it > 1 && !mbar_wait(smem_u32(&v_empty[(it - 2) % S::V_STAGES]), ((it - 2) / S::V_STAGES) & 1, abort_flag, a.status, RLB_ERR_WAIT_TMEM_EMPTY))
+        if (!S::OWN_P && it > 1 && !one_wait(&v_empty[(it - 2) % S::V_STAGES], ((it - 2) / S::V_STAGES) & 1, abort_flag, a.status, RLB_ERR_WAIT_TMEM_EMPTY))
           return false;
-        if (!mbar_wait(smem_u32(&k_full[ks]), (it / S::K_STAGES) & 1, abort_flag, a.status, RLB_ERR_WAIT_FULL)) return false;
+        if (!one_wait(&k_full[ks], (it / S::K_STAGES) & 1, abort_flag, a.status, RLB_ERR_WAIT_FULL)) return false;
         tc_fence_after();
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
@@ -463,38 +486,42 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       int it = 0;
       for (int unit = 0; ok && cur.next(a, g); ++unit) {
         const int n = g.t1 - g.t0;
-        ok = mbar_wait(smem_u32(q_full), unit & 1, abort_flag, a.status, RLB_ERR_WAIT_FULL) && scores(it, n == 1);
-        for (int t = 0; t < n && ok; ++t, ++it) {
-          const int vs = it % S::V_STAGES;
-          if (t + 1 < n && !scores(it + 1, t + 2 == n)) ok = false;
-          if (ok && t == 0 && unit > 0) ok = mbar_wait(smem_u32(o_empty), (unit - 1) & 1, abort_flag, a.status, RLB_ERR_WAIT_TMEM_EMPTY);
-          ok = ok && mbar_wait(smem_u32(&p_full[it & 1]), (it >> 1) & 1, abort_flag, a.status, RLB_ERR_WAIT_FLAG) &&
-               mbar_wait(smem_u32(&v_full[vs]), (it / S::V_STAGES) & 1, abort_flag, a.status, RLB_ERR_WAIT_FULL);
+        ok = one_wait(q_full, unit & 1, abort_flag, a.status, RLB_ERR_WAIT_FULL);
+        for (int t = -1; t < n && ok; ++t) {      // the scores of tile t + 1, the output of tile t
+          if (t + 1 < n && !scores(it + t + 1, t + 2 == n)) ok = false;
+          if (t < 0) continue;
+          const int i = it + t, vs = i % S::V_STAGES;
+          if (ok && t == 0 && unit > 0) ok = one_wait(o_empty, (unit - 1) & 1, abort_flag, a.status, RLB_ERR_WAIT_TMEM_EMPTY);
+          ok = ok && one_wait(&p_full[i & 1], (i >> 1) & 1, abort_flag, a.status, RLB_ERR_WAIT_FLAG) &&
+               one_wait(&v_full[vs], (i / S::V_STAGES) & 1, abort_flag, a.status, RLB_ERR_WAIT_FULL);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < TILE / 16; ++kk)      // 16 keys each, 8 columns of P
-            umma_f16_ts(tmem_o, tmem_base + S::P_COL + (it & 1) * S::P_STEP + kk * 8, make_smem_desc_sw128(smem_u32(v_s + vs * S::KV_BYTES) + kk * (16 * 128), S::KV_ATOM, 1024), idesc_o,
+            umma_f16_ts(tmem_o, tmem_base + S::P_COL + (i & 1) * S::P_STEP + kk * 8, make_smem_desc_sw128(smem_u32(v_s + vs * S::KV_BYTES) + kk * (16 * 128), S::KV_ATOM, 1024), idesc_o,
                         (t | kk) != 0 ? 1u : 0u);
           umma_commit(smem_u32(&v_empty[vs]));
         }
+        it += n;
       }
     }
   } else {
     // ------------------------------------------------------------ softmax: a thread per row
     const int quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
-    // scores are compared before scaling; a negative scale turns the comparison round
-    const int own_j = r / a.G, own_h = r % a.G;
+    const int own_j = (r * a.group_inv) >> 16, own_h = r - own_j * a.G;
     const bool neg = a.scale_log2 < 0.f;
-    const float hidden = neg ? INFINITY : -INFINITY;
+    const float hidden = neg ? INFINITY : -INFINITY, size = fabsf(a.scale_log2);
     bool ok = true;
     int it = 0;
     for (int unit = 0; ok && cur.next(a, g); ++unit) {
       const bool active = quarter * 32 < g.rows;      // of the warp
       const int j = min(g.j0 + own_j, g.s.n - 1);   // (rows behind the block's compute as its last one)
-      RowView view{a.masks ? a.masks + (g.s.lo + j) * a.masks_ld : nullptr, (a.max_rows + 31) >> 5, j, a.window > 0 ? max(a.positions[g.s.lo + j], g.s.ctx) : 0};
-      if (a.masks) asm volatile("prefetch.global.L1 [%0];" ::"l"(view.mask));
+      RowView view{a.masks ? a.masks + (g.s.lo + j) * a.masks_ld : nullptr, (a.max_rows + 31) >> 5, j, a.window > 0 ? max(a.positions[g.s.lo + j], g.s.ctx) : 0, 0u, 0u};
+      if (a.masks) {      // (on their way while the first tiles go by)
+        view.w0 = static_cast<uint32_t>(view.mask[0]);
+        view.w1 = view.words > 1 ? static_cast<uint32_t>(view.mask[1]) : 0u;
+      }
       int edge = 0;      // keys before it are out of some row's window
       if (a.window > 0) {
         int far = g.s.ctx;
@@ -512,6 +539,84 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         tc_fence_after();
         const int lost = bad[it % BAD_RING];
         const bool cut = k0 + TILE > g.s.ctx || k0 < edge || lost;      // some row does not see some key
+        if (active) {
+          uint32_t s0[32], s1[32];
+          tmem_ld_32x32b_x32(tmem_s, s0);
+          tmem_ld_32x32b_x32(tmem_s + 32, s1);
+          tmem_ld_wait();
+          if (cut) {
+            const uint64_t seen = without_pages(seen_keys(a, g.s.ctx, g.s.keys, g.s.lo, g.s.n, view, k0), lost);
+            const uint32_t lo = static_cast<uint32_t>(seen), hi = static_cast<uint32_t>(seen >> 32);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              if (!(lo >> i & 1)) s0[i] = __float_as_uint(hidden);
+              if (!(hi >> i & 1)) s1[i] = __float_as_uint(hidden);
+            }
+          }
+          if (neg) {      // scores are compared before scaling
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              s0[i] ^= 0x80000000u;
+              s1[i] ^= 0x80000000u;
+            }
+          }
+          float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            best[0] = max3(best[0], __uint_as_float(s0[i]), __uint_as_float(s0[i + 1]));
+            best[1] = max3(best[1], __uint_as_float(s0[i + 2]), __uint_as_float(s0[i + 3]));
+            best[2] = max3(best[2], __uint_as_float(s1[i]), __uint_as_float(s1[i + 1]));
+            best[3] = max3(best[3], __uint_as_float(s1[i + 2]), __uint_as_float(s1[i + 3]));
+          }
+          best[0] = max3(best[0], best[1], fmaxf(best[2], best[3]));
+          const float mx = best[0] * size;
+          float factor = 1.f;
+          bool need = false;
+          if (mx > m_ref + RESCALE || m_ref == -INFINITY) {
+            const float m_new = fmaxf(mx, m_ref);
+            if (m_new != -INFINITY) {
+              factor = m_ref == -INFINITY ? 0.f : exp2_fast(m_ref - m_new);
+              need = m_ref != -INFINITY;      // (nothing in O yet otherwise)
+              m_ref = m_new;
+            }
+          }
+          const float mr = m_ref == -INFINITY ? 0.f : -m_ref;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          uint32_t pk[32];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float e0 = exp2_fast(fmaf(__uint_as_float(s0[2 * i]), size, mr)), e1 = exp2_fast(fmaf(__uint_as_float(s0[2 * i + 1]), size, mr));
+            const float f0 = exp2_fast(fmaf(__uint_as_float(s1[2 * i]), size, mr)), f1 = exp2_fast(fmaf(__uint_as_float(s1[2 * i + 1]), size, mr));
+            sum[0] += e0;
+            sum[1] += e1;
+            sum[2] += f0;
+            sum[3] += f1;
+            pk[i] = pack_bf16x2(e0, e1);
+            pk[16 + i] = pack_bf16x2(f0, f1);
+          }
+          l = l * factor + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+          // (the product with what stood there has been completed: these scores were issued after it)
+          tmem_st_32x32b_x32(tmem_base + S::P_COL + (it & 1) * S::P_STEP + lane_addr, pk);
+          if (__any_sync(0xffffffffu, need)) {
+            // O may be touched only after the previous product has completed (the next one waits for p_full)
+            if (!warp_wait(&v_empty[(it - 1) % S::V_STAGES], ((it - 1) / S::V_STAGES) & 1, abort_flag, a.status, RLB_ERR_WAIT_TMEM_EMPTY)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld_32x32b_x32(tmem_o + lane_addr + c * 32, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+              tmem_st_32x32b_x32(tmem_o + lane_addr + c * 32, o);
+            }
+          }
+          tmem_st_wait();
+          tc_fence_before();
+        }
         if (cut) {
           const int vs = it % S::V_STAGES;
           if (!warp_wait(&v_full[vs], (it / S::V_STAGES) & 1, abort_flag, a.status, RLB_ERR_WAIT_FULL)) {
@@ -520,7 +625,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           }
           uint4* v = reinterpret_cast<uint4*>(v_s + vs * S::KV_BYTES);
           bool found = false;
-#pragma unroll
+#pragma unroll 2
           for (int i = 0; i < S::KV_BYTES / 16 / 128; ++i) {
             uint4 x = v[i * 128 + r];
             if (not_finite(x.x) || not_finite(x.y) || not_finite(x.z) || not_finite(x.w)) {
@@ -540,88 +645,6 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           }
           __syncwarp();
         }
-        if (active) {
-          uint32_t s0[32], s1[32];
-          tmem_ld_32x32b_x32(tmem_s, s0);
-          tmem_ld_32x32b_x32(tmem_s + 32, s1);
-          tmem_ld_wait();
-          if (cut) {
-            const uint64_t seen = without_pages(seen_keys(a, g.s, view, k0), lost);
-            const uint32_t lo = static_cast<uint32_t>(seen), hi = static_cast<uint32_t>(seen >> 32);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              if (!(lo >> i & 1)) s0[i] = __float_as_uint(hidden);
-              if (!(hi >> i & 1)) s1[i] = __float_as_uint(hidden);
-            }
-          }
-          float best[4] = {__uint_as_float(s0[0]), __uint_as_float(s0[1]), __uint_as_float(s1[0]), __uint_as_float(s1[1])};
-          if (!neg) {
-#pragma unroll
-            for (int i = 2; i < 32; i += 2) {
-              best[0] = fmaxf(best[0], __uint_as_float(s0[i]));
-              best[1] = fmaxf(best[1], __uint_as_float(s0[i + 1]));
-              best[2] = fmaxf(best[2], __uint_as_float(s1[i]));
-              best[3] = fmaxf(best[3], __uint_as_float(s1[i + 1]));
-            }
-            best[0] = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
-          } else {
-#pragma unroll
-            for (int i = 2; i < 32; i += 2) {
-              best[0] = fminf(best[0], __uint_as_float(s0[i]));
-              best[1] = fminf(best[1], __uint_as_float(s0[i + 1]));
-              best[2] = fminf(best[2], __uint_as_float(s1[i]));
-              best[3] = fminf(best[3], __uint_as_float(s1[i + 1]));
-            }
-            best[0] = fminf(fminf(best[0], best[1]), fminf(best[2], best[3]));
-          }
-          const float mx = best[0] * a.scale_log2;
-          float factor = 1.f;
-          bool need = false;
-          if (mx > m_ref + RESCALE || m_ref == -INFINITY) {
-            const float m_new = fmaxf(mx, m_ref);
-            if (m_new != -INFINITY) {
-              factor = m_ref == -INFINITY ? 0.f : exp2_fast(m_ref - m_new);
-              need = m_ref != -INFINITY;      // (nothing in O yet otherwise)
-              m_ref = m_new;
-            }
-          }
-          const float mr = m_ref == -INFINITY ? 0.f : -m_ref;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-          uint32_t pk[32];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float e0 = exp2_fast(fmaf(__uint_as_float(s0[2 * i]), a.scale_log2, mr)), e1 = exp2_fast(fmaf(__uint_as_float(s0[2 * i + 1]), a.scale_log2, mr));
-            const float f0 = exp2_fast(fmaf(__uint_as_float(s1[2 * i]), a.scale_log2, mr)), f1 = exp2_fast(fmaf(__uint_as_float(s1[2 * i + 1]), a.scale_log2, mr));
-            sum[0] += e0;
-            sum[1] += e1;
-            sum[2] += f0;
-            sum[3] += f1;
-            pk[i] = pack_bf16x2(e0, e1);
-            pk[16 + i] = pack_bf16x2(f0, f1);
-          }
-          l = l * factor + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-          // (the product with what stood there has been completed: these scores were issued after it)
-          tmem_st_32x32b_x32(tmem_base + S::P_COL + (it & 1) * S::P_STEP + lane_addr, pk);
-          if (__any_sync(0xffffffffu, need)) {
-            // O may be touched only after the previous product has completed (the next one waits for p_full)
-            if (!warp_wait(&v_empty[(it - 1) % S::V_STAGES], ((it - 1) / S::V_STAGES) & 1, abort_flag, a.status, RLB_ERR_WAIT_TMEM_EMPTY)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld_32x32b_x32(tmem_o + lane_addr + c * 32, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
-              tmem_st_32x32b_x32(tmem_o + lane_addr + c * 32, o);
-            }
-          }
-          tmem_st_wait();
-          tc_fence_before();
-        }
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&p_full[it & 1]));
       }
@@ -636,7 +659,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         const float inv = l == 0.f ? 0.f : 1.f / l;
         if (there && !g.whole) a.part_ml[slot] = make_float2(m_ref, l);
         __nv_bfloat16* dst = a.out + (g.s.lo + j) * a.ldo + (g.kv_head * a.G + own_h) * D;
-#pragma unroll 2
+#pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           __syncwarp();
@@ -644,10 +667,9 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           tmem_ld_wait();
           if (!there) continue;
           if (!g.whole) {
-            float4* to = reinterpret_cast<float4*>(a.part_o + slot * D + c * 32);
+            float* to = a.part_o + slot * D + c * 32;
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
-              to[q] = make_float4(__uint_as_float(o[4 * q]), __uint_as_float(o[4 * q + 1]), __uint_as_float(o[4 * q + 2]), __uint_as_float(o[4 * q + 3]));
+            for (int q = 0; q < 32; q += 8) store32(to + q, o[q], o[q + 1], o[q + 2], o[q + 3], o[q + 4], o[q + 5], o[q + 6], o[q + 7]);
             continue;
           }
           uint32_t w[16];
@@ -655,7 +677,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           for (int q = 0; q < 16; ++q) w[q] = pack_bf16x2(__uint_as_float(o[2 * q]) * inv, __uint_as_float(o[2 * q + 1]) * inv);
           if (a.vec) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(dst + c * 32 + q * 8) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+            for (int q = 0; q < 16; q += 8) store32(dst + c * 32 + q * 2, w[q], w[q + 1], w[q + 2], w[q + 3], w[q + 4], w[q + 5], w[q + 6], w[q + 7]);
           } else {
 #pragma unroll
             for (int q = 0; q < 16; ++q) {
@@ -749,8 +771,8 @@ int launch(const void* q, long long ldq, const void* k, const void* v, TreeArgs 
 }
 }  // namespace
 
-// ctas > 0: so many CTAs share all tiles, at least `least` each; part_o [2 ctas, part_rows, D] and part_ml [2 ctas, part_rows, 2] fp32 with part_rows = min(max_rows, 128 / G) * G, cuts 32 bytes
-// for each CTA.
+// ctas > 0: so many CTAs share all tiles, at least `least` each; part_o [2 ctas, part_rows, D] and part_ml [2 ctas, part_rows, 2] fp32 with part_rows = min(max_rows, 128 / G) * G, on 32 bytes,
+// cuts 32 bytes for each CTA.
 // ctas 0: a CTA for each unit. q: rows on 16 bytes.
 RLB_API int rlb_tree_decode(const void* q, long long ldq, const void* k, const void* v, int blocks, int block, const int* table, long long table_ld, int pages,
                             const int* ctx, const int* cu, int B, int T, int max_rows, int Hq, int Hkv, int D, const int* masks, long long masks_ld,
@@ -779,6 +801,7 @@ RLB_API int rlb_tree_decode(const void* q, long long ldq, const void* k, const v
   a.G = Hq / Hkv;
   a.block_rows = M_ROWS / a.G;
   a.block_inv = 65536 / a.block_rows + 1;
+  a.group_inv = 65536 / a.G + 1;
   a.q_rows = a.block_rows < max_rows ? a.block_rows : max_rows;
   a.masks = masks;
   a.masks_ld = masks_ld;
@@ -788,7 +811,7 @@ RLB_API int rlb_tree_decode(const void* q, long long ldq, const void* k, const v
   a.scale_log2 = fabsf(scale) < 1e-30f ? copysignf(1e-30f, scale) : scale * LOG2E_F;
   a.out = static_cast<__nv_bfloat16*>(out);
   a.ldo = ldo;
-  a.vec = ldo % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  a.vec = ldo % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 32 == 0;
   a.v = static_cast<const __nv_bfloat16*>(v);
   a.part_o = ctas ? part_o : nullptr;
   a.part_ml = reinterpret_cast<float2*>(part_ml);

@@ -155,7 +155,7 @@ def tree_plan(B: int, Hq: int, Hkv: int, max_rows: int, max_len: int, sm_count: 
 
 def tree_scratch_size(ctas: int, Hq: int, Hkv: int, D: int, max_rows: int) -> int:
     """Floats of the scratch tensor of :func:`tree_paged_decode` with this many CTAs."""
-    return 2 * ctas * min(max_rows, 128 // (Hq // Hkv)) * (Hq // Hkv) * (D + 2) + 12 * ctas
+    return 2 * ctas * min(max_rows, 128 // (Hq // Hkv)) * (Hq // Hkv) * (D + 2) + 16 * ctas
 
 
 def tree_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, ctx_lens: torch.Tensor, cu_rows: torch.Tensor,
@@ -226,11 +226,11 @@ def tree_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         size = tree_scratch_size(plan, Hq, Hkv, D, max_rows)
         if scratch is None:
             scratch = torch.empty(size, dtype=torch.float32, device=device)
-        elif scratch.dtype is not torch.float32 or not scratch.is_contiguous() or scratch.numel() < size or scratch.data_ptr() % 16 or scratch.device != device:
-            raise ValueError(f"scratch is a contiguous float32 tensor of {size} elements on {device} that starts on 16 bytes")
+        elif scratch.dtype is not torch.float32 or not scratch.is_contiguous() or scratch.numel() < size or scratch.data_ptr() % 32 or scratch.device != device:
+            raise ValueError(f"scratch is a contiguous float32 tensor of {size} elements on {device} that starts on 32 bytes")
         cuts = scratch.data_ptr()
-        parts = cuts + 48 * plan
-        sums = parts + (size - 12 * plan) // (D + 2) * D * 4
+        parts = cuts + 64 * plan
+        sums = parts + (size - 16 * plan) // (D + 2) * D * 4
     with torch.cuda.device(device):
         if q.stride(1) != 1 or q.stride(0) % 8 or q.data_ptr() % 16:      # rows that do not start on 16 bytes
             q = q[:, :width].clone(memory_format=torch.contiguous_format)
