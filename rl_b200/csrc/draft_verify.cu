@@ -188,7 +188,7 @@ __device__ __forceinline__ double power(const double* table, double t, double r)
   return fma(s, p, s);
 }
 // log2 of a sum: 32 bits, then one step on 2^-l s = 1 + d.
-__device__ __forceinline__ double log2_of(const double* table, double s) {
+__device__ __noinline__ double log2_of(const double* table, double s) {
   const int hi = __double2hiint(s), e = (hi >> 20) - 1023;
   const double f = __hiloint2double((hi & 0xfffff) | 0x3ff00000, __double2loint(s));
   const double l = static_cast<double>(__log2f(static_cast<float>(f))), t = MAGIC - l, d = fma(f, power(table, t, -l - (t - MAGIC)), -1.0);
@@ -204,7 +204,12 @@ struct Frame {
   double add;          // MAGIC - N
   float top, low;      // logits below `low` weigh nothing (2^-1000 of top's)
   int kind;            // 0: what is below `low` may be taken as `low` in a sum; 1: it may not; 2: so far apart are the logits (top c beyond 2^42) that top's equals alone have weight
-  __device__ __forceinline__ void set(float x, const Temperature& q) {
+  static __device__ __noinline__ Frame frame_of(float x, const Temperature q) {
+    Frame f;
+    f.set(x, q);
+    return f;
+  }
+  __device__ __forceinline__ void set(float x, const Temperature q) {
     top = x;
     low = fmaxf(fminf(__fsub_ru(x, q.far), x), -F_MAX);
     const double m = lowered(x) * q.c, n = (m + 256 * MAGIC) - 256 * MAGIC;
@@ -217,21 +222,21 @@ struct Frame {
     return static_cast<uint32_t>(__double2hiint(d)) <= 0xc090e000u ? v * __hiloint2double((1123 + __double2loint(d + 256 * MAGIC)) << 20, 0) * 0x1p-100 : 0.0;      // (-1080)
   }
   __device__ __forceinline__ void move(float x, const Temperature& q, double& total) {
-    const double before = add;
-    const bool first = top == -INFINITY;
-    set(x, q);
-    total = first ? 0.0 : moved(total, before, add);
+    const Frame before = *this;
+    *this = frame_of(x, q);
+    total = before.top == -INFINITY ? 0.0 : moved(total, before.add, add);
   }
   __device__ __forceinline__ double depth(double c, float x) const { return kind == 2 ? 0.0 : fma(lowered(x), c, add - MAGIC); }      // x c - N
   __device__ __forceinline__ double near(const double* table, double c, float x) const {
     const double v = lowered(x), t = fma(v, c, add);
     return power(table, t, fma(v, c, add - t));
   }
-  __device__ __forceinline__ double operator()(const double* table, double c, float x) const {
-    return !(x >= low) ? 0.0 : kind == 2 ? (x == top ? 1.0 : 0.0) : near(table, c, x);
-  }
 };
 
+// One weight in a frame of any kind.
+__device__ __noinline__ double weight_of(const Frame* f, const double* table, double c, float x) {
+  return !(x >= f->low) ? 0.0 : f->kind == 2 ? (x == f->top ? 1.0 : 0.0) : f->near(table, c, x);
+}
 __device__ __forceinline__ void push_d(uint32_t addr, double v) { asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory"); }
 
 struct Part {      // of a warp's range, target and draft: sum of weights in its frame, the frame's MAGIC - N and logit (-inf: none)
@@ -253,7 +258,7 @@ struct RowLogits {
     if (g < g1 && vec && e >= 0 && e + VEC <= V) return __ldg(reinterpret_cast<const uint4*>(p + e));
     return edge(p, e, g < g1 ? V : 0);
   }
-  static __device__ __noinline__ uint4 edge(const T* p, int e, int V) {
+  static __device__ __noinline__ uint4 edge(const T* p, int e, int V) {      // (a call waits for what it loads)
     uint4 v;
     uint32_t* w = &v.x;
     if (sizeof(T) == 4) {
@@ -278,7 +283,10 @@ struct RowLogits {
   static __device__ __noinline__ double seldom(uint4 v, Frame f, const double* table, double c) {      // a group's weights in frames of the other kinds
     double t = 0.0;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) t += f(table, c, element(v, i));
+    for (int i = 0; i < VEC; ++i) {
+      const float x = element(v, i);
+      t += !(x >= f.low) ? 0.0 : f.kind == 2 ? (x == f.top ? 1.0 : 0.0) : f.near(table, c, x);
+    }
     return t;
   }
   __device__ __forceinline__ float at(int i) const { return usable(static_cast<float>(p[i])); }
@@ -288,6 +296,135 @@ struct RowSum {      // of all parts
   Frame f;
   double inv, sum;      // the sum's reciprocal (0: no logit above -inf)
 };
+
+// A visited row: its logits, the draft's, and what its sums and rejections came to (in shared memory).
+template <typename T, bool DRAFT>
+struct Visit {
+  RowLogits<T> z, d;
+  const RowSum* row;      // [1 + DRAFT]
+  const double* table;
+  const double* grow;
+  const int* gone;
+  double c;
+};
+// What is left of the probability of token i after `r` rejections, from its logits.
+template <typename T, bool DRAFT>
+__device__ __noinline__ double rest_of(const Visit<T, DRAFT>& v, int i, float x, float y, int r) {
+  double w = weight_of(&v.row[0].f, v.table, v.c, x) * v.row[0].inv;
+  if (r == 0) return w;
+  if (DRAFT) {
+    const double g = weight_of(&v.row[DRAFT].f, v.table, v.c, y) * v.row[DRAFT].inv;
+#pragma unroll 1
+    for (int k = 0; k < r; ++k) w = fmax(fma(w, v.grow[k], -g), 0.0);
+  } else {
+#pragma unroll 1
+    for (int k = 0; k < r; ++k) w = v.gone[k] == i ? 0.0 : w;
+  }
+  return w;
+}
+// The same of the tokens from e0 to e1, summed over the warp.
+template <typename T, bool DRAFT>
+__device__ __noinline__ double sum_of(const Visit<T, DRAFT>& v, int e0, int e1, int r) {
+  double sum = 0.0;
+  int e = e0 + (threadIdx.x & 31);
+  float x[4], y[4];
+  auto fetch = [&](int from) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = from + 32 * k;
+      x[k] = i < e1 ? v.z.at(i) : -INFINITY;
+      y[k] = DRAFT && i < e1 ? v.d.at(i) : 0.f;
+    }
+  };
+  const Frame f = v.row[0].f;
+  if (f.kind == 0 && (!DRAFT || r == 0)) {      // as in the row's own sums
+    const double inv = v.row[0].inv, c = v.c;
+    const double* table = v.table;
+#pragma unroll 1
+    for (; e < e1; e += 128) {
+      fetch(e);
+      double w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = x[k] >= f.low ? f.near(table, c, x[k]) : 0.0;
+#pragma unroll 1
+      for (int g = 0; g < r; ++g) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = v.gone[g] == e + 32 * k ? 0.0 : w[k];
+      }
+      sum += (w[0] + w[1]) + (w[2] + w[3]);
+    }
+    return warp_sum_d(sum) * inv;
+  }
+#pragma unroll 1
+  for (; e < e1; e += 128) {
+    fetch(e);
+    sum += rest_of<T, DRAFT>(v, e, x[0], y[0], r);
+    if (e + 32 < e1) sum += rest_of<T, DRAFT>(v, e + 32, x[1], y[1], r);
+    if (e + 64 < e1) sum += rest_of<T, DRAFT>(v, e + 64, x[2], y[2], r);
+    if (e + 96 < e1) sum += rest_of<T, DRAFT>(v, e + 96, x[3], y[3], r);
+  }
+  return warp_sum_d(sum);
+}
+// The same of the groups from g0 to g1 of a row and its draft's, both of kind 0 and without infinities: as in the row's own sums.
+template <typename T>
+__device__ __noinline__ double sum_left(const Visit<T, true>& v, int g0, int g1, int r) {
+  constexpr int VEC = RowLogits<T>::VEC;
+  const int lane = threadIdx.x & 31;
+  const RowLogits<T> z = v.z, d = v.d;
+  const Frame p = v.row[0].f, q = v.row[1].f;
+  const double inv = v.row[0].inv, dinv = v.row[1].inv, c = v.c;
+  const double* table = v.table;
+  double even = 0.0, odd = 0.0;
+  uint4 x = z.load(g0 + lane, g1), y = d.load(g0 + lane, g1);
+#pragma unroll 1
+  for (int g = g0; g < g1; g += 32) {
+    const uint4 xx = x, yy = y;
+    if (g + 32 < g1) {
+      x = z.load(g + 32 + lane, g1);
+      y = d.load(g + 32 + lane, g1);
+    }
+    double w[VEC], e[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      w[i] = p.near(table, c, fmaxf(RowLogits<T>::raw(xx, i), p.low)) * inv;
+      e[i] = q.near(table, c, fmaxf(RowLogits<T>::raw(yy, i), q.low)) * dinv;
+    }
+#pragma unroll 1
+    for (int k = 0; k < r; ++k) {
+      const double grow = v.grow[k];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) w[i] = fmax(fma(w[i], grow, -e[i]), 0.0);
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) {
+      even += w[i];
+      odd += w[i + 1];
+    }
+  }
+  return warp_sum_d(even + odd);
+}
+// The token of [e0, e1) at which the running sum from `start` passes `aim` (none: the last with a share; -1: none has). By a warp.
+template <typename T, bool DRAFT>
+__device__ __noinline__ int find_token(const Visit<T, DRAFT>& v, int e0, int e1, int r, double start, double aim, bool inside) {
+  const int lane = threadIdx.x & 31;
+  int last = -1;
+#pragma unroll 1
+  for (int e = e0; e < e1; e += 32) {
+    const int i = e + lane;
+    const double w = i < e1 ? rest_of<T, DRAFT>(v, i, v.z.at(i), DRAFT ? v.d.at(i) : 0.f, r) : 0.0;
+    double run = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double u = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += u;
+    }
+    const unsigned over = __ballot_sync(0xffffffffu, inside && w > 0.0 && start + run > aim), any = __ballot_sync(0xffffffffu, w > 0.0);
+    if (over) return e + __ffs(over) - 1;
+    if (any) last = e + 31 - __clz(any);
+    start += __shfl_sync(0xffffffffu, run, 31);
+  }
+  return last;
+}
 
 template <typename T, bool DRAFT>
 __global__ void __launch_bounds__(DV_THREADS, 2)
@@ -483,8 +620,7 @@ verify_kernel(const VerifyArgs a) {
           m[k] = lane * 4 + k < W ? got[k].peak : -INFINITY;
           top = fmaxf(top, m[k]);
         }
-        Frame whole;
-        whole.set(warp_top(top), tp);
+        const Frame whole = Frame::frame_of(warp_top(top), tp);
         double v[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {      // of rows with one logit far above the others the parts that have it
@@ -516,63 +652,8 @@ verify_kernel(const VerifyArgs a) {
         __syncwarp();
       }
       if (DRAFT) __syncthreads();
-      // what is left of the probability of a token after `r` rejections, from its logits
-      auto rest = [&](int i, float x, float y, int r) {
-        double w = row[0].f(table, tp.c, x) * row[0].inv;
-        if (DRAFT) {
-          if (r > 0) {
-            const double g = row[DRAFT].f(table, tp.c, y) * row[DRAFT].inv;
-            for (int k = 0; k < r; ++k) w = fmax(fma(w, grow[k], -g), 0.0);
-          }
-        } else {
-          for (int k = 0; k < r; ++k) w = gone[k] == i ? 0.0 : w;
-        }
-        return w;
-      };
-      const bool simple = DRAFT && row[0].f.kind == 0 && row[DRAFT].f.kind == 0 && row[0].f.top < 0.5f * F_MAX && row[DRAFT].f.top < 0.5f * F_MAX;
-      auto sum_rest = [&](int g0, int g1, int r) {
-        double v = 0.0;
-        if (simple) {      // as in the row's own sums
-          const Frame p = row[0].f, q = row[DRAFT].f;
-          const double inv = row[0].inv, dinv = row[DRAFT].inv;
-          if (g0 < g1) fetch(g0, g1);
-          for (int g = g0; g < g1; g += STEP) {
-            uint4 wz[LOADS], wd[LOADS];
-#pragma unroll
-            for (int u = 0; u < LOADS; ++u) {
-              wz[u] = vz[u];
-              wd[u] = vd[DRAFT ? u : 0];
-            }
-            if (g + STEP < g1) fetch(g + STEP, g1);
-#pragma unroll
-            for (int u = 0; u < LOADS; ++u)
-#pragma unroll
-              for (int i = 0; i < VEC; ++i) {
-                double w = p.near(table, tp.c, fmaxf(Row::raw(wz[u], i), p.low)) * inv;
-                const double e = q.near(table, tp.c, fmaxf(Row::raw(wd[u], i), q.low)) * dinv;
-                for (int k = 0; k < r; ++k) w = fmax(fma(w, grow[k], -e), 0.0);
-                v += w;
-              }
-          }
-          return warp_sum_d(v);
-        }
-        uint4 x = z.load(g0 + lane, g1), y = DRAFT ? d.load(g0 + lane, g1) : x;
-        for (int g = g0; g < g1; g += 32) {
-          const uint4 xx = x, yy = y;
-          if (g + 32 < g1) {
-            x = z.load(g + 32 + lane, g1);
-            y = DRAFT ? d.load(g + 32 + lane, g1) : x;
-          }
-          double even = 0.0, odd = 0.0;
-#pragma unroll
-          for (int i = 0; i < VEC; i += 2) {
-            even += rest((g + lane) * VEC - z.shift + i, Row::element(xx, i), Row::element(yy, i), r);
-            odd += rest((g + lane) * VEC - z.shift + i + 1, Row::element(xx, i + 1), Row::element(yy, i + 1), r);
-          }
-          v += even + odd;
-        }
-        return warp_sum_d(v);
-      };
+      Visit<T, DRAFT> visit{z, d, row, table, grow, gone, tp.c};
+      const int e0 = max(0, g0 * VEC - z.shift), e1 = min(a.V, g1 * VEC - z.shift);      // the range's tokens
       double mine[4], total = 0.0;
       auto take = [&](double v) {      // this warp's part of new sums; the parts and the whole sum of all
         begin();
@@ -595,8 +676,8 @@ verify_kernel(const VerifyArgs a) {
               continue;
             }
             if (t < 0 || t >= a.V) continue;      // has no probability, and is none of the draft's
-            const double w = rest(t, lz[j], DRAFT ? ld[j] : 0.f, r);
-            const double g = DRAFT ? row[DRAFT].f(table, tp.c, ld[j]) * row[DRAFT].inv : 1.0;
+            const double w = rest_of<T, DRAFT>(visit, t, lz[j], DRAFT ? ld[j] : 0.f, r);
+            const double g = DRAFT ? weight_of(&row[DRAFT].f, table, tp.c, ld[j]) * row[DRAFT].inv : 1.0;
             if (static_cast<double>(num[j]) * g * left[r] < w) {
               v = j;
             } else if (DRAFT) {
@@ -619,7 +700,10 @@ verify_kernel(const VerifyArgs a) {
           break;
         }
         ++rejected;
-        take(sum_rest(g0, g1, rejected));
+        if constexpr (DRAFT) {
+          const bool simple = row[0].f.kind == 0 && row[1].f.kind == 0 && row[0].f.top < 0.5f * F_MAX && row[1].f.top < 0.5f * F_MAX;
+          take(simple ? sum_left<T>(visit, g0, g1, rejected) : sum_of<T, DRAFT>(visit, e0, e1, rejected));
+        }
         if (tid == 0) {
           left[rejected] = total;
           grow[rejected] = 1.0 / total;
@@ -667,7 +751,7 @@ verify_kernel(const VerifyArgs a) {
             const int g = (gone[k] + z.shift) / VEC;
             hit |= g >= g0 && g < g1;
           }
-          take(hit ? sum_rest(g0, g1, rejected) : share[me]);
+          take(hit ? sum_of<T, DRAFT>(visit, e0, e1, rejected) : share[me]);
         }
       }
       if (rejected == 0 || !(total > 0.0)) {      // (nothing is left: from p itself)
@@ -706,9 +790,9 @@ verify_kernel(const VerifyArgs a) {
         owner = __shfl_sync(0xffffffffu, last, 31 - __clz(any));
       }
       if (rank == owner / DV_WARPS) {      // the range once more, by all warps of its CTA
-        const int r0 = min(groups, owner * groups_per), r1 = min(groups, r0 + groups_per), piece = (r1 - r0 + DV_WARPS - 1) / DV_WARPS;
-        const int q0 = min(r1, r0 + warp * piece), q1 = min(r1, q0 + piece);
-        const double own = sum_rest(q0, q1, rejected);
+        const int r0 = max(0, min(groups, owner * groups_per) * VEC - z.shift), r1 = min(a.V, (owner + 1) * groups_per * VEC - z.shift);
+        const int piece = (r1 - r0 + DV_WARPS - 1) / DV_WARPS, q0 = min(r1, r0 + warp * piece), q1 = min(r1, q0 + piece);
+        const double own = sum_of<T, DRAFT>(visit, q0, q1, rejected);
         if (lane == 0) pieces[warp] = own;
         __syncthreads();
         int mover = -1, filled = -1;
@@ -726,40 +810,7 @@ verify_kernel(const VerifyArgs a) {
         }
         const bool inside = mover >= 0;      // (otherwise the last that has a share)
         if (warp == (inside ? mover : filled)) {
-          int hit = -1, end = 0;
-          for (int g = q0; g < q1 && hit < 0; g += 32) {
-            const int e = (g + lane) * VEC - z.shift;
-            const uint4 x = z.load(g + lane, q1), y = DRAFT ? d.load(g + lane, q1) : x;
-            double w[VEC], own = 0.0;
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-              w[i] = rest(e + i, Row::element(x, i), Row::element(y, i), rejected);
-              own += w[i];
-            }
-            double sofar = own;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-              const double v = __shfl_up_sync(0xffffffffu, sofar, o);
-              if (lane >= o) sofar += v;
-            }
-            double at_lane = __shfl_up_sync(0xffffffffu, sofar, 1);
-            if (lane == 0) at_lane = 0.0;
-            at_lane += start;
-            int pass = -1, has = -1;
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-              at_lane += w[i];
-              if (w[i] > 0.0) {
-                has = e + i;
-                if (pass < 0 && inside && at_lane > aim) pass = e + i;
-              }
-            }
-            const unsigned passed = __ballot_sync(0xffffffffu, pass >= 0), there = __ballot_sync(0xffffffffu, has >= 0);
-            if (there) end = __shfl_sync(0xffffffffu, has, 31 - __clz(there));
-            if (passed) hit = __shfl_sync(0xffffffffu, pass, __ffs(passed) - 1);
-            start += __shfl_sync(0xffffffffu, sofar, 31);
-          }
-          if (hit < 0) hit = end;
+          const int hit = max(0, find_token<T, DRAFT>(visit, q0, q1, rejected, start, aim, inside));
           if (lane == 0) {
             drawn = hit;
             drawn_z = z.at(hit);

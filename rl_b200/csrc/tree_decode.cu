@@ -52,6 +52,7 @@ struct TreeArgs {
   float2* part_ml;             // [2 CTAs][part_rows] maximum (log2) and sum
   Cut* cuts;                   // [CTAs]
   int part_rows, least;        // least: tiles of a share at least
+  int sorted;                  // whole units: in order of their sequences' lengths (at most THREADS of them)
   int* status;
 };
 
@@ -235,6 +236,20 @@ __device__ __forceinline__ float max3(float a, float b, float c) {      // of th
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+// Two at a time.
+__device__ __forceinline__ uint64_t pair(float a, float b) { return static_cast<uint64_t>(__float_as_uint(b)) << 32 | __float_as_uint(a); }
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float low_of(uint64_t a) { return __uint_as_float(static_cast<uint32_t>(a)); }
+__device__ __forceinline__ float high_of(uint64_t a) { return __uint_as_float(static_cast<uint32_t>(a >> 32)); }
 __device__ __forceinline__ bool not_finite(uint32_t w) { return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
 
 // Adds values that are not finite, of tiles that some row does not see as a whole, to the row that sees them: to its output, or to its part.
@@ -372,6 +387,22 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     }
   } else {
     cur.b = blockIdx.z;
+    if (a.sorted) {      // the longest sequences' units first: the last ones to run are short
+      int* keys = reinterpret_cast<int*>(smem);      // (the loads' place)
+      const int b = threadIdx.x;
+      int mine = 0;
+      if (b < a.B) {
+        const Seq s = sequence(a, b);
+        keys[b] = mine = s.n > 0 ? s.tiles : 0;
+      }
+      __syncthreads();
+      int before = 0;
+      for (int i = 0; i < a.B; ++i) before += keys[i] > mine || (keys[i] == mine && i < b);
+      if (b < a.B && before == static_cast<int>(blockIdx.z)) start[0] = b;
+      __syncthreads();
+      cur.b = start[0];
+      fence_proxy_async();
+    }
     if (threadIdx.x == 0 && a.window == 0) asm volatile("prefetch.global.L1 [%0];" ::"l"(a.table + cur.b * a.table_ld));
     cur.s = sequence(a, cur.b);
     if (static_cast<int>(blockIdx.x) >= cur.s.blocks) return;
@@ -581,20 +612,21 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             }
           }
           const float mr = m_ref == -INFINITY ? 0.f : -m_ref;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint64_t size2 = pair(size, size), mr2 = pair(mr, mr);
+          uint64_t sum[2] = {0ull, 0ull};
           uint32_t pk[32];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float e0 = exp2_fast(fmaf(__uint_as_float(s0[2 * i]), size, mr)), e1 = exp2_fast(fmaf(__uint_as_float(s0[2 * i + 1]), size, mr));
-            const float f0 = exp2_fast(fmaf(__uint_as_float(s1[2 * i]), size, mr)), f1 = exp2_fast(fmaf(__uint_as_float(s1[2 * i + 1]), size, mr));
-            sum[0] += e0;
-            sum[1] += e1;
-            sum[2] += f0;
-            sum[3] += f1;
+            const uint64_t x = fma_pair(pair(__uint_as_float(s0[2 * i]), __uint_as_float(s0[2 * i + 1])), size2, mr2);
+            const uint64_t y = fma_pair(pair(__uint_as_float(s1[2 * i]), __uint_as_float(s1[2 * i + 1])), size2, mr2);
+            const float e0 = exp2_fast(low_of(x)), e1 = exp2_fast(high_of(x)), f0 = exp2_fast(low_of(y)), f1 = exp2_fast(high_of(y));
+            sum[0] = add_pair(sum[0], pair(e0, e1));
+            sum[1] = add_pair(sum[1], pair(f0, f1));
             pk[i] = pack_bf16x2(e0, e1);
             pk[16 + i] = pack_bf16x2(f0, f1);
           }
-          l = l * factor + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+          sum[0] = add_pair(sum[0], sum[1]);
+          l = l * factor + (low_of(sum[0]) + high_of(sum[0]));
           // (the product with what stood there has been completed: these scores were issued after it)
           tmem_st_32x32b_x32(tmem_base + S::P_COL + (it & 1) * S::P_STEP + lane_addr, pk);
           if (__any_sync(0xffffffffu, need)) {
@@ -818,6 +850,8 @@ RLB_API int rlb_tree_decode(const void* q, long long ldq, const void* k, const v
   a.part_rows = a.q_rows * a.G;
   a.cuts = static_cast<Cut*>(cuts);
   a.least = least;
+  // (more units than run at once)
+  a.sorted = !ctas && B > 1 && B <= THREADS && static_cast<long long>(B) * Hkv * ((max_rows + a.block_rows - 1) / a.block_rows) > 2 * 148;
   a.status = status;
   return D == 64 ? launch<64>(q, ldq, k, v, a, ctas, static_cast<cudaStream_t>(stream)) : launch<128>(q, ldq, k, v, a, ctas, static_cast<cudaStream_t>(stream));
 }

@@ -149,8 +149,10 @@ def _tree_decode_ref(q, k_cache, v_cache, table, ctx, spans, Hq, Hkv, D, masks, 
 @lru_cache(maxsize=4096)
 def tree_plan(B: int, Hq: int, Hkv: int, max_rows: int, max_len: int, sm_count: int = 148) -> int:
     """CTAs that share all tiles of 64 keys evenly in :func:`tree_paged_decode`, or 0: a CTA for each sequence, key/value head and block of 128 / (Hq / Hkv) rows."""
-    units, tiles = B * Hkv * -(-max_rows // (128 // (Hq // Hkv))), -(-max_len // 64)
-    return 0 if tiles <= 4 or units >= 6 * sm_count else 2 * sm_count
+    units, tiles, slots = B * Hkv * -(-max_rows // (128 // (Hq // Hkv))), -(-max_len // 64), 2 * sm_count
+    if units > slots:
+        return 0 if units <= 2 * slots and min(max_rows, 128 // (Hq // Hkv)) * (Hq // Hkv) >= 64 else slots
+    return slots if tiles * (slots - units) > 6 * slots else 0
 
 
 def tree_scratch_size(ctas: int, Hq: int, Hkv: int, D: int, max_rows: int) -> int:
