@@ -36,6 +36,7 @@ BF16 = torch.bfloat16
 HEAD_DIMS = (64, 128)
 MAX_ROWS = 256
 COLDEST = torch.finfo(torch.float32).tiny
+MAX_SCALE = torch.finfo(torch.float32).max
 MAX_TOKENS = 0x7FFF0000      # of a sequence: places are 32-bit numbers
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else lambda index: torch.cuda.current_stream(index).cuda_stream
 
@@ -44,6 +45,16 @@ def _same_device(device: torch.device, *ts: Optional[torch.Tensor]) -> None:
     for t in ts:
         if t is not None and t.device != device:
             raise ValueError(f"tensors on several devices: {device} and {t.device}")
+
+
+def _launch(device: torch.device, name: str, *args) -> None:
+    """Enqueues on the device's current stream, whichever device is the current one; the status word and the stream are the entry's last arguments."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        call(name, *args, _L.status_word(device).data_ptr(), _raw_stream(index))
+        return
+    with torch.cuda.device(index):
+        call(name, *args, _L.status_word(device).data_ptr(), _raw_stream(index))
 
 
 def _ints(t: torch.Tensor, shape: tuple, what: str) -> torch.Tensor:
@@ -110,12 +121,9 @@ def tree_rows(parents: torch.Tensor, cu_rows: torch.Tensor, ctx_lens: torch.Tens
                 if 0 <= place < room:
                     slots[lo + j] = int(table[b, place // block_size]) * block_size + place % block_size
         return masks, positions, slots
-    with torch.cuda.device(device):
-        masks = torch.empty((T, words), dtype=torch.int32, device=device)
-        positions = torch.empty(T, dtype=torch.int32, device=device)
-        slots = torch.empty(T, dtype=torch.int64, device=device)
-        call("rlb_tree_rows", parents.data_ptr(), cu.data_ptr(), ctx.data_ptr(), table.data_ptr(), table.stride(0), table.shape[1], block_size, B, T, max_rows, words,
-             masks.data_ptr(), positions.data_ptr(), slots.data_ptr(), _L.status_word(device).data_ptr(), _raw_stream(device.index))
+    masks, positions, slots = parents.new_empty((T, words)), parents.new_empty(T), parents.new_empty(T, dtype=torch.int64)
+    _launch(device, "rlb_tree_rows", parents.data_ptr(), cu.data_ptr(), ctx.data_ptr(), table.data_ptr(), table.stride(0), table.shape[1], block_size, B, T, max_rows, words,
+            masks.data_ptr(), positions.data_ptr(), slots.data_ptr())
     return masks, positions, slots
 
 
@@ -179,13 +187,14 @@ def tree_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         raise ValueError(f"heads of {HEAD_DIMS} dimensions, not {D}")
     if Hkv < 1 or Hq < 1 or Hq % Hkv or Hq // Hkv > 128 or q.dim() != 2 or q.shape[1] < width:
         raise ValueError(f"q is [T, {width}] with {Hq} heads, 1 to 128 times {Hkv}, not {tuple(q.shape)}")
-    T = q.shape[0]
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1] != Hkv or k_cache.shape[3] != D or not k_cache.is_contiguous() or not v_cache.is_contiguous():
-        raise ValueError(f"the caches are contiguous [blocks, {Hkv}, block size, {D}], not {tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
-    block = k_cache.shape[2]
+    T, shape = q.shape[0], k_cache.shape
+    if len(shape) != 4 or shape != v_cache.shape or shape[1] != Hkv or shape[3] != D or not k_cache.is_contiguous() or not v_cache.is_contiguous():
+        raise ValueError(f"the caches are contiguous [blocks, {Hkv}, block size, {D}], not {tuple(shape)} and {tuple(v_cache.shape)}")
+    blocks, block = shape[0], shape[2]
     if block < 16 or block % 16:
         raise ValueError(f"pages hold a multiple of 16 tokens, not {block}")
-    if q.dtype != k_cache.dtype or q.dtype != v_cache.dtype:
+    dtype = q.dtype
+    if dtype != k_cache.dtype or dtype != v_cache.dtype:
         raise ValueError(f"queries and caches are of one type, not {q.dtype}, {k_cache.dtype} and {v_cache.dtype}")
     _same_device(device, k_cache, v_cache, block_table, ctx_lens, cu_rows, masks, positions, out)
     table, ctx, cu = _table(block_table, B, block), _ints(ctx_lens, (B,), "ctx_lens"), cu_rows.contiguous()
@@ -199,11 +208,11 @@ def tree_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     if window:
         positions = _ints(positions, (T,), "positions")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not abs(scale) <= torch.finfo(torch.float32).max:
+    if not abs(scale) <= MAX_SCALE:
         raise ValueError(f"scale {scale} is not a number of 32 bits")
     _no_gradient(q, k_cache, v_cache)
     if out is None:
-        out = torch.empty((T, width), dtype=q.dtype, device=device)
+        out = q.new_empty((T, width))
     elif out.shape != (T, width) or out.dtype != q.dtype:
         raise ValueError(f"out is {q.dtype} [{T}, {width}], not {out.dtype} {tuple(out.shape)}")
     elif out.stride(1) != 1 or (T > 1 and out.stride(0) < width):
@@ -212,16 +221,18 @@ def tree_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         return out
     if not use_native(q):
         return _tree_decode_ref(q, k_cache, v_cache, table, ctx, _spans(cu, T, max_rows), Hq, Hkv, D, masks, positions, window, scale, out)
-    if q.dtype is not BF16:
+    if dtype is not BF16:
         raise ValueError(f"the kernels take bf16 queries and caches, not {q.dtype}")
-    if (k_cache.data_ptr() | v_cache.data_ptr()) % 16 or k_cache.shape[0] * Hkv * block > 0x7FFFFFFE or B > 65535 or Hkv * -(-max_rows // (128 // (Hq // Hkv))) > 65535:
+    if (k_cache.data_ptr() | v_cache.data_ptr()) % 16 or blocks * Hkv * block > 0x7FFFFFFE or B > 65535 or Hkv * -(-max_rows // (128 // (Hq // Hkv))) > 65535:
         raise ValueError(f"caches {tuple(k_cache.shape)} start on 16 bytes and have less than 2^31 - 1 places of all heads, for at most 65535 sequences, and units of a sequence")
-    room = table.shape[1] * block
+    pages = table.shape[1]
+    room = pages * block
+    longest = min(room, window + max_rows) if window else room
     if plan is None:
-        plan = tree_plan(B, Hq, Hkv, max_rows, min(room, window + max_rows) if window else room)
+        plan = tree_plan(B, Hq, Hkv, max_rows, longest)
     elif plan < 0 or plan > 65535:
         raise ValueError(f"plan is 0 to 65535 CTAs, not {plan}")
-    if plan and B * Hkv * -(-max_rows // (128 // (Hq // Hkv))) * ((min(room, window + max_rows) if window else room) // 64 + 2) > 0x7FFFFFFF:
+    if plan and B * Hkv * -(-max_rows // (128 // (Hq // Hkv))) * (longest // 64 + 2) > 0x7FFFFFFF:
         plan = 0      # (more tiles than the kernel counts to)
     parts = sums = cuts = None
     if plan:
@@ -233,12 +244,12 @@ def tree_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         cuts = scratch.data_ptr()
         parts = cuts + 64 * plan
         sums = parts + (size - 16 * plan) // (D + 2) * D * 4
-    with torch.cuda.device(device):
-        if q.stride(1) != 1 or q.stride(0) % 8 or q.data_ptr() % 16:      # rows that do not start on 16 bytes
-            q = q[:, :width].clone(memory_format=torch.contiguous_format)
-        call("rlb_tree_decode", q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], block, table.data_ptr(), table.stride(0), table.shape[1],
-             ctx.data_ptr(), cu.data_ptr(), B, T, max_rows, Hq, Hkv, D, _L.ptr(masks), masks.stride(0) if masks is not None else 0, _L.ptr(positions) if window else None,
-             window, scale, plan, 4, parts, sums, cuts, out.data_ptr(), out.stride(0), _L.status_word(device).data_ptr(), _raw_stream(device.index))
+    stride = q.stride()
+    if stride[1] != 1 or stride[0] % 8 or q.data_ptr() % 16:      # rows that do not start on 16 bytes
+        q = q[:, :width].clone(memory_format=torch.contiguous_format)
+    _launch(device, "rlb_tree_decode", q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), blocks, block, table.data_ptr(), table.stride(0), pages,
+            ctx.data_ptr(), cu.data_ptr(), B, T, max_rows, Hq, Hkv, D, _L.ptr(masks), masks.stride(0) if masks is not None else 0, _L.ptr(positions) if window else None,
+            window, scale, plan, 4, parts, sums, cuts, out.data_ptr(), out.stride(0))
     return out
 
 
@@ -347,8 +358,7 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Ten
     if not 1 <= steps <= max_rows:
         raise ValueError(f"max_steps is 1 to max_rows = {max_rows}, not {steps}")
     _no_gradient(logits, draft_logits)
-    out = (torch.empty((B, steps), dtype=torch.int32, device=device), torch.empty(B, dtype=torch.int32, device=device),
-           torch.empty((B, steps), dtype=torch.int32, device=device), torch.empty((B, steps), dtype=torch.float32, device=device))
+    out = tokens.new_empty((B, steps)), tokens.new_empty(B), tokens.new_empty((B, steps)), uniforms.new_empty((B, steps))
     if B == 0:
         return out
     if not use_native(logits):
@@ -356,14 +366,13 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Ten
             x.fill_(fill)
         each = temps.tolist() if temps is not None else [float(temperature)] * B
         return _verify_ref(logits, tokens, parents, _spans(cu, T, max_rows), uniforms, draft_logits, each, greedy, steps, out)
-    with torch.cuda.device(device):
-        logits = logits if logits.stride(1) == 1 else logits.contiguous()
-        if draft_logits is not None and draft_logits.stride(1) != 1:
-            draft_logits = draft_logits.contiguous()
-        uniforms, temps = uniforms.contiguous(), None if temps is None else temps.contiguous()
-        call("rlb_verify_drafts", logits.data_ptr(), logits.stride(0), _L.ptr(draft_logits), draft_logits.stride(0) if draft_logits is not None else 0,
-             int(logits.dtype is torch.float32), V, T, B, max_rows, steps, tokens.data_ptr(), parents.data_ptr(), cu.data_ptr(), uniforms.data_ptr(), _L.ptr(temps),
-             float(temperature), int(greedy), *(x.data_ptr() for x in out), _L.status_word(device).data_ptr(), _raw_stream(device.index))
+    logits = logits if logits.stride(1) == 1 else logits.contiguous()
+    if draft_logits is not None and draft_logits.stride(1) != 1:
+        draft_logits = draft_logits.contiguous()
+    uniforms, temps = uniforms.contiguous(), None if temps is None else temps.contiguous()
+    _launch(device, "rlb_verify_drafts", logits.data_ptr(), logits.stride(0), _L.ptr(draft_logits), draft_logits.stride(0) if draft_logits is not None else 0,
+            int(logits.dtype is torch.float32), V, T, B, max_rows, steps, tokens.data_ptr(), parents.data_ptr(), cu.data_ptr(), uniforms.data_ptr(), _L.ptr(temps),
+            float(temperature), int(greedy), *(x.data_ptr() for x in out))
     return out
 
 
@@ -376,16 +385,22 @@ def kv_cache_keep(caches: Sequence[tuple[torch.Tensor, torch.Tensor]], block_tab
         raise ValueError(f"rows is int32 [B, steps], not {rows.dtype} {tuple(rows.shape)}")
     B, S = rows.shape
     rows, counts, ctx = _ints(rows, (B, S), "rows"), _ints(counts, (B,), "counts"), _ints(ctx_lens, (B,), "ctx_lens")
+    _same_device(rows.device, block_table, counts, ctx)
     kinds: dict[tuple, dict[int, torch.Tensor]] = {}
+    last, places, grad = None, {}, torch.is_grad_enabled()
     for pair in caches:
         for x in pair if pair is not None else ():
             if x is None:
                 continue
-            if x.dim() != 4 or not x.is_contiguous() or x.shape[3] * x.element_size() % 16 or x.data_ptr() % 16:
-                raise ValueError(f"caches are contiguous [blocks, heads, block size, D] in places of 16 bytes, not {x.dtype} {tuple(x.shape)}")
-            kinds.setdefault((x.shape[0], x.shape[1], x.shape[2], x.shape[3] * x.element_size() // 16), {})[x.data_ptr()] = x
-            _same_device(x.device, block_table, rows, counts, ctx)
-            _no_gradient(x)
+            at, kind = x.data_ptr(), (x.shape, x.dtype)
+            if kind != last:
+                if x.dim() != 4 or x.shape[3] * x.element_size() % 16:
+                    raise ValueError(f"caches are [blocks, heads, block size, D] in places of 16 bytes, not {x.dtype} {tuple(x.shape)}")
+                last = kind
+                places = kinds.setdefault((x.shape[0], x.shape[1], x.shape[2], x.shape[3] * x.element_size() // 16), {})
+            if at % 16 or not x.is_contiguous() or x.device != rows.device or (grad and x.requires_grad):
+                raise ValueError(f"caches are contiguous, start on 16 bytes, lie on {rows.device} and have no gradient, not {x.dtype} {tuple(x.shape)} on {x.device}")
+            places[at] = x
     for (blocks, heads, block, vecs), tensors in kinds.items():
         table = _table(block_table, B, block)
         if B == 0 or blocks == 0:
@@ -405,6 +420,5 @@ def kv_cache_keep(caches: Sequence[tuple[torch.Tensor, torch.Tensor]], block_tab
                     for x in tensors.values():
                         x[int(table[b, (c + i) // block]), :, (c + i) % block] = x[int(table[b, (c + r) // block]), :, (c + r) % block]
             continue
-        with torch.cuda.device(one.device):
-            call("rlb_kv_keep", (C.c_void_p * len(tensors))(*tensors), len(tensors), table.data_ptr(), table.stride(0), table.shape[1], block, blocks, heads, vecs, ctx.data_ptr(),
-                 rows.data_ptr(), S, counts.data_ptr(), B, _L.status_word(one.device).data_ptr(), _raw_stream(one.device.index))
+        _launch(one.device, "rlb_kv_keep", (C.c_void_p * len(tensors))(*tensors), len(tensors), table.data_ptr(), table.stride(0), table.shape[1], block, blocks, heads, vecs,
+                ctx.data_ptr(), rows.data_ptr(), S, counts.data_ptr(), B)
