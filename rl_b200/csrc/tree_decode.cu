@@ -620,10 +620,11 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             const uint64_t x = fma_pair(pair(__uint_as_float(s0[2 * i]), __uint_as_float(s0[2 * i + 1])), size2, mr2);
             const uint64_t y = fma_pair(pair(__uint_as_float(s1[2 * i]), __uint_as_float(s1[2 * i + 1])), size2, mr2);
             const float e0 = exp2_fast(low_of(x)), e1 = exp2_fast(high_of(x)), f0 = exp2_fast(low_of(y)), f1 = exp2_fast(high_of(y));
-            sum[0] = add_pair(sum[0], pair(e0, e1));
-            sum[1] = add_pair(sum[1], pair(f0, f1));
             pk[i] = pack_bf16x2(e0, e1);
             pk[16 + i] = pack_bf16x2(f0, f1);
+            // (of the rounded weights: what a row's heaviest key lost by its rounding, the sum has lost too)
+            sum[0] = add_pair(sum[0], pair(__uint_as_float(pk[i] << 16), __uint_as_float(pk[i] & 0xffff0000u)));
+            sum[1] = add_pair(sum[1], pair(__uint_as_float(pk[16 + i] << 16), __uint_as_float(pk[16 + i] & 0xffff0000u)));
           }
           sum[0] = add_pair(sum[0], sum[1]);
           l = l * factor + (low_of(sum[0]) + high_of(sum[0]));
