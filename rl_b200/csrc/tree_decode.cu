@@ -52,6 +52,7 @@ struct TreeArgs {
   float2* part_ml;             // [2 CTAs][part_rows] maximum (log2) and sum
   Cut* cuts;                   // [CTAs]
   int part_rows, least;        // least: tiles of a share at least
+  int group;                   // CTAs beside one another that have the same tiles, each a block of its own
   int sorted;                  // whole units: in order of their sequences' lengths (at most THREADS of them)
   int* status;
 };
@@ -117,7 +118,7 @@ __device__ __noinline__ Seq sequence(const TreeArgs& a, int b) {
   s.tiles = max((s.keys + TILE - 1) / TILE - s.first, s.n > 0 ? 1 : 0);      // (rows without any key have a tile too, which they do not see)
   return s;
 }
-__device__ __forceinline__ int tiles_of(const TreeArgs& a, const Seq& s) { return s.tiles * s.blocks * a.Hkv; }      // (shared tiles are less than 2^31 in all)
+__device__ __forceinline__ int tiles_of(const TreeArgs& a, const Seq& s) { return s.tiles * (a.group > 1 ? min(s.blocks, 1) : s.blocks) * a.Hkv; }      // (shared tiles are less than 2^31 in all)
 
 // Sums over the block's threads: of those before this one, and of all. `red`: a word for each warp.
 __device__ __forceinline__ int block_scan(int v, int* red, int& all) {
@@ -162,13 +163,17 @@ struct Cursor {
     if (left <= 0) return false;
     if (t == s.tiles) {
       t = 0;
-      if (++m == s.blocks) {
-        m = 0;
+      if (a.group > 1 || ++m == s.blocks) {
+        if (a.group <= 1) m = 0;
         ++kv_head;
       }
     }
-    while (s.blocks == 0 || kv_head == a.Hkv) {
-      kv_head = 0;
+    while (s.blocks == 0 || kv_head == a.Hkv || m >= s.blocks) {
+      if (kv_head < a.Hkv && s.blocks > 0) {      // a sequence without a block of this number
+        left -= (a.Hkv - kv_head) * s.tiles - t;
+        if (left <= 0) return false;
+      }
+      kv_head = t = 0;
       if (++b >= a.B) return false;
       s = sequence(a, b);
     }
@@ -352,8 +357,9 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       before = total + block_scan(mine, red, all);
       total += all;
     }
-    const int share = max(a.least, static_cast<int>((static_cast<unsigned>(total) + gridDim.x - 1) / gridDim.x));
-    const long long from = static_cast<long long>(share) * blockIdx.x;
+    const unsigned groups = gridDim.x / a.group, mine_of = blockIdx.x / a.group;
+    const int share = max(a.least, static_cast<int>((static_cast<unsigned>(total) + groups - 1) / groups));
+    const long long from = static_cast<long long>(share) * mine_of;
     if (from >= total) {
       if (threadIdx.x == 0) a.cuts[blockIdx.x].before = 0;
       return;
@@ -378,12 +384,17 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     cur.s = sequence(a, cur.b);
     const int unit = start[1] / cur.s.tiles;
     cur.t = start[1] - unit * cur.s.tiles;
-    cur.kv_head = unit / cur.s.blocks;
-    cur.m = unit - cur.kv_head * cur.s.blocks;
+    if (a.group > 1) {
+      cur.kv_head = unit;
+      cur.m = blockIdx.x - mine_of * a.group;
+    } else {
+      cur.kv_head = unit / cur.s.blocks;
+      cur.m = unit - cur.kv_head * cur.s.blocks;
+    }
     cur.left = min(share, total - begin);
     if (threadIdx.x == 0) {
       const int j0 = cur.m * a.block_rows;
-      a.cuts[blockIdx.x] = Cut{share, cur.s.lo + j0, min(a.block_rows, cur.s.n - j0) * a.G, cur.kv_head * a.G, cur.t, cur.s.tiles, {0, 0}};
+      a.cuts[blockIdx.x] = Cut{share, cur.s.lo + j0, min(a.block_rows, cur.s.n - j0) * a.G, cur.kv_head * a.G, cur.m < cur.s.blocks ? cur.t : 0, cur.s.tiles, {0, 0}};
     }
   } else {
     cur.b = blockIdx.z;
@@ -744,10 +755,10 @@ tree_join_kernel(const TreeArgs a) {
   const int c = blockIdx.y, r = blockIdx.x * JOIN_ROWS + threadIdx.x / (D / 8), d = (threadIdx.x % (D / 8)) * 8;
   const Cut cut = a.cuts[c];
   if (cut.before == 0 || cut.before > cut.share || r >= cut.rows) return;
-  const int last = c + (cut.tiles - cut.before - 1) / cut.share;
+  const int last = c + (cut.tiles - cut.before - 1) / cut.share * a.group;
   float o[8] = {}, l = 0.f, top = -INFINITY;
 #pragma unroll 2
-  for (int k = c - 1; k <= last; ++k) {      // the first one is its CTA's last part, the others their CTA's first
+  for (int k = c - a.group; k <= last; k += a.group) {      // the first one is its CTA's last part, the others their CTA's first
     const long long i = (2 * static_cast<long long>(k) + (k < c)) * a.part_rows + r;
     const float2 ml = a.part_ml[i];
     const float4 x = *reinterpret_cast<const float4*>(a.part_o + i * D + d), y = *reinterpret_cast<const float4*>(a.part_o + i * D + d + 4);
@@ -804,15 +815,16 @@ int launch(const void* q, long long ldq, const void* k, const void* v, TreeArgs 
 }
 }  // namespace
 
-// ctas > 0: so many CTAs share all tiles, at least `least` each; part_o [2 ctas, part_rows, D] and part_ml [2 ctas, part_rows, 2] fp32 with part_rows = min(max_rows, 128 / G) * G, on 32 bytes,
+// ctas > 0: so many CTAs share all tiles, at least `least` each, in groups that have the same tiles, each a block of a sequence's rows (group: the blocks of max_rows rows; 1: blocks one after the
+// other); part_o [2 ctas, part_rows, D] and part_ml [2 ctas, part_rows, 2] fp32 with part_rows = min(max_rows, 128 / G) * G, on 32 bytes,
 // cuts 32 bytes for each CTA.
 // ctas 0: a CTA for each unit. q: rows on 16 bytes.
 RLB_API int rlb_tree_decode(const void* q, long long ldq, const void* k, const void* v, int blocks, int block, const int* table, long long table_ld, int pages,
                             const int* ctx, const int* cu, int B, int T, int max_rows, int Hq, int Hkv, int D, const int* masks, long long masks_ld,
-                            const int* positions, int window, float scale, int ctas, int least, float* part_o, float* part_ml, void* cuts, void* out, long long ldo, int* status,
+                            const int* positions, int window, float scale, int ctas, int group, int least, float* part_o, float* part_ml, void* cuts, void* out, long long ldo, int* status,
                             void* stream) {
   if (D != 64 && D != 128) return -2;
-  if (Hkv < 1 || Hkv > 65535 || Hq % Hkv || Hq / Hkv > M_ROWS || B > 65535 || block < 16 || block % 16 || max_rows < 1 || max_rows > 256 || ldq % 8 || least < 1) return -2;
+  if (Hkv < 1 || Hkv > 65535 || Hq % Hkv || Hq / Hkv > M_ROWS || B > 65535 || block < 16 || block % 16 || max_rows < 1 || max_rows > 256 || ldq % 8 || least < 1 || group < 1 || (ctas && ctas % group)) return -2;
   if (static_cast<long long>(blocks) * Hkv * block >= 0x7fffffffll || (ctas && (!part_o || !part_ml || !cuts))) return -2;
   TreeArgs a;
   a.blocks = blocks;
@@ -851,6 +863,7 @@ RLB_API int rlb_tree_decode(const void* q, long long ldq, const void* k, const v
   a.part_rows = a.q_rows * a.G;
   a.cuts = static_cast<Cut*>(cuts);
   a.least = least;
+  a.group = ctas ? group : 1;
   // (more units than run at once)
   a.sorted = !ctas && B > 1 && B <= THREADS && static_cast<long long>(B) * Hkv * ((max_rows + a.block_rows - 1) / a.block_rows) > 2 * 148;
   a.status = status;

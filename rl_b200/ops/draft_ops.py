@@ -30,7 +30,7 @@ _P, _I, _LL, _F = _L.P, _L.I, _L.L, _L.F
 _L.register("rlb_tree_rows", [_P, _P, _P, _P, _LL, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P])
 _L.register("rlb_kv_keep", [_P, _I, _P, _LL, _I, _I, _I, _I, _I, _P, _P, _I, _P, _I, _P, _P])
 _L.register("rlb_verify_drafts", [_P, _LL, _P, _LL, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, C.c_double, _I, _P, _P, _P, _P, _P, _P])
-_L.register("rlb_tree_decode", [_P, _LL, _P, _P, _I, _I, _P, _LL, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _LL, _P, _I, _F, _I, _I, _P, _P, _P, _P, _LL, _P, _P])
+_L.register("rlb_tree_decode", [_P, _LL, _P, _P, _I, _I, _P, _LL, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _LL, _P, _I, _F, _I, _I, _I, _P, _P, _P, _P, _LL, _P, _P])
 
 BF16 = torch.bfloat16
 HEAD_DIMS = (64, 128)
@@ -155,12 +155,24 @@ def _tree_decode_ref(q, k_cache, v_cache, table, ctx, spans, Hq, Hkv, D, masks, 
 
 
 @lru_cache(maxsize=4096)
-def tree_plan(B: int, Hq: int, Hkv: int, max_rows: int, max_len: int, sm_count: int = 148) -> int:
-    """CTAs that share all tiles of 64 keys evenly in :func:`tree_paged_decode`, or 0: a CTA for each sequence, key/value head and block of 128 / (Hq / Hkv) rows."""
-    units, tiles, slots = B * Hkv * -(-max_rows // (128 // (Hq // Hkv))), -(-max_len // 64), 2 * sm_count
+def tree_plan(B: int, Hq: int, Hkv: int, D: int, max_rows: int, max_len: int, sm_count: int = 148) -> tuple[int, int]:
+    """How :func:`tree_paged_decode` is cut up. A unit is a sequence, a key/value head and a block of 128 / (Hq / Hkv) rows of its tree; keys go by in tiles of 64. (0, 1): a CTA
+    for each unit, the longest sequences' first. (n, 1): n CTAs share all tiles evenly, units one after another, and a second kernel joins what they cut through. (n, blocks): the CTAs of a
+    sequence's blocks have the same tiles, so that its keys and values come from memory once.
+
+    Two CTAs are on an SM at a time. With fewer units than that, sharing pays where the longest unit has six tiles more than a share (us in a graph, a CTA each / shared: one
+    sequence of 1000 tokens, 8 KV heads of 128, trees of 8: 18.7 / 13.8; two of 500 13.1 / 13.7; 16 of 8000 with trees of 64 146 / 103). With more, sharing keeps the loads of the next unit on
+    their way (128 of 1000, trees of 8: 83 / 73; 180 of 500 79 / 64; 64 of 1200 49 / 49), but for less than twice as many of 64 rows and more, whose parts are large
+    (64 of 1280 with trees of 17, 4 query heads each: 52 / 56; 16 of 500 with trees of 128: 36 / 46). Blocks one after another read a sequence of 131072 tokens, trees of 33 with 5 query
+    heads, twice from memory: 189, beside one another 154; where all keys stay in the second level cache there is no difference, and trees of fewer blocks leave CTAs without work."""
+    blocks = -(-max_rows // (128 // (Hq // Hkv)))
+    units, tiles, slots = B * Hkv * blocks, -(-max_len // 64), 2 * sm_count
+    group = blocks if blocks <= 4 and B * Hkv * max_len * 4 * D > 2**27 else 1
     if units > slots:
-        return 0 if units <= 2 * slots and min(max_rows, 128 // (Hq // Hkv)) * (Hq // Hkv) >= 64 else slots
-    return slots if tiles * (slots - units) > 6 * slots else 0
+        share = units > 2 * slots or min(max_rows, 128 // (Hq // Hkv)) * (Hq // Hkv) < 64
+    else:
+        share = tiles * (slots - units) > 6 * slots
+    return (slots - slots % group, group) if share else (0, 1)
 
 
 def tree_scratch_size(ctas: int, Hq: int, Hkv: int, D: int, max_rows: int) -> int:
@@ -170,14 +182,14 @@ def tree_scratch_size(ctas: int, Hq: int, Hkv: int, D: int, max_rows: int) -> in
 
 def tree_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, ctx_lens: torch.Tensor, cu_rows: torch.Tensor,
                       Hq: int, Hkv: int, D: int, *, max_rows: int, masks: Optional[torch.Tensor] = None, scale: Optional[float] = None, window: int = 0,
-                      positions: Optional[torch.Tensor] = None, plan: Optional[int] = None, scratch: Optional[torch.Tensor] = None,
+                      positions: Optional[torch.Tensor] = None, plan: Optional[tuple[int, int]] = None, scratch: Optional[torch.Tensor] = None,
                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of the trees' rows, ``q`` [T, >= Hq D] (rows may be strided: the fused rows do), against the paged cache [blocks, Hkv, block size, D], which holds their own
     keys and values behind the context. A row sees the whole context of its sequence and the tree rows whose bits ``masks`` (as :func:`tree_rows` gives them; any bits
     do) has set; without ``masks`` the rows up to itself, which is a chain. ``window`` > 0: of these only keys whose position is less than ``window`` before the row's own
     (sliding-window layers): ``positions`` [T] int32 has the rows' (from the context's end on), a context place's is its number. A row that sees nothing gives zeros. Rows of no sequence are left as
-    they are in ``out`` (a new ``out`` has no values there). Heads of 64 and 128, at most 128 query heads to a key/value head, pages of a multiple of 16 tokens. ``plan``: CTAs that
-    share the keys (None: :func:`tree_plan` for the table's width); ``scratch``: float32 tensor of :func:`tree_scratch_size` elements, for callers that keep their own (one call at a
+    they are in ``out`` (a new ``out`` has no values there). Heads of 64 and 128, at most 128 query heads to a key/value head, pages of a multiple of 16 tokens. ``plan``: as
+    :func:`tree_plan` gives it (None: for the table's width); ``scratch``: float32 tensor of :func:`tree_scratch_size` elements, for callers that keep their own (one call at a
     time). Returns [T, Hq D].
 
     Scores, maxima and sums are in 32 bits, weights are rounded to bf16 before they meet the values."""
@@ -228,28 +240,28 @@ def tree_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     pages = table.shape[1]
     room = pages * block
     longest = min(room, window + max_rows) if window else room
-    if plan is None:
-        plan = tree_plan(B, Hq, Hkv, max_rows, longest)
-    elif plan < 0 or plan > 65535:
-        raise ValueError(f"plan is 0 to 65535 CTAs, not {plan}")
-    if plan and B * Hkv * -(-max_rows // (128 // (Hq // Hkv))) * (longest // 64 + 2) > 0x7FFFFFFF:
-        plan = 0      # (more tiles than the kernel counts to)
+    blocks_of = -(-max_rows // (128 // (Hq // Hkv)))
+    ctas, group = tree_plan(B, Hq, Hkv, D, max_rows, longest) if plan is None else plan
+    if not 0 <= ctas <= 65535 or group not in (1, blocks_of) or ctas % group or (group > 1 and not ctas):
+        raise ValueError(f"plan {(ctas, group)} is neither (0, 1) nor up to 65535 CTAs in groups of 1 or {blocks_of}")
+    if ctas and B * Hkv * blocks_of * (longest // 64 + 2) + 64 * ctas > 0x7FFFFFFF:
+        ctas, group = 0, 1      # (more tiles than the kernel counts to)
     parts = sums = cuts = None
-    if plan:
-        size = tree_scratch_size(plan, Hq, Hkv, D, max_rows)
+    if ctas:
+        size = tree_scratch_size(ctas, Hq, Hkv, D, max_rows)
         if scratch is None:
             scratch = torch.empty(size, dtype=torch.float32, device=device)
         elif scratch.dtype is not torch.float32 or not scratch.is_contiguous() or scratch.numel() < size or scratch.data_ptr() % 32 or scratch.device != device:
             raise ValueError(f"scratch is a contiguous float32 tensor of {size} elements on {device} that starts on 32 bytes")
         cuts = scratch.data_ptr()
-        parts = cuts + 64 * plan
-        sums = parts + (size - 16 * plan) // (D + 2) * D * 4
+        parts = cuts + 64 * ctas
+        sums = parts + (size - 16 * ctas) // (D + 2) * D * 4
     stride = q.stride()
     if stride[1] != 1 or stride[0] % 8 or q.data_ptr() % 16:      # rows that do not start on 16 bytes
         q = q[:, :width].clone(memory_format=torch.contiguous_format)
     _launch(device, "rlb_tree_decode", q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), blocks, block, table.data_ptr(), table.stride(0), pages,
             ctx.data_ptr(), cu.data_ptr(), B, T, max_rows, Hq, Hkv, D, _L.ptr(masks), masks.stride(0) if masks is not None else 0, _L.ptr(positions) if window else None,
-            window, scale, plan, 4, parts, sums, cuts, out.data_ptr(), out.stride(0))
+            window, scale, ctas, group, 4, parts, sums, cuts, out.data_ptr(), out.stride(0))
     return out
 
 

@@ -66,13 +66,13 @@ def _masks(bits, most):
     return torch.cat([O.words(x, -(-most // 32)) for x in bits])
 
 
-def _check(case, Hq, Hkv, D, most, bits=None, **kw):
+def _check(case, Hq, Hkv, D, most, bits=None, plan=None, **kw):
     q, k, v, table, ctx, cu, _ = case
     masks = _masks(bits, most) if bits is not None else None
     want, tol = O.attend(q, k, v, table, ctx, cu, Hq, Hkv, D, bits, **kw)
     if "positions" in kw:
         kw["positions"] = kw["positions"].cuda()
-    got = S.tree_paged_decode(q.cuda()[:, : Hq * D], *_dev(k, v, table, ctx, cu), Hq, Hkv, D, max_rows=most, masks=masks.cuda() if masks is not None else None, **kw)
+    got = S.tree_paged_decode(q.cuda()[:, : Hq * D], *_dev(k, v, table, ctx, cu), Hq, Hkv, D, max_rows=most, masks=masks.cuda() if masks is not None else None, plan=plan, **kw)
     assert L.check_status() == 0
     n = int(cu[-1])
     off = (got.cpu().double() - want).abs()[:n] - tol[:n] - 1e-30
@@ -449,3 +449,37 @@ def test_verify_of_logits_that_grow(native_lib):
             got = S.verify_drafts(*_dev(z, tokens, parents, cu, torch.full((4,), u)), max_rows=1)
             assert torch.equal(got[0].cpu(), want[0])
             assert torch.allclose(got[3].cpu(), want[3], rtol=2.0**-23, atol=1e-12)
+
+
+@pytest.mark.parametrize("D,Hq,Hkv", [(128, 8, 2), (64, 7, 1), (128, 40, 1)])
+@pytest.mark.parametrize("ctas", [0, 1, 3, 40, 296])
+def test_every_plan_is_the_same_attention(native_lib, D, Hq, Hkv, ctas):
+    """A CTA for each unit, few and many CTAs that share the tiles, blocks one after another or beside one another, trees of fewer blocks than others, callers' own scratch."""
+    sizes, ctx = [70, 3, 0, 40, 33, 1], [700, 1000, 9, 64, 0, 127]
+    case = _attend_case(sizes, ctx, Hq, Hkv, D, 32, seed=8)
+    q, k, v, table, ctx_t, cu, parents = case
+    bits = _bits(parents, cu)
+    want, tol = O.attend(q, k, v, table, ctx_t, cu, Hq, Hkv, D, bits)
+    blocks = -(-70 // (128 // (Hq // Hkv)))
+    for group in {1, blocks} if ctas else {1}:
+        n = max(group, ctas - ctas % group)
+        scratch = torch.full((S.tree_scratch_size(n, Hq, Hkv, D, 70) + 3,), math.nan, device="cuda") if ctas else None
+        got = S.tree_paged_decode(*_dev(q, k, v, table, ctx_t, cu), Hq, Hkv, D, max_rows=70, masks=_masks(bits, 70).cuda(), plan=(n if ctas else 0, group), scratch=scratch)
+        assert ((got.cpu().double() - want).abs() <= tol).all() and L.check_status() == 0
+
+
+def test_attention_of_more_sequences_than_a_block_counts_at_once(native_lib):
+    sizes, ctx = [1 + i % 3 if i % 7 else 0 for i in range(500)], [i % 90 for i in range(500)]
+    case = _attend_case(sizes, ctx, 4, 2, 64, 16, seed=1)
+    for plan in (None, (0, 1), (296, 1)):
+        _check(case, 4, 2, 64, 3, _bits(case[6], case[5]), plan=plan)
+
+
+def test_plans_that_are_refused(native_lib):
+    q, k, v, table, ctx, cu, _ = _dev(*_attend_case([5, 18], [70, 3], 8, 2, 128, 16, seed=6))
+    for plan in ((-1, 1), (70000, 1), (10, 2), (0, 2)):
+        with pytest.raises(ValueError):
+            S.tree_paged_decode(q, k, v, table, ctx, cu, 8, 2, 128, max_rows=18, plan=plan)
+    for scratch in (torch.zeros(10, device="cuda"), torch.zeros(10**6, device="cuda", dtype=torch.bfloat16), torch.zeros(10**6), torch.zeros(10**6, device="cuda")[1:]):
+        with pytest.raises(ValueError):
+            S.tree_paged_decode(q, k, v, table, ctx, cu, 8, 2, 128, max_rows=18, plan=(8, 1), scratch=scratch)
