@@ -237,6 +237,7 @@ struct Frame {
 __device__ __noinline__ double weight_of(const Frame* f, const double* table, double c, float x) {
   return !(x >= f->low) ? 0.0 : f->kind == 2 ? (x == f->top ? 1.0 : 0.0) : f->near(table, c, x);
 }
+__device__ __forceinline__ void push_u(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ void push_d(uint32_t addr, double v) { asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory"); }
 
 struct Part {      // of a warp's range, target and draft: sum of weights in its frame, the frame's MAGIC - N and logit (-inf: none)
@@ -466,7 +467,8 @@ verify_kernel(const VerifyArgs a) {
     const Temperature tp{LOG2E / temp * 0x1p896, __double2float_rd(1000 * LN2 * temp), __double2float_rd(60 * LN2 * temp)};
     const int groups_per = (a.V + 2 * VEC - 2) / VEC / W + 1;      // groups of a range, whatever the row's alignment
     depth_c = tp.c;
-    int turn = 0, node = 0;
+    int turn = 0, node = 0, own_up = -1, own_tok = -1;
+    float own_num = 0.f;
     bool started = false;
     cluster_arrive();
 
@@ -515,17 +517,18 @@ verify_kernel(const VerifyArgs a) {
         }
       };
       if (g0 < g1) fetch(g0, g1);
-      if (count == 0)
-        for (int j = tid; j < s.n; j += DV_THREADS) {
-          up[j] = j ? a.parents[s.lo + j] : -1;
-          tok[j] = a.tokens[s.lo + j];
-          num[j] = a.uniforms[s.lo + j];
-        }
-      const bool child = tid > node && tid < s.n && up[tid] == node && tok[tid] >= 0 && tok[tid] < a.V;
+      // The tree and its children's logits are read by the first CTA alone, for all: what the CTAs decide comes from the same numbers even where another stream is writing them.
+      const bool mine_of_tree = rank == 0 && tid < s.n, first_row = count == 0;
+      if (first_row && mine_of_tree) {
+        own_up = tid ? a.parents[s.lo + tid] : -1;
+        own_tok = a.tokens[s.lo + tid];
+        own_num = a.uniforms[s.lo + tid];
+      }
+      const bool child = mine_of_tree && tid > node && own_up == node && own_tok >= 0 && own_tok < a.V;
       float own_z = 0.f, own_d = 0.f;
       if (child) {
-        own_z = z.at(tok[tid]);
-        if (DRAFT) own_d = d.at(tok[tid]);
+        own_z = z.at(own_tok);
+        if (DRAFT) own_d = d.at(own_tok);
       }
       // ---------------------------------------------------------------- the sums of the row
       float peak = -INFINITY;      // the largest that a lane has met first
@@ -602,11 +605,19 @@ verify_kernel(const VerifyArgs a) {
           }
         }
       }
-      if (child) {
-        lz[tid] = own_z;
-        if (DRAFT) ld[tid] = own_d;
-      }
       begin();
+      if (mine_of_tree && (first_row || child))
+        for (uint32_t to = 0; to < ctas; ++to) {
+          if (first_row) {
+            push_u(mapa_shared(smem_u32(&up[tid]), to), static_cast<uint32_t>(own_up));
+            push_u(mapa_shared(smem_u32(&tok[tid]), to), static_cast<uint32_t>(own_tok));
+            push_u(mapa_shared(smem_u32(&num[tid]), to), __float_as_uint(own_num));
+          }
+          if (child) {
+            push_u(mapa_shared(smem_u32(&lz[tid]), to), __float_as_uint(own_z));
+            if (DRAFT) push_u(mapa_shared(smem_u32(&ld[tid]), to), __float_as_uint(own_d));
+          }
+        }
       push(0, sum, f.add, f.top, at, fminf(warp_top(most), F_MAX));
       if (DRAFT) push(1, dsum, fd.add, fd.top, 0, fminf(warp_top(dmost), F_MAX));
       end();

@@ -235,8 +235,8 @@ def tree_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         return _tree_decode_ref(q, k_cache, v_cache, table, ctx, _spans(cu, T, max_rows), Hq, Hkv, D, masks, positions, window, scale, out)
     if dtype is not BF16:
         raise ValueError(f"the kernels take bf16 queries and caches, not {q.dtype}")
-    if (k_cache.data_ptr() | v_cache.data_ptr()) % 16 or blocks * Hkv * block > 0x7FFFFFFE or B > 65535 or Hkv * -(-max_rows // (128 // (Hq // Hkv))) > 65535:
-        raise ValueError(f"caches {tuple(k_cache.shape)} start on 16 bytes and have less than 2^31 - 1 places of all heads, for at most 65535 sequences, and units of a sequence")
+    if (k_cache.data_ptr() | v_cache.data_ptr()) % 16 or blocks < 1 or blocks * Hkv * block > 0x7FFFFFFE or B > 65535 or Hkv * -(-max_rows // (128 // (Hq // Hkv))) > 65535:
+        raise ValueError(f"caches {tuple(k_cache.shape)} start on 16 bytes and have some pages, and less than 2^31 - 1 places of all heads, for at most 65535 sequences, and units of a sequence")
     pages = table.shape[1]
     room = pages * block
     longest = min(room, window + max_rows) if window else room
@@ -257,7 +257,7 @@ def tree_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         parts = cuts + 64 * ctas
         sums = parts + (size - 16 * ctas) // (D + 2) * D * 4
     stride = q.stride()
-    if stride[1] != 1 or stride[0] % 8 or q.data_ptr() % 16:      # rows that do not start on 16 bytes
+    if stride[1] != 1 or stride[0] % 8 or stride[0] < width or q.data_ptr() % 16:      # rows that do not start on 16 bytes, or share places
         q = q[:, :width].clone(memory_format=torch.contiguous_format)
     _launch(device, "rlb_tree_decode", q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), blocks, block, table.data_ptr(), table.stride(0), pages,
             ctx.data_ptr(), cu.data_ptr(), B, T, max_rows, Hq, Hkv, D, _L.ptr(masks), masks.stride(0) if masks is not None else 0, _L.ptr(positions) if window else None,

@@ -191,6 +191,9 @@ def test_rows_of_any_place(native_lib):
     odd = torch.empty(27, Hq * D + 3, dtype=torch.bfloat16, device="cuda")[:, 1 : 1 + Hq * D].copy_(q[:, : Hq * D])
     wide = torch.full((23 + 4, masks.shape[1] + 2), -1, dtype=I32, device="cuda")
     wide[:, : masks.shape[1]] = masks
+    same = q[:1, : Hq * D].expand(27, -1)      # rows that share their place
+    one = S.tree_paged_decode(same.contiguous(), *args, Hq, Hkv, D, max_rows=18, masks=masks)[:23]
+    assert torch.equal(S.tree_paged_decode(same, *args, Hq, Hkv, D, max_rows=18, masks=masks)[:23], one)
     for x, m in ((q, masks), (odd, masks), (q, wide[:, : masks.shape[1]])):
         out = torch.full((27, Hq * D + 5), 9.0, dtype=torch.bfloat16, device="cuda")
         for place in (out[:, : Hq * D], out[:, 3 : 3 + Hq * D]):
