@@ -35,16 +35,20 @@ tree_rows_kernel(const int* __restrict__ parents, const int* __restrict__ cu, co
   __shared__ int up[DR_ROWS];
   pdl_sync();
   const int b = blockIdx.x, j = threadIdx.x;
-  if (b == B) {      // rows of no sequence see nothing and have no place
-    const int end = B > 0 ? min(max(cu[B], 0), T) : 0;
-    for (long long t = end + j; t < T; t += blockDim.x) {
+  auto none = [&](int from, int to) {      // rows of no sequence see nothing and have no place
+    for (long long t = from + j; t < to; t += blockDim.x) {
       for (int w = 0; w < words; ++w) masks[t * words + w] = 0;
       positions[t] = 0;
       slots[t] = -1;
     }
+  };
+  if (b == B) {
+    none(0, B > 0 ? min(max(cu[0], 0), T) : 0);
+    none(B > 0 ? min(max(cu[B], 0), T) : 0, T);
     return;
   }
   const TreeSpan s = tree_span(cu, b, T, max_rows, status, j == 0);
+  none(s.lo + s.n, min(max(cu[b + 1], s.lo), T));      // (rows over max_rows)
   if (j < s.n) {
     const int p = parents[s.lo + j];
     up[j] = p >= 0 && p < j ? p : -1;

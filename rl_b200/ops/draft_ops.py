@@ -11,7 +11,8 @@ The rows of all sequences' trees lie one after the other: sequence ``b``'s are `
 before the tree; row ``j``'s key and value stand at place ``ctx_lens[b] + j`` of the pages that ``block_table`` [B, pages] int32 names.
 
 On the GPU offsets that do not ascend, rows over ``max_rows``, parents that are not above their row, pages that are not there and places outside the table are left
-out, and reported as ``RLB_ERR_BOUNDS`` in the status word. CPU tensors run the PyTorch restatement. Everything here is for inference: nothing has a gradient.
+out. The status word then has ``RLB_ERR_BOUNDS``: from :func:`tree_rows` for offsets, rows, parents and places, from :func:`verify_drafts` for offsets and rows, from
+:func:`tree_paged_decode` for pages, from :func:`kv_cache_keep` for rows, pages and places. CPU tensors run the PyTorch restatement. Everything here is for inference: nothing has a gradient.
 """
 
 from __future__ import annotations

@@ -48,6 +48,20 @@ def test_rows_reports_what_is_left_out(native_lib):
         assert L.check_status() == 8
 
 
+@pytest.mark.parametrize("cu,most", [([3, 5, 9], 4), ([0, 6, 9], 4), ([2, 300, 301], 256)])
+def test_rows_that_are_left_out_have_no_place(native_lib, cu, most):
+    """Rows before the first sequence, and those over max_rows: whatever the results' memory held."""
+    T = cu[-1] + 3
+    args = [torch.tensor(x, dtype=I32) for x in ([-1] * T, cu, [7, 20], [list(range(30)), list(range(30, 60))])]
+    want = S.tree_rows(*args, 16, max_rows=most)
+    held = [torch.full((T, n), 77, dtype=t, device="cuda") for n, t in ((-(-most // 32), I32), (1, I32), (1, torch.int64))]
+    del held      # (their places are the next ones to be given out)
+    got = S.tree_rows(*_dev(*args), 16, max_rows=most)
+    for x, y in zip(got, want):
+        assert torch.equal(x.cpu(), y)
+    assert L.check_status() == (8 if cu[1] - cu[0] > most else 0)
+
+
 def _attend_case(sizes, ctx, Hq, Hkv, D, block, seed=0, chain=False):
     g = torch.Generator().manual_seed(seed)
     parents, cu = O.forest(sizes, seed, chain=chain)
