@@ -156,11 +156,20 @@ struct VerifyArgs {
 
 constexpr int DV_THREADS = 512, DV_WARPS = DV_THREADS / 32, DV_CLUSTER = 8, DV_PARTS = DV_WARPS * DV_CLUSTER;
 constexpr int DV_ELEMS = 8;      // logits a lane has at a time
+constexpr int DV_SLOTS = 8;      // loads of 16 bytes that a lane has on their way
 constexpr int EXP_STEPS = 256;
 constexpr double LOG2E = 1.4426950408889634074, LN2 = 0.69314718055994530942;
 constexpr double MAGIC = 6755399441055744.0 / EXP_STEPS;      // 1.5 * 2^52 / 256: a sum with it has the nearest number of 256ths in its low word
 constexpr float F_MAX = 3.402823466e38f;
 constexpr float COLDEST = 1.17549435e-38f;      // temperatures below are greedy
+
+// Copies of 16 bytes to shared memory, which the lane that issued them reads itself.
+__device__ __forceinline__ void copy16(uint4* to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory"); }
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
 
 // NaN weighs nothing, +inf as much as the largest number.
 __device__ __forceinline__ float usable(float x) { return fminf(fmaxf(x, -INFINITY), F_MAX); }
@@ -244,11 +253,14 @@ __device__ __noinline__ double weight_of(const Frame* f, const double* table, do
 __device__ __forceinline__ void push_u(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ void push_d(uint32_t addr, double v) { asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory"); }
 
-struct Part {      // of a warp's range, target and draft: sum of weights in its frame, the frame's MAGIC - N and logit (-inf: none)
-  double sum, add;
-  float m, peak;   // the range's largest logit
-  int at, none;    // and its place, where that is asked for
+// Of the warps' ranges, target or draft: sum of weights in its frame, the frame's MAGIC - N, the range's largest logit (-inf: none) and, where that is asked for, its place.
+// A lane that joins has four ranges beside one another: these lie in as many rows.
+struct Parts {
+  double sum[DV_PARTS], add[DV_PARTS];
+  float peak[DV_PARTS];
+  int at[DV_PARTS];
 };
+__device__ __forceinline__ int part_place(int w) { return (w & 3) * 32 + (w >> 2); }
 
 template <typename T>
 struct RowLogits {
@@ -257,11 +269,17 @@ struct RowLogits {
   int V;
   int shift;      // elements before the row's first that its first group of 16 bytes has
   bool vec;
-  // group g: elements g * VEC - shift and on; those outside of the row are -inf
-  __device__ __forceinline__ uint4 load(int g, int g1) const {
+  // Group g's elements, g * VEC - shift and on, to the lane's place in shared memory; those behind group g1 or outside of the row are -inf.
+  __device__ __forceinline__ void stage(uint4* to, int g, int g1) const {
     const int e = g * VEC - shift;
-    if (g < g1 && vec && e >= 0 && e + VEC <= V) return __ldg(reinterpret_cast<const uint4*>(p + e));
-    return edge(p, e, g < g1 ? V : 0);
+    if (g >= g1) {
+      constexpr uint32_t none = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+      *to = make_uint4(none, none, none, none);
+    } else if (vec && e >= 0 && e + VEC <= V) {
+      copy16(to, p + e);
+    } else {
+      *to = edge(p, e, V);
+    }
   }
   static __device__ __noinline__ uint4 edge(const T* p, int e, int V) {      // (a call waits for what it loads)
     uint4 v;
@@ -310,6 +328,7 @@ struct Visit {
   const double* table;
   const double* grow;
   const int* gone;
+  uint4* slots;      // this lane's in shared memory, DV_THREADS apart
   double c;
 };
 // What is left of the probability of token i after `r` rejections, from its logits.
@@ -358,6 +377,7 @@ __device__ __noinline__ double sum_of(const Visit<T, DRAFT>& v, int e0, int e1, 
       }
       sum += (w[0] + w[1]) + (w[2] + w[3]);
     }
+    __syncwarp();
     return warp_sum_d(sum) * inv;
   }
 #pragma unroll 1
@@ -368,6 +388,7 @@ __device__ __noinline__ double sum_of(const Visit<T, DRAFT>& v, int e0, int e1, 
     if (e + 64 < e1) sum += rest_of<T, DRAFT>(v, e + 64, x[2], y[2], r);
     if (e + 96 < e1) sum += rest_of<T, DRAFT>(v, e + 96, x[3], y[3], r);
   }
+  __syncwarp();
   return warp_sum_d(sum);
 }
 // The same of the groups from g0 to g1 of a row and its draft's, both of kind 0 and without infinities: as in the row's own sums.
@@ -380,14 +401,26 @@ __device__ __noinline__ double sum_left(const Visit<T, true>& v, int g0, int g1,
   const double inv = v.row[0].inv, dinv = v.row[1].inv, c = v.c;
   const double* table = v.table;
   double even = 0.0, odd = 0.0;
-  uint4 x = z.load(g0 + lane, g1), y = d.load(g0 + lane, g1);
+  constexpr int AHEAD = DV_SLOTS / 2;
+  uint4* to = v.slots;
+#pragma unroll 1
+  for (int k = 0; k < AHEAD; ++k, to += 2 * DV_THREADS) {
+    z.stage(to, g0 + 32 * k + lane, g1);
+    d.stage(to + DV_THREADS, g0 + 32 * k + lane, g1);
+    copies_commit();
+  }
+  int at = 0;
 #pragma unroll 1
   for (int g = g0; g < g1; g += 32) {
-    const uint4 xx = x, yy = y;
-    if (g + 32 < g1) {
-      x = z.load(g + 32 + lane, g1);
-      y = d.load(g + 32 + lane, g1);
+    copies_wait<AHEAD - 1>();
+    to = v.slots + at * (2 * DV_THREADS);
+    const uint4 xx = to[0], yy = to[DV_THREADS];
+    at = (at + 1) % AHEAD;
+    if (g + 32 * AHEAD < g1) {
+      z.stage(to, g + 32 * AHEAD + lane, g1);
+      d.stage(to + DV_THREADS, g + 32 * AHEAD + lane, g1);
     }
+    copies_commit();
     double w[VEC], e[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
@@ -406,6 +439,7 @@ __device__ __noinline__ double sum_left(const Visit<T, true>& v, int g0, int g1,
       odd += w[i + 1];
     }
   }
+  __syncwarp();
   return warp_sum_d(even + odd);
 }
 // The token of [e0, e1) at which the running sum from `start` passes `aim` (none: the last with a share; -1: none has). By a warp.
@@ -417,6 +451,7 @@ __device__ __noinline__ int find_token(const Visit<T, DRAFT>& v, int e0, int e1,
   for (int e = e0; e < e1; e += 32) {
     const int i = e + lane;
     const double w = i < e1 ? rest_of<T, DRAFT>(v, i, v.z.at(i), DRAFT ? v.d.at(i) : 0.f, r) : 0.0;
+    __syncwarp();
     double run = w;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -435,9 +470,10 @@ template <typename T, bool DRAFT>
 __global__ void __launch_bounds__(DV_THREADS, 2)
 verify_kernel(const VerifyArgs a) {
   using Row = RowLogits<T>;
-  constexpr int VEC = Row::VEC, LOADS = Row::LOADS, STEP = 32 * LOADS;
+  constexpr int VEC = Row::VEC, LOADS = Row::LOADS, STEP = 32 * LOADS, STEP_SLOTS = LOADS * (1 + DRAFT), AHEAD = DV_SLOTS / STEP_SLOTS;
+  extern __shared__ uint4 ring[];                     // [DV_SLOTS][DV_THREADS]
   __shared__ double table[EXP_STEPS];
-  __shared__ Part parts[2][1 + DRAFT][DV_PARTS];      // of all warps of the cluster, by turns
+  __shared__ Parts parts[2][1 + DRAFT];      // of all warps of the cluster, by turns
   __shared__ double share[DV_PARTS], pieces[DV_WARPS];      // the ranges' probabilities; sums of a range's pieces
   __shared__ RowSum row[1 + DRAFT];
   __shared__ int row_best;
@@ -446,7 +482,9 @@ verify_kernel(const VerifyArgs a) {
   __shared__ double left[DR_ROWS + 1], grow[DR_ROWS + 1];       // what is left to be given after so many rejections, and its reciprocal
   __shared__ double chosen[DR_ROWS], sums[DR_ROWS];             // of each accepted step: l c - N of its token, the sum of weights
   __shared__ int verdict, tried, turned_down;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // (A shuffle or a vote where the compiler cannot rule out that the warp's lanes have parted costs some 260 cycles in place of 20: what decides on loops and branches goes
+  // through one first.)
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   uint32_t ctas;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
   const int rank = static_cast<int>(cluster_ctarank()), b = blockIdx.x / ctas, W = static_cast<int>(ctas) * DV_WARPS, me = rank * DV_WARPS + warp;
@@ -459,14 +497,14 @@ verify_kernel(const VerifyArgs a) {
   }
   __syncthreads();
   pdl_sync();
-  const TreeSpan s = tree_span(a.cu, b, a.T, a.max_rows, a.status, tid == 0 && rank == 0);
+  const TreeSpan span = tree_span(a.cu, b, a.T, a.max_rows, a.status, tid == 0 && rank == 0), s{__shfl_sync(0xffffffffu, span.lo, 0), __shfl_sync(0xffffffffu, span.n, 0)};
   const long long out = static_cast<long long>(b) * a.steps;
   int count = 0, drawn = -1;      // the last token, of the thread that has it
   float drawn_z = 0.f;
   double depth_c = 0.0;
   if (s.n > 0) {
     const float given = a.temps ? a.temps[b] : static_cast<float>(a.temp);
-    const bool cold = a.greedy || !(given >= COLDEST);
+    const bool cold = __any_sync(0xffffffffu, a.greedy || !(given >= COLDEST));
     const double temp = !(given >= COLDEST) ? 1.0 : a.temps ? static_cast<double>(given) : a.temp;
     const Temperature tp{LOG2E / temp * 0x1p896, __double2float_rd(1000 * LN2 * temp), __double2float_rd(60 * LN2 * temp)};
     const int groups_per = (a.V + 2 * VEC - 2) / VEC / W + 1;      // groups of a range, whatever the row's alignment
@@ -481,13 +519,14 @@ verify_kernel(const VerifyArgs a) {
       if (!started) cluster_wait();      // (all CTAs of the cluster run before one writes into another's memory)
       started = true;
     };
-    auto push = [&](int which, double sum, double add, float m, int at, float peak) {      // this warp's part to all CTAs
+    auto push = [&](int which, double sum, double add, float peak, int at) {      // this warp's part to all CTAs
       if (lane < static_cast<int>(ctas)) {
-        const uint32_t p = mapa_shared(smem_u32(&parts[turn][which][me]), lane);
-        push_d(p, sum);
-        push_d(p + 8, add);
-        push_d(p + 16, __hiloint2double(__float_as_int(peak), __float_as_int(m)));
-        if (cold) push_d(p + 24, __hiloint2double(0, at));
+        Parts& to = parts[turn][which];
+        const int place = part_place(me);
+        push_d(mapa_shared(smem_u32(&to.sum[place]), lane), sum);
+        push_d(mapa_shared(smem_u32(&to.add[place]), lane), add);
+        push_u(mapa_shared(smem_u32(&to.peak[place]), lane), __float_as_uint(peak));
+        if (cold) push_u(mapa_shared(smem_u32(&to.at[place]), lane), static_cast<uint32_t>(at));
       }
     };
     auto end = [&]() {
@@ -503,24 +542,18 @@ verify_kernel(const VerifyArgs a) {
         d.vec = reinterpret_cast<uintptr_t>(d.p) % 16 / sizeof(T) == z.shift;
       }
       const int groups = (a.V + z.shift + VEC - 1) / VEC, g0 = min(groups, me * groups_per), g1 = min(groups, g0 + groups_per);
-      uint4 vz[LOADS], vd[DRAFT ? LOADS : 1];      // the groups of the next step
-      auto fetch = [&](int g, int g1) {
-        if (z.vec && (!DRAFT || d.vec) && g * VEC >= z.shift && g + STEP <= g1 && (g + STEP) * VEC - z.shift <= a.V) {      // all inside
-          const int e = (g + lane) * VEC - z.shift;
-#pragma unroll
-          for (int u = 0; u < LOADS; ++u) {
-            vz[u] = __ldg(reinterpret_cast<const uint4*>(z.p + e) + u * 32);
-            if (DRAFT) vd[u] = __ldg(reinterpret_cast<const uint4*>(d.p + e) + u * 32);
-          }
-          return;
-        }
+      auto stage = [&](uint4* to, int g) {      // of a step
 #pragma unroll
         for (int u = 0; u < LOADS; ++u) {
-          vz[u] = z.load(g + u * 32 + lane, g1);
-          if (DRAFT) vd[u] = d.load(g + u * 32 + lane, g1);
+          z.stage(to + u * DV_THREADS, g + u * 32 + lane, g1);
+          if (DRAFT) d.stage(to + (LOADS + u) * DV_THREADS, g + u * 32 + lane, g1);
         }
       };
-      if (g0 < g1) fetch(g0, g1);
+#pragma unroll 1
+      for (int k = 0; k < AHEAD; ++k) {
+        if (g0 + k * STEP < g1) stage(ring + tid + k * (STEP_SLOTS * DV_THREADS), g0 + k * STEP);
+        copies_commit();
+      }
       // The tree and its children's logits are read by the first CTA alone, for all: what the CTAs decide comes from the same numbers even where another stream is writing them.
       const bool mine_of_tree = rank == 0 && tid < s.n, first_row = count == 0;
       if (first_row && mine_of_tree) {
@@ -571,14 +604,20 @@ verify_kernel(const VerifyArgs a) {
           }
         total += even + odd;
       };
+      int slot = 0;
+#pragma unroll 1
       for (int g = g0; g < g1; g += STEP) {
+        copies_wait<AHEAD - 1>();
+        uint4* from = ring + tid + slot * (STEP_SLOTS * DV_THREADS);
         uint4 wz[LOADS], wd[LOADS];
 #pragma unroll
         for (int u = 0; u < LOADS; ++u) {
-          wz[u] = vz[u];
-          if (DRAFT) wd[u] = vd[DRAFT ? u : 0];
+          wz[u] = from[u * DV_THREADS];
+          if (DRAFT) wd[u] = from[(LOADS + u) * DV_THREADS];
         }
-        if (g + STEP < g1) fetch(g + STEP, g1);
+        slot = (slot + 1) % AHEAD;
+        if (g + AHEAD * STEP < g1) stage(from, g + AHEAD * STEP);
+        copies_commit();
         add(f, high, most, sum, wz);
         if (DRAFT) {
           if (!cold) add(fd, dhigh, dmost, dsum, wd);
@@ -596,6 +635,7 @@ verify_kernel(const VerifyArgs a) {
             }
         }
       }
+      __syncwarp();
       sum = warp_sum_d(sum);
       if (DRAFT) dsum = warp_sum_d(dsum);
       if (cold) {
@@ -622,43 +662,42 @@ verify_kernel(const VerifyArgs a) {
             if (DRAFT) push_u(mapa_shared(smem_u32(&ld[tid]), to), __float_as_uint(own_d));
           }
         }
-      push(0, sum, f.add, f.top, at, fminf(warp_top(most), F_MAX));
-      if (DRAFT) push(1, dsum, fd.add, fd.top, 0, fminf(warp_top(dmost), F_MAX));
+      push(0, sum, f.add, fminf(warp_top(most), F_MAX), at);
+      if (DRAFT) push(1, dsum, fd.add, fminf(warp_top(dmost), F_MAX), 0);
       end();
       // a warp joins the target's parts, another the draft's: lane i has four of them, in their order
       if (warp < 1 + DRAFT) {
-        const Part* got = &parts[turn][warp][lane * 4];
+        const Parts& got = parts[turn][warp];
         RowSum& to = row[warp];
         float m[4], top = -INFINITY;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          m[k] = lane * 4 + k < W ? got[k].peak : -INFINITY;
+          m[k] = lane * 4 + k < W ? got.peak[k * 32 + lane] : -INFINITY;
           top = fmaxf(top, m[k]);
         }
         const Frame whole = Frame::frame_of(warp_top(top), tp);
         double v[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {      // of rows with one logit far above the others the parts that have it
-          v[k] = !(m[k] >= whole.low) ? 0.0 : whole.kind == 2 ? (m[k] == whole.top ? got[k].sum : 0.0) : Frame::moved(got[k].sum, got[k].add, whole.add);
+          const double sum = got.sum[k * 32 + lane], moved = Frame::moved(sum, got.add[k * 32 + lane], whole.add);
+          v[k] = !(m[k] >= whole.low) ? 0.0 : whole.kind == 2 ? (m[k] == whole.top ? sum : 0.0) : moved;
         }
         const double all = warp_sum_d((v[0] + v[1]) + (v[2] + v[3])), inv = whole.top > -INFINITY && !(cold && warp) ? 1.0 / all : 0.0;
         if (warp == 0)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) share[lane * 4 + k] = v[k] * inv;
+          for (int k = 0; k < 4; ++k) share[k * 32 + lane] = v[k] * inv;
+        int best = -1;
+        if (cold && warp == 0 && whole.top > -INFINITY) {      // the first range that has the largest (ranges lie in the tokens' order)
+#pragma unroll
+          for (int k = 3; k >= 0; --k) best = m[k] == whole.top ? got.at[k * 32 + lane] : best;
+        }
+        if (cold) best = __shfl_sync(0xffffffffu, best, max(0, __ffs(__ballot_sync(0xffffffffu, best >= 0)) - 1));
         if (lane == 0) {
           to.f = whole;
           to.inv = inv;
           to.sum = all;
           if (warp == 0) {
-            if (cold) {
-              float x = -INFINITY;
-              row_best = 0;
-              for (int w = 0; w < W; ++w)
-                if (parts[turn][0][w].peak > x) {      // (parts lie in the tokens' order)
-                  x = parts[turn][0][w].peak;
-                  row_best = parts[turn][0][w].at;
-                }
-            }
+            if (cold) row_best = max(0, best);
             left[0] = grow[0] = 1.0;
             tried = node;
             turned_down = 0;
@@ -667,49 +706,71 @@ verify_kernel(const VerifyArgs a) {
         __syncwarp();
       }
       if (DRAFT) __syncthreads();
-      Visit<T, DRAFT> visit{z, d, row, table, grow, gone, tp.c};
+      Visit<T, DRAFT> visit{z, d, row, table, grow, gone, ring + tid, tp.c};
       const int e0 = max(0, g0 * VEC - z.shift), e1 = min(a.V, g1 * VEC - z.shift);      // the range's tokens
       double mine[4], total = 0.0;
       auto take = [&](double v) {      // this warp's part of new sums; the parts and the whole sum of all
         begin();
-        push(0, v, 0.0, 0.f, 0, 0.f);
+        push(0, v, 0.0, 0.f, 0);
         end();
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mine[k] = lane * 4 + k < W ? parts[turn][0][lane * 4 + k].sum : 0.0;
+        for (int k = 0; k < 4; ++k) mine[k] = lane * 4 + k < W ? parts[turn][0].sum[k * 32 + lane] : 0.0;
         total = warp_sum_d((mine[0] + mine[1]) + (mine[2] + mine[3]));
       };
       // ---------------------------------------------------------------- the children
       int next = -1, rejected = 0;
       while (true) {
-        if (tid == 0) {      // verdict: an accepted row, -1 none, -2 one rejected after which the sums are taken again
-          int v = -1, j = tried + 1, r = rejected;
-          for (; j < s.n && v == -1 && count + 1 < a.steps; ++j) {
-            if (up[j] != node) continue;
-            const int t = tok[j];
+        if (warp == 0) {      // verdict: an accepted row, -1 none, -2 one rejected after which the sums are taken again
+          int v = -1, r = rejected, j0 = tried + 1, stop = s.n;      // 32 rows at a time, each lane has the weight of its own
+          double rest = left[r];
+          for (int c0 = j0 & ~31; __any_sync(0xffffffffu, c0 < s.n && v == -1 && count + 1 < a.steps); c0 += 32) {
+            const int j = c0 + lane, t = j < s.n ? tok[j] : -1;
+            const bool child = j >= j0 && j < s.n && up[j] == node && t >= 0 && t < a.V;      // (others have no probability, and are none of the draft's)
+            unsigned todo = __ballot_sync(0xffffffffu, child);
+            if (todo == 0) continue;
             if (cold) {
-              if (row[0].inv > 0.0 && t == row_best) v = j;
+              todo = __ballot_sync(0xffffffffu, child && row[0].inv > 0.0 && t == row_best);
+              if (todo) v = c0 + __ffs(todo) - 1;
               continue;
             }
-            if (t < 0 || t >= a.V) continue;      // has no probability, and is none of the draft's
-            const double w = rest_of<T, DRAFT>(visit, t, lz[j], DRAFT ? ld[j] : 0.f, r);
-            const double g = DRAFT ? weight_of(&row[DRAFT].f, table, tp.c, ld[j]) * row[DRAFT].inv : 1.0;
-            if (static_cast<double>(num[j]) * g * left[r] < w) {
-              v = j;
-            } else if (DRAFT) {
-              v = -2;
-            } else if (w > 0.0) {
-              gone[r] = t;
-              left[r + 1] = left[r] - w;
-              ++r;
+            const float x = child ? lz[j] : -INFINITY, y = DRAFT && child ? ld[j] : -INFINITY;
+            double w = rest_of<T, DRAFT>(visit, t, x, y, r);
+            double asked = child ? static_cast<double>(num[j]) : 0.0;
+            if (DRAFT) asked *= weight_of(&row[DRAFT].f, table, tp.c, y) * row[DRAFT].inv;
+            __syncwarp();
+            for (; todo; todo &= todo - 1) {
+              const int l = __ffs(todo) - 1, tl = __shfl_sync(0xffffffffu, t, l);
+              const double wl = __shfl_sync(0xffffffffu, w, l), al = __shfl_sync(0xffffffffu, asked, l);
+              if (__any_sync(0xffffffffu, al * rest < wl)) {
+                v = c0 + l;
+                break;
+              }
+              if (DRAFT) {
+                v = -2;
+                stop = c0 + l;
+                break;
+              }
+              if (__any_sync(0xffffffffu, wl > 0.0)) {
+                rest -= wl;
+                if (lane == 0) {
+                  gone[r] = tl;
+                  left[r + 1] = rest;
+                }
+                ++r;
+                if (t == tl) w = 0.0;      // (a token that is out)
+              }
             }
+            __syncwarp();
           }
-          tried = j - 1;
-          verdict = v;
-          if (!DRAFT) turned_down = r;
+          if (lane == 0) {
+            tried = stop;
+            verdict = v;
+            if (!DRAFT) turned_down = r;
+          }
         }
         __syncthreads();
-        const int v = verdict;
-        if (!DRAFT) rejected = turned_down;
+        const int v = __reduce_max_sync(0xffffffffu, verdict);
+        if (!DRAFT) rejected = __reduce_max_sync(0xffffffffu, turned_down);
         if (v != -2) {
           next = v;
           break;
@@ -724,10 +785,10 @@ verify_kernel(const VerifyArgs a) {
           grow[rejected] = 1.0 / total;
         }
         __syncthreads();
-        if (!(total > 0.0)) break;
+        if (__any_sync(0xffffffffu, !(total > 0.0))) break;
       }
       // ---------------------------------------------------------------- the token
-      const bool some = row[0].inv > 0.0;      // a row without a number above -inf has no probabilities
+      const bool some = __any_sync(0xffffffffu, row[0].inv > 0.0);      // a row without a number above -inf has no probabilities
       if (rank == 0 && tid == 0) a.out_rows[out + count] = node;
       if (next >= 0) {
         if (rank == 0 && tid == 0) {
@@ -749,9 +810,9 @@ verify_kernel(const VerifyArgs a) {
         break;
       }
       if (!DRAFT && rejected > 0) {      // without the rejected tokens
-        if (left[rejected] >= 1.0 / 1024) {      // their weights are taken off their ranges' sums, of which no more than ten bits are lost
+        if (__any_sync(0xffffffffu, left[rejected] >= 1.0 / 1024)) {      // their weights are taken off their ranges' sums, of which no more than ten bits are lost
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mine[k] = share[lane * 4 + k];
+          for (int k = 0; k < 4; ++k) mine[k] = share[k * 32 + lane];
           for (int r = 0; r < rejected; ++r) {
             const int w = (gone[r] + z.shift) / VEC / groups_per;
             const double off = left[r] - left[r + 1];
@@ -766,15 +827,16 @@ verify_kernel(const VerifyArgs a) {
             const int g = (gone[k] + z.shift) / VEC;
             hit |= g >= g0 && g < g1;
           }
-          take(hit ? sum_of<T, DRAFT>(visit, e0, e1, rejected) : share[me]);
+          take(__any_sync(0xffffffffu, hit) ? sum_of<T, DRAFT>(visit, e0, e1, rejected) : share[part_place(me)]);
         }
       }
-      if (rejected == 0 || !(total > 0.0)) {      // (nothing is left: from p itself)
+      if (__any_sync(0xffffffffu, rejected == 0 || !(total > 0.0))) {      // (nothing is left: from p itself)
         rejected = 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mine[k] = share[lane * 4 + k];
+        for (int k = 0; k < 4; ++k) mine[k] = share[k * 32 + lane];
         total = warp_sum_d((mine[0] + mine[1]) + (mine[2] + mine[3]));
       }
+      __syncwarp();
       const double aim = static_cast<double>(num[0]) * total;
       double run = (mine[0] + mine[1]) + (mine[2] + mine[3]);
 #pragma unroll
@@ -810,19 +872,17 @@ verify_kernel(const VerifyArgs a) {
         const double own = sum_of<T, DRAFT>(visit, q0, q1, rejected);
         if (lane == 0) pieces[warp] = own;
         __syncthreads();
-        int mover = -1, filled = -1;
-        double from = start;
-        for (int w = 0; w < DV_WARPS; ++w) {
-          const double v = pieces[w];
-          if (v > 0.0) {
-            filled = w;
-            if (mover < 0 && over && from + v > aim) {
-              mover = w;
-              start = from;
-            }
-          }
-          from += v;
+        __syncwarp();
+        const double piece_sum = lane < DV_WARPS ? pieces[lane] : 0.0;
+        double upto = piece_sum;
+#pragma unroll
+        for (int o = 1; o < DV_WARPS; o <<= 1) {
+          const double v = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += v;
         }
+        const int filled = 31 - __clz(__ballot_sync(0xffffffffu, piece_sum > 0.0));      // -1: none
+        const int mover = over ? __ffs(__ballot_sync(0xffffffffu, piece_sum > 0.0 && start + upto > aim)) - 1 : -1;
+        if (mover >= 0) start += __shfl_sync(0xffffffffu, upto - piece_sum, mover);
         const bool inside = mover >= 0;      // (otherwise the last that has a share)
         if (warp == (inside ? mover : filled)) {
           const int hit = max(0, find_token<T, DRAFT>(visit, q0, q1, rejected, start, aim, inside));
@@ -865,6 +925,9 @@ int launch_verify(const VerifyArgs& a, int B, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(B) * cluster);
   cfg.blockDim = dim3(DV_THREADS);
+  cfg.dynamicSmemBytes = DV_SLOTS * DV_THREADS * 16;
+  e = cudaFuncSetAttribute(verify_kernel<T, DRAFT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(cfg.dynamicSmemBytes));
+  if (e != cudaSuccess) return static_cast<int>(e);
   cfg.stream = stream;
   cudaLaunchAttribute attrs[2];
   attrs[0].id = cudaLaunchAttributeClusterDimension;
