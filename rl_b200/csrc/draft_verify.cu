@@ -231,8 +231,8 @@ struct Frame {
   }
   // `v` in a frame with a larger N
   static __device__ __forceinline__ double moved(double v, double add, double larger) {
-    const double d = larger - add;
-    return static_cast<uint32_t>(__double2hiint(d)) <= 0xc090e000u ? v * __hiloint2double((1123 + __double2loint(d + 256 * MAGIC)) << 20, 0) * 0x1p-100 : 0.0;      // (-1080)
+    const double d = larger - add, scaled = v * __hiloint2double((1123 + __double2loint(d + 256 * MAGIC)) << 20, 0) * 0x1p-100;
+    return static_cast<uint32_t>(__double2hiint(d)) <= 0xc090e000u ? scaled : 0.0;      // (-1080)
   }
   __device__ __forceinline__ void move(float x, const Temperature& q, double& total) {
     const Frame before = *this;
@@ -251,8 +251,15 @@ __device__ __noinline__ double weight_of(const Frame* f, const double* table, do
   return !(x >= f->low) ? 0.0 : f->kind == 2 ? (x == f->top ? 1.0 : 0.0) : f->near(table, c, x);
 }
 __device__ __forceinline__ void push_u(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+__device__ __forceinline__ void push_row(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
 __device__ __forceinline__ void push_d(uint32_t addr, double v) { asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory"); }
 
+struct __align__(16) TreeRow {
+  int up, token;
+  float number, z;      // z: of a child of the visited row, its token's logit there
+};
 // Of the warps' ranges, target or draft: sum of weights in its frame, the frame's MAGIC - N, the range's largest logit (-inf: none) and, where that is asked for, its place.
 // A lane that joins has four ranges beside one another: these lie in as many rows.
 struct Parts {
@@ -269,13 +276,15 @@ struct RowLogits {
   int V;
   int shift;      // elements before the row's first that its first group of 16 bytes has
   bool vec;
+  bool inner;     // all of this warp's range lies on 16 bytes and within the row
+  __device__ __forceinline__ void range(int g0, int g1) { inner = vec && g0 * VEC >= shift && g1 * VEC - shift <= V; }
   // Group g's elements, g * VEC - shift and on, to the lane's place in shared memory; those behind group g1 or outside of the row are -inf.
   __device__ __forceinline__ void stage(uint4* to, int g, int g1) const {
     const int e = g * VEC - shift;
     if (g >= g1) {
       constexpr uint32_t none = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
       *to = make_uint4(none, none, none, none);
-    } else if (vec && e >= 0 && e + VEC <= V) {
+    } else if (inner || (vec && e >= 0 && e + VEC <= V)) {
       copy16(to, p + e);
     } else {
       *to = edge(p, e, V);
@@ -477,8 +486,9 @@ verify_kernel(const VerifyArgs a) {
   __shared__ double share[DV_PARTS], pieces[DV_WARPS];      // the ranges' probabilities; sums of a range's pieces
   __shared__ RowSum row[1 + DRAFT];
   __shared__ int row_best;
-  __shared__ int up[DR_ROWS], tok[DR_ROWS], gone[DR_ROWS];
-  __shared__ float num[DR_ROWS], lz[DR_ROWS], ld[DR_ROWS];      // numbers, logits of the children's tokens in their parent's rows
+  __shared__ TreeRow tree[DR_ROWS];
+  __shared__ float ld[DR_ROWS];      // as TreeRow::z, the draft's
+  __shared__ int gone[DR_ROWS];
   __shared__ double left[DR_ROWS + 1], grow[DR_ROWS + 1];       // what is left to be given after so many rejections, and its reciprocal
   __shared__ double chosen[DR_ROWS], sums[DR_ROWS];             // of each accepted step: l c - N of its token, the sum of weights
   __shared__ int verdict, tried, turned_down;
@@ -535,13 +545,15 @@ verify_kernel(const VerifyArgs a) {
     };
 
     while (true) {
-      Row z{static_cast<const T*>(a.logits) + (s.lo + node) * a.ld, a.V, 0, true}, d{};
+      Row z{static_cast<const T*>(a.logits) + (s.lo + node) * a.ld, a.V, 0, true, false}, d{};
       z.shift = static_cast<int>(reinterpret_cast<uintptr_t>(z.p) % 16 / sizeof(T));
       if (DRAFT) {
-        d = Row{static_cast<const T*>(a.draft) + (s.lo + node) * a.ld_draft, a.V, z.shift, false};
+        d = Row{static_cast<const T*>(a.draft) + (s.lo + node) * a.ld_draft, a.V, z.shift, false, false};
         d.vec = reinterpret_cast<uintptr_t>(d.p) % 16 / sizeof(T) == z.shift;
       }
       const int groups = (a.V + z.shift + VEC - 1) / VEC, g0 = min(groups, me * groups_per), g1 = min(groups, g0 + groups_per);
+      z.range(g0, g1);
+      if (DRAFT) d.range(g0, g1);
       auto stage = [&](uint4* to, int g) {      // of a step
 #pragma unroll
         for (int u = 0; u < LOADS; ++u) {
@@ -652,13 +664,10 @@ verify_kernel(const VerifyArgs a) {
       begin();
       if (mine_of_tree && (first_row || child))
         for (uint32_t to = 0; to < ctas; ++to) {
-          if (first_row) {
-            push_u(mapa_shared(smem_u32(&up[tid]), to), static_cast<uint32_t>(own_up));
-            push_u(mapa_shared(smem_u32(&tok[tid]), to), static_cast<uint32_t>(own_tok));
-            push_u(mapa_shared(smem_u32(&num[tid]), to), __float_as_uint(own_num));
-          }
+          const uint32_t at = mapa_shared(smem_u32(&tree[tid]), to);
+          if (first_row) push_row(at, static_cast<uint32_t>(own_up), static_cast<uint32_t>(own_tok), __float_as_uint(own_num), __float_as_uint(own_z));
           if (child) {
-            push_u(mapa_shared(smem_u32(&lz[tid]), to), __float_as_uint(own_z));
+            if (!first_row) push_u(at + 12, __float_as_uint(own_z));
             if (DRAFT) push_u(mapa_shared(smem_u32(&ld[tid]), to), __float_as_uint(own_d));
           }
         }
@@ -724,8 +733,8 @@ verify_kernel(const VerifyArgs a) {
           int v = -1, r = rejected, j0 = tried + 1, stop = s.n;      // 32 rows at a time, each lane has the weight of its own
           double rest = left[r];
           for (int c0 = j0 & ~31; __any_sync(0xffffffffu, c0 < s.n && v == -1 && count + 1 < a.steps); c0 += 32) {
-            const int j = c0 + lane, t = j < s.n ? tok[j] : -1;
-            const bool child = j >= j0 && j < s.n && up[j] == node && t >= 0 && t < a.V;      // (others have no probability, and are none of the draft's)
+            const int j = c0 + lane, t = j < s.n ? tree[j].token : -1;
+            const bool child = j >= j0 && j < s.n && tree[j].up == node && t >= 0 && t < a.V;      // (others have no probability, and are none of the draft's)
             unsigned todo = __ballot_sync(0xffffffffu, child);
             if (todo == 0) continue;
             if (cold) {
@@ -733,9 +742,8 @@ verify_kernel(const VerifyArgs a) {
               if (todo) v = c0 + __ffs(todo) - 1;
               continue;
             }
-            const float x = child ? lz[j] : -INFINITY, y = DRAFT && child ? ld[j] : -INFINITY;
-            double w = rest_of<T, DRAFT>(visit, t, x, y, r);
-            double asked = child ? static_cast<double>(num[j]) : 0.0;
+            const float x = child ? tree[j].z : -INFINITY, y = DRAFT && child ? ld[j] : -INFINITY;
+            double w = rest_of<T, DRAFT>(visit, t, x, y, r), asked = child ? static_cast<double>(tree[j].number) : 0.0;
             if (DRAFT) asked *= weight_of(&row[DRAFT].f, table, tp.c, y) * row[DRAFT].inv;
             __syncwarp();
             for (; todo; todo &= todo - 1) {
@@ -792,8 +800,8 @@ verify_kernel(const VerifyArgs a) {
       if (rank == 0 && tid == 0) a.out_rows[out + count] = node;
       if (next >= 0) {
         if (rank == 0 && tid == 0) {
-          a.out_tokens[out + count] = tok[next];
-          chosen[count] = row[0].f.depth(tp.c, lz[next]);
+          a.out_tokens[out + count] = tree[next].token;
+          chosen[count] = row[0].f.depth(tp.c, tree[next].z);
           sums[count] = row[0].sum;
         }
         ++count;
@@ -837,7 +845,7 @@ verify_kernel(const VerifyArgs a) {
         total = warp_sum_d((mine[0] + mine[1]) + (mine[2] + mine[3]));
       }
       __syncwarp();
-      const double aim = static_cast<double>(num[0]) * total;
+      const double aim = static_cast<double>(tree[0].number) * total;
       double run = (mine[0] + mine[1]) + (mine[2] + mine[3]);
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
