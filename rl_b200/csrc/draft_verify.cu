@@ -156,7 +156,7 @@ struct VerifyArgs {
 
 constexpr int DV_THREADS = 512, DV_WARPS = DV_THREADS / 32, DV_CLUSTER = 8, DV_PARTS = DV_WARPS * DV_CLUSTER;
 constexpr int DV_ELEMS = 8;      // logits a lane has at a time
-constexpr int DV_SLOTS = 8;      // loads of 16 bytes that a lane has on their way
+constexpr int DV_SLOTS = 4;      // loads of 16 bytes that a lane has on their way (eight are no faster)
 constexpr int EXP_STEPS = 256;
 constexpr double LOG2E = 1.4426950408889634074, LN2 = 0.69314718055994530942;
 constexpr double MAGIC = 6755399441055744.0 / EXP_STEPS;      // 1.5 * 2^52 / 256: a sum with it has the nearest number of 256ths in its low word
@@ -479,7 +479,7 @@ template <typename T, bool DRAFT>
 __global__ void __launch_bounds__(DV_THREADS, 2)
 verify_kernel(const VerifyArgs a) {
   using Row = RowLogits<T>;
-  constexpr int VEC = Row::VEC, LOADS = Row::LOADS, STEP = 32 * LOADS, STEP_SLOTS = LOADS * (1 + DRAFT), AHEAD = DV_SLOTS / STEP_SLOTS;
+  constexpr int VEC = Row::VEC, LOADS = Row::LOADS, STEP = 32 * LOADS, AHEAD = DV_SLOTS / LOADS;
   extern __shared__ uint4 ring[];                     // [DV_SLOTS][DV_THREADS]
   __shared__ double table[EXP_STEPS];
   __shared__ Parts parts[2][1 + DRAFT];      // of all warps of the cluster, by turns
@@ -554,18 +554,18 @@ verify_kernel(const VerifyArgs a) {
       const int groups = (a.V + z.shift + VEC - 1) / VEC, g0 = min(groups, me * groups_per), g1 = min(groups, g0 + groups_per);
       z.range(g0, g1);
       if (DRAFT) d.range(g0, g1);
-      auto stage = [&](uint4* to, int g) {      // of a step
+      auto stage = [&](const Row& r, uint4* to, int g) {      // of a step
 #pragma unroll
-        for (int u = 0; u < LOADS; ++u) {
-          z.stage(to + u * DV_THREADS, g + u * 32 + lane, g1);
-          if (DRAFT) d.stage(to + (LOADS + u) * DV_THREADS, g + u * 32 + lane, g1);
+        for (int u = 0; u < LOADS; ++u) r.stage(to + u * DV_THREADS, g + u * 32 + lane, g1);
+      };
+      auto first_steps = [&](const Row& r) {
+#pragma unroll 1
+        for (int k = 0; k < AHEAD; ++k) {
+          if (g0 + k * STEP < g1) stage(r, ring + tid + k * (LOADS * DV_THREADS), g0 + k * STEP);
+          copies_commit();
         }
       };
-#pragma unroll 1
-      for (int k = 0; k < AHEAD; ++k) {
-        if (g0 + k * STEP < g1) stage(ring + tid + k * (STEP_SLOTS * DV_THREADS), g0 + k * STEP);
-        copies_commit();
-      }
+      first_steps(z);
       // The tree and its children's logits are read by the first CTA alone, for all: what the CTAs decide comes from the same numbers even where another stream is writing them.
       const bool mine_of_tree = rank == 0 && tid < s.n, first_row = count == 0;
       if (first_row && mine_of_tree) {
@@ -579,89 +579,85 @@ verify_kernel(const VerifyArgs a) {
         own_z = z.at(own_tok);
         if (DRAFT) own_d = d.at(own_tok);
       }
-      // ---------------------------------------------------------------- the sums of the row
-      float peak = -INFINITY;      // the largest that a lane has met first
-      int at = 0x7fffffff;
-      Frame f, fd;
-      f.top = fd.top = -INFINITY;
-      float high = -INFINITY, dhigh = -INFINITY, most = -INFINITY, dmost = -INFINITY;
-      double sum = 0.0, dsum = 0.0;
-      auto add = [&](Frame& q, float& high, float& most, double& total, const uint4 (&v)[LOADS]) {
-        float top = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < LOADS; ++u)
-#pragma unroll
-          for (int i = 0; i < VEC; i += 2) top = max3(top, Row::raw(v[u], i), Row::raw(v[u], i + 1));
-        most = fmaxf(most, top);
-        if (__any_sync(0xffffffffu, top > high)) {      // the first numbers, or some that weigh 2^60 and more
-          top = fminf(warp_top(top), F_MAX);
-          if (top > q.top) {
-            q.move(top, tp, total);
-            high = fmaxf(__fadd_rd(top, tp.near), top);
-          }
-        }
-        if (q.top == -INFINITY) return;
-        if (q.kind != 0 || high >= F_MAX) {      // (F_MAX: there may be +inf)
-#pragma unroll
-          for (int u = 0; u < LOADS; ++u) total += Row::seldom(v[u], q, table, tp.c);
-          return;
-        }
-        double even = 0.0, odd = 0.0;      // what is below `low`, and what is not a number, is taken as 2^-1000
-#pragma unroll
-        for (int u = 0; u < LOADS; ++u)
-#pragma unroll
-          for (int i = 0; i < VEC; i += 2) {
-            even += q.near(table, tp.c, fmaxf(Row::raw(v[u], i), q.low));
-            odd += q.near(table, tp.c, fmaxf(Row::raw(v[u], i + 1), q.low));
-          }
-        total += even + odd;
-      };
-      int slot = 0;
+      // ---------------------------------------------------------------- the sums of the row, the target's and then the draft's
+      begin();
 #pragma unroll 1
-      for (int g = g0; g < g1; g += STEP) {
-        copies_wait<AHEAD - 1>();
-        uint4* from = ring + tid + slot * (STEP_SLOTS * DV_THREADS);
-        uint4 wz[LOADS], wd[LOADS];
+      for (int which = 0; which < (DRAFT && !cold ? 2 : 1); ++which) {
+        const Row r = DRAFT && which ? d : z;
+        float peak = -INFINITY;      // the largest that a lane has met first
+        int at = 0x7fffffff;
+        Frame f;
+        f.top = -INFINITY;
+        float high = -INFINITY, most = -INFINITY;
+        double sum = 0.0;
+        int slot = 0;
+#pragma unroll 1
+        for (int g = g0; g < g1; g += STEP) {
+          copies_wait<AHEAD - 1>();
+          uint4* from = ring + tid + slot * (LOADS * DV_THREADS);
+          uint4 v[LOADS];
 #pragma unroll
-        for (int u = 0; u < LOADS; ++u) {
-          wz[u] = from[u * DV_THREADS];
-          if (DRAFT) wd[u] = from[(LOADS + u) * DV_THREADS];
-        }
-        slot = (slot + 1) % AHEAD;
-        if (g + AHEAD * STEP < g1) stage(from, g + AHEAD * STEP);
-        copies_commit();
-        add(f, high, most, sum, wz);
-        if (DRAFT) {
-          if (!cold) add(fd, dhigh, dmost, dsum, wd);
-        }
-        if (cold) {
+          for (int u = 0; u < LOADS; ++u) v[u] = from[u * DV_THREADS];
+          slot = (slot + 1) % AHEAD;
+          if (g + AHEAD * STEP < g1) stage(r, from, g + AHEAD * STEP);
+          copies_commit();
+          if (cold) {
+#pragma unroll
+            for (int u = 0; u < LOADS; ++u)
+#pragma unroll
+              for (int i = 0; i < VEC; ++i) {
+                const float x = Row::element(v[u], i);
+                if (x > peak) {
+                  peak = x;
+                  at = (g + u * 32 + lane) * VEC - r.shift + i;
+                }
+              }
+          }
+          float top = -INFINITY;
 #pragma unroll
           for (int u = 0; u < LOADS; ++u)
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-              const float x = Row::element(wz[u], i);
-              if (x > peak) {
-                peak = x;
-                at = (g + u * 32 + lane) * VEC - z.shift + i;
-              }
+            for (int i = 0; i < VEC; i += 2) top = max3(top, Row::raw(v[u], i), Row::raw(v[u], i + 1));
+          most = fmaxf(most, top);
+          if (__any_sync(0xffffffffu, top > high)) {      // the first numbers, or some that weigh 2^60 and more
+            top = fminf(warp_top(top), F_MAX);
+            if (top > f.top) {
+              f.move(top, tp, sum);
+              high = fmaxf(__fadd_rd(top, tp.near), top);
             }
-        }
-      }
-      __syncwarp();
-      sum = warp_sum_d(sum);
-      if (DRAFT) dsum = warp_sum_d(dsum);
-      if (cold) {
+          }
+          if (f.top == -INFINITY) continue;
+          if (f.kind != 0 || high >= F_MAX) {      // (F_MAX: there may be +inf)
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          const float x = __shfl_xor_sync(0xffffffffu, peak, o);
-          const int i = __shfl_xor_sync(0xffffffffu, at, o);
-          if (x > peak || (x == peak && i < at)) {
-            peak = x;
-            at = i;
+            for (int u = 0; u < LOADS; ++u) sum += Row::seldom(v[u], f, table, tp.c);
+            continue;
+          }
+          double even = 0.0, odd = 0.0;      // what is below `low`, and what is not a number, is taken as 2^-1000
+#pragma unroll
+          for (int u = 0; u < LOADS; ++u)
+#pragma unroll
+            for (int i = 0; i < VEC; i += 2) {
+              even += f.near(table, tp.c, fmaxf(Row::raw(v[u], i), f.low));
+              odd += f.near(table, tp.c, fmaxf(Row::raw(v[u], i + 1), f.low));
+            }
+          sum += even + odd;
+        }
+        if (DRAFT && which == 0 && !cold) first_steps(d);
+        __syncwarp();
+        sum = warp_sum_d(sum);
+        if (cold) {
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) {
+            const float x = __shfl_xor_sync(0xffffffffu, peak, o);
+            const int i = __shfl_xor_sync(0xffffffffu, at, o);
+            if (x > peak || (x == peak && i < at)) {
+              peak = x;
+              at = i;
+            }
           }
         }
+        push(which, sum, f.add, fminf(warp_top(most), F_MAX), at);
       }
-      begin();
       if (mine_of_tree && (first_row || child))
         for (uint32_t to = 0; to < ctas; ++to) {
           const uint32_t at = mapa_shared(smem_u32(&tree[tid]), to);
@@ -671,8 +667,6 @@ verify_kernel(const VerifyArgs a) {
             if (DRAFT) push_u(mapa_shared(smem_u32(&ld[tid]), to), __float_as_uint(own_d));
           }
         }
-      push(0, sum, f.add, fminf(warp_top(most), F_MAX), at);
-      if (DRAFT) push(1, dsum, fd.add, fminf(warp_top(dmost), F_MAX), 0);
       end();
       // a warp joins the target's parts, another the draft's: lane i has four of them, in their order
       if (warp < 1 + DRAFT) {
