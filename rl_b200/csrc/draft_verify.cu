@@ -247,8 +247,9 @@ struct Frame {
 };
 
 // One weight in a frame of any kind.
-__device__ __noinline__ double weight_of(const Frame* f, const double* table, double c, float x) {
-  return !(x >= f->low) ? 0.0 : f->kind == 2 ? (x == f->top ? 1.0 : 0.0) : f->near(table, c, x);
+__device__ __forceinline__ double weight_of(const Frame& f, const double* table, double c, float x) {
+  const double near = f.near(table, c, fminf(fmaxf(x, f.low), f.top));
+  return !(x >= f.low) ? 0.0 : f.kind == 2 ? (x == f.top ? 1.0 : 0.0) : near;
 }
 __device__ __forceinline__ void push_u(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ void push_row(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -337,16 +338,16 @@ struct Visit {
   const double* table;
   const double* grow;
   const int* gone;
-  uint4* slots;      // this lane's in shared memory, DV_THREADS apart
+  uint4* slots;      // of all lanes, DV_THREADS apart
   double c;
 };
 // What is left of the probability of token i after `r` rejections, from its logits.
 template <typename T, bool DRAFT>
 __device__ __noinline__ double rest_of(const Visit<T, DRAFT>& v, int i, float x, float y, int r) {
-  double w = weight_of(&v.row[0].f, v.table, v.c, x) * v.row[0].inv;
+  double w = weight_of(v.row[0].f, v.table, v.c, x) * v.row[0].inv;
   if (r == 0) return w;
   if (DRAFT) {
-    const double g = weight_of(&v.row[DRAFT].f, v.table, v.c, y) * v.row[DRAFT].inv;
+    const double g = weight_of(v.row[DRAFT].f, v.table, v.c, y) * v.row[DRAFT].inv;
 #pragma unroll 1
     for (int k = 0; k < r; ++k) w = fmax(fma(w, v.grow[k], -g), 0.0);
   } else {
@@ -405,13 +406,15 @@ template <typename T>
 __device__ __noinline__ double sum_left(const Visit<T, true>& v, int g0, int g1, int r) {
   constexpr int VEC = RowLogits<T>::VEC;
   const int lane = threadIdx.x & 31;
-  const RowLogits<T> z = v.z, d = v.d;
+  RowLogits<T> z = v.z, d = v.d;
+  z.range(g0, g1);
+  d.range(g0, g1);
   const Frame p = v.row[0].f, q = v.row[1].f;
   const double inv = v.row[0].inv, dinv = v.row[1].inv, c = v.c;
   const double* table = v.table;
   double even = 0.0, odd = 0.0;
   constexpr int AHEAD = DV_SLOTS / 2;
-  uint4* to = v.slots;
+  uint4* to = v.slots + threadIdx.x;
 #pragma unroll 1
   for (int k = 0; k < AHEAD; ++k, to += 2 * DV_THREADS) {
     z.stage(to, g0 + 32 * k + lane, g1);
@@ -422,7 +425,7 @@ __device__ __noinline__ double sum_left(const Visit<T, true>& v, int g0, int g1,
 #pragma unroll 1
   for (int g = g0; g < g1; g += 32) {
     copies_wait<AHEAD - 1>();
-    to = v.slots + at * (2 * DV_THREADS);
+    to = v.slots + threadIdx.x + at * (2 * DV_THREADS);
     const uint4 xx = to[0], yy = to[DV_THREADS];
     at = (at + 1) % AHEAD;
     if (g + 32 * AHEAD < g1) {
@@ -492,6 +495,7 @@ verify_kernel(const VerifyArgs a) {
   __shared__ double left[DR_ROWS + 1], grow[DR_ROWS + 1];       // what is left to be given after so many rejections, and its reciprocal
   __shared__ double chosen[DR_ROWS], sums[DR_ROWS];             // of each accepted step: l c - N of its token, the sum of weights
   __shared__ int verdict, tried, turned_down;
+  __shared__ Visit<T, DRAFT> visit;
   // (A shuffle or a vote where the compiler cannot rule out that the warp's lanes have parted costs some 260 cycles in place of 20: what decides on loops and branches goes
   // through one first.)
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -565,7 +569,6 @@ verify_kernel(const VerifyArgs a) {
           copies_commit();
         }
       };
-      first_steps(z);
       // The tree and its children's logits are read by the first CTA alone, for all: what the CTAs decide comes from the same numbers even where another stream is writing them.
       const bool mine_of_tree = rank == 0 && tid < s.n, first_row = count == 0;
       if (first_row && mine_of_tree) {
@@ -573,11 +576,13 @@ verify_kernel(const VerifyArgs a) {
         own_tok = a.tokens[s.lo + tid];
         own_num = a.uniforms[s.lo + tid];
       }
+      first_steps(z);
+      if (tid == 0) visit = Visit<T, DRAFT>{z, d, row, table, grow, gone, ring, tp.c};      // (read behind this row's barrier)
       const bool child = mine_of_tree && tid > node && own_up == node && own_tok >= 0 && own_tok < a.V;
-      float own_z = 0.f, own_d = 0.f;
+      T own_z{}, own_d{};      // (waited for where they are passed on)
       if (child) {
-        own_z = z.at(own_tok);
-        if (DRAFT) own_d = d.at(own_tok);
+        own_z = z.p[own_tok];
+        if (DRAFT) own_d = d.p[own_tok];
       }
       // ---------------------------------------------------------------- the sums of the row, the target's and then the draft's
       begin();
@@ -661,10 +666,10 @@ verify_kernel(const VerifyArgs a) {
       if (mine_of_tree && (first_row || child))
         for (uint32_t to = 0; to < ctas; ++to) {
           const uint32_t at = mapa_shared(smem_u32(&tree[tid]), to);
-          if (first_row) push_row(at, static_cast<uint32_t>(own_up), static_cast<uint32_t>(own_tok), __float_as_uint(own_num), __float_as_uint(own_z));
+          if (first_row) push_row(at, static_cast<uint32_t>(own_up), static_cast<uint32_t>(own_tok), __float_as_uint(own_num), __float_as_uint(usable(static_cast<float>(own_z))));
           if (child) {
-            if (!first_row) push_u(at + 12, __float_as_uint(own_z));
-            if (DRAFT) push_u(mapa_shared(smem_u32(&ld[tid]), to), __float_as_uint(own_d));
+            if (!first_row) push_u(at + 12, __float_as_uint(usable(static_cast<float>(own_z))));
+            if (DRAFT) push_u(mapa_shared(smem_u32(&ld[tid]), to), __float_as_uint(usable(static_cast<float>(own_d))));
           }
         }
       end();
@@ -709,7 +714,6 @@ verify_kernel(const VerifyArgs a) {
         __syncwarp();
       }
       if (DRAFT) __syncthreads();
-      Visit<T, DRAFT> visit{z, d, row, table, grow, gone, ring + tid, tp.c};
       const int e0 = max(0, g0 * VEC - z.shift), e1 = min(a.V, g1 * VEC - z.shift);      // the range's tokens
       double mine[4], total = 0.0;
       auto take = [&](double v) {      // this warp's part of new sums; the parts and the whole sum of all
@@ -738,7 +742,7 @@ verify_kernel(const VerifyArgs a) {
             }
             const float x = child ? tree[j].z : -INFINITY, y = DRAFT && child ? ld[j] : -INFINITY;
             double w = rest_of<T, DRAFT>(visit, t, x, y, r), asked = child ? static_cast<double>(tree[j].number) : 0.0;
-            if (DRAFT) asked *= weight_of(&row[DRAFT].f, table, tp.c, y) * row[DRAFT].inv;
+            if (DRAFT) asked *= weight_of(row[DRAFT].f, table, tp.c, y) * row[DRAFT].inv;
             __syncwarp();
             for (; todo; todo &= todo - 1) {
               const int l = __ffs(todo) - 1, tl = __shfl_sync(0xffffffffu, t, l);
