@@ -308,8 +308,8 @@ struct RowLogits {
     }
     return v;
   }
-  static __device__ __forceinline__ float raw(const uint4& v, int i) {
-    const uint32_t* w = &v.x;
+  static __device__ __forceinline__ float raw(const uint4& v, int i) { return raw(&v.x, i); }
+  static __device__ __forceinline__ float raw(const uint32_t* w, int i) {
     return sizeof(T) == 4 ? __uint_as_float(w[i]) : __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
   }
   static __device__ __forceinline__ float element(const uint4& v, int i) { return usable(raw(v, i)); }
@@ -426,30 +426,30 @@ __device__ __noinline__ double sum_left(const Visit<T, true>& v, int g0, int g1,
   for (int g = g0; g < g1; g += 32) {
     copies_wait<AHEAD - 1>();
     to = v.slots + threadIdx.x + at * (2 * DV_THREADS);
-    const uint4 xx = to[0], yy = to[DV_THREADS];
+    const uint32_t *xs = reinterpret_cast<const uint32_t*>(to), *ys = reinterpret_cast<const uint32_t*>(to + DV_THREADS);
+#pragma unroll 1
+    for (int h = 0; h < VEC; h += 4, xs += sizeof(T), ys += sizeof(T)) {      // four at a time: more do not fit the registers
+      double w[4], e[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i] = p.near(table, c, fmaxf(RowLogits<T>::raw(xs, i), p.low)) * inv;
+        e[i] = q.near(table, c, fmaxf(RowLogits<T>::raw(ys, i), q.low)) * dinv;
+      }
+#pragma unroll 1
+      for (int k = 0; k < r; ++k) {
+        const double grow = v.grow[k];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = fmax(fma(w[i], grow, -e[i]), 0.0);
+      }
+      even += w[0] + w[2];
+      odd += w[1] + w[3];
+    }
     at = (at + 1) % AHEAD;
     if (g + 32 * AHEAD < g1) {
       z.stage(to, g + 32 * AHEAD + lane, g1);
       d.stage(to + DV_THREADS, g + 32 * AHEAD + lane, g1);
     }
     copies_commit();
-    double w[VEC], e[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      w[i] = p.near(table, c, fmaxf(RowLogits<T>::raw(xx, i), p.low)) * inv;
-      e[i] = q.near(table, c, fmaxf(RowLogits<T>::raw(yy, i), q.low)) * dinv;
-    }
-#pragma unroll 1
-    for (int k = 0; k < r; ++k) {
-      const double grow = v.grow[k];
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) w[i] = fmax(fma(w[i], grow, -e[i]), 0.0);
-    }
-#pragma unroll
-    for (int i = 0; i < VEC; i += 2) {
-      even += w[i];
-      odd += w[i + 1];
-    }
   }
   __syncwarp();
   return warp_sum_d(even + odd);
@@ -482,8 +482,8 @@ template <typename T, bool DRAFT>
 __global__ void __launch_bounds__(DV_THREADS, 2)
 verify_kernel(const VerifyArgs a) {
   using Row = RowLogits<T>;
-  constexpr int VEC = Row::VEC, LOADS = Row::LOADS, STEP = 32 * LOADS, AHEAD = DV_SLOTS / LOADS;
-  extern __shared__ uint4 ring[];                     // [DV_SLOTS][DV_THREADS]
+  constexpr int VEC = Row::VEC, LOADS = Row::LOADS, STEP = 32 * LOADS, AHEAD = 2;
+  extern __shared__ uint4 ring[];                     // [AHEAD steps][LOADS][DV_THREADS]
   __shared__ double table[EXP_STEPS];
   __shared__ Parts parts[2][1 + DRAFT];      // of all warps of the cluster, by turns
   __shared__ double share[DV_PARTS], pieces[DV_WARPS];      // the ranges' probabilities; sums of a range's pieces
@@ -549,15 +549,14 @@ verify_kernel(const VerifyArgs a) {
     };
 
     while (true) {
-      Row z{static_cast<const T*>(a.logits) + (s.lo + node) * a.ld, a.V, 0, true, false}, d{};
-      z.shift = static_cast<int>(reinterpret_cast<uintptr_t>(z.p) % 16 / sizeof(T));
-      if (DRAFT) {
-        d = Row{static_cast<const T*>(a.draft) + (s.lo + node) * a.ld_draft, a.V, z.shift, false, false};
-        d.vec = reinterpret_cast<uintptr_t>(d.p) % 16 / sizeof(T) == z.shift;
-      }
-      const int groups = (a.V + z.shift + VEC - 1) / VEC, g0 = min(groups, me * groups_per), g1 = min(groups, g0 + groups_per);
-      z.range(g0, g1);
-      if (DRAFT) d.range(g0, g1);
+      const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(static_cast<const T*>(a.logits) + (s.lo + node) * a.ld) % 16 / sizeof(T));
+      const int groups = (a.V + shift + VEC - 1) / VEC, g0 = min(groups, me * groups_per), g1 = min(groups, g0 + groups_per);
+      auto row_of = [&](int which) {      // the target's, the draft's (made again where it is asked for: registers are short)
+        Row r{static_cast<const T*>(DRAFT && which ? a.draft : a.logits) + (s.lo + node) * (DRAFT && which ? a.ld_draft : a.ld), a.V, shift, false, false};
+        r.vec = reinterpret_cast<uintptr_t>(r.p) % 16 / sizeof(T) == shift;
+        r.range(g0, g1);
+        return r;
+      };
       auto stage = [&](const Row& r, uint4* to, int g) {      // of a step
 #pragma unroll
         for (int u = 0; u < LOADS; ++u) r.stage(to + u * DV_THREADS, g + u * 32 + lane, g1);
@@ -576,19 +575,19 @@ verify_kernel(const VerifyArgs a) {
         own_tok = a.tokens[s.lo + tid];
         own_num = a.uniforms[s.lo + tid];
       }
-      first_steps(z);
-      if (tid == 0) visit = Visit<T, DRAFT>{z, d, row, table, grow, gone, ring, tp.c};      // (read behind this row's barrier)
+      first_steps(row_of(0));
+      if (tid == 0) visit = Visit<T, DRAFT>{row_of(0), DRAFT ? row_of(1) : Row{}, row, table, grow, gone, ring, tp.c};      // (read behind this row's barrier)
       const bool child = mine_of_tree && tid > node && own_up == node && own_tok >= 0 && own_tok < a.V;
       T own_z{}, own_d{};      // (waited for where they are passed on)
       if (child) {
-        own_z = z.p[own_tok];
-        if (DRAFT) own_d = d.p[own_tok];
+        own_z = row_of(0).p[own_tok];
+        if (DRAFT) own_d = row_of(1).p[own_tok];
       }
       // ---------------------------------------------------------------- the sums of the row, the target's and then the draft's
       begin();
 #pragma unroll 1
       for (int which = 0; which < (DRAFT && !cold ? 2 : 1); ++which) {
-        const Row r = DRAFT && which ? d : z;
+        const Row r = row_of(which);
         float peak = -INFINITY;      // the largest that a lane has met first
         int at = 0x7fffffff;
         Frame f;
@@ -647,7 +646,7 @@ verify_kernel(const VerifyArgs a) {
             }
           sum += even + odd;
         }
-        if (DRAFT && which == 0 && !cold) first_steps(d);
+        if (DRAFT && which == 0 && !cold) first_steps(row_of(1));
         __syncwarp();
         sum = warp_sum_d(sum);
         if (cold) {
@@ -714,7 +713,7 @@ verify_kernel(const VerifyArgs a) {
         __syncwarp();
       }
       if (DRAFT) __syncthreads();
-      const int e0 = max(0, g0 * VEC - z.shift), e1 = min(a.V, g1 * VEC - z.shift);      // the range's tokens
+      const int e0 = max(0, g0 * VEC - shift), e1 = min(a.V, g1 * VEC - shift);      // the range's tokens
       double mine[4], total = 0.0;
       auto take = [&](double v) {      // this warp's part of new sums; the parts and the whole sum of all
         begin();
@@ -810,7 +809,7 @@ verify_kernel(const VerifyArgs a) {
       if (cold || !some) {
         if (rank == 0 && tid == 0) {
           drawn = some ? row_best : 0;
-          drawn_z = some ? z.at(drawn) : 0.f;
+          drawn_z = some ? visit.z.at(drawn) : 0.f;
         }
         ++count;
         break;
@@ -820,7 +819,7 @@ verify_kernel(const VerifyArgs a) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) mine[k] = share[k * 32 + lane];
           for (int r = 0; r < rejected; ++r) {
-            const int w = (gone[r] + z.shift) / VEC / groups_per;
+            const int w = (gone[r] + shift) / VEC / groups_per;
             const double off = left[r] - left[r + 1];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
@@ -830,7 +829,7 @@ verify_kernel(const VerifyArgs a) {
         } else {
           bool hit = false;
           for (int k = 0; k < rejected; ++k) {
-            const int g = (gone[k] + z.shift) / VEC;
+            const int g = (gone[k] + shift) / VEC;
             hit |= g >= g0 && g < g1;
           }
           take(__any_sync(0xffffffffu, hit) ? sum_of<T, DRAFT>(visit, e0, e1, rejected) : share[part_place(me)]);
@@ -873,7 +872,7 @@ verify_kernel(const VerifyArgs a) {
         owner = __shfl_sync(0xffffffffu, last, 31 - __clz(any));
       }
       if (rank == owner / DV_WARPS) {      // the range once more, by all warps of its CTA
-        const int r0 = max(0, min(groups, owner * groups_per) * VEC - z.shift), r1 = min(a.V, (owner + 1) * groups_per * VEC - z.shift);
+        const int r0 = max(0, min(groups, owner * groups_per) * VEC - shift), r1 = min(a.V, (owner + 1) * groups_per * VEC - shift);
         const int piece = (r1 - r0 + DV_WARPS - 1) / DV_WARPS, q0 = min(r1, r0 + warp * piece), q1 = min(r1, q0 + piece);
         const double own = sum_of<T, DRAFT>(visit, q0, q1, rejected);
         if (lane == 0) pieces[warp] = own;
@@ -894,7 +893,7 @@ verify_kernel(const VerifyArgs a) {
           const int hit = max(0, find_token<T, DRAFT>(visit, q0, q1, rejected, start, aim, inside));
           if (lane == 0) {
             drawn = hit;
-            drawn_z = z.at(hit);
+            drawn_z = visit.z.at(hit);
           }
         }
       }
