@@ -320,7 +320,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   int* red = reinterpret_cast<int*>(smem + S::SMEM - 128);      // [THREADS / 32]
   int* start = red + THREADS / 32;                              // [2]
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;      // (one of the warp's, as the compiler sees then)
   if (threadIdx.x == 0) {
     prefetch_tmap(&tmap_q);
     prefetch_tmap(&tmap_k);
