@@ -129,13 +129,18 @@ keep_kernel(const __grid_constant__ KeepCaches caches, const int* __restrict__ t
 // p = softmax(l / T) of a node, in 64 bits throughout: the last token is the first whose running sum passes a given number, and with 32 bits the running sums of a flat
 // distribution over 10^5 tokens would be off by as much as a token has. A weight is 2^(l c - N), c = log2(e) / T, with a whole number N next to the largest l c that a warp has met first: so
 // sums of several warps are joined by their exponents. l c - N is cut into 256ths, a table's entry, and a rest r, |r| <= 1 / 512, for which a polynomial of third degree is off by
-// (r ln 2)^4 / 24 < 1.5e-13. Eight instructions of the 64-bit pipe and some ten others a logit.
+// (r ln 2)^4 / 24 < 1.5e-13. Eight instructions of the 64-bit pipe a logit and, with the loads,
+// some twenty others.
 //
 // A cluster of CTAs has a sequence. It walks down the accepted rows and reads the logits of these rows alone, which is what the operator cannot do without: each warp has a range
 // of tokens and leaves its sum in every CTA's shared memory; all CTAs come to the same decision. The ranges' sums say in which range the last token lies, whose CTA
 // goes through it once more. With draft logits the sums are taken again behind a rejection; without, the rejected tokens' weights are taken off their ranges.
 //
-// Bound by the instructions' rate and, for few sequences, by latency: the row, the exchange and the decision one after another (a 64-bit instruction takes 18 cycles).
+// Bound by the instructions' rate (64 trees of 17 rows, 128256 logits: 54 us for 56 MB, 58 % of the issue slots while an SM has work) and by latency: a row is its sums (5500 cycles of
+// 11000), the exchange (1400), the joining of the parts (1000) and the children (1000), one after another; a single row of 128256 logits takes 10 us, a chain of 6 with 32000 logits 10.
+// 48 sequences of 8 drawn rows, 151936 logits: 127 us for 82 MB. A first pass in 32 bits with sums in 64 where they decide was slower, so were 256 threads in clusters of 16, a table
+// entry for each of 128ths in 16 copies without conflicts of banks, and eight loads of a lane on their way in place of four.
+// What the functions behind a row's sums read lies in shared memory: in every thread's own memory (52 KB a CTA) it came from the second level cache (59 us in place of 52).
 struct VerifyArgs {
   const void* logits;
   const void* draft;      // null: children are taken without chance
@@ -920,7 +925,7 @@ verify_kernel(const VerifyArgs a) {
 template <typename T, bool DRAFT>
 int launch_verify(const VerifyArgs& a, int B, cudaStream_t stream) {
   // Two CTAs to an SM. The largest cluster with which all sequences run at once, or in two turns where they may go down several rows: the last sequences' rows
-  // are what the others wait for (64 trees of 17 rows: four CTAs 70 us, eight 69; 48 of 8 drawn ones 213 and 191; 64 single rows 27 and 36).
+  // are what the others wait for (us with two turns and with one: 64 trees of 17 rows 54 and 57, 48 of 8 drawn ones 127 and 142, 256 trees of 5 113 and 145; 64 single rows 26 and 21).
   int dev = 0, sms = 148;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);

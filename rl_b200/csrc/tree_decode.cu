@@ -15,6 +15,10 @@
 // The tiles of all units form one sequence, of which each CTA takes an equal share (two CTAs to an SM, all resident): contexts of any lengths fill the device. Units that
 // are cut leave sums, maximum and 32-bit output of their parts in a workspace, and a second kernel joins them in their order. With few tiles to a unit a CTA takes a whole unit instead.
 //
+// Long contexts of few rows are bound by memory (32 chains of 5 on 32768 tokens, 32 / 8 heads of 128: 4.3 GB of keys and values in 624 us, above the rate of a plain copy). With 64 rows and more the
+// tensor cores and the softmax take turns: a product of 64 keys costs as much as one of 128, and a pair of tiles takes 2100 cycles, 1540 of them the products' (16 trees of 64 on 8001, 28 / 4 heads: 104 us,
+// 0.17 GB; one tree of 33 on 131072, 40 / 8 heads: 147 us, 0.54 GB). Short contexts pay for a unit's start and end (64 trees of 17 rows to 1280 tokens: 52 us where memory takes 35).
+//
 // This file is compiled without fast math.
 #include "common.cuh"
 
@@ -864,7 +868,7 @@ RLB_API int rlb_tree_decode(const void* q, long long ldq, const void* k, const v
   a.cuts = static_cast<Cut*>(cuts);
   a.least = least;
   a.group = ctas ? group : 1;
-  // (more units than run at once)
+  // (more units than run at once: 64 trees of 17 rows on ragged contexts to 1280 55 -> 52 us; where all have 804 tokens 46 -> 49)
   a.sorted = !ctas && B > 1 && B <= THREADS && static_cast<long long>(B) * Hkv * ((max_rows + a.block_rows - 1) / a.block_rows) > 2 * 148;
   a.status = status;
   return D == 64 ? launch<64>(q, ldq, k, v, a, ctas, static_cast<cudaStream_t>(stream)) : launch<128>(q, ldq, k, v, a, ctas, static_cast<cudaStream_t>(stream));
