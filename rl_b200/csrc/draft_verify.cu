@@ -977,7 +977,7 @@ RLB_API int rlb_kv_keep(void* const* caches, int tensors, const int* table, long
 RLB_API int rlb_verify_drafts(const void* logits, long long ld, const void* draft, long long ld_draft, int f32, int V, int T, int B, int max_rows, int steps,
                               const int* tokens, const int* parents, const int* cu, const float* uniforms, const float* temps, double temp, int greedy,
                               int* out_tokens, int* out_counts, int* out_rows, float* out_logprobs, int* status, void* stream) {
-  if (max_rows < 1 || max_rows > DR_ROWS || steps < 1 || steps > max_rows || V < 1) return -2;
+  if (max_rows < 1 || max_rows > DR_ROWS || steps < 1 || steps > max_rows || V < 1 || V > 1 << 30) return -2;
   const VerifyArgs a{logits, draft, ld, ld_draft, V, T, max_rows, steps, greedy, tokens, parents, cu, uniforms, temps, temp, out_tokens, out_counts, out_rows,
                      out_logprobs, status};
   if (static_cast<long long>(B) * DV_CLUSTER > 0x7fffffffll) return -2;

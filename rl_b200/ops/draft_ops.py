@@ -37,7 +37,8 @@ BF16 = torch.bfloat16
 HEAD_DIMS = (64, 128)
 MAX_ROWS = 256
 COLDEST = torch.finfo(torch.float32).tiny
-MAX_SCALE = torch.finfo(torch.float32).max
+MAX_SCALE = torch.finfo(torch.float32).max / 2      # (times log2(e) it has to be a number still)
+MAX_VOCAB = 1 << 30
 MAX_TOKENS = 0x7FFF0000      # of a sequence: places are 32-bit numbers
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else lambda index: torch.cuda.current_stream(index).cuda_stream
 
@@ -222,7 +223,7 @@ def tree_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         positions = _ints(positions, (T,), "positions")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not abs(scale) <= MAX_SCALE:
-        raise ValueError(f"scale {scale} is not a number of 32 bits")
+        raise ValueError(f"scale {scale} is no number of at most {MAX_SCALE}")
     _no_gradient(q, k_cache, v_cache)
     if out is None:
         out = q.new_empty((T, width))
@@ -354,8 +355,8 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Ten
     Returns ``tokens`` int32 [B, max_steps] (accepted ones and the last; -1 behind them), ``counts`` int32 [B], ``rows`` int32 [B, max_steps] (row 0 and the accepted rows, as :func:`kv_cache_keep`
     takes them; -1 behind them) and ``logprobs`` fp32 [B, max_steps], the tokens' logarithms of p (0 behind them; -inf where no logit is above -inf, whose token is 0). Sums are in 64 bits."""
     B = _rows_of(cu_rows, max_rows)
-    if logits.dim() != 2 or logits.dtype not in (torch.float32, BF16) or logits.shape[1] < 1:
-        raise ValueError(f"logits are fp32 or bf16 [T, V], not {logits.dtype} {tuple(logits.shape)}")
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, BF16) or not 1 <= logits.shape[1] <= MAX_VOCAB:
+        raise ValueError(f"logits are fp32 or bf16 [T, V] with V up to 2^30, not {logits.dtype} {tuple(logits.shape)}")
     T, V = logits.shape
     device = logits.device
     if draft_logits is not None and (draft_logits.shape != logits.shape or draft_logits.dtype != logits.dtype):

@@ -193,6 +193,18 @@ def test_refusals():
             S.kv_cache_keep(**{**dict(caches=[(k, v)], block_table=table, ctx_lens=ctx, rows=rows, counts=counts), **bad})
 
 
+def test_refusals_of_what_32_bits_do_not_count():
+    """Scales that are infinite times log2(e), more tokens than places of a row are counted to (rows of none, so that nothing of that size is held)."""
+    q, k, v, table, ctx, cu, _ = _attend_case([2], [5], 4, 2, 64, 16)
+    for scale in (3e38, -2.4e38):
+        with pytest.raises(ValueError):
+            S.tree_paged_decode(q, k, v, table, ctx, cu, 4, 2, 64, max_rows=3, scale=scale)
+    none, zero = torch.zeros(0, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        S.verify_drafts(torch.zeros((0, 2**30 + 1)), none, none, zero, torch.zeros(0), max_rows=4)
+    assert S.verify_drafts(torch.zeros((0, 2**30)), none, none, zero, torch.zeros(0), max_rows=4)[1].tolist() == [0]
+
+
 def test_empty_batches():
     none = torch.zeros(0, dtype=torch.int32)
     cu, table = torch.zeros(1, dtype=torch.int32), torch.zeros((0, 1), dtype=torch.int32)
