@@ -454,6 +454,23 @@ def test_streams(native_lib):
     assert all(torch.equal(x, want) for x in got) and L.check_status() == 0
 
 
+def test_verify_on_two_streams(native_lib):
+    """Calls on side streams, two at once: the same results every time, whoever of a cluster is first."""
+    cases = []
+    for draft, dtype in ((False, torch.float32), (True, torch.bfloat16)):
+        logits, guess, tokens, parents, cu, u = _verify_case([9, 1, 6, 0, 9] * 4, 30011, 5, 2, draft, dtype)
+        cases.append((_dev(logits, tokens, parents, cu, u), dict(max_rows=9, draft_logits=guess.cuda() if draft else None)))
+    want = [S.verify_drafts(*args, **more) for args, more in cases]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((i, S.verify_drafts(*cases[i][0], **cases[i][1])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for i, g in got for x, y in zip(g, want[i])) and L.check_status() == 0
+
+
 def test_verify_of_logits_that_grow(native_lib):
     """Ranges whose later logits weigh far more than their first ones, up to what has no place beside them."""
     V = 40000
