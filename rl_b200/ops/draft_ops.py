@@ -101,7 +101,7 @@ def tree_rows(parents: torch.Tensor, cu_rows: torch.Tensor, ctx_lens: torch.Tens
               ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """What the layers need of the trees' rows: ``masks`` int32 [T, ceil(max_rows / 32)], in which bit ``i % 32`` of word ``i // 32`` says that a row sees row ``i`` of its
     sequence (itself and the rows that it continues); ``positions`` int32 [T], the context's length and the rows before it on its path; ``slots`` int64 [T], the
-    cache places as ``rope_kv_cache_write`` takes them. Rows behind the last sequence see nothing, with position 0 and slot -1 (which is skipped)."""
+    cache places as ``rope_kv_cache_write`` takes them. Rows of no sequence (behind the last, before the first, over ``max_rows``) see nothing, with position 0 and slot -1 (which is skipped)."""
     B = _rows_of(cu_rows, max_rows)
     T, device, words = parents.shape[0] if parents.dim() == 1 else -1, parents.device, -(-max_rows // 32)
     parents = _ints(parents, (T,), "parents")
