@@ -139,7 +139,7 @@ keep_kernel(const __grid_constant__ KeepCaches caches, const int* __restrict__ t
 // Bound by the instructions' rate (64 trees of 17 rows, 128256 logits: 54 us for 56 MB, 58 % of the issue slots while an SM has work) and by latency: a row is its sums (5500 cycles of
 // 11000), the exchange (1400), the joining of the parts (1000) and the children (1000), one after another; a single row of 128256 logits takes 10 us, a chain of 6 with 32000 logits 10.
 // 48 sequences of 8 drawn rows, 151936 logits: 127 us for 82 MB. A first pass in 32 bits with sums in 64 where they decide was slower, so were 256 threads in clusters of 16, a table
-// entry for each of 128ths in 16 copies without conflicts of banks, and eight loads of a lane on their way in place of four.
+// entry for each of 128ths in 16 copies without conflicts of banks, eight loads of a lane on their way in place of four, and the first child's logits fetched while a row's parts are exchanged.
 // What the functions behind a row's sums read lies in shared memory: in every thread's own memory (52 KB a CTA) it came from the second level cache (59 us in place of 52).
 struct VerifyArgs {
   const void* logits;
