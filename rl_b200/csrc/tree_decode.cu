@@ -349,6 +349,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     mbar_fence_init();
     fence_proxy_async();
   }
+  __syncthreads();      // (no warp waits for a barrier before it is one, whichever way it goes below)
   pdl_sync();
 
   // ---------------------------------------------------------------- this CTA's tiles
