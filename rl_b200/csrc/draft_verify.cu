@@ -497,7 +497,7 @@ verify_kernel(const VerifyArgs a) {
   __shared__ TreeRow tree[DR_ROWS];
   __shared__ float ld[DR_ROWS];      // as TreeRow::z, the draft's
   __shared__ int gone[DR_ROWS];
-  __shared__ double left[DR_ROWS + 1], grow[DR_ROWS + 1];       // what is left to be given after so many rejections, and its reciprocal
+  __shared__ double left[DR_ROWS + 1], grow[DR_ROWS + 1];       // what is left to be given after so many rejections; its reciprocal, without draft logits the rejected tokens' weights
   __shared__ double chosen[DR_ROWS], sums[DR_ROWS];             // of each accepted step: l c - N of its token, the sum of weights
   __shared__ int verdict, tried, turned_down;
   __shared__ Visit<T, DRAFT> visit;
@@ -764,6 +764,7 @@ verify_kernel(const VerifyArgs a) {
                 rest -= wl;
                 if (lane == 0) {
                   gone[r] = tl;
+                  grow[r] = wl;
                   left[r + 1] = rest;
                 }
                 ++r;
@@ -820,16 +821,20 @@ verify_kernel(const VerifyArgs a) {
         break;
       }
       if (!DRAFT && rejected > 0) {      // without the rejected tokens
-        if (__any_sync(0xffffffffu, left[rejected] >= 1.0 / 1024)) {      // their weights are taken off their ranges' sums, of which no more than ten bits are lost
+        // Their weights are taken off their ranges' sums, of which no more than ten bits are lost. A range without any other token keeps some 500 roundings of its sum (2^-44 of it), which
+        // are no token's weight: where a range has lost all but 2^-40, or is so light that its roundings are coarser, the sums are taken again. So a range that has something has a token.
+        bool again = left[rejected] < 1.0 / 1024;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mine[k] = share[k * 32 + lane];
-          for (int r = 0; r < rejected; ++r) {
-            const int w = (gone[r] + shift) / VEC / groups_per;
-            const double off = left[r] - left[r + 1];
+        for (int k = 0; k < 4; ++k) mine[k] = share[k * 32 + lane];
+        for (int r = 0; r < rejected; ++r) {
+          const int w = (gone[r] + shift) / VEC / groups_per;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (w == lane * 4 + k) mine[k] = fmax(mine[k] - off, 0.0);
-          }
+          for (int k = 0; k < 4; ++k)
+            if (w == lane * 4 + k) mine[k] -= grow[r];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) again |= share[k * 32 + lane] > 0.0 && mine[k] < fma(0x1p-40, share[k * 32 + lane], 0x1p-960);
+        if (!__any_sync(0xffffffffu, again)) {
           total = warp_sum_d((mine[0] + mine[1]) + (mine[2] + mine[3]));
         } else {
           bool hit = false;
@@ -894,7 +899,7 @@ verify_kernel(const VerifyArgs a) {
         const int mover = over ? __ffs(__ballot_sync(0xffffffffu, piece_sum > 0.0 && start + upto > aim)) - 1 : -1;
         if (mover >= 0) start += __shfl_sync(0xffffffffu, upto - piece_sum, mover);
         const bool inside = mover >= 0;      // (otherwise the last that has a share)
-        if (warp == (inside ? mover : filled)) {
+        if (warp == (inside ? mover : max(filled, 0))) {      // (a token is written, whatever the logits became meanwhile)
           const int hit = max(0, find_token<T, DRAFT>(visit, q0, q1, rejected, start, aim, inside));
           if (lane == 0) {
             drawn = hit;

@@ -213,3 +213,42 @@ def test_empty_batches():
     assert S.tree_paged_decode(torch.zeros(0, 64), k, k, table, none, cu, 1, 1, 64, max_rows=4).shape == (0, 64)
     assert S.verify_drafts(torch.zeros(0, 5), none, none, cu, torch.zeros(0), max_rows=4)[0].shape == (0, 4)
     S.kv_cache_keep([(k, k)], table, none, torch.zeros((0, 4), dtype=torch.int32), none)
+
+
+def masked_case(V, sizes, seed, draft, dtype=torch.float32, most=6):
+    """Rows of which a filter or a grammar has left a few tokens (the draft's has left others beside some of them), children that are often turned down, and row 0's number zero for
+    every other sequence."""
+    g = torch.Generator().manual_seed(seed)
+    parents, cu = O.forest(sizes, seed, 3)
+    T = int(cu[-1])
+    logits, guess = torch.full((T, V), -math.inf), torch.full((T, V), -math.inf)
+    for t in range(T):
+        few = torch.randperm(V, generator=g)[: 2 + int(torch.randint(most - 1, (1,), generator=g))]
+        logits[t, few] = torch.randn(len(few), generator=g)
+        both = few[torch.rand(len(few), generator=g) < 0.8]
+        guess[t, both] = logits[t, both] + torch.randn(len(both), generator=g)
+        guess[t, torch.randint(V, (2,), generator=g)] = 0.3
+    logits, guess = logits.to(dtype), guess.to(dtype)
+    tokens, used = torch.zeros(T, dtype=torch.int32), {}
+    for b, n in enumerate(sizes):
+        for j in range(1, n):
+            p = int(cu[b]) + int(parents[int(cu[b]) + j])
+            used[p] = used.get(p, -1) + 1
+            best = logits[p].float().topk(min(2, V)).indices
+            tokens[int(cu[b]) + j] = int(torch.multinomial(torch.softmax(guess[p].float(), -1), 1, generator=g)) if draft else int(best[-1 - used[p] % len(best)])
+    u = torch.rand(T, generator=g) ** 0.1
+    u = u.clamp(max=1 - 2.0**-20)
+    u[cu[:-1].long()[::2]] = 0.0
+    u[cu[:-1].long()[1::2]] = torch.rand(len(u[cu[:-1].long()[1::2]]), generator=g)
+    return logits, guess if draft else None, tokens, parents, cu, u
+
+
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("V", [9, 1000])
+def test_verify_restatement_on_masked_logits(V, draft):
+    for seed in range(4):
+        sizes = [4, 1, 7, 2, 5, 3]
+        logits, guess, tokens, parents, cu, u = masked_case(V, sizes, seed, draft)
+        want = O.verify(logits, tokens, parents, cu, u, guess)
+        assert min(w[3] for w in want) > 1e-9
+        _same(S.verify_drafts(logits, tokens, parents, cu, u, max_rows=7, draft_logits=guess), want, 7)

@@ -5,7 +5,7 @@ import math
 import draft_oracle as O
 import pytest
 import torch
-from test_draft_ops import _same, _verify_case
+from test_draft_ops import _same, _verify_case, masked_case
 
 from rl_b200.ops import draft_ops as S
 from rl_b200.ops import engine_ops as E
@@ -517,3 +517,41 @@ def test_plans_that_are_refused(native_lib):
     for scratch in (torch.zeros(10, device="cuda"), torch.zeros(10**6, device="cuda", dtype=torch.bfloat16), torch.zeros(10**6), torch.zeros(10**6, device="cuda")[1:]):
         with pytest.raises(ValueError):
             S.tree_paged_decode(q, k, v, table, ctx, cu, 8, 2, 128, max_rows=18, plan=(8, 1), scratch=scratch)
+
+
+def _poisoned(args, **kw):
+    """A call whose results' memory held other numbers."""
+    held = [torch.full((n,), 77, dtype=I32, device="cuda") for n in (len(args[3]) - 1, (len(args[3]) - 1) * kw["max_rows"]) for _ in range(4)]
+    torch.cuda.synchronize()
+    del held      # (their places are the next ones to be given out)
+    return S.verify_drafts(*_dev(*args), **{k: x.cuda() if torch.is_tensor(x) else x for k, x in kw.items()})
+
+
+def _as_on_the_cpu(args, **kw):
+    want = S.verify_drafts(*args, **kw)
+    for x, y in zip(_poisoned(args, **kw)[:3], want[:3]):
+        assert torch.equal(x.cpu(), y)
+    got = _poisoned(args, **kw)[3].cpu()
+    assert torch.allclose(got, want[3], rtol=2.0**-23, atol=1e-12)
+    assert L.check_status() == 0
+    return want
+
+
+def test_verify_behind_the_only_token_of_a_range(native_lib):
+    """A turned-down token that is all, or nearly all, of what its range of the vocabulary weighs: the range has nothing left, or what is far below the sum's roundings."""
+    V = 128256
+    for low, high in ((0.0, 1.0), (0.3, -0.2), (-1.7, 2.9), (0.11, 0.13)):
+        for third in (-math.inf, -35.0, -60.0, -300.0):
+            z = torch.full((2, V), -math.inf)
+            z[:, 5], z[:, 6], z[:, 2000] = low, third, high
+            for u0 in (0.0, 0.3, 1 - 2.0**-24):
+                want = _as_on_the_cpu((z, *(torch.tensor(x, dtype=I32) for x in ([0, 5], [-1, 0], [0, 2])), torch.tensor([u0, 0.999])), max_rows=2)
+                assert int(want[0][0, 0]) == (6 if u0 == 0 and third > -math.inf else 2000)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,batch", [(9, 3), (1003, 40), (30011, 6), (4096, 400)])
+def test_verify_of_masked_logits(native_lib, V, batch, dtype):
+    for seed in range(3):
+        logits, _, tokens, parents, cu, u = masked_case(V, [1 + (3 * b + seed) % 7 for b in range(batch)], seed, False, dtype)
+        _as_on_the_cpu((logits, tokens, parents, cu, u), max_rows=7)
