@@ -406,7 +406,9 @@ __device__ __noinline__ double sum_of(const Visit<T, DRAFT>& v, int e0, int e1, 
   __syncwarp();
   return warp_sum_d(sum);
 }
-// The same of the groups from g0 to g1 of a row and its draft's, both of kind 0 and without infinities: as in the row's own sums.
+// The same of the groups from g0 to g1 of a row and its draft's, both of kind 0 and without infinities: as in the row's own sums, but that what weighs nothing in the target is nothing, or a
+// difference would be left where no token has a share and the last token could fall there. (2^-500 and less, `low`'s weight, times a factor without exponent, below 2^-1042, is zero: 127 us for 48 of
+// 8 drawn rows, 151936 logits, as without it; 131 with the weight itself chosen.) The draft's may be too much by as much: a sum is never more than its tokens' shares.
 template <typename T>
 __device__ __noinline__ double sum_left(const Visit<T, true>& v, int g0, int g1, int r) {
   constexpr int VEC = RowLogits<T>::VEC;
@@ -437,7 +439,8 @@ __device__ __noinline__ double sum_left(const Visit<T, true>& v, int g0, int g1,
       double w[4], e[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        w[i] = p.near(table, c, fmaxf(RowLogits<T>::raw(xs, i), p.low)) * inv;
+        const float x = RowLogits<T>::raw(xs, i);
+        w[i] = p.near(table, c, fmaxf(x, p.low)) * __hiloint2double(x >= p.low ? __double2hiint(inv) : 0, __double2loint(inv));
         e[i] = q.near(table, c, fmaxf(RowLogits<T>::raw(ys, i), q.low)) * dinv;
       }
 #pragma unroll 1

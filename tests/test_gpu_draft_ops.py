@@ -555,3 +555,22 @@ def test_verify_of_masked_logits(native_lib, V, batch, dtype):
     for seed in range(3):
         logits, _, tokens, parents, cu, u = masked_case(V, [1 + (3 * b + seed) % 7 for b in range(batch)], seed, False, dtype)
         _as_on_the_cpu((logits, tokens, parents, cu, u), max_rows=7)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,batch", [(9, 3), (1003, 40), (30011, 6), (4096, 400)])
+def test_verify_of_masked_logits_of_both_models(native_lib, V, batch, dtype):
+    for seed in range(3):
+        logits, guess, tokens, parents, cu, u = masked_case(V, [1 + (3 * b + seed) % 7 for b in range(batch)], seed, True, dtype)
+        _as_on_the_cpu((logits, tokens, parents, cu, u), max_rows=7, draft_logits=guess)
+
+
+@pytest.mark.parametrize("hidden", [-math.inf, math.nan, O.FMAX * -1, -3e4])
+def test_verify_of_one_allowed_token(native_lib, hidden):
+    """One token is left in both models and a child is a hidden one: nothing is left behind it, and the last token comes from the target's own probabilities."""
+    V = 4000
+    z, d = torch.full((2, V), hidden), torch.full((2, V), hidden)
+    z[:, 7], d[:, 7] = 0.3, 0.1
+    for u0 in (0.0, 1e-30, 0.3, 0.999, 1 - 2.0**-24):
+        want = _as_on_the_cpu((z, *(torch.tensor(x, dtype=I32) for x in ([0, 3], [-1, 0], [0, 2])), torch.tensor([u0, 0.5])), max_rows=2, draft_logits=d)
+        assert want[0][0].tolist() == [7, -1] and want[1].tolist() == [1]
