@@ -273,10 +273,15 @@ def _rounded_down(x: float) -> float:
     return float(f) if float(f) <= x else float(torch.nextafter(f, torch.tensor(-math.inf)))
 
 
+def _usable(z: torch.Tensor) -> torch.Tensor:
+    """Logits in 64 bits, -inf for what is not a number, the largest number for +inf."""
+    z = z.double()
+    return torch.where(z.isnan(), -math.inf, z).clamp(max=torch.finfo(torch.float32).max)
+
+
 def _weights(z: torch.Tensor, temp: float) -> tuple[torch.Tensor, torch.Tensor]:
     """Probabilities and their logarithms in 64 bits; zeros and -inf where no number is above -inf."""
-    z = z.double()
-    z = torch.where(z.isnan(), -math.inf, z).clamp(max=torch.finfo(torch.float32).max)
+    z = _usable(z)
     top = z.max()
     if top == -math.inf:
         return torch.zeros_like(z), z
@@ -295,7 +300,7 @@ def _verify_ref(logits, tokens, parents, spans, uniforms, draft, temps, greedy, 
         while n:
             p, logp = _weights(logits[lo + node], temp)
             some = bool(p.sum() > 0)
-            best = int(torch.argmax(logp)) if some else 0
+            best = int(torch.argmax(_usable(logits[lo + node]))) if some else 0
             q = _weights(draft[lo + node], temp)[0] if draft is not None and not cold else None
             w, left, went = p.clone(), 1.0, -1
             for j in range(node + 1, n) if step + 1 < steps else ():

@@ -252,3 +252,15 @@ def test_verify_restatement_on_masked_logits(V, draft):
         want = O.verify(logits, tokens, parents, cu, u, guess)
         assert min(w[3] for w in want) > 1e-9
         _same(S.verify_drafts(logits, tokens, parents, cu, u, max_rows=7, draft_logits=guess), want, 7)
+
+
+def test_greedy_takes_the_largest_logit_at_any_temperature():
+    """Logits that are alike once a large temperature has divided them."""
+    z = torch.tensor([[0.0, 1.0, 5.0, 2.0], [3.0, 3.0 + 2.0**-21, math.nan, -1.0], [O.FMAX, math.inf, 0.0, O.FMAX], [-math.inf, -2.0, -2.0, -math.inf]])
+    parents, cu = torch.tensor([-1, -1, -1, -1], dtype=torch.int32), torch.arange(5, dtype=torch.int32)
+    for kw in (dict(temperature=x) for x in (1e-30, 1.0, 1e20, math.inf)):
+        got = S.verify_drafts(z, torch.zeros(4, dtype=torch.int32), parents, cu, torch.full((4,), 0.9), max_rows=1, greedy=True, **kw)
+        assert got[0][:, 0].tolist() == [2, 1, 0, 1]
+    tokens, _, rows, _ = S.verify_drafts(z[[0, 0, 0]], torch.tensor([0, 0, 2], dtype=torch.int32), torch.tensor([-1, 0, 0], dtype=torch.int32), torch.tensor([0, 3], dtype=torch.int32),
+                                         torch.zeros(3), max_rows=3, greedy=True, temperature=1e20)
+    assert tokens[0].tolist() == [2, 2, -1] and rows[0].tolist() == [0, 2, -1]

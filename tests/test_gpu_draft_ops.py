@@ -574,3 +574,12 @@ def test_verify_of_one_allowed_token(native_lib, hidden):
     for u0 in (0.0, 1e-30, 0.3, 0.999, 1 - 2.0**-24):
         want = _as_on_the_cpu((z, *(torch.tensor(x, dtype=I32) for x in ([0, 3], [-1, 0], [0, 2])), torch.tensor([u0, 0.5])), max_rows=2, draft_logits=d)
         assert want[0][0].tolist() == [7, -1] and want[1].tolist() == [1]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("temperature", [1e-30, 1.0, 1e20, math.inf])
+def test_greedy_takes_the_largest_logit_at_any_temperature(native_lib, temperature, dtype):
+    """As on the CPU, where a large temperature makes logits alike and where some are not numbers or infinite."""
+    logits, _, tokens, parents, cu, u = _verify_case([9, 1, 5, 7], 3001, 6, 2, False, dtype)
+    logits[0, 70], logits[3, 5:9], logits[9, 2999] = math.nan, math.inf, math.inf
+    _as_on_the_cpu((logits, tokens, parents, cu, u), max_rows=9, greedy=True, temperature=temperature)
