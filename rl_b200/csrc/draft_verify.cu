@@ -27,12 +27,13 @@ __device__ __forceinline__ TreeSpan tree_span(const int* cu, int b, int T, int m
 }
 
 // ------------------------------------------------------------------------------------------------ rows
-// One CTA per sequence (and one for the rows behind the last), a thread per row: it walks up its parents.
+// One CTA per sequence (and one for the rows before the first and behind the last), a thread per row: it walks up its parents. Every row is written by one CTA, whatever the offsets are: a
+// sequence's begin at the largest offset up to its own.
 __global__ void __launch_bounds__(DR_ROWS)
 tree_rows_kernel(const int* __restrict__ parents, const int* __restrict__ cu, const int* __restrict__ ctx, const int* __restrict__ table, long long table_ld,
                  int pages, int block, int B, int T, int max_rows, int words, int* __restrict__ masks, int* __restrict__ positions,
                  long long* __restrict__ slots, int* status) {
-  __shared__ int up[DR_ROWS];
+  __shared__ int up[DR_ROWS], before[DR_ROWS / 32];
   pdl_sync();
   const int b = blockIdx.x, j = threadIdx.x;
   auto none = [&](int from, int to) {      // rows of no sequence see nothing and have no place
@@ -42,20 +43,28 @@ tree_rows_kernel(const int* __restrict__ parents, const int* __restrict__ cu, co
       slots[t] = -1;
     }
   };
-  if (b == B) {
-    none(0, B > 0 ? min(max(cu[0], 0), T) : 0);
-    none(B > 0 ? min(max(cu[B], 0), T) : 0, T);
-    return;
-  }
-  const TreeSpan s = tree_span(cu, b, T, max_rows, status, j == 0);
-  none(s.lo + s.n, min(max(cu[b + 1], s.lo), T));      // (rows over max_rows)
+  int own = 0;
+  for (int i = j; i <= b; i += DR_ROWS) own = max(own, cu[i]);
+  own = __reduce_max_sync(0xffffffffu, own);
+  if ((j & 31) == 0) before[j >> 5] = own;
+  const TreeSpan s = b < B ? tree_span(cu, b, T, max_rows, status, j == 0) : TreeSpan{0, 0};
   if (j < s.n) {
     const int p = parents[s.lo + j];
     up[j] = p >= 0 && p < j ? p : -1;
     if ((p >= j || p < -1) && status) atomicCAS(status, 0, RLB_ERR_BOUNDS);
   }
   __syncthreads();
-  if (j >= s.n) return;
+  own = 0;
+#pragma unroll
+  for (int w = 0; w < DR_ROWS / 32; ++w) own = max(own, before[w]);
+  own = min(own, T);
+  if (b == B) {
+    none(0, min(max(cu[0], 0), T));
+    none(own, T);
+    return;
+  }
+  none(max(s.lo + s.n, own), min(max(cu[b + 1], s.lo), T));      // (rows over max_rows)
+  if (j >= s.n || s.lo + j < own) return;
   uint32_t bits[DR_ROWS / 32] = {};
   int depth = 0;
   for (int a = j; a >= 0; a = up[a], ++depth) {

@@ -101,7 +101,8 @@ def tree_rows(parents: torch.Tensor, cu_rows: torch.Tensor, ctx_lens: torch.Tens
               ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """What the layers need of the trees' rows: ``masks`` int32 [T, ceil(max_rows / 32)], in which bit ``i % 32`` of word ``i // 32`` says that a row sees row ``i`` of its
     sequence (itself and the rows that it continues); ``positions`` int32 [T], the context's length and the rows before it on its path; ``slots`` int64 [T], the
-    cache places as ``rope_kv_cache_write`` takes them. Rows of no sequence (behind the last, before the first, over ``max_rows``) see nothing, with position 0 and slot -1 (which is skipped)."""
+    cache places as ``rope_kv_cache_write`` takes them. Rows of no sequence (behind the last, before the first, over ``max_rows``) see nothing, with position 0 and slot -1 (which is skipped).
+    Where offsets do not ascend, a row that several sequences name is the first one's."""
     B = _rows_of(cu_rows, max_rows)
     T, device, words = parents.shape[0] if parents.dim() == 1 else -1, parents.device, -(-max_rows // 32)
     parents = _ints(parents, (T,), "parents")
@@ -110,12 +111,15 @@ def tree_rows(parents: torch.Tensor, cu_rows: torch.Tensor, ctx_lens: torch.Tens
     if not use_native(parents):
         masks, positions = torch.zeros((T, words), dtype=torch.int32), torch.zeros(T, dtype=torch.int32)
         slots = torch.full((T,), -1, dtype=torch.int64)
-        room = table.shape[1] * block_size
+        room, taken = table.shape[1] * block_size, 0      # taken: rows before are earlier sequences'
         for b, (lo, n) in enumerate(_spans(cu, T, max_rows)):
             seen: list[int] = []
+            taken = max(taken, min(int(cu[b]), T))
             for j in range(n):
                 p, place = int(parents[lo + j]), int(ctx[b]) + j
                 seen.append(1 << j | (seen[p] if 0 <= p < j else 0))
+                if lo + j < taken:
+                    continue
                 for w in range(words):
                     x = seen[j] >> (32 * w) & 0xFFFFFFFF
                     masks[lo + j, w] = x - (1 << 32) if x >> 31 else x

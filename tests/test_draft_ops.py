@@ -264,3 +264,17 @@ def test_greedy_takes_the_largest_logit_at_any_temperature():
     tokens, _, rows, _ = S.verify_drafts(z[[0, 0, 0]], torch.tensor([0, 0, 2], dtype=torch.int32), torch.tensor([-1, 0, 0], dtype=torch.int32), torch.tensor([0, 3], dtype=torch.int32),
                                          torch.zeros(3), max_rows=3, greedy=True, temperature=1e20)
     assert tokens[0].tolist() == [2, 2, -1] and rows[0].tolist() == [0, 2, -1]
+
+
+@pytest.mark.parametrize("cu,T,owners", [([0, 5, 2], 5, [0] * 5), ([0, 5, 3, 8], 9, [0] * 5 + [2] * 3 + [None]), ([4, 2, 6], 7, [None] * 4 + [1] * 2 + [None]), ([0, 4, 1, 3, 6], 6, [0] * 4 + [3] * 2),
+                                         ([0, 9, 2], 5, [0] * 5)])
+def test_rows_that_several_sequences_name(cu, T, owners):
+    """Offsets that do not ascend: a row is the first one's that names it, and one that a sequence has is not one behind the last."""
+    ctx = torch.arange(len(cu) - 1, dtype=torch.int32) * 100
+    table = torch.arange(30 * len(ctx), dtype=torch.int32).reshape(-1, 30)
+    parents = torch.full((T,), -1, dtype=torch.int32)
+    masks, positions, slots = S.tree_rows(parents, torch.tensor(cu, dtype=torch.int32), ctx, table, 16, max_rows=8)
+    for t, b in enumerate(owners):
+        j = t - cu[b] if b is not None else 0
+        assert int(masks[t, 0]) == (1 << j if b is not None else 0) and int(positions[t]) == (int(ctx[b]) if b is not None else 0)
+        assert int(slots[t]) == (30 * 16 * b + int(ctx[b]) + j if b is not None else -1)

@@ -583,3 +583,16 @@ def test_greedy_takes_the_largest_logit_at_any_temperature(native_lib, temperatu
     logits, _, tokens, parents, cu, u = _verify_case([9, 1, 5, 7], 3001, 6, 2, False, dtype)
     logits[0, 70], logits[3, 5:9], logits[9, 2999] = math.nan, math.inf, math.inf
     _as_on_the_cpu((logits, tokens, parents, cu, u), max_rows=9, greedy=True, temperature=temperature)
+
+
+@pytest.mark.parametrize("cu,T", [([0, 5, 2], 5), ([0, 5, 3, 8], 9), ([4, 2, 6], 7), ([0, 4, 1, 3, 6], 6), ([0, 9, 2], 5), ([0, 256, 1, 256] * 60 + [300], 310)])
+def test_rows_that_several_sequences_name(native_lib, cu, T):
+    """As on the CPU, every time."""
+    g = torch.Generator().manual_seed(T)
+    args = [(torch.rand(T, generator=g) * 3).to(I32) - 1, torch.tensor(cu, dtype=I32), torch.arange(len(cu) - 1, dtype=I32), torch.arange(30 * (len(cu) - 1), dtype=I32).reshape(-1, 30)]
+    want = S.tree_rows(*args, 16, max_rows=256)
+    dev = _dev(*args)
+    for _ in range(20):
+        for x, y in zip(S.tree_rows(*dev, 16, max_rows=256), want):
+            assert torch.equal(x.cpu(), y)
+    assert L.check_status() == 8
