@@ -143,7 +143,8 @@ def _tree_decode_ref(q, k_cache, v_cache, table, ctx, spans, Hq, Hkv, D, masks, 
         c = min(max(int(ctx[b]), 0), room)
         keys = min(c + n, room)
         pages = table[b, : -(-keys // block)].long()
-        k, v = (x[pages].transpose(0, 1).reshape(Hkv, -1, D)[:, :keys].float() for x in (k_cache, v_cache))
+        there = (pages >= 0) & (pages < k_cache.shape[0])
+        k, v = (torch.where(there[:, None, None, None], x[torch.where(there, pages, 0)], 0).transpose(0, 1).reshape(Hkv, -1, D)[:, :keys].float() for x in (k_cache, v_cache))
         i = torch.arange(keys) - c
         sees = (i < 0).expand(n, -1).clone()
         for j in range(n):
@@ -153,6 +154,7 @@ def _tree_decode_ref(q, k_cache, v_cache, table, ctx, spans, Hq, Hkv, D, masks, 
             pos = positions[lo : lo + n].long().clamp(min=c)
             own = positions[lo : lo + n].long()
             sees &= pos[:, None] - torch.cat([torch.arange(c), own[: keys - c]]) < window
+        sees &= there.repeat_interleave(block)[:keys]
         s = torch.einsum("nhgd,htd->hgnt", q[lo : lo + n, : Hq * D].reshape(n, Hkv, g, D).float() * scale, k)
         p = torch.softmax(s.masked_fill(~sees, float("-inf")), -1)
         p = torch.where(sees.any(-1)[:, None], p, 0.0)      # (rows that see nothing)
@@ -440,8 +442,11 @@ def kv_cache_keep(caches: Sequence[tuple[torch.Tensor, torch.Tensor]], block_tab
                     last = r
                     if r == i or not (0 <= c + i and c + r < room):
                         continue
+                    to, source = int(table[b, (c + i) // block]), int(table[b, (c + r) // block])
+                    if not (0 <= to < blocks and 0 <= source < blocks):
+                        continue
                     for x in tensors.values():
-                        x[int(table[b, (c + i) // block]), :, (c + i) % block] = x[int(table[b, (c + r) // block]), :, (c + r) % block]
+                        x[to, :, (c + i) % block] = x[source, :, (c + r) % block]
             continue
         _launch(one.device, "rlb_kv_keep", (C.c_void_p * len(tensors))(*tensors), len(tensors), table.data_ptr(), table.stride(0), table.shape[1], block, blocks, heads, vecs,
                 ctx.data_ptr(), rows.data_ptr(), S, counts.data_ptr(), B)

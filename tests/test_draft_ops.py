@@ -278,3 +278,27 @@ def test_rows_that_several_sequences_name(cu, T, owners):
         j = t - cu[b] if b is not None else 0
         assert int(masks[t, 0]) == (1 << j if b is not None else 0) and int(positions[t]) == (int(ctx[b]) if b is not None else 0)
         assert int(slots[t]) == (30 * 16 * b + int(ctx[b]) + j if b is not None else -1)
+
+
+def test_pages_that_are_not_there_are_left_out():
+    """Of a table's entries below zero and behind the cache's last page nothing is read, moved or written."""
+    q, k, v, table, ctx, cu, _ = _attend_case([5, 18], [70, 3], 4, 2, 64, 16, seed=6)
+    bad = table.clone()
+    bad[0, 1], bad[0, 3] = k.shape[0], -1
+    got = S.tree_paged_decode(q, k, v, bad, ctx, cu, 4, 2, 64, max_rows=18)
+    left = torch.tensor([t for t in range(75) if not (16 <= t < 32 or 48 <= t < 64)])
+    kk, vv = (torch.zeros((3, 2, 16, 64)) for _ in range(2))
+    for x, y in ((kk, k), (vv, v)):
+        for i, t in enumerate(left.tolist()):
+            x[i // 16, :, i % 16] = y[table[0, t // 16], :, t % 16]
+    want = S.tree_paged_decode(q[:5], kk, vv, torch.arange(3, dtype=torch.int32)[None], torch.tensor([38], dtype=torch.int32), torch.tensor([0, 5], dtype=torch.int32), 4, 2, 64, max_rows=18)
+    assert torch.allclose(got[:5], want, rtol=1e-4, atol=1e-5)
+    assert torch.equal(got[5:], S.tree_paged_decode(q, k, v, table, ctx, cu, 4, 2, 64, max_rows=18)[5:])
+    none = S.tree_paged_decode(q, k, v, torch.full_like(table, -1), ctx, cu, 4, 2, 64, max_rows=18)
+    assert not none.any()
+    for page, rows in ((-1, [0, 1, 2, 20]), (9, [0, 1, 2, 20]), (-3, [0, 17, 20, 21])):      # the source's page, the targets'
+        caches = [(torch.randn((4, 2, 16, 8)), torch.randn((4, 2, 16, 8)))]
+        t = torch.tensor([[1, page]] if rows[1] == 1 else [[page, 2]], dtype=torch.int32)
+        before = caches[0][0].clone(), caches[0][1].clone()
+        S.kv_cache_keep(caches, t, torch.tensor([0], dtype=torch.int32), torch.tensor([rows], dtype=torch.int32), torch.tensor([4], dtype=torch.int32))
+        assert torch.equal(caches[0][0], before[0]) and torch.equal(caches[0][1], before[1])
