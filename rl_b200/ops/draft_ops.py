@@ -158,7 +158,11 @@ def _tree_decode_ref(q, k_cache, v_cache, table, ctx, spans, Hq, Hkv, D, masks, 
         s = torch.einsum("nhgd,htd->hgnt", q[lo : lo + n, : Hq * D].reshape(n, Hkv, g, D).float() * scale, k)
         p = torch.softmax(s.masked_fill(~sees, float("-inf")), -1)
         p = torch.where(sees.any(-1)[:, None], p, 0.0)      # (rows that see nothing)
-        out[lo : lo + n] = torch.einsum("hgnt,htd->nhgd", p, v).reshape(n, Hq * D).to(out.dtype)
+        finite = v.isfinite()
+        o = torch.einsum("hgnt,htd->nhgd", p, torch.where(finite, v, 0))
+        for t in (~finite).any(-1).any(0).nonzero().flatten().tolist():      # (a weight of zero times these is not zero)
+            o[sees[:, t]] += torch.where(finite, 0, v)[:, t, None]
+        out[lo : lo + n] = o.reshape(n, Hq * D).to(out.dtype)
     return out
 
 

@@ -302,3 +302,20 @@ def test_pages_that_are_not_there_are_left_out():
         before = caches[0][0].clone(), caches[0][1].clone()
         S.kv_cache_keep(caches, t, torch.tensor([0], dtype=torch.int32), torch.tensor([rows], dtype=torch.int32), torch.tensor([4], dtype=torch.int32))
         assert torch.equal(caches[0][0], before[0]) and torch.equal(caches[0][1], before[1])
+
+
+def test_values_that_are_not_finite_reach_the_rows_that_see_them():
+    """And no others: rows of other branches, rows whose window or context ends before."""
+    q, k, v, table, ctx, _, _ = _attend_case([6, 4], [20, 33], 4, 2, 64, 16, seed=3)
+    parents, cu = torch.tensor([-1, 0, 0, 1, 2, 4, -1, 0, 1, 1], dtype=torch.int32), torch.tensor([0, 6, 10], dtype=torch.int32)
+    masks, positions, _ = S.tree_rows(parents, cu, ctx, table.clamp(min=0), 16, max_rows=6)
+    run = lambda values, **kw: S.tree_paged_decode(q, k, values, table, ctx, cu, 4, 2, 64, max_rows=6, masks=masks, **kw)  # noqa: E731
+    for place, blind, window in ((22, [0, 1, 3, 6, 7, 8, 9], 0), (0, [0, 1, 2, 3, 4, 5, 6, 7, 8, 9], 8), (14, [1, 2, 3, 4, 5, 6, 7, 8, 9], 7)):
+        kw = dict(window=window, positions=positions) if window else {}
+        bad = v.clone()
+        bad[table[0, place // 16], :, place % 16] = torch.tensor([math.nan, math.inf, -math.inf])[torch.arange(64) % 3]
+        got, want = run(bad, **kw), run(v, **kw)
+        assert torch.equal(got[blind], want[blind])
+        for r in set(range(10)) - set(blind):
+            x = got[r].reshape(4, 64)
+            assert x[:, 0::3].isnan().all() and (x[:, 1::3] == math.inf).all() and (x[:, 2::3] == -math.inf).all()
