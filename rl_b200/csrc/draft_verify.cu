@@ -175,6 +175,8 @@ constexpr int EXP_STEPS = 256;
 constexpr double LOG2E = 1.4426950408889634074, LN2 = 0.69314718055994530942;
 constexpr double MAGIC = 6755399441055744.0 / EXP_STEPS;      // 1.5 * 2^52 / 256: a sum with it has the nearest number of 256ths in its low word
 constexpr float F_MAX = 3.402823466e38f;
+// Two probabilities are off by up to 3e-13 from one another, relatively, where they are equal: a draft's are taken as 4.5e-13 more, so that nothing is left of tokens that are as probable in both.
+constexpr double DRAFT_MORE = 1.0 + 0x1p-41;
 constexpr float COLDEST = 1.17549435e-38f;      // temperatures below are greedy
 
 // Copies of 16 bytes to shared memory, which the lane that issued them reads itself.
@@ -718,7 +720,7 @@ verify_kernel(const VerifyArgs a) {
         if (cold) best = __shfl_sync(0xffffffffu, best, max(0, __ffs(__ballot_sync(0xffffffffu, best >= 0)) - 1));
         if (lane == 0) {
           to.f = whole;
-          to.inv = inv;
+          to.inv = DRAFT && warp ? inv * DRAFT_MORE : inv;
           to.sum = all;
           if (warp == 0) {
             if (cold) row_best = max(0, best);

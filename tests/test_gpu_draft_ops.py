@@ -596,3 +596,24 @@ def test_rows_that_several_sequences_name(native_lib, cu, T):
         for x, y in zip(S.tree_rows(*dev, 16, max_rows=256), want):
             assert torch.equal(x.cpu(), y)
     assert L.check_status() == 8
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("temperature", [1.0, 0.7, 20.0])
+def test_verify_where_both_models_agree(native_lib, temperature, dtype):
+    """Tokens that are as probable in the draft as in the target have nothing left behind a rejection: of all tokens (the child is a hidden one: the last token is the target's own), and of all but
+    one, which is the last token whatever the number is. Logits are whole numbers and differ by a constant, so that the probabilities are equal in exact arithmetic."""
+    V, g = 4096, torch.Generator().manual_seed(3)
+    for seed in range(12):
+        few = torch.randperm(V, generator=g)[:6].sort().values
+        z, d = torch.full((2, V), -math.inf), torch.full((2, V), -math.inf)
+        z[:, few] = torch.randint(-3, 4, (6,), generator=g).float() if seed % 2 else 0.0
+        d[:, few] = z[:, few] + 10.0 * seed + 1
+        child = int((few[-1] + 1) % V)
+        one = seed % 4 > 1 and seed % 2 == 0      # the draft has the hidden child in place of the last token
+        if one:
+            d[:, child], d[:, few[-1]] = d[0, few[-1]].item(), -math.inf
+        for u0 in (0.0, 1e-9, 0.4, 1 - 2.0**-24):
+            args = (z.to(dtype), torch.tensor([0, child], dtype=I32), torch.tensor([-1, 0], dtype=I32), torch.tensor([0, 2], dtype=I32), torch.tensor([u0, 0.5]))
+            want = _as_on_the_cpu(args, max_rows=2, draft_logits=d.to(dtype), temperature=temperature)
+            assert not one or want[0][0].tolist() == [int(few[-1]), -1]
