@@ -363,7 +363,8 @@ __device__ __noinline__ double rest_of(const Visit<T, DRAFT>& v, int i, float x,
   double w = weight_of(v.row[0].f, v.table, v.c, x) * v.row[0].inv;
   if (r == 0) return w;
   if (DRAFT) {
-    const double g = weight_of(v.row[DRAFT].f, v.table, v.c, y) * v.row[DRAFT].inv;
+    const Frame& f = v.row[DRAFT].f;      // (what is below `low` as much as that, where sum_left may be asked for the same)
+    const double g = (f.kind == 0 ? f.near(v.table, v.c, fminf(fmaxf(y, f.low), f.top)) : weight_of(f, v.table, v.c, y)) * v.row[DRAFT].inv;
 #pragma unroll 1
     for (int k = 0; k < r; ++k) w = fmax(fma(w, v.grow[k], -g), 0.0);
   } else {
@@ -419,7 +420,7 @@ __device__ __noinline__ double sum_of(const Visit<T, DRAFT>& v, int e0, int e1, 
 }
 // The same of the groups from g0 to g1 of a row and its draft's, both of kind 0 and without infinities: as in the row's own sums, but that what weighs nothing in the target is nothing, or a
 // difference would be left where no token has a share and the last token could fall there. (2^-500 and less, `low`'s weight, times a factor without exponent, below 2^-1042, is zero: 127 us for 48 of
-// 8 drawn rows, 151936 logits, as without it; 131 with the weight itself chosen.) The draft's may be too much by as much: a sum is never more than its tokens' shares.
+// 8 drawn rows, 151936 logits, as without it; 131 with the weight itself chosen.) The draft's is at least `low`'s, here and in rest_of.
 template <typename T>
 __device__ __noinline__ double sum_left(const Visit<T, true>& v, int g0, int g1, int r) {
   constexpr int VEC = RowLogits<T>::VEC;

@@ -328,7 +328,7 @@ def _verify_ref(logits, tokens, parents, spans, uniforms, draft, temps, greedy, 
                     went = j
                     break
                 if q is not None:
-                    w = (w / left - q).clamp_(min=0.0)
+                    w = (w / left - q.clamp(min=2.0**-1000 * float(q.max()))).clamp_(min=0.0)
                     left = float(w.sum())
                     if not left > 0:
                         break
@@ -365,7 +365,7 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Ten
     accepted if u Z q(x) < w(x), and is the next node. Otherwise, with ``draft_logits`` [T, V] (the logits, at the same temperature, that a row's children were drawn from,
     independently), w becomes max(w / Z - q, 0) and Z its sum; without (children were taken without chance, each token once; q = 1) Z loses w(x) and x is out. Where no child
     is accepted, the last token is the first whose running sum of w passes row 0's number times the whole sum. Greedy: a child is accepted if its token has the largest logit (of equal ones the lowest), which is the last token too.
-    Logits that are not numbers weigh nothing, nor does what is less than 2^-1000 of the largest; +inf as much as the largest number. At most ``max_steps`` tokens (None: ``max_rows``).
+    Logits that are not numbers weigh nothing, nor does what is less than 2^-1000 of the largest (what the draft takes off a token is at least that); +inf as much as the largest number. At most ``max_steps`` tokens (None: ``max_rows``).
 
     Returns ``tokens`` int32 [B, max_steps] (accepted ones and the last; -1 behind them), ``counts`` int32 [B], ``rows`` int32 [B, max_steps] (row 0 and the accepted rows, as :func:`kv_cache_keep`
     takes them; -1 behind them) and ``logprobs`` fp32 [B, max_steps], the tokens' logarithms of p (0 behind them; -inf where no logit is above -inf, whose token is 0). Sums are in 64 bits."""

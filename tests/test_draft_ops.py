@@ -319,3 +319,18 @@ def test_values_that_are_not_finite_reach_the_rows_that_see_them():
         for r in set(range(10)) - set(blind):
             x = got[r].reshape(4, 64)
             assert x[:, 0::3].isnan().all() and (x[:, 1::3] == math.inf).all() and (x[:, 2::3] == -math.inf).all()
+
+
+def faint_case(V=4096):
+    """Two tokens have the target's weight and two the draft's; all others are so faint (2^-999 and 2^-1001 of the largest) that a draft which took nothing off them would leave them."""
+    z, d = torch.full((4, V), -692.2), torch.full((4, V), -690.4)
+    z[:, 300], z[:, 2000], d[:, 300], d[:, 17] = 0.0, 0.02, 3.0, 0.3
+    tokens, parents = torch.tensor([0, 17, 300, 300], dtype=torch.int32), torch.tensor([-1, 0, 0, 0], dtype=torch.int32)
+    return (z, tokens, parents, torch.tensor([0, 4], dtype=torch.int32), torch.tensor([0.0, 0.999, 0.999, 0.999])), d
+
+
+def test_verify_of_what_is_nearly_nothing():
+    args, d = faint_case()
+    want = O.verify(args[0], *args[1:4], args[4], d)
+    assert want[0][:2] == ([2000], [0])
+    _same(S.verify_drafts(*args, max_rows=4, draft_logits=d), want, 4)

@@ -5,7 +5,7 @@ import math
 import draft_oracle as O
 import pytest
 import torch
-from test_draft_ops import _same, _verify_case, masked_case
+from test_draft_ops import _same, _verify_case, faint_case, masked_case
 
 from rl_b200.ops import draft_ops as S
 from rl_b200.ops import engine_ops as E
@@ -617,3 +617,8 @@ def test_verify_where_both_models_agree(native_lib, temperature, dtype):
             args = (z.to(dtype), torch.tensor([0, child], dtype=I32), torch.tensor([-1, 0], dtype=I32), torch.tensor([0, 2], dtype=I32), torch.tensor([u0, 0.5]))
             want = _as_on_the_cpu(args, max_rows=2, draft_logits=d.to(dtype), temperature=temperature)
             assert not one or want[0][0].tolist() == [int(few[-1]), -1]
+
+
+def test_verify_of_what_is_nearly_nothing(native_lib):
+    args, d = faint_case()
+    assert int(_as_on_the_cpu(args, max_rows=4, draft_logits=d)[0][0, 0]) == 2000
