@@ -145,7 +145,7 @@ keep_kernel(const __grid_constant__ KeepCaches caches, const int* __restrict__ t
 // of tokens and leaves its sum in every CTA's shared memory; all CTAs come to the same decision. The ranges' sums say in which range the last token lies, whose CTA
 // goes through it once more. With draft logits the sums are taken again behind a rejection; without, the rejected tokens' weights are taken off their ranges.
 //
-// Bound by the instructions' rate (64 trees of 17 rows, 128256 logits: 54 us for 56 MB, 58 % of the issue slots while an SM has work) and by latency: a row is its sums (5500 cycles of
+// Bound by the instructions' rate (64 trees of 17 rows, 128256 logits: 52 us for 56 MB, 58 % of the issue slots while an SM has work) and by latency: a row is its sums (5500 cycles of
 // 11000), the exchange (1400), the joining of the parts (1000) and the children (1000), one after another; a single row of 128256 logits takes 10 us, a chain of 6 with 32000 logits 10.
 // 48 sequences of 8 drawn rows, 151936 logits: 127 us for 82 MB. A first pass in 32 bits with sums in 64 where they decide was slower, so were 256 threads in clusters of 16, a table
 // entry for each of 128ths in 16 copies without conflicts of banks, eight loads of a lane on their way in place of four, and the first child's logits fetched while a row's parts are exchanged.

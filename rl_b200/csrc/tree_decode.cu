@@ -7,7 +7,7 @@
 //   warp 0      TMA producer: the unit's queries, then K tiles through a ring and V tiles through another. A tile is 64 / R boxes of R = gcd(page, 64) keys; a box whose page is not
 //               there (behind the last key, or no page of the cache) starts behind the cache's last row, and arrives as zeros
 //   warp 1      tcgen05.mma issuer: S = Q K^T (128 x 64 x D) into one of two TMEM buffers, one tile ahead of the softmax, then O += P V (128 x D x 64) with P read from TMEM
-//   warps 2..5  softmax, a thread per row: maximum and sum in 32 bits; P is rounded to bf16 (half a step: 2^-9 of a weight's share, about what the output's own rounding costs)
+//   warps 2..5  softmax, a thread per row: maximum and sum in 32 bits; P is rounded to bf16 (half a step: up to 2^-8 of a weight, as the output's own rounding)
 //               over the scores that were read; O is rescaled only when the maximum moved by more than 2^8.
 // In tiles that some row does not see as a whole (the tree's, the window's edge, the last) a row has a word of 64 bits, and V is searched for values that are not finite: these would
 // reach every row through weights of zero. They are set to zero there and added in the end to the rows that see them.
@@ -15,9 +15,10 @@
 // The tiles of all units form one sequence, of which each CTA takes an equal share (two CTAs to an SM, all resident): contexts of any lengths fill the device. Units that
 // are cut leave sums, maximum and 32-bit output of their parts in a workspace, and a second kernel joins them in their order. With few tiles to a unit a CTA takes a whole unit instead.
 //
-// Long contexts of few rows are bound by memory (32 chains of 5 on 32768 tokens, 32 / 8 heads of 128: 4.3 GB of keys and values in 624 us, above the rate of a plain copy). With 64 rows and more the
-// tensor cores and the softmax take turns: a product of 64 keys costs as much as one of 128, and a pair of tiles takes 2100 cycles, 1540 of them the products' (16 trees of 64 on 8001, 28 / 4 heads: 104 us,
-// 0.17 GB; one tree of 33 on 131072, 40 / 8 heads: 147 us, 0.54 GB). Short contexts pay for a unit's start and end (64 trees of 17 rows to 1280 tokens: 52 us where memory takes 35).
+// Long contexts of few rows are bound by memory (31 chains of 5 on 32768 tokens, 32 / 8 heads of 128: 4.2 GB of keys and values, 637 us at the rate of a plain copy: 605 in a graph of short runs,
+// 670 to 741 in calls one after another, board by board). With 64 rows and more the
+// tensor cores and the softmax take turns: a product of 64 keys costs as much as one of 128, and a pair of tiles takes 2100 cycles, 1540 of them the products' (16 trees of 64 on 8001, 28 / 4 heads: 103 us,
+// 0.17 GB; one tree of 33 on 131072, 40 / 8 heads: 152 us, 0.54 GB). Short contexts pay for a unit's start and end (64 trees of 17 rows to 1280 tokens: 52 us where memory takes 35).
 //
 // This file is compiled without fast math.
 #include "common.cuh"

@@ -12,7 +12,8 @@ before the tree; row ``j``'s key and value stand at place ``ctx_lens[b] + j`` of
 
 On the GPU offsets that do not ascend, rows over ``max_rows``, parents that are not above their row, pages that are not there and places outside the table are left
 out. The status word then has ``RLB_ERR_BOUNDS``: from :func:`tree_rows` for offsets, rows, parents and places, from :func:`verify_drafts` for offsets and rows, from
-:func:`tree_paged_decode` for pages, from :func:`kv_cache_keep` for rows, pages and places. CPU tensors run the PyTorch restatement. Everything here is for inference: nothing has a gradient.
+:func:`tree_paged_decode` for pages, from :func:`kv_cache_keep` for rows, pages and places. Where offsets that do not ascend have several sequences name a row, :func:`tree_paged_decode` gives it
+the attention of one of them. CPU tensors run the PyTorch restatement. Everything here is for inference: nothing has a gradient.
 """
 
 from __future__ import annotations
@@ -368,7 +369,8 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Ten
     Logits that are not numbers weigh nothing, nor does what is less than 2^-1000 of the largest (what the draft takes off a token is at least that); +inf as much as the largest number. At most ``max_steps`` tokens (None: ``max_rows``).
 
     Returns ``tokens`` int32 [B, max_steps] (accepted ones and the last; -1 behind them), ``counts`` int32 [B], ``rows`` int32 [B, max_steps] (row 0 and the accepted rows, as :func:`kv_cache_keep`
-    takes them; -1 behind them) and ``logprobs`` fp32 [B, max_steps], the tokens' logarithms of p (0 behind them; -inf where no logit is above -inf, whose token is 0). Sums are in 64 bits."""
+    takes them; -1 behind them) and ``logprobs`` fp32 [B, max_steps], the tokens' logarithms of p (0 behind them; -inf where no logit is above -inf, whose token is 0). Sums are in 64 bits, weights to 1.5e-13; on the GPU a draft's probabilities count as 2^-41 more, so
+    that of tokens as probable in both nothing is left."""
     B = _rows_of(cu_rows, max_rows)
     if logits.dim() != 2 or logits.dtype not in (torch.float32, BF16) or not 1 <= logits.shape[1] <= MAX_VOCAB:
         raise ValueError(f"logits are fp32 or bf16 [T, V] with V up to 2^30, not {logits.dtype} {tuple(logits.shape)}")
